@@ -1,0 +1,867 @@
+// The paged cache that is held in 8 bits (format: kv8.cuh): its write, and the attention that reads it.
+//
+//   kv8_write_kernel     rotates q and k, stores k and v with a scale for every page and kv head
+//   kv8_decode_kernel    single tokens on the CUDA cores: any head size in steps of 16 up to 256, float32 or bfloat16
+//   kv8_prefill_kernel   portions of prompts on the CUDA cores, for the same types and sizes
+#include "kv8.cuh"
+
+#ifndef RL_HEAD_DIM
+#define RL_HEAD_DIM 64
+#endif
+
+namespace rl {
+
+constexpr int kD = RL_HEAD_DIM;
+static_assert(kD % 16 == 0 && kD >= 16 && kD <= 256, "head size must be a multiple of 16, at most 256");
+
+// ------------------------------------------------------------------------------------------------ write
+
+// Eight consecutive elements.
+__device__ __forceinline__ void load8(const float* p, float* out) {
+  load16(p, out);
+  load16(p + 4, out + 4);
+}
+__device__ __forceinline__ void load8(const bf16* p, float* out) { load16(p, out); }
+__device__ __forceinline__ void store8(float* p, const float* in) {
+  store16(p, in);
+  store16(p + 4, in + 4);
+}
+__device__ __forceinline__ void store8(bf16* p, const float* in) { store16(p, in); }
+
+// Entries i and i + D/2 of a head by the angle's cosine and sine.  (Each product is rounded before the sum: what is
+// stored next is rounded to 4 bits, and a fused sum would land on the other side of a border now and then.)
+__device__ __forceinline__ void kv8_rotate8(float* x0, float* x1, const float* cos, const float* sin) {
+  float c[8], s[8];
+  load8(cos, c);
+  load8(sin, s);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float a = x0[i], b = x1[i];
+    x0[i] = __fsub_rn(__fmul_rn(a, c[i]), __fmul_rn(b, s[i]));
+    x1[i] = __fadd_rn(__fmul_rn(b, c[i]), __fmul_rn(a, s[i]));
+  }
+}
+
+template <typename T>
+struct Kv8WriteArgs {
+  const T* qkv;                // [tokens, qkv_stride]: q heads, then k heads, then v heads
+  int qkv_stride;
+  const int32_t* positions;
+  const int32_t* slots;        // [tokens] place in the cache; negative: none.  With items instead: null
+  const int4* items;           // (token, sequence, context): the slot is that of position context - 1
+  const int32_t* block_table;
+  int max_blocks;
+  const float* cos;            // [max_pos, D/2], null: no rotation
+  const float* sin;
+  uint8_t* kcache;
+  uint8_t* vcache;
+  uint8_t* kscale;
+  uint8_t* vscale;
+  T* q_out;                    // [tokens, q_stride], null: q is left alone
+  int q_stride;
+  int tokens, hq, hkv, page_shift, max_pos;
+  long long num_slots;
+  int* status;
+};
+
+// Slot of token t (-1: none).
+template <typename T>
+__device__ __forceinline__ long long kv8_slot(const Kv8WriteArgs<T>& a, int t) {
+  if (a.slots != nullptr) return a.slots[t];
+  const int4 info = a.items[t];
+  if (info.z <= 0) return -1;
+  const int pos = info.z - 1;
+  return (static_cast<long long>(a.block_table[static_cast<size_t>(info.y) * a.max_blocks + (pos >> a.page_shift)])
+          << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
+}
+
+// A position whose angles the tables have.
+template <typename T>
+__device__ __forceinline__ int kv8_position(const Kv8WriteArgs<T>& a, int pos) {
+  if (pos >= 0 && pos < a.max_pos) return pos;
+  atomicOr(a.status, 2);
+  return 0;
+}
+
+constexpr int kWriteThreads = 512;
+
+// The first `kv_blocks` CTAs are one to a token (or item): where a RUN begins there, the tokens that follow one another in
+// one page, the CTA stores the run, a warp to the keys or the values of a kv head; the others have nothing to do.  (A
+// warp to 16 tokens of a head: 32 bytes of each lane's asked for at once.  With one CTA to a fixed window of tokens, single
+// tokens would queue in one CTA, and where a prompt's pages begin among the tokens is not known to the host.)  The CTAs
+// behind them rotate q, eight pairs of entries to a thread.
+// The scale needs the block's largest magnitude before the first byte can be written: two passes over the run, the
+// second of which finds it in L1.
+template <typename T>
+__global__ void __launch_bounds__(kWriteThreads)
+kv8_write_kernel(const Kv8WriteArgs<T> a, int kv_blocks) {
+  pdl_wait();
+  pdl_launch();    // (behind the wait: a kernel after this one may read, before its own wait, what kernels before this one wrote)
+  constexpr int CH = kD / 16;                    // lanes to a token: each has 8 entries of either half of the head
+  if (static_cast<int>(blockIdx.x) >= kv_blocks) {
+    const int per = a.hq * CH;
+    const long long idx = static_cast<long long>(blockIdx.x - kv_blocks) * kWriteThreads + threadIdx.x;
+    if (idx >= static_cast<long long>(a.tokens) * per) return;
+    const int t = static_cast<int>(idx / per), rest = static_cast<int>(idx - static_cast<long long>(t) * per);
+    const int col = rest / CH * kD + rest % CH * 8;
+    const T* src = a.qkv + static_cast<size_t>(t) * a.qkv_stride + col;
+    float x0[8], x1[8];
+    load8(src, x0);
+    load8(src + kD / 2, x1);
+    if (a.cos != nullptr) {
+      const size_t at = static_cast<size_t>(kv8_position(a, a.positions[t])) * (kD / 2) + rest % CH * 8;
+      kv8_rotate8(x0, x1, a.cos + at, a.sin + at);
+    }
+    T* dst = a.q_out + static_cast<size_t>(t) * a.q_stride + col;
+    store8(dst, x0);
+    store8(dst + kD / 2, x1);
+    return;
+  }
+  const int t = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int ps = 1 << a.page_shift;
+  const long long slot = kv8_slot(a, t);
+  if (slot < 0) return;
+  if (slot >= a.num_slots) {
+    if (threadIdx.x == 0) atomicOr(a.status, 4);
+    return;
+  }
+  const int off = static_cast<int>(slot & (ps - 1));
+  const long long page = slot >> a.page_shift;
+  if (t > 0 && off > 0 && kv8_slot(a, t - 1) == slot - 1) return;      // not the first of its run
+  // Two runs of one page in one call would each set its scale without the other's: only the first is stored.  (Page 0
+  // is the reserved one that padding rows write to: nothing to tell of there.)
+  bool before = false;
+  for (int i = threadIdx.x; i < t; i += blockDim.x) {
+    const long long s = kv8_slot(a, i);
+    before |= s >= 0 && (s >> a.page_shift) == page;
+  }
+  if (__syncthreads_or(before)) {
+    if (threadIdx.x == 0 && page != 0) atomicOr(a.status, 8);
+    return;
+  }
+  int n = 1;                                     // tokens of the run
+  {
+    bool same = true;
+    for (int i0 = 0; same && i0 < ps; i0 += 32) {
+      const int i = i0 + lane;
+      const bool in = t + i < a.tokens && off + i < ps && kv8_slot(a, t + i) == slot + i;
+      const unsigned m = __ballot_sync(0xffffffffu, in);
+      n = m == 0xffffffffu ? i0 + 32 : i0 + __ffs(~m) - 1;
+      same = m == 0xffffffffu;
+    }
+  }
+  constexpr int TPR = 32 / CH;                   // tokens that a warp takes at once
+  const int tl = lane / CH, ch = lane - tl * CH;
+  for (int w = warp; w < 2 * a.hkv; w += blockDim.x >> 5) {
+    const bool is_v = w >= a.hkv;
+    const int h = is_v ? w - a.hkv : w;
+    const T* src = a.qkv + static_cast<size_t>(t) * a.qkv_stride + static_cast<size_t>(a.hq + w) * kD + ch * 8;
+    const bool turn = !is_v && a.cos != nullptr;
+    auto load = [&](int i, float* x0, float* x1) {
+      const T* p = src + static_cast<size_t>(i) * a.qkv_stride;
+      load8(p, x0);
+      load8(p + kD / 2, x1);
+      if (turn) {
+        const int pos = a.items != nullptr ? a.items[t + i].z - 1 : a.positions[t + i];
+        const size_t at = static_cast<size_t>(kv8_position(a, pos)) * (kD / 2) + ch * 8;
+        kv8_rotate8(x0, x1, a.cos + at, a.sin + at);
+      }
+    };
+    float amax = 0.f;
+#pragma unroll 2
+    for (int i = tl; i < n; i += TPR) {
+      if (tl >= TPR) break;
+      float x0[8], x1[8];
+      load(i, x0, x1);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float u = fabsf(x0[e]), v = fabsf(x1[e]);
+        amax = fmaxf(amax, fmaxf(u < INFINITY ? u : 0.f, v < INFINITY ? v : 0.f));
+      }
+    }
+    amax = warp_max(amax);
+    uint8_t* cache = is_v ? a.vcache : a.kcache;
+    uint8_t* scale = (is_v ? a.vscale : a.kscale) + static_cast<size_t>(page) * a.hkv + h;
+    uint8_t* base = cache + (static_cast<size_t>(page) * a.hkv + h) * (static_cast<size_t>(ps) * kD);
+    int code = kv8_code(amax);
+    if (off > 0) {
+      const int old = min(static_cast<int>(*scale), 254);
+      if (code > old) {                          // what is in the page goes over to the larger scale
+        const float f = kv8_exp2i(max(old - code, -127));
+        for (int c = lane; c < off * (kD / 16); c += 32) {
+          uint4* p = reinterpret_cast<uint4*>(base) + c;
+          float x[16];
+          kv8_f16(*p, x);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[e] *= f;
+          *p = make_uint4(kv8_pack4(x), kv8_pack4(x + 4), kv8_pack4(x + 8), kv8_pack4(x + 12));
+        }
+      } else {
+        code = old;
+      }
+      __syncwarp();                              // (every lane has read the scale)
+    }
+    if (lane == 0) *scale = static_cast<uint8_t>(code);
+    const float inv = kv8_exp2i(127 - code);
+#pragma unroll 2
+    for (int i = tl; i < n; i += TPR) {
+      if (tl >= TPR) break;
+      float x0[8], x1[8];
+      load(i, x0, x1);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {              // (what is not finite is stored as not a number, and left out of the scale)
+        x0[e] = fabsf(x0[e]) < INFINITY ? x0[e] * inv : __uint_as_float(0x7fc00000u);
+        x1[e] = fabsf(x1[e]) < INFINITY ? x1[e] * inv : __uint_as_float(0x7fc00000u);
+      }
+      uint8_t* dst = base + static_cast<size_t>(off + i) * kD + ch * 8;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(kv8_pack4(x0), kv8_pack4(x0 + 4));
+      *reinterpret_cast<uint2*>(dst + kD / 2) = make_uint2(kv8_pack4(x1), kv8_pack4(x1 + 4));
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ single tokens
+
+constexpr int kUnit = 64;                  // keys of a unit of work (an absolute boundary; the largest page)
+constexpr int kMaxItems = 1024;            // items whose first units are kept in shared memory
+
+// The launch's units: start[i] is the first unit of item i (all its kv heads), start[nitems] their number.
+// Called by all threads of the CTA; `start` is shared memory for nitems + 1.
+__device__ __forceinline__ int kv8_units(const Kv8Args& a, int* start) {
+  __shared__ int warp_sums[33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
+  int run = 0;
+  for (int i0 = 0; i0 < a.nitems; i0 += blockDim.x) {
+    const int i = i0 + threadIdx.x;
+    int n = 0;
+    if (i < a.nitems) {
+      const int ctx = a.items[i].z;
+      if (ctx > 0) {
+        const int lo = a.window > 0 && ctx > a.window ? ctx - a.window : 0;
+        n = ((ctx - 1) / kUnit - lo / kUnit + 1) * a.hkv;
+      }
+    }
+    int inc = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += up;
+    }
+    if (lane == 31) warp_sums[warp] = inc;
+    __syncthreads();
+    int below = 0, all = 0;
+    for (int w = 0; w < nwarps; ++w) {
+      if (w < warp) below += warp_sums[w];
+      all += warp_sums[w];
+    }
+    if (i < a.nitems) start[i] = run + below + inc - n;
+    run += all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) start[a.nitems] = run;
+  __syncthreads();
+  return run;
+}
+
+// A share's part of one row: keys [key_lo, key_hi).
+struct Kv8Segment {
+  int item, kvh, tok, seq, ctx;
+  int key_lo, key_hi;
+  int next;                 // the unit after the segment
+  int row_begin, row_end;   // the row's units
+  bool whole;
+};
+
+// The units of share s of `shares`: [s U / shares, (s + 1) U / shares).
+__device__ __forceinline__ int kv8_share_begin(int s, int units, int shares) {
+  return static_cast<int>(static_cast<long long>(units) * s / shares);
+}
+// The share that unit u lies in.
+__device__ __forceinline__ int kv8_share_of(int u, int units, int shares) {
+  int s = static_cast<int>((static_cast<long long>(u) * shares) / units);
+  while (kv8_share_begin(s + 1, units, shares) <= u) ++s;
+  return s;
+}
+
+__device__ __forceinline__ Kv8Segment kv8_segment(const Kv8Args& a, const int* start, int u, int end) {
+  int lo = 0, hi = a.nitems - 1;            // the largest i with start[i] <= u (items without keys have no units)
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (start[mid] <= u) lo = mid; else hi = mid - 1;
+  }
+  Kv8Segment g;
+  g.item = lo;
+  const int4 info = a.items[lo];
+  g.tok = info.x;
+  g.seq = info.y;
+  g.ctx = info.z;
+  const int first = a.window > 0 && g.ctx > a.window ? g.ctx - a.window : 0;
+  const int u0 = first / kUnit, n = (g.ctx - 1) / kUnit - u0 + 1;
+  g.kvh = (u - start[lo]) / n;
+  g.row_begin = start[lo] + g.kvh * n;
+  g.row_end = g.row_begin + n;
+  g.next = min(end, g.row_end);
+  g.key_lo = max(first, (u0 + u - g.row_begin) * kUnit);
+  g.key_hi = min(g.ctx, (u0 + g.next - g.row_begin) * kUnit);
+  g.whole = u == g.row_begin && g.next == g.row_end;
+  return g;
+}
+
+// The pieces of a cut row, added in the order of the keys and written out, by `nthreads` threads.
+template <typename T>
+__device__ __forceinline__ void kv8_merge(const Kv8Args& a, const Kv8Segment& g, int units, int shares, int tid, int nthreads) {
+  const int G = a.hq / a.hkv;
+  const int s0 = kv8_share_of(g.row_begin, units, shares), s1 = kv8_share_of(g.row_end - 1, units, shares);
+  const int row = G * (kD + 2);
+  for (int i = tid; i < G * kD; i += nthreads) {
+    const int r = i / kD, d = i - r * kD;
+    float m = -INFINITY, den = 0.f, num = 0.f;
+    for (int s = s0; s <= s1; ++s) {
+      // (the first piece ends its share unless it begins it: its place is 0 then, as everybody else's)
+      const int place = s == s0 && kv8_share_begin(s, units, shares) != g.row_begin ? 1 : 0;
+      const float* p = a.part + (static_cast<size_t>(s) * 2 + place) * row + r * (kD + 2);
+      const float pm = __ldcg(p + kD), pl = __ldcg(p + kD + 1), pn = __ldcg(p + d);
+      const float mn = fmaxf(m, pm);
+      const float f = m == -INFINITY ? 0.f : exp2f(m - mn), w = pm == -INFINITY ? 0.f : exp2f(pm - mn);
+      den = den * f + pl * w;
+      num = num * f + pn * w;
+      m = mn;
+    }
+    static_cast<T*>(a.out)[static_cast<size_t>(g.tok) * a.out_stride + (g.kvh * G + r) * kD + d] = from_float<T>(num / den);
+  }
+}
+
+constexpr int kGenThreads = 128;
+constexpr int kGenHeads = 4;               // query heads in one pass over the keys
+constexpr int kGenLanes = kD <= 16 ? 1 : kD <= 32 ? 2 : kD <= 64 ? 4 : kD <= 128 ? 8 : 16;     // lanes to a key: 16 entries each
+
+// Single tokens on the CUDA cores.  A CTA to a share; a key to kGenLanes lanes of a warp, each with 16 entries of four
+// query heads and their numerators in registers and a running (max, denominator) of its own keys.
+template <typename T>
+__global__ void __launch_bounds__(kGenThreads)
+kv8_decode_kernel(const Kv8Args a) {
+  __shared__ int start[kMaxItems + 1];
+  __shared__ float parts[kGenThreads / 32][kGenHeads][kD + 2];
+  __shared__ int last;
+  pdl_launch();
+  pdl_wait();
+  constexpr float kLog2e = 1.4426950408889634f;
+  constexpr int KPW = 32 / kGenLanes;       // keys that a warp takes at once
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int G = a.hq / a.hkv, ps = 1 << a.page_shift;
+  const int ch = lane % kGenLanes, slot = lane / kGenLanes;
+  const bool in_head = ch * 16 < kD;
+  const int units = kv8_units(a, start);
+  const int shares = min(static_cast<int>(gridDim.x), units);      // every share has a unit
+  if (static_cast<int>(blockIdx.x) >= shares) return;
+  const int end = kv8_share_begin(blockIdx.x + 1, units, shares);
+  const int begin = kv8_share_begin(blockIdx.x, units, shares);
+  for (int u = begin; u < end;) {
+    const Kv8Segment g = kv8_segment(a, start, u, end);
+    const int32_t* bt = a.block_table + static_cast<size_t>(g.seq) * a.max_blocks;
+    float* piece = a.part + (static_cast<size_t>(blockIdx.x) * 2 + (u == begin ? 0 : 1)) * (G * (kD + 2));
+    for (int g0 = 0; g0 < G; g0 += kGenHeads) {
+      const int ng = min(kGenHeads, G - g0);
+      float q[kGenHeads][16], acc[kGenHeads][16], m[kGenHeads], l[kGenHeads];
+#pragma unroll
+      for (int h = 0; h < kGenHeads; ++h) {
+        m[h] = -INFINITY;
+        l[h] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) q[h][e] = acc[h][e] = 0.f;
+        if (h < ng && in_head) {
+          const T* row = static_cast<const T*>(a.q) + static_cast<size_t>(g.tok) * a.q_stride + (g.kvh * G + g0 + h) * kD;
+          load8(row + ch * 16, q[h]);
+          load8(row + ch * 16 + 8, q[h] + 8);
+          if (a.cos != nullptr) {           // the other half's entries come from the row, too
+            int pos = g.ctx - 1;
+            if (pos >= a.max_pos) {
+              atomicOr(a.status, 2);
+              pos = 0;
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int d = ch * 16 + e, dh = d < kD / 2 ? d : d - kD / 2;
+              const float other = to_float(row[d < kD / 2 ? d + kD / 2 : dh]);
+              const float c = a.cos[static_cast<size_t>(pos) * (kD / 2) + dh], s = a.sin[static_cast<size_t>(pos) * (kD / 2) + dh];
+              const float x = d < kD / 2 ? __fsub_rn(__fmul_rn(q[h][e], c), __fmul_rn(other, s))
+                                         : __fadd_rn(__fmul_rn(q[h][e], c), __fmul_rn(other, s));
+              q[h][e] = to_float(from_float<T>(x));      // (as the write leaves it for prompt steps)
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) q[h][e] *= a.scale * kLog2e;
+        }
+      }
+      // (the trip count is the same for all lanes of a warp: the shuffles below need all of them)
+      for (int k0 = g.key_lo + warp * KPW; k0 < g.key_hi; k0 += KPW * (kGenThreads / 32)) {
+        const int key = k0 + slot;
+        const bool live = key < g.key_hi;
+        const size_t block = static_cast<size_t>(bt[(live ? key : k0) >> a.page_shift]) * a.hkv + g.kvh;
+        const size_t at = (block * ps + (key & (ps - 1))) * kD + ch * 16;
+        float s[kGenHeads] = {};
+        uint4 vraw = make_uint4(0, 0, 0, 0);
+        if (live && in_head) {
+          const uint4 kraw = *reinterpret_cast<const uint4*>(a.kcache + at);
+          vraw = *reinterpret_cast<const uint4*>(a.vcache + at);
+          float k[16];
+          kv8_f16(kraw, k);
+#pragma unroll
+          for (int h = 0; h < kGenHeads; ++h)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[h] += q[h][e] * k[e];
+        }
+#pragma unroll
+        for (int h = 0; h < kGenHeads; ++h)
+#pragma unroll
+          for (int o = 1; o < kGenLanes; o <<= 1) s[h] += __shfl_xor_sync(0xffffffffu, s[h], o);
+        if (live) {
+          const float ks = kv8_scale(a.kscale[block]), vs = kv8_scale(a.vscale[block]);
+          float v[16];
+          kv8_f16(vraw, v);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) v[e] *= vs;
+#pragma unroll
+          for (int h = 0; h < kGenHeads; ++h) {
+            const float x = s[h] * ks;
+            if (x > m[h]) {
+              const float f = exp2f(m[h] - x);           // 0 the first time
+              l[h] *= f;
+#pragma unroll
+              for (int e = 0; e < 16; ++e) acc[h][e] *= f;
+              m[h] = x;
+            }
+            // (a score that is not a number makes the row not a number; one of -inf weighs nothing)
+            const float p = x == -INFINITY ? 0.f : exp2f(x - m[h]);
+            l[h] += p;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[h][e] += p * v[e];
+          }
+        }
+      }
+      // the warp's slots, then its partial result
+#pragma unroll
+      for (int h = 0; h < kGenHeads; ++h) {
+#pragma unroll
+        for (int o = kGenLanes; o < 32; o <<= 1) {
+          const float om = __shfl_xor_sync(0xffffffffu, m[h], o), ol = __shfl_xor_sync(0xffffffffu, l[h], o);
+          const float mn = fmaxf(m[h], om);
+          const float f = m[h] == -INFINITY ? 0.f : exp2f(m[h] - mn), w = om == -INFINITY ? 0.f : exp2f(om - mn);
+          l[h] = l[h] * f + ol * w;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float oa = __shfl_xor_sync(0xffffffffu, acc[h][e], o);
+            acc[h][e] = acc[h][e] * f + oa * w;
+          }
+          m[h] = mn;
+        }
+        if (slot == 0 && in_head) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) parts[warp][h][ch * 16 + e] = acc[h][e];
+          if (ch == 0) {
+            parts[warp][h][kD] = m[h];
+            parts[warp][h][kD + 1] = l[h];
+          }
+        }
+      }
+      __syncthreads();
+      for (int i = threadIdx.x; i < ng * kD; i += kGenThreads) {
+        const int h = i / kD, d = i - h * kD;
+        float mx = -INFINITY, den = 0.f, num = 0.f;
+#pragma unroll
+        for (int w = 0; w < kGenThreads / 32; ++w) mx = fmaxf(mx, parts[w][h][kD]);
+#pragma unroll
+        for (int w = 0; w < kGenThreads / 32; ++w) {
+          const float f = parts[w][h][kD] == -INFINITY ? 0.f : exp2f(parts[w][h][kD] - mx);
+          den += f * parts[w][h][kD + 1];
+          num += f * parts[w][h][d];
+        }
+        const int r = g0 + h;
+        if (g.whole) {
+          static_cast<T*>(a.out)[static_cast<size_t>(g.tok) * a.out_stride + (g.kvh * G + r) * kD + d] = from_float<T>(num / den);
+        } else {
+          piece[r * (kD + 2) + d] = num;
+          if (d == 0) {
+            piece[r * (kD + 2) + kD] = mx;
+            piece[r * (kD + 2) + kD + 1] = den;
+          }
+        }
+      }
+      __syncthreads();
+    }
+    if (!g.whole) {
+      __threadfence();                       // the piece, before it is counted
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        const int pieces = kv8_share_of(g.row_end - 1, units, shares) - kv8_share_of(g.row_begin, units, shares) + 1;
+        int* c = a.counters + static_cast<size_t>(g.item) * a.hkv + g.kvh;
+        last = atomicAdd(c, 1) == pieces - 1;
+        if (last) *c = 0;
+      }
+      __syncthreads();
+      if (last) {
+        __threadfence();
+        kv8_merge<T>(a, g, units, shares, threadIdx.x, kGenThreads);
+      }
+      __syncthreads();
+    }
+    u = g.next;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ portions of prompts
+
+template <typename T>
+struct Kv8PrefillArgs {
+  const T* q;
+  int q_stride;
+  const uint8_t* kcache;
+  const uint8_t* vcache;
+  const uint8_t* kscale;
+  const uint8_t* vscale;
+  const int32_t* block_table;
+  int max_blocks;
+  const int32_t* tile_seq;
+  const int32_t* tile_tok;
+  const int32_t* tile_rows;
+  const int32_t* positions;
+  T* out;
+  int out_stride;
+  int hq, hkv, page_shift, window;
+  float scale;
+};
+
+constexpr int kPR = 64, kPK = 64, kPreThreads = 256;      // query rows and keys of a tile
+constexpr int kPLd = 68;                                  // floats to a row of 64 in shared memory
+constexpr size_t kPreSmem = sizeof(float) * (2 * kD * kPLd + kPK * kD + kPK * kPLd);
+
+// Portions of prompts on the CUDA cores: a CTA to 64 consecutive query rows (half a tile of the launch) of one head;
+// keys in tiles of 64.  Thread (ty, tx) has rows 4 ty .. + 3; of S their keys 4 tx .. + 3 (operands as four rows and four
+// keys side by side: two 16-byte reads for 16 products), of O their columns tx + 16 j.
+template <typename T>
+__global__ void __launch_bounds__(kPreThreads)
+kv8_prefill_kernel(const Kv8PrefillArgs<T> a) {
+  extern __shared__ __align__(16) float smem[];
+  float* qs = smem;                         // [D][68], scaled
+  float* ks = qs + kD * kPLd;               // [D][68]
+  float* vs = ks + kD * kPLd;               // [64][D]
+  float* ps = vs + kPK * kD;                // [64 keys][68]
+  constexpr float kLog2e = 1.4426950408889634f;
+  constexpr int NC = kD / 16;
+  pdl_launch();
+  pdl_wait();
+  const int tile = blockIdx.x >> 1, head = blockIdx.y, kvh = head / (a.hq / a.hkv);
+  const int half = (blockIdx.x & 1) * kPR;
+  const int rows = min(a.tile_rows[tile] - half, kPR);
+  if (rows <= 0) return;
+  const int tok0 = a.tile_tok[tile] + half;
+  const int pos0 = a.positions[tok0], page = 1 << a.page_shift;
+  const int32_t* bt = a.block_table + static_cast<size_t>(a.tile_seq[tile]) * a.max_blocks;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  for (int i = threadIdx.x; i < kPR * (kD / 8); i += kPreThreads) {
+    const int r = i % kPR, c = i / kPR;
+    float x[8] = {};
+    if (r < rows) load8(a.q + static_cast<size_t>(tok0 + r) * a.q_stride + head * kD + c * 8, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) qs[(c * 8 + e) * kPLd + r] = x[e] * (a.scale * kLog2e);
+  }
+  const int k_end = pos0 + rows;
+  const int first = a.window > 0 && pos0 + 1 > a.window ? pos0 + 1 - a.window : 0;
+  float m[4], l[4], acc[4][NC];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < NC; ++j) acc[i][j] = 0.f;
+  }
+  for (int k0 = first / kPK * kPK; k0 < k_end; k0 += kPK) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < kPK * (kD / 16); i += kPreThreads) {
+      const int key = i % kPK, c = i / kPK, j = k0 + key;
+      float k[16] = {}, v[16] = {};
+      if (j < k_end && j >= first) {
+        const size_t block = static_cast<size_t>(bt[j >> a.page_shift]) * a.hkv + kvh;
+        const size_t at = (block * page + (j & (page - 1))) * kD + c * 16;
+        const float fk = kv8_scale(a.kscale[block]), fv = kv8_scale(a.vscale[block]);
+        kv8_f16(*reinterpret_cast<const uint4*>(a.kcache + at), k);
+        kv8_f16(*reinterpret_cast<const uint4*>(a.vcache + at), v);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          k[e] *= fk;
+          v[e] *= fv;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        ks[(c * 16 + e) * kPLd + key] = k[e];
+        vs[key * kD + c * 16 + e] = v[e];
+      }
+    }
+    __syncthreads();
+    float s[4][4] = {};
+#pragma unroll 4
+    for (int d = 0; d < kD; ++d) {
+      const float4 x = *reinterpret_cast<const float4*>(qs + d * kPLd + ty * 4);
+      const float4 y = *reinterpret_cast<const float4*>(ks + d * kPLd + tx * 4);
+      const float xr[4] = {x.x, x.y, x.z, x.w}, yr[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][j] += xr[i] * yr[j];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int pos = pos0 + ty * 4 + i;
+      const int lo = a.window > 0 && pos + 1 > a.window ? pos + 1 - a.window : 0;
+      float top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = k0 + tx * 4 + j;
+        if (key > pos || key < lo) s[i][j] = -INFINITY;
+        top = fmaxf(top, s[i][j]);
+      }
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float mn = fmaxf(m[i], top);
+      const float use = mn == -INFINITY ? 0.f : mn;       // (no key of the row yet)
+      const float f = m[i] == -INFINITY ? 0.f : exp2f(m[i] - use);
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[i][j] = exp2f(s[i][j] - use);
+        sum += s[i][j];
+      }
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      l[i] = l[i] * f + sum;
+      m[i] = mn;
+#pragma unroll
+      for (int j = 0; j < NC; ++j) acc[i][j] *= f;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      *reinterpret_cast<float4*>(ps + (tx * 4 + j) * kPLd + ty * 4) = make_float4(s[0][j], s[1][j], s[2][j], s[3][j]);
+    __syncwarp();                                          // (a row's sixteen threads are half a warp)
+#pragma unroll 4
+    for (int c = 0; c < kPK; ++c) {
+      const float4 p = *reinterpret_cast<const float4*>(ps + c * kPLd + ty * 4);
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+        const float v = vs[c * kD + tx + 16 * j];
+        acc[0][j] += p.x * v;
+        acc[1][j] += p.y * v;
+        acc[2][j] += p.z * v;
+        acc[3][j] += p.w * v;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = ty * 4 + i;
+    if (r >= rows) continue;
+    const float inv = 1.f / l[i];
+#pragma unroll
+    for (int j = 0; j < NC; ++j)
+      a.out[static_cast<size_t>(tok0 + r) * a.out_stride + head * kD + tx + 16 * j] = from_float<T>(acc[i][j] * inv);
+  }
+}
+
+}  // namespace rl
+
+using namespace rl;
+
+namespace {
+
+constexpr int kMaxDevices = 64;
+
+int device_sms(int* sms) {
+  static int sms_of[kMaxDevices];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (dev < 0 || dev >= kMaxDevices) return static_cast<int>(cudaErrorInvalidDevice);
+  if (sms_of[dev] == 0) {
+    int n = 0;
+    e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    sms_of[dev] = n > 0 ? n : 1;
+  }
+  *sms = sms_of[dev];
+  return 0;
+}
+
+int shift_of(int page_size) {
+  int s = 0;
+  while ((1 << s) < page_size) ++s;
+  return s;
+}
+
+template <typename T>
+int launch_write(const void* qkv, int qkv_stride, const int32_t* positions, const int32_t* slots, const int4* items,
+                 const int32_t* bt, int max_blocks, const float* cos, const float* sin, uint8_t* kc, uint8_t* vc, uint8_t* ks,
+                 uint8_t* vs, void* q_out, int q_stride, int tokens, int hq, int hkv, int page_size, int max_pos,
+                 long long num_slots, int* status, cudaStream_t stream) {
+  Kv8WriteArgs<T> a;
+  a.qkv = static_cast<const T*>(qkv);
+  a.qkv_stride = qkv_stride;
+  a.positions = positions;
+  a.slots = slots;
+  a.items = items;
+  a.block_table = bt;
+  a.max_blocks = max_blocks;
+  a.cos = cos;
+  a.sin = sin;
+  a.kcache = kc;
+  a.vcache = vc;
+  a.kscale = ks;
+  a.vscale = vs;
+  a.q_out = static_cast<T*>(q_out);
+  a.q_stride = q_stride;
+  a.tokens = tokens;
+  a.hq = hq;
+  a.hkv = hkv;
+  a.page_shift = shift_of(page_size);
+  a.max_pos = max_pos;
+  a.num_slots = num_slots;
+  a.status = status;
+  const int kv_blocks = slots != nullptr || items != nullptr ? tokens : 0;
+  const long long pairs = q_out != nullptr ? static_cast<long long>(tokens) * hq * (kD / 16) : 0;
+  const long long blocks = kv_blocks + (pairs + kWriteThreads - 1) / kWriteThreads;
+  if (blocks == 0) return 0;
+  if (blocks > 0x7fffffffLL) return static_cast<int>(cudaErrorInvalidValue);
+  launch_kernel(kv8_write_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(kWriteThreads), 0, stream, a, kv_blocks);
+  return static_cast<int>(cudaGetLastError());
+}
+
+// The largest number of shares that a launch is cut into: the workspace has two places for each.
+constexpr int kMaxShares = 148 * 12;
+
+}  // namespace
+
+extern "C" {
+
+// The floats of the workspace for groups of G heads (kv8.cuh: Kv8Args::part).
+long long rl_kv8_part_floats(int G) { return static_cast<long long>(kMaxShares) * 2 * G * (kD + 2); }
+
+int rl_kv8_write(int dtype, const void* qkv, int qkv_stride, const int32_t* positions, const int32_t* slots,
+                 const float* cos, const float* sin, void* kc, void* vc, void* ks, void* vs, void* q_out, int q_stride,
+                 int tokens, int hq, int hkv, int page_size, int max_pos, long long num_slots, int* status, void* stream) {
+  auto run = dtype == 0 ? launch_write<float> : launch_write<bf16>;
+  return run(qkv, qkv_stride, positions, slots, nullptr, nullptr, 0, cos, sin, static_cast<uint8_t*>(kc),
+             static_cast<uint8_t*>(vc), static_cast<uint8_t*>(ks), static_cast<uint8_t*>(vs), q_out, q_stride, tokens, hq, hkv,
+             page_size, max_pos, num_slots, status, static_cast<cudaStream_t>(stream));
+}
+
+// Single tokens.  store: q holds the unrotated rows [q | k | v]; the tokens' keys and values are stored first, in a
+// launch of their own, and the attention rotates q on its way in.
+int rl_kv8_attn_decode(int dtype, const void* q, int q_stride, void* kc, void* vc, void* ks, void* vs, const int32_t* bt,
+                       int max_blocks, const void* items, int nitems, float* part, int* counters, void* out, int out_stride,
+                       int hq, int hkv, int page_size, int window, float scale, const float* cos, const float* sin, int max_pos,
+                       int store, long long num_slots, int* status, long long max_units, void* stream_) {
+  if (max_units <= 0) return 0;
+  const cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  int sms = 0;
+  int e = device_sms(&sms);
+  if (e) return e;
+  if (store) {
+    auto run = dtype == 0 ? launch_write<float> : launch_write<bf16>;
+    e = run(q, q_stride, nullptr, nullptr, static_cast<const int4*>(items), bt, max_blocks, cos, sin, static_cast<uint8_t*>(kc),
+            static_cast<uint8_t*>(vc), static_cast<uint8_t*>(ks), static_cast<uint8_t*>(vs), nullptr, 0, nitems, hq, hkv, page_size,
+            max_pos, num_slots, status, stream);
+    if (e) return e;
+  }
+  Kv8Args a;
+  a.q = q;
+  a.q_stride = q_stride;
+  a.kcache = static_cast<const uint8_t*>(kc);
+  a.vcache = static_cast<const uint8_t*>(vc);
+  a.kscale = static_cast<const uint8_t*>(ks);
+  a.vscale = static_cast<const uint8_t*>(vs);
+  a.block_table = bt;
+  a.max_blocks = max_blocks;
+  a.items = static_cast<const int4*>(items);
+  a.nitems = nitems;
+  a.part = part;
+  a.counters = counters;
+  a.out = out;
+  a.out_stride = out_stride;
+  a.hq = hq;
+  a.hkv = hkv;
+  a.page_shift = shift_of(page_size);
+  a.window = window;
+  a.scale = scale;
+  a.cos = store ? cos : nullptr;
+  a.sin = sin;
+  a.max_pos = max_pos;
+  a.status = status;
+  for (int i0 = 0; i0 < nitems; i0 += kMaxItems) {         // (one launch unless there are very many items)
+    a.items = static_cast<const int4*>(items) + i0;
+    a.nitems = nitems - i0 < kMaxItems ? nitems - i0 : kMaxItems;
+    // a CTA to a unit, as far as they are resident together
+    const int most = sms * 2 < kMaxShares ? sms * 2 : kMaxShares;
+    const int ctas = static_cast<int>(max_units < most ? max_units : most);
+    if (dtype == 0)
+      launch_kernel(kv8_decode_kernel<float>, dim3(ctas), dim3(kGenThreads), 0, stream, a);
+    else
+      launch_kernel(kv8_decode_kernel<bf16>, dim3(ctas), dim3(kGenThreads), 0, stream, a);
+    e = static_cast<int>(cudaGetLastError());
+    if (e) return e;
+  }
+  return 0;
+}
+
+}  // extern "C"
+
+namespace {
+
+template <typename T>
+int launch_prefill(const void* q, int q_stride, const void* kc, const void* vc, const void* ks, const void* vs, const int32_t* bt,
+                   int max_blocks, const int32_t* tile_seq, const int32_t* tile_tok, const int32_t* tile_rows,
+                   const int32_t* positions, void* out, int out_stride, int tiles, int hq, int hkv, int page_size, int window,
+                   float scale, cudaStream_t stream) {
+  Kv8PrefillArgs<T> a;
+  a.q = static_cast<const T*>(q);
+  a.q_stride = q_stride;
+  a.kcache = static_cast<const uint8_t*>(kc);
+  a.vcache = static_cast<const uint8_t*>(vc);
+  a.kscale = static_cast<const uint8_t*>(ks);
+  a.vscale = static_cast<const uint8_t*>(vs);
+  a.block_table = bt;
+  a.max_blocks = max_blocks;
+  a.tile_seq = tile_seq;
+  a.tile_tok = tile_tok;
+  a.tile_rows = tile_rows;
+  a.positions = positions;
+  a.out = static_cast<T*>(out);
+  a.out_stride = out_stride;
+  a.hq = hq;
+  a.hkv = hkv;
+  a.page_shift = shift_of(page_size);
+  a.window = window;
+  a.scale = scale;
+  static bool attr_set[kMaxDevices];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (dev < 0 || dev >= kMaxDevices) return static_cast<int>(cudaErrorInvalidDevice);
+  if (!attr_set[dev]) {
+    e = cudaFuncSetAttribute(kv8_prefill_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kPreSmem));
+    if (e != cudaSuccess) return static_cast<int>(e);
+    attr_set[dev] = true;
+  }
+  launch_kernel(kv8_prefill_kernel<T>, dim3(tiles * 2, hq), dim3(kPreThreads), kPreSmem, stream, a);
+  return static_cast<int>(cudaGetLastError());
+}
+
+}  // namespace
+
+extern "C" int rl_kv8_attn_prefill(int dtype, const void* q, int q_stride, const void* kc, const void* vc, const void* ks,
+                                   const void* vs, const int32_t* bt, int max_blocks, const int32_t* tile_seq,
+                                   const int32_t* tile_tok, const int32_t* tile_rows, const int32_t* positions, void* out,
+                                   int out_stride, int tiles, int hq, int hkv, int page_size, int window, float scale,
+                                   void* stream) {
+  auto run = dtype == 0 ? launch_prefill<float> : launch_prefill<bf16>;
+  return run(q, q_stride, kc, vc, ks, vs, bt, max_blocks, tile_seq, tile_tok, tile_rows, positions, out, out_stride, tiles, hq,
+             hkv, page_size, window, scale, static_cast<cudaStream_t>(stream));
+}

@@ -91,6 +91,22 @@ def _need_cuda(*ts: Optional[torch.Tensor]) -> None:
             raise KernelError("redline_b200 kernels run on CUDA tensors only; there is no CPU fallback")
 
 
+class _Here:
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *_):
+        pass
+
+
+_here = _Here()
+
+
+def _on(t: torch.Tensor):
+    """A guard under which the current device is ``t``'s (nothing to do where it is already, which is nearly always)."""
+    return _here if t.device.index == _device_index() else torch.cuda.device(t.device)
+
+
 # ------------------------------------------------------------------ elementwise
 
 def _ew() -> ctypes.CDLL:
@@ -643,6 +659,230 @@ def attn_prefill(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, vcache: t
              block_table.shape[1], _ptr(tile_seq), _ptr(tile_tok), _ptr(tile_rows), _ptr(positions),
              _ptr(out), out.stride(0), tiles, num_heads, num_kv_heads, page_size, window, float(scale), impl,
              _ptr(tc_status(q.device)), _stream()), "attn_prefill")
+
+
+# ------------------------------------------- the cache in 8 bits (csrc/kv8.cu)
+
+KV8_DTYPE, KV8_SCALE_DTYPE = torch.float8_e4m3fn, torch.float8_e8m0fnu
+KV8_PAGE_SIZES = (16, 32, 64)
+KV8_UNIT = 64                     # keys of a unit of work (kUnit)
+
+
+def _kv8(head_dim: int) -> ctypes.CDLL:
+    if head_dim % 16 != 0 or head_dim < 16 or head_dim > MAX_HEAD_DIM:
+        raise KernelError(f"attention kernels take head sizes that are multiples of 16 up to "
+                          f"{MAX_HEAD_DIM}; got {head_dim}")
+    return _lib(f"kv8_d{head_dim}", "kv8.cu", {"RL_HEAD_DIM": head_dim})
+
+
+def _kv8_check(what: str, kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch.Tensor, vscale: torch.Tensor, num_heads: int,
+               num_kv_heads: int, head_dim: int, page_size: int) -> None:
+    """The cache's tensors have the types and shapes that the kernels take."""
+    shape = kcache.shape
+    if (kcache.dtype is not KV8_DTYPE or vcache.dtype is not KV8_DTYPE or kscale.dtype is not KV8_SCALE_DTYPE
+            or vscale.dtype is not KV8_SCALE_DTYPE):
+        raise KernelError(f"{what}: the cache is float8_e4m3fn and its scales float8_e8m0fnu; got {kcache.dtype}, "
+                          f"{vcache.dtype}, {kscale.dtype}, {vscale.dtype}")
+    if page_size not in KV8_PAGE_SIZES:
+        raise KernelError(f"{what}: pages of 16, 32 or 64 tokens; got {page_size}")
+    if num_kv_heads <= 0 or num_heads <= 0 or num_heads % num_kv_heads:
+        raise KernelError(f"{what}: {num_heads} query heads are no multiple of {num_kv_heads} kv heads")
+    if (len(shape) != 4 or shape[1] != num_kv_heads or shape[2] != page_size or shape[3] != head_dim
+            or vcache.shape != shape or kscale.shape != shape[:2] or vscale.shape != shape[:2]):
+        raise KernelError(f"{what}: caches [pages, {num_kv_heads}, {page_size}, {head_dim}] and scales [pages, {num_kv_heads}]; "
+                          f"got {tuple(shape)}, {tuple(vcache.shape)}, {tuple(kscale.shape)}, {tuple(vscale.shape)}")
+    if not (kcache.is_contiguous() and vcache.is_contiguous() and kscale.is_contiguous() and vscale.is_contiguous()):
+        raise KernelError(f"{what}: the cache and its scales must be contiguous")
+    if (kcache.data_ptr() | vcache.data_ptr()) % 16:
+        raise KernelError(f"{what}: the cache must start on a 16-byte boundary")
+    if not kcache.is_cuda or not (kcache.device == vcache.device == kscale.device == vscale.device):
+        raise KernelError("redline_b200 kernels run on CUDA tensors only; there is no CPU fallback")
+
+
+def _kv8_rows(what: str, name: str, x: torch.Tensor, stride: int, columns: int, cache: torch.Tensor) -> None:
+    """``x``: rows of at least ``columns`` elements, ``stride`` apart, in 16-byte pieces, on the cache's device."""
+    piece = 8 if x.dtype is torch.bfloat16 else 4
+    if x.device != cache.device:
+        raise KernelError(f"{what}: {name} is on {x.device}, the cache on {cache.device}")
+    if x.dim() != 2 or x.stride(1) != 1 or x.stride(0) != stride or x.shape[1] < columns or (x.shape[0] > 1 and stride < columns):
+        raise KernelError(f"{what}: {name} must be rows of {columns} contiguous elements, {stride} apart; got "
+                          f"{tuple(x.shape)} with strides {x.stride()}")
+    if stride % piece or x.data_ptr() % 16:
+        raise KernelError(f"{what}: the rows of {name} must start on 16-byte boundaries")
+
+
+def _kv8_ints(what: str, cache: torch.Tensor, **tensors: torch.Tensor) -> None:
+    for name, t in tensors.items():
+        if t.dtype is not torch.int32 or t.device != cache.device or not t.is_contiguous():
+            raise KernelError(f"{what}: {name} must be a contiguous int32 tensor on {cache.device}; got {t.dtype} on {t.device}")
+
+
+def _kv8_tables(what: str, cos: torch.Tensor, sin: torch.Tensor, head_dim: int, cache: torch.Tensor) -> None:
+    if (cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or cos.dim() != 2 or cos.shape[1] != head_dim // 2
+            or sin.shape != cos.shape or not cos.is_contiguous() or not sin.is_contiguous() or cos.device != cache.device
+            or sin.device != cache.device or (cos.data_ptr() | sin.data_ptr()) % 16):
+        raise KernelError(f"{what}: cos / sin must be contiguous float32 [positions, {head_dim // 2}] on the cache's device")
+
+
+def kv8_write(qkv: torch.Tensor, positions: torch.Tensor, slots: Optional[torch.Tensor], cos: Optional[torch.Tensor],
+              sin: Optional[torch.Tensor], kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch.Tensor,
+              vscale: torch.Tensor, q_out: Optional[torch.Tensor], num_heads: int, num_kv_heads: int, head_dim: int,
+              page_size: int, status: torch.Tensor, tokens: Optional[int] = None) -> None:
+    """``rope_kv_write`` for a cache in 8 bits: the rows of qkv [T, (Hq + 2 Hkv) D] are read, q is rotated into ``q_out`` (rows of
+    Hq D; it may be qkv itself; None: q is left alone), k is rotated, and k and v are stored at each token's slot (``slots`` None or
+    negative: not stored; beyond the pool: not stored, bit 4 of ``status``).  cos / sin None: nothing is rotated.
+
+    The cache is float8_e4m3fn [pages, Hkv, page_size, D] with float8_e8m0fnu scales [pages, Hkv]: a page of a head stands for
+    its bytes times its scale, the smallest power of two with which its largest magnitude fits (at least 2^-126, at most 2^119,
+    beyond which numbers saturate).  Pages are filled in order: the first place of a page sets the scale anew; a later token
+    may raise it, and what lies in the places before it is rescaled.  What is not finite is stored as not a number and
+    left out of the scale.  The tokens of a page follow one another in a call: of several runs in one page the first is
+    stored, and the others set bit 8 of ``status`` (not in page 0, which belongs to the padding rows)."""
+    what = "kv8_write"
+    T = tokens if tokens is not None else qkv.shape[0]
+    _kv8_check(what, kcache, vcache, kscale, vscale, num_heads, num_kv_heads, head_dim, page_size)
+    _kv8_rows(what, "qkv", qkv, qkv.stride(0), (num_heads + 2 * num_kv_heads) * head_dim, kcache)
+    _kv8_ints(what, kcache, positions=positions, status=status)
+    if not 0 <= T <= qkv.shape[0] or positions.numel() < T:
+        raise KernelError(f"{what}: {T} tokens of {qkv.shape[0]} rows and {positions.numel()} positions")
+    if slots is not None:
+        _kv8_ints(what, kcache, slots=slots)
+        if slots.numel() < T:
+            raise KernelError(f"{what}: {slots.numel()} slots for {T} tokens")
+    if (cos is None) != (sin is None):
+        raise KernelError(f"{what}: cos and sin come together")
+    if cos is not None:
+        _kv8_tables(what, cos, sin, head_dim, kcache)
+    if q_out is not None:
+        _kv8_rows(what, "q_out", q_out, q_out.stride(0), num_heads * head_dim, kcache)
+        if q_out.dtype is not qkv.dtype or q_out.shape[0] < T:
+            raise KernelError(f"{what}: q_out must be {qkv.dtype} with {T} rows")
+    f = _fn(_kv8(head_dim), "rl_kv8_write",
+            [c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+             c_int, c_int, c_int, c_int, c_int, c_int, c_longlong, c_void_p, c_void_p])
+    with _on(kcache):
+        _check(f(_code(qkv.dtype), qkv.data_ptr(), qkv.stride(0), positions.data_ptr(), _ptr(slots), _ptr(cos), _ptr(sin),
+                 kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(), vscale.data_ptr(), _ptr(q_out),
+                 0 if q_out is None else q_out.stride(0), T, num_heads, num_kv_heads, page_size,
+                 cos.shape[0] if cos is not None else 2 ** 31 - 1, kcache.shape[0] * page_size, status.data_ptr(), _stream()),
+               what)
+
+
+def kv8_decode_workspace(nitems: int, num_heads: int, num_kv_heads: int, head_dim: int,
+                         device: torch.device) -> Tuple[torch.Tensor, torch.Tensor]:
+    """What ``kv8_attn_decode`` and ``kv8_attn_decode_rope`` need beside their arguments for up to ``nitems`` items: room for
+    the pieces of rows that are shared out, and counters, which launches leave zero.  One stream uses a workspace at a time
+    (two graphs that may run side by side need one each)."""
+    f = _kv8(head_dim).rl_kv8_part_floats
+    f.restype, f.argtypes = c_longlong, [c_int]
+    return (torch.empty(f(num_heads // num_kv_heads), dtype=torch.float32, device=device),
+            torch.zeros(max(nitems, 1) * num_kv_heads, dtype=torch.int32, device=device))
+
+
+def _kv8_decode(what: str, q, q_stride, kcache, vcache, kscale, vscale, block_table, items, workspace, out, nitems, num_heads,
+                num_kv_heads, head_dim, page_size, window, scale, cos, sin, status, max_ctx, sum_ctx) -> None:
+    store = cos is not None
+    _kv8_check(what, kcache, vcache, kscale, vscale, num_heads, num_kv_heads, head_dim, page_size)
+    _kv8_rows(what, "qkv" if store else "q", q, q_stride, (num_heads + (2 * num_kv_heads if store else 0)) * head_dim, kcache)
+    _kv8_rows(what, "out", out, out.stride(0), num_heads * head_dim, kcache)
+    part, counters = workspace
+    _kv8_ints(what, kcache, block_table=block_table, items=items, counters=counters)
+    if out.dtype is not q.dtype:
+        raise KernelError(f"{what}: out must be {q.dtype}")
+    if nitems < 0 or items.numel() < 4 * nitems or items.data_ptr() % 16:
+        raise KernelError(f"{what}: items must be int32 [{nitems}, 4] on a 16-byte boundary")
+    if block_table.dim() != 2:
+        raise KernelError(f"{what}: block_table must be [sequences, blocks]")
+    if window < 0:
+        raise KernelError(f"{what}: a window of {window} keys")
+    lib = _kv8(head_dim)
+    need = _kv8_part.get((head_dim, num_heads // num_kv_heads))
+    if need is None:
+        g = lib.rl_kv8_part_floats
+        g.restype, g.argtypes = c_longlong, [c_int]
+        need = _kv8_part[(head_dim, num_heads // num_kv_heads)] = g(num_heads // num_kv_heads)
+    if part.numel() < need or part.dtype is not torch.float32 or part.device != kcache.device or counters.numel() < nitems * num_kv_heads:
+        raise KernelError(f"{what}: the workspace is too small (kv8_decode_workspace)")
+    if store:
+        _kv8_tables(what, cos, sin, head_dim, kcache)
+        _kv8_ints(what, kcache, status=status)
+    capacity = block_table.shape[1] * page_size
+    max_ctx = min(max_ctx, capacity) if max_ctx > 0 else capacity
+    seen = min(max_ctx, window) if window > 0 else max_ctx
+    f = _fn(lib, "rl_kv8_attn_decode",
+            [c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p,
+             c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_int, c_int, c_longlong, c_void_p,
+             c_longlong, c_void_p])
+    with _on(kcache):
+        _check(f(_code(q.dtype), q.data_ptr(), q_stride, kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(),
+                 vscale.data_ptr(), block_table.data_ptr(), block_table.shape[1], items.data_ptr(), nitems, part.data_ptr(),
+                 counters.data_ptr(), out.data_ptr(), out.stride(0), num_heads, num_kv_heads, page_size, window, float(scale),
+                 _ptr(cos), _ptr(sin), cos.shape[0] if store else 0, 1 if store else 0, kcache.shape[0] * page_size,
+                 status.data_ptr() if store else None, nitems * num_kv_heads * (seen // KV8_UNIT + 2), _stream()),
+               what, 2 if store else 1)
+
+
+def kv8_attn_decode(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch.Tensor,
+                    vscale: torch.Tensor, block_table: torch.Tensor, items: torch.Tensor,
+                    workspace: Tuple[torch.Tensor, torch.Tensor], out: torch.Tensor, nitems: int, num_heads: int,
+                    num_kv_heads: int, head_dim: int, page_size: int, window: int, scale: float, max_ctx: int = 0,
+                    sum_ctx: int = 0) -> None:
+    """``attn_decode`` over a cache in 8 bits (kv8_write): one query token per item.
+
+    items      int32 [nitems, 4]: (token index of the query, sequence index, context length, 0); an item of context 0 has
+               no keys, and its row of ``out`` is left as it was
+    workspace  of kv8_decode_workspace
+    max_ctx, sum_ctx  the longest context and their sum, as far as the host knows them (0: unknown); the work is shared out by
+               the items' own contexts, these choose between ways to do so
+    """
+    _kv8_decode("kv8_attn_decode", q, q_stride, kcache, vcache, kscale, vscale, block_table, items, workspace, out, nitems,
+                num_heads, num_kv_heads, head_dim, page_size, window, scale, None, None, None, max_ctx, sum_ctx)
+
+
+def kv8_attn_decode_rope(qkv: torch.Tensor, q_stride: int, kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch.Tensor,
+                         vscale: torch.Tensor, block_table: torch.Tensor, items: torch.Tensor,
+                         workspace: Tuple[torch.Tensor, torch.Tensor], out: torch.Tensor, nitems: int, num_heads: int,
+                         num_kv_heads: int, head_dim: int, page_size: int, window: int, scale: float, cos: torch.Tensor,
+                         sin: torch.Tensor, status: torch.Tensor, max_ctx: int = 0, sum_ctx: int = 0) -> None:
+    """``kv8_attn_decode`` from the UNROTATED rows [q | k | v] of the query tokens: a token's position is its context length - 1;
+    its rotated k and its v are stored there first (as kv8_write does), and q is rotated on its way into the attention."""
+    _kv8_decode("kv8_attn_decode_rope", qkv, q_stride, kcache, vcache, kscale, vscale, block_table, items, workspace, out, nitems,
+                num_heads, num_kv_heads, head_dim, page_size, window, scale, cos, sin, status, max_ctx, sum_ctx)
+
+
+_kv8_part: Dict[Tuple[int, int], int] = {}
+
+
+def kv8_attn_prefill(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch.Tensor,
+                     vscale: torch.Tensor, block_table: torch.Tensor, tile_seq: torch.Tensor, tile_tok: torch.Tensor,
+                     tile_rows: torch.Tensor, positions: torch.Tensor, out: torch.Tensor, tiles: int, num_heads: int,
+                     num_kv_heads: int, head_dim: int, page_size: int, window: int, scale: float) -> None:
+    """``attn_prefill`` over a cache in 8 bits (kv8_write): tiles of up to 128 consecutive query tokens of one sequence
+    (tile_seq, tile_tok, tile_rows); rows of ``out`` that no tile names are left as they were."""
+    what = "kv8_attn_prefill"
+    _kv8_check(what, kcache, vcache, kscale, vscale, num_heads, num_kv_heads, head_dim, page_size)
+    _kv8_rows(what, "q", q, q_stride, num_heads * head_dim, kcache)
+    _kv8_rows(what, "out", out, out.stride(0), num_heads * head_dim, kcache)
+    _kv8_ints(what, kcache, block_table=block_table, tile_seq=tile_seq, tile_tok=tile_tok, tile_rows=tile_rows,
+              positions=positions)
+    if out.dtype is not q.dtype:
+        raise KernelError(f"{what}: out must be {q.dtype}")
+    if tiles < 0 or min(tile_seq.numel(), tile_tok.numel(), tile_rows.numel()) < tiles:
+        raise KernelError(f"{what}: lists of {tile_seq.numel()}, {tile_tok.numel()} and {tile_rows.numel()} for {tiles} tiles")
+    if block_table.dim() != 2:
+        raise KernelError(f"{what}: block_table must be [sequences, blocks]")
+    if window < 0:
+        raise KernelError(f"{what}: a window of {window} keys")
+    if tiles == 0:
+        return
+    f = _fn(_kv8(head_dim), "rl_kv8_attn_prefill",
+            [c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+             c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p])
+    with _on(kcache):
+        _check(f(_code(q.dtype), q.data_ptr(), q_stride, kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(), vscale.data_ptr(),
+                 block_table.data_ptr(), block_table.shape[1], tile_seq.data_ptr(), tile_tok.data_ptr(), tile_rows.data_ptr(),
+                 positions.data_ptr(), out.data_ptr(), out.stride(0), tiles, num_heads, num_kv_heads, page_size, window,
+                 float(scale), _stream()), what)
 
 
 # ------------------------------------------- row-wise kernels of blocks with norms on both sides
@@ -1657,8 +1897,8 @@ def gather_logprob(logits: torch.Tensor, rows: int, target: torch.Tensor, out: t
 
 
 def build_all(head_dims=(64, 128), maps_dims=((64, 128, 2), (128, 128, 1)), linear_dims=(64,), memory_dims=(64,),
-              delta_dims=(128,), state_dims=(), verbose: bool = True) -> None:
-    """Compiles every kernel family (attention for the given head sizes, attention with score maps for the
+              delta_dims=(128,), state_dims=(), kv8_dims=(64, 128), verbose: bool = True) -> None:
+    """Compiles every kernel family (attention for the given head sizes, the 8-bit cache likewise, attention with score maps for the
     given (key size, value size, maps), linear attention, the matrix memory, the delta rule and the state-space
     recurrence for the given key sizes) and
     removes built files of these modules that belong to other versions of the sources."""
@@ -1667,6 +1907,7 @@ def build_all(head_dims=(64, 128), maps_dims=((64, 128, 2), (128, 128, 1)), line
     jobs.append(("prompt_layers", "prompt_layers.cpp", None))      # host-only: the launches of a prompt step
     jobs.append(("host_core", "host_core.cpp", None))              # host-only: cache manager, batch filler
     jobs += [(f"attention_d{d}", "attention.cu", {"RL_HEAD_DIM": d}) for d in head_dims]
+    jobs += [(f"kv8_d{d}", "kv8.cu", {"RL_HEAD_DIM": d}) for d in kv8_dims]
     for d, v, m, *stride in maps_dims:         # (key size, value size, maps[, length of a value row if longer])
         name, defines = f"attention_maps_d{d}_v{v}_m{m}", {"RL_QK_DIM": d, "RL_V_DIM": v, "RL_MAPS": m}
         if stride and stride[0] not in (0, v):

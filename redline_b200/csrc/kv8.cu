@@ -3,6 +3,8 @@
 //   kv8_write_kernel     rotates q and k, stores k and v with a scale for every page and kv head
 //   kv8_decode_kernel    single tokens on the CUDA cores: any head size in steps of 16 up to 256, float32 or bfloat16
 //   kv8_prefill_kernel   portions of prompts on the CUDA cores, for the same types and sizes
+#include <mutex>
+
 #include "kv8.cuh"
 
 #ifndef RL_HEAD_DIM
@@ -312,22 +314,28 @@ template <typename T>
 __device__ __forceinline__ void kv8_merge(const Kv8Args& a, const Kv8Segment& g, int units, int shares, int tid, int nthreads) {
   const int G = a.hq / a.hkv;
   const int s0 = kv8_share_of(g.row_begin, units, shares), s1 = kv8_share_of(g.row_end - 1, units, shares);
-  const int row = G * (kD + 2);
+  const int row = G * (kD + 3);
+  // (the first piece ends its share unless it begins it: its place is 0 then, as everybody else's)
+  const int first = kv8_share_begin(s0, units, shares) != g.row_begin ? 1 : 0;
   for (int i = tid; i < G * kD; i += nthreads) {
     const int r = i / kD, d = i - r * kD;
-    float m = -INFINITY, den = 0.f, num = 0.f;
-    for (int s = s0; s <= s1; ++s) {
-      // (the first piece ends its share unless it begins it: its place is 0 then, as everybody else's)
-      const int place = s == s0 && kv8_share_begin(s, units, shares) != g.row_begin ? 1 : 0;
-      const float* p = a.part + (static_cast<size_t>(s) * 2 + place) * row + r * (kD + 2);
-      const float pm = __ldcg(p + kD), pl = __ldcg(p + kD + 1), pn = __ldcg(p + d);
-      const float mn = fmaxf(m, pm);
-      const float f = m == -INFINITY ? 0.f : exp2f(m - mn), w = pm == -INFINITY ? 0.f : exp2f(pm - mn);
-      den = den * f + pl * w;
-      num = num * f + pn * w;
-      m = mn;
+    const float* base = a.part + r * (kD + 3);
+    Kv8Piece sum;
+    for (int s = s0; s <= s1; s += 8) {        // eight pieces' loads in flight together
+      float pd[8], m[8], den[8], num[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float* p = base + (static_cast<size_t>(min(s + k, s1)) * 2 + (s + k == s0 ? first : 0)) * row;
+        pd[k] = __ldcg(p + kD);
+        m[k] = __ldcg(p + kD + 1);
+        den[k] = __ldcg(p + kD + 2);
+        num[k] = __ldcg(p + d);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (s + k <= s1) sum.add(pd[k], m[k], den[k], num[k]);
     }
-    static_cast<T*>(a.out)[static_cast<size_t>(g.tok) * a.out_stride + (g.kvh * G + r) * kD + d] = from_float<T>(num / den);
+    static_cast<T*>(a.out)[static_cast<size_t>(g.tok) * a.out_stride + (g.kvh * G + r) * kD + d] = from_float<T>(sum.value());
   }
 }
 
@@ -359,7 +367,7 @@ kv8_decode_kernel(const Kv8Args a) {
   for (int u = begin; u < end;) {
     const Kv8Segment g = kv8_segment(a, start, u, end);
     const int32_t* bt = a.block_table + static_cast<size_t>(g.seq) * a.max_blocks;
-    float* piece = a.part + (static_cast<size_t>(blockIdx.x) * 2 + (u == begin ? 0 : 1)) * (G * (kD + 2));
+    float* piece = a.part + (static_cast<size_t>(blockIdx.x) * 2 + (u == begin ? 0 : 1)) * (G * (kD + 3));
     for (int g0 = 0; g0 < G; g0 += kGenHeads) {
       const int ng = min(kGenHeads, G - g0);
       float q[kGenHeads][16], acc[kGenHeads][16], m[kGenHeads], l[kGenHeads];
@@ -384,9 +392,7 @@ kv8_decode_kernel(const Kv8Args a) {
               const int d = ch * 16 + e, dh = d < kD / 2 ? d : d - kD / 2;
               const float other = to_float(row[d < kD / 2 ? d + kD / 2 : dh]);
               const float c = a.cos[static_cast<size_t>(pos) * (kD / 2) + dh], s = a.sin[static_cast<size_t>(pos) * (kD / 2) + dh];
-              const float x = d < kD / 2 ? __fsub_rn(__fmul_rn(q[h][e], c), __fmul_rn(other, s))
-                                         : __fadd_rn(__fmul_rn(q[h][e], c), __fmul_rn(other, s));
-              q[h][e] = to_float(from_float<T>(x));      // (as the write leaves it for prompt steps)
+              q[h][e] = d < kD / 2 ? q[h][e] * c - other * s : q[h][e] * c + other * s;
             }
           }
 #pragma unroll
@@ -480,11 +486,12 @@ kv8_decode_kernel(const Kv8Args a) {
         if (g.whole) {
           static_cast<T*>(a.out)[static_cast<size_t>(g.tok) * a.out_stride + (g.kvh * G + r) * kD + d] = from_float<T>(num / den);
         } else {
-          piece[r * (kD + 2) + d] = num;
-          if (d == 0) {
-            piece[r * (kD + 2) + kD] = mx;
-            piece[r * (kD + 2) + kD + 1] = den;
-          }
+          Kv8Piece x;
+          x.m = mx;
+          x.d = 0.f;
+          x.den = den;
+          x.num = num;
+          kv8_leave(piece + r * (kD + 3), kD, d, x);
         }
       }
       __syncthreads();
@@ -508,6 +515,15 @@ kv8_decode_kernel(const Kv8Args a) {
     u = g.next;
   }
 }
+
+}  // namespace rl
+
+#if RL_HEAD_DIM == 64 || RL_HEAD_DIM == 128
+#include "kv8_decode_tc.cuh"
+#define RL_KV8_TC 1
+#endif
+
+namespace rl {
 
 // ------------------------------------------------------------------------------------------------ portions of prompts
 
@@ -541,8 +557,8 @@ constexpr size_t kPreSmem = sizeof(float) * (2 * kD * kPLd + kPK * kD + kPK * kP
 template <typename T>
 __global__ void __launch_bounds__(kPreThreads)
 kv8_prefill_kernel(const Kv8PrefillArgs<T> a) {
-  extern __shared__ __align__(16) float smem[];
-  float* qs = smem;                         // [D][68], scaled
+  extern __shared__ __align__(16) float tiles[];
+  float* qs = tiles;                        // [D][68], scaled
   float* ks = qs + kD * kPLd;               // [D][68]
   float* vs = ks + kD * kPLd;               // [64][D]
   float* ps = vs + kPK * kD;                // [64 keys][68]
@@ -735,14 +751,126 @@ int launch_write(const void* qkv, int qkv_stride, const int32_t* positions, cons
 }
 
 // The largest number of shares that a launch is cut into: the workspace has two places for each.
-constexpr int kMaxShares = 148 * 12;
+constexpr int kMaxShares = 1776;
+
+#ifdef RL_KV8_TC
+
+typedef void (*TcKernel)(Kv8Args, int, int);
+const TcKernel kTcKernels[2] = {kv8_decode_tc_kernel<false>, kv8_decode_tc_kernel<true>};      // (true: groups of more than 8 heads)
+
+struct TcDevice {
+  bool ready;
+  int sms;
+  int resident[kMaxCluster + 1];     // clusters of so many CTAs that fit the device at once (one row's slots of 16 heads)
+  int smem_most;
+};
+
+size_t tc_smem(int csize, int G) {
+  return static_cast<size_t>(kTcWarps) * (kRingBytes + kHeadBytes) + (csize > 1 ? sizeof(float) * csize * G * (kD + 3) : 0);
+}
+
+// What is asked of the device once.
+int tc_device(const TcDevice** out) {
+  static TcDevice devices[kMaxDevices];
+  static std::mutex lock;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (dev < 0 || dev >= kMaxDevices) return static_cast<int>(cudaErrorInvalidDevice);
+  std::lock_guard<std::mutex> guard(lock);
+  TcDevice& d = devices[dev];
+  if (!d.ready) {
+    int n = 0, most = 0;
+    e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev);
+    cudaFuncAttributes fa;
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&fa, kTcKernels[0]);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    d.sms = n > 0 ? n : 1;
+    d.smem_most = most - static_cast<int>(fa.sharedSizeBytes);
+    for (TcKernel k : kTcKernels) {
+      e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, d.smem_most);
+      if (e != cudaSuccess) return static_cast<int>(e);
+    }
+    for (int c = 1; c <= kMaxCluster; ++c) {
+      cudaLaunchConfig_t q = {};
+      q.gridDim = dim3(c);
+      q.blockDim = dim3(kTcThreads);
+      q.dynamicSmemBytes = tc_smem(c, 1);
+      cudaLaunchAttribute at[1];
+      at[0].id = cudaLaunchAttributeClusterDimension;
+      at[0].val.clusterDim.x = c;
+      at[0].val.clusterDim.y = 1;
+      at[0].val.clusterDim.z = 1;
+      q.attrs = at;
+      q.numAttrs = 1;
+      int k = 0;
+      if (cudaOccupancyMaxActiveClusters(&k, kTcKernels[0], &q) != cudaSuccess) {
+        cudaGetLastError();
+        k = 0;
+      }
+      d.resident[c] = k;
+    }
+    d.ready = true;
+  }
+  *out = &d;
+  return 0;
+}
+
+// impl 2: by rows; 3: by shares; 0: the one that is expected to be faster.
+int launch_decode_tc(Kv8Args a, int max_ctx, long long sum_ctx, int impl, cudaStream_t stream) {
+  const TcDevice* d = nullptr;
+  const int err = tc_device(&d);
+  if (err) return err;
+  const int G = a.hq / a.hkv;
+  const long long rows = static_cast<long long>(a.nitems) * a.hkv;
+  int csize = 1;
+  for (int c = kMaxCluster; c > 1; --c)
+    if (d->resident[c] >= rows && tc_smem(c, G) <= static_cast<size_t>(d->smem_most)) {
+      csize = c;
+      break;
+    }
+  const int resident = d->resident[1] > 0 ? d->resident[1] : d->sms;
+  // as few groups (a divisor of the warps) as give every row one at once, else a warp to a row
+  int groups = 1;
+  if (rows > resident) {
+    groups = kTcWarps;
+    for (int k = 2; k < kTcWarps; ++k)
+      if (kTcWarps % k == 0 && static_cast<long long>(resident) * k >= rows) {
+        groups = k;
+        break;
+      }
+  }
+  const bool by_shares = impl == 3;
+  if (by_shares) csize = 1;
+  const long long wanted = by_shares ? resident : (csize > 1 ? rows : (rows + groups - 1) / groups);
+  const int clusters = static_cast<int>(wanted < resident || csize > 1 ? wanted : resident);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(clusters * csize);
+  cfg.blockDim = dim3(kTcThreads);
+  cfg.dynamicSmemBytes = tc_smem(csize, G);
+  cfg.stream = stream;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = csize;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  const int shares_flag = by_shares ? 1 : 0;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, kTcKernels[G > 8 ? 1 : 0], a, groups, shares_flag));
+}
+
+#endif
 
 }  // namespace
 
 extern "C" {
 
 // The floats of the workspace for groups of G heads (kv8.cuh: Kv8Args::part).
-long long rl_kv8_part_floats(int G) { return static_cast<long long>(kMaxShares) * 2 * G * (kD + 2); }
+long long rl_kv8_part_floats(int G) { return static_cast<long long>(kMaxShares) * 2 * G * (kD + 3); }
 
 int rl_kv8_write(int dtype, const void* qkv, int qkv_stride, const int32_t* positions, const int32_t* slots,
                  const float* cos, const float* sin, void* kc, void* vc, void* ks, void* vs, void* q_out, int q_stride,
@@ -758,8 +886,7 @@ int rl_kv8_write(int dtype, const void* qkv, int qkv_stride, const int32_t* posi
 int rl_kv8_attn_decode(int dtype, const void* q, int q_stride, void* kc, void* vc, void* ks, void* vs, const int32_t* bt,
                        int max_blocks, const void* items, int nitems, float* part, int* counters, void* out, int out_stride,
                        int hq, int hkv, int page_size, int window, float scale, const float* cos, const float* sin, int max_pos,
-                       int store, long long num_slots, int* status, long long max_units, void* stream_) {
-  if (max_units <= 0) return 0;
+                       int store, long long num_slots, int* status, int max_ctx, long long sum_ctx, int impl, void* stream_) {
   const cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   int sms = 0;
   int e = device_sms(&sms);
@@ -798,7 +925,16 @@ int rl_kv8_attn_decode(int dtype, const void* q, int q_stride, void* kc, void* v
   for (int i0 = 0; i0 < nitems; i0 += kMaxItems) {         // (one launch unless there are very many items)
     a.items = static_cast<const int4*>(items) + i0;
     a.nitems = nitems - i0 < kMaxItems ? nitems - i0 : kMaxItems;
+#ifdef RL_KV8_TC
+    if (dtype == 1 && hq / hkv <= 16 && impl != 1) {
+      e = launch_decode_tc(a, max_ctx, sum_ctx, impl, stream);
+      if (e) return e;
+      continue;
+    }
+#endif
+    if (impl > 1) return static_cast<int>(cudaErrorInvalidValue);
     // a CTA to a unit, as far as they are resident together
+    const long long max_units = static_cast<long long>(a.nitems) * hkv * (max_ctx / kUnit + 2);
     const int most = sms * 2 < kMaxShares ? sms * 2 : kMaxShares;
     const int ctas = static_cast<int>(max_units < most ? max_units : most);
     if (dtype == 0)

@@ -69,7 +69,7 @@ __device__ __forceinline__ uint32_t kv8_pack4(const float* f) { return kv8_pack2
 // A row is an (item, kv head): the query heads of one kv head of one sequence's token.  Its live keys are counted in
 // units of kUnit keys from an absolute boundary.  The units of all rows, one after another, are cut into as many
 // equal shares as there are groups of warps at work: a share holds whole rows, and at its two ends at most one row
-// each that is cut.  A whole row is written by its group; of a cut row every group leaves (max, denominator, numerators) in a
+// each that is cut.  A whole row is written by its group; of a cut row every group leaves its piece in a
 // place of its own in the workspace (two places a share: 0 for the row that goes on from the share before, 1 for a row
 // that begins here and goes on), counts itself, and the last one to count adds the pieces in the order of the keys.  Nobody waits
 // for anybody.
@@ -84,7 +84,7 @@ struct Kv8Args {
   int max_blocks;
   const int4* items;           // (token index of the query, sequence index, context length, 0)
   int nitems;
-  float* part;                 // [shares, 2, G, D + 2] numerators, max (log2 units), denominator
+  float* part;                 // [shares, 2, G, D + 3] pieces: numerators, d, m, denominator (Kv8Piece)
   int* counters;               // [items * Hkv], zero between launches
   void* out;                   // [tokens, out_stride]
   int out_stride;
@@ -95,5 +95,33 @@ struct Kv8Args {
   int max_pos;
   int* status;
 };
+
+// What a part of a row's keys comes to, for one head and one entry of its result (log2 units): the denominator times 2^m and
+// the numerator times 2^(m + d).  Two references, because a numerator's terms carry the scales of their pages; the second as a
+// distance from the first, so that it keeps its bits when the scores are large.
+struct Kv8Piece {
+  float m = -INFINITY, d = -INFINITY, den = 0.f, num = 0.f;
+  __device__ __forceinline__ void add(float od, float om, float oden, float onum) {
+    if (om == -INFINITY && oden == 0.f) return;          // (a part without keys)
+    const float t = fmaxf(m, om);
+    const float a = m == -INFINITY ? -INFINITY : m - t, b = om == -INFINITY ? 0.f : om - t;
+    const float td = fmaxf(d + a, od + b);
+    const float wa = a == -INFINITY ? 0.f : exp2f(d + a - td);
+    num = num * wa + onum * exp2f(od + b - td);
+    den = den * exp2f(a) + oden * exp2f(b);
+    m = t;
+    d = td;
+  }
+  __device__ __forceinline__ float value() const { return num / den * exp2f(d); }
+};
+// Entry d of a piece into its place (all entries of a head are left by somebody).
+__device__ __forceinline__ void kv8_leave(float* place, int dim, int d, const Kv8Piece& x) {
+  place[d] = x.num;
+  if (d == 0) {
+    place[dim] = x.d;
+    place[dim + 1] = x.m;
+    place[dim + 2] = x.den;
+  }
+}
 
 }  // namespace rl

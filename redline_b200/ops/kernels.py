@@ -665,7 +665,6 @@ def attn_prefill(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, vcache: t
 
 KV8_DTYPE, KV8_SCALE_DTYPE = torch.float8_e4m3fn, torch.float8_e8m0fnu
 KV8_PAGE_SIZES = (16, 32, 64)
-KV8_UNIT = 64                     # keys of a unit of work (kUnit)
 
 
 def _kv8(head_dim: int) -> ctypes.CDLL:
@@ -780,7 +779,7 @@ def kv8_decode_workspace(nitems: int, num_heads: int, num_kv_heads: int, head_di
 
 
 def _kv8_decode(what: str, q, q_stride, kcache, vcache, kscale, vscale, block_table, items, workspace, out, nitems, num_heads,
-                num_kv_heads, head_dim, page_size, window, scale, cos, sin, status, max_ctx, sum_ctx) -> None:
+                num_kv_heads, head_dim, page_size, window, scale, cos, sin, status, max_ctx, sum_ctx, impl) -> None:
     store = cos is not None
     _kv8_check(what, kcache, vcache, kscale, vscale, num_heads, num_kv_heads, head_dim, page_size)
     _kv8_rows(what, "qkv" if store else "q", q, q_stride, (num_heads + (2 * num_kv_heads if store else 0)) * head_dim, kcache)
@@ -812,13 +811,13 @@ def _kv8_decode(what: str, q, q_stride, kcache, vcache, kscale, vscale, block_ta
     f = _fn(lib, "rl_kv8_attn_decode",
             [c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p,
              c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_int, c_int, c_longlong, c_void_p,
-             c_longlong, c_void_p])
+             c_int, c_longlong, c_int, c_void_p])
     with _on(kcache):
         _check(f(_code(q.dtype), q.data_ptr(), q_stride, kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(),
                  vscale.data_ptr(), block_table.data_ptr(), block_table.shape[1], items.data_ptr(), nitems, part.data_ptr(),
                  counters.data_ptr(), out.data_ptr(), out.stride(0), num_heads, num_kv_heads, page_size, window, float(scale),
                  _ptr(cos), _ptr(sin), cos.shape[0] if store else 0, 1 if store else 0, kcache.shape[0] * page_size,
-                 status.data_ptr() if store else None, nitems * num_kv_heads * (seen // KV8_UNIT + 2), _stream()),
+                 status.data_ptr() if store else None, seen, sum_ctx, impl, _stream()),
                what, 2 if store else 1)
 
 
@@ -826,7 +825,7 @@ def kv8_attn_decode(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, vcache
                     vscale: torch.Tensor, block_table: torch.Tensor, items: torch.Tensor,
                     workspace: Tuple[torch.Tensor, torch.Tensor], out: torch.Tensor, nitems: int, num_heads: int,
                     num_kv_heads: int, head_dim: int, page_size: int, window: int, scale: float, max_ctx: int = 0,
-                    sum_ctx: int = 0) -> None:
+                    sum_ctx: int = 0, impl: int = 0) -> None:
     """``attn_decode`` over a cache in 8 bits (kv8_write): one query token per item.
 
     items      int32 [nitems, 4]: (token index of the query, sequence index, context length, 0); an item of context 0 has
@@ -834,20 +833,23 @@ def kv8_attn_decode(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, vcache
     workspace  of kv8_decode_workspace
     max_ctx, sum_ctx  the longest context and their sum, as far as the host knows them (0: unknown); the work is shared out by
                the items' own contexts, these choose between ways to do so
+    impl       0: the best kernel that applies; 1: CUDA cores; 2: tensor cores, a cluster or a group of warps to a row, or an
+               error; 3: tensor cores, the keys in equal shares, or an error (tensor cores: bfloat16, head size 64 or 128, up to 16
+               query heads to a kv head)
     """
     _kv8_decode("kv8_attn_decode", q, q_stride, kcache, vcache, kscale, vscale, block_table, items, workspace, out, nitems,
-                num_heads, num_kv_heads, head_dim, page_size, window, scale, None, None, None, max_ctx, sum_ctx)
+                num_heads, num_kv_heads, head_dim, page_size, window, scale, None, None, None, max_ctx, sum_ctx, impl)
 
 
 def kv8_attn_decode_rope(qkv: torch.Tensor, q_stride: int, kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch.Tensor,
                          vscale: torch.Tensor, block_table: torch.Tensor, items: torch.Tensor,
                          workspace: Tuple[torch.Tensor, torch.Tensor], out: torch.Tensor, nitems: int, num_heads: int,
                          num_kv_heads: int, head_dim: int, page_size: int, window: int, scale: float, cos: torch.Tensor,
-                         sin: torch.Tensor, status: torch.Tensor, max_ctx: int = 0, sum_ctx: int = 0) -> None:
+                         sin: torch.Tensor, status: torch.Tensor, max_ctx: int = 0, sum_ctx: int = 0, impl: int = 0) -> None:
     """``kv8_attn_decode`` from the UNROTATED rows [q | k | v] of the query tokens: a token's position is its context length - 1;
     its rotated k and its v are stored there first (as kv8_write does), and q is rotated on its way into the attention."""
     _kv8_decode("kv8_attn_decode_rope", qkv, q_stride, kcache, vcache, kscale, vscale, block_table, items, workspace, out, nitems,
-                num_heads, num_kv_heads, head_dim, page_size, window, scale, cos, sin, status, max_ctx, sum_ctx)
+                num_heads, num_kv_heads, head_dim, page_size, window, scale, cos, sin, status, max_ctx, sum_ctx, impl)
 
 
 _kv8_part: Dict[Tuple[int, int], int] = {}

@@ -236,12 +236,19 @@ DECODE = [  # heads, kv heads, head size, page, window, contexts
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
 @pytest.mark.parametrize("heads,kv_heads,dim,page,window,ctxs", DECODE)
-def test_decode(heads, kv_heads, dim, page, window, ctxs, dtype):
+@pytest.mark.parametrize("impl", [0, 1, 2, 3])
+def test_decode(heads, kv_heads, dim, page, window, ctxs, dtype, impl):
+    if impl >= 2 and (dtype == "float32" or dim not in (64, 128) or heads > 16 * kv_heads):
+        with pytest.raises(kernels.KernelError):
+            cache, table = filled((3,), heads, kv_heads, dim, page, seed=1)
+            decode(torch.zeros(1, heads * dim, dtype=DT[dtype], device=DEV), on_gpu(cache), table, (3,), heads, kv_heads, dim, page, 0,
+                   1.0, impl=impl)
+        return
     cache, table = filled(ctxs, heads, kv_heads, dim, page, seed=dim + len(ctxs))
     g = torch.Generator().manual_seed(9)
     q = torch.randn(len(ctxs), heads * dim, generator=g).to(DT[dtype])
     scale = 1.0 / math.sqrt(dim)
-    out = decode(q.to(DEV), on_gpu(cache), table, ctxs, heads, kv_heads, dim, page, window, scale)
+    out = decode(q.to(DEV), on_gpu(cache), table, ctxs, heads, kv_heads, dim, page, window, scale, impl=impl)
     k, v = P.values(cache[0], cache[2]), P.values(cache[1], cache[3])
     for s, n in enumerate(ctxs):
         ref = P.attend(q[s].view(1, heads, dim), k, v, table[s], [n - 1], window, scale)
@@ -267,10 +274,11 @@ def test_decode_of_many_and_of_very_different_lengths(dim, dtype):
             near(out[s].view(1, heads, dim), ref, v[table[s][:-(-ctxs[s] // page)].long()], dtype)
         again = decode(qg, gpu, table, ctxs, heads, kv_heads, dim, page, 0, scale)
         assert torch.equal(out, again)
-        told = decode(qg, gpu, table, ctxs, heads, kv_heads, dim, page, 0, scale, max_ctx=max(ctxs), sum_ctx=sum(ctxs))
-        for s in range(len(ctxs)):      # (another way to share the work out: other last bits)
-            mine = v[table[s][:-(-ctxs[s] // page)].long()]
-            near(told[s], out[s].double(), mine, dtype)
+        for kw in (dict(max_ctx=max(ctxs), sum_ctx=sum(ctxs)), dict(impl=1)) + ((dict(impl=2), dict(impl=3)) if dtype == "bfloat16" else ()):
+            told = decode(qg, gpu, table, ctxs, heads, kv_heads, dim, page, 0, scale, **kw)
+            for s in range(len(ctxs)):      # (another way to share the work out: other last bits)
+                mine = v[table[s][:-(-ctxs[s] // page)].long()]
+                near(told[s], out[s].double(), mine, dtype)
 
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
@@ -354,12 +362,13 @@ def test_decode_with_the_tokens_own_keys(heads, kv_heads, dim, page, window, dty
         assert torch.equal(xg.cpu(), x) and status.item() == 0
         positions = [n - 1 for n in ctxs]
         slots = [int(table[s, p // page]) * page + p % page for s, p in enumerate(positions)]
-        q = check_write(x, positions, slots, cos, sin, cache, heads, kv_heads, dim, page)
+        check_write(x, positions, slots, cos, sin, cache, heads, kv_heads, dim, page)
+        q = P.rotate(x.float()[:, :heads * dim].view(-1, heads, dim), cos[positions], sin[positions])     # (not rounded on its way)
         for got, want in zip(gpu, cache):
             assert torch.equal(got.view(torch.uint8).cpu(), want)
         k, v = P.values(cache[0], cache[2]), P.values(cache[1], cache[3])
         for s, n in enumerate(ctxs):
-            ref = P.attend(q[s].cpu().view(1, heads, dim), k, v, table[s], [n - 1], window, scale)
+            ref = P.attend(q[s].view(1, heads, dim), k, v, table[s], [n - 1], window, scale)
             near(out[s].view(1, heads, dim), ref, v[table[s][:-(-n // page)].long()], dtype)
     items[3, 2] = 500                                 # a position beyond the tables is told, and nothing beyond them is read
     kernels.kv8_attn_decode_rope(xg, xg.stride(0), *gpu, torch.zeros(len(ctxs), 500 // page + 1, dtype=torch.int32, device=DEV), items,
@@ -495,7 +504,7 @@ def test_a_run_of_steps(heads, kv_heads, dim, page, dtype):
         graph.replay()
         slots = [int(table[s, at[s] // page]) * page + at[s] % page for s in range(2)]
         f = x.float()
-        q = P.rotate(f[:, :heads * dim].view(2, heads, dim), cos[at], sin[at]).to(DT[dtype])
+        q = P.rotate(f[:, :heads * dim].view(2, heads, dim), cos[at], sin[at])
         P.store(P.rotate(f[:, heads * dim:-kv_heads * dim].view(2, kv_heads, dim), cos[at], sin[at]), slots, cache[0], cache[2])
         P.store(f[:, -kv_heads * dim:].reshape(2, kv_heads, dim), slots, cache[1], cache[3])
         for got, want in zip(gpu, cache):

@@ -32,10 +32,7 @@ __device__ __forceinline__ void store8(bf16* p, const float* in) { store16(p, in
 
 // Entries i and i + D/2 of a head by the angle's cosine and sine.  (Each product is rounded before the sum: what is
 // stored next is rounded to 4 bits, and a fused sum would land on the other side of a border now and then.)
-__device__ __forceinline__ void kv8_rotate8(float* x0, float* x1, const float* cos, const float* sin) {
-  float c[8], s[8];
-  load8(cos, c);
-  load8(sin, s);
+__device__ __forceinline__ void kv8_rotate8(float* x0, float* x1, const float* c, const float* s) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float a = x0[i], b = x1[i];
@@ -98,7 +95,7 @@ template <typename T>
 __global__ void __launch_bounds__(kWriteThreads)
 kv8_write_kernel(const Kv8WriteArgs<T> a, int kv_blocks) {
   pdl_wait();
-  pdl_launch();    // (behind the wait: a kernel after this one may read, before its own wait, what kernels before this one wrote)
+  pdl_launch();
   constexpr int CH = kD / 16;                    // lanes to a token: each has 8 entries of either half of the head
   if (static_cast<int>(blockIdx.x) >= kv_blocks) {
     const int per = a.hq * CH;
@@ -112,7 +109,10 @@ kv8_write_kernel(const Kv8WriteArgs<T> a, int kv_blocks) {
     load8(src + kD / 2, x1);
     if (a.cos != nullptr) {
       const size_t at = static_cast<size_t>(kv8_position(a, a.positions[t])) * (kD / 2) + rest % CH * 8;
-      kv8_rotate8(x0, x1, a.cos + at, a.sin + at);
+      float c[8], s[8];
+      load8(a.cos + at, c);
+      load8(a.sin + at, s);
+      kv8_rotate8(x0, x1, c, s);
     }
     T* dst = a.q_out + static_cast<size_t>(t) * a.q_stride + col;
     store8(dst, x0);
@@ -121,7 +121,10 @@ kv8_write_kernel(const Kv8WriteArgs<T> a, int kv_blocks) {
   }
   const int t = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int ps = 1 << a.page_shift;
-  const long long slot = kv8_slot(a, t);
+  // (asked for together: the slots of the token before, of this one and of 30 more, and those of all before it)
+  const int near = t - 1 + lane;
+  const long long theirs = near >= 0 && near < a.tokens ? kv8_slot(a, near) : -1;
+  const long long slot = __shfl_sync(0xffffffffu, theirs, 1);
   if (slot < 0) return;
   if (slot >= a.num_slots) {
     if (threadIdx.x == 0) atomicOr(a.status, 4);
@@ -129,7 +132,7 @@ kv8_write_kernel(const Kv8WriteArgs<T> a, int kv_blocks) {
   }
   const int off = static_cast<int>(slot & (ps - 1));
   const long long page = slot >> a.page_shift;
-  if (t > 0 && off > 0 && kv8_slot(a, t - 1) == slot - 1) return;      // not the first of its run
+  if (off > 0 && __shfl_sync(0xffffffffu, theirs, 0) == slot - 1) return;      // not the first of its run
   // Two runs of one page in one call would each set its scale without the other's: only the first is stored.  (Page 0
   // is the reserved one that padding rows write to: nothing to tell of there.)
   bool before = false;
@@ -141,15 +144,19 @@ kv8_write_kernel(const Kv8WriteArgs<T> a, int kv_blocks) {
     if (threadIdx.x == 0 && page != 0) atomicOr(a.status, 8);
     return;
   }
-  int n = 1;                                     // tokens of the run
+  int n;                                         // tokens of the run
   {
-    bool same = true;
-    for (int i0 = 0; same && i0 < ps; i0 += 32) {
-      const int i = i0 + lane;
-      const bool in = t + i < a.tokens && off + i < ps && kv8_slot(a, t + i) == slot + i;
-      const unsigned m = __ballot_sync(0xffffffffu, in);
-      n = m == 0xffffffffu ? i0 + 32 : i0 + __ffs(~m) - 1;
-      same = m == 0xffffffffu;
+    // (lane l has token t - 1 + l; lane 0 stands for itself)
+    unsigned m = __ballot_sync(0xffffffffu, lane == 0 || (off + lane - 1 < ps && theirs == slot + lane - 1));
+    n = m == 0xffffffffu ? 31 : __ffs(~m) - 2;
+    while (n >= 31 && off + n < ps) {
+      const int i = n + lane;
+      m = __ballot_sync(0xffffffffu, t + i < a.tokens && off + i < ps && kv8_slot(a, t + i) == slot + i);
+      if (m != 0xffffffffu) {
+        n += __ffs(~m) - 1;
+        break;
+      }
+      n += 32;
     }
   }
   constexpr int TPR = 32 / CH;                   // tokens that a warp takes at once
@@ -166,7 +173,10 @@ kv8_write_kernel(const Kv8WriteArgs<T> a, int kv_blocks) {
       if (turn) {
         const int pos = a.items != nullptr ? a.items[t + i].z - 1 : a.positions[t + i];
         const size_t at = static_cast<size_t>(kv8_position(a, pos)) * (kD / 2) + ch * 8;
-        kv8_rotate8(x0, x1, a.cos + at, a.sin + at);
+        float c[8], s[8];
+        load8(a.cos + at, c);
+        load8(a.sin + at, s);
+        kv8_rotate8(x0, x1, c, s);
       }
     };
     float amax = 0.f;
@@ -309,33 +319,39 @@ __device__ __forceinline__ Kv8Segment kv8_segment(const Kv8Args& a, const int* s
   return g;
 }
 
-// The pieces of a cut row, added in the order of the keys and written out, by `nthreads` threads.
+// The pieces of a cut row, added in the order of the keys and written out, by `nwarps` warps: a warp to 32 (or 16) entries of a
+// head.  First a lane to a piece, for the references and the weights, then an entry to a lane, the pieces' loads in flight together.
 template <typename T>
-__device__ __forceinline__ void kv8_merge(const Kv8Args& a, const Kv8Segment& g, int units, int shares, int tid, int nthreads) {
-  const int G = a.hq / a.hkv;
+__device__ __forceinline__ void kv8_merge(const Kv8Args& a, const Kv8Segment& g, int units, int shares, int warp, int nwarps) {
+  constexpr int W = kD % 32 == 0 ? 32 : 16, NB = kD / W;
+  const int lane = threadIdx.x & 31, G = a.hq / a.hkv;
   const int s0 = kv8_share_of(g.row_begin, units, shares), s1 = kv8_share_of(g.row_end - 1, units, shares);
-  const int row = G * (kD + 3);
+  const int row = G * (kD + 4);
   // (the first piece ends its share unless it begins it: its place is 0 then, as everybody else's)
   const int first = kv8_share_begin(s0, units, shares) != g.row_begin ? 1 : 0;
-  for (int i = tid; i < G * kD; i += nthreads) {
-    const int r = i / kD, d = i - r * kD;
-    const float* base = a.part + r * (kD + 3);
-    Kv8Piece sum;
-    for (int s = s0; s <= s1; s += 8) {        // eight pieces' loads in flight together
-      float pd[8], m[8], den[8], num[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float* p = base + (static_cast<size_t>(min(s + k, s1)) * 2 + (s + k == s0 ? first : 0)) * row;
-        pd[k] = __ldcg(p + kD);
-        m[k] = __ldcg(p + kD + 1);
-        den[k] = __ldcg(p + kD + 2);
-        num[k] = __ldcg(p + d);
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (s + k <= s1) sum.add(pd[k], m[k], den[k], num[k]);
+  for (int i = warp; i < G * NB; i += nwarps) {
+    const int r = i / NB, d = (i - r * NB) * W + lane % W;
+    const float* base = a.part + r * (kD + 4);
+    auto piece = [&](int s) { return base + (static_cast<size_t>(s) * 2 + (s == s0 ? first : 0)) * row; };
+    float top = -INFINITY, dtop = -INFINITY, den = 0.f, num = 0.f;
+    for (int c = s0; c <= s1; c += 32) {                 // (32 pieces at a time; the sums so far are carried over)
+      const bool in = c + lane <= s1;
+      const float4 x = in ? __ldcg(reinterpret_cast<const float4*>(piece(c + lane) + kD)) : make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
+      const bool none = x.y == -INFINITY && x.z == 0.f;
+      const float t = fmaxf(top, warp_max(x.y));
+      const float dm = none ? 0.f : x.y - t, od = top == -INFINITY ? 0.f : top - t;
+      const float dt = fmaxf(dtop + od, warp_max(none ? -INFINITY : x.x + dm));
+      const float w = none ? 0.f : exp2f(x.x + dm - dt);
+      num *= dtop == -INFINITY ? 0.f : exp2f(dtop + od - dt);
+      den = den * exp2f(od) + warp_sum(none ? 0.f : x.z * exp2f(dm));
+      top = t;
+      dtop = dt;
+      const int n = min(32, s1 - c + 1);
+#pragma unroll 8
+      for (int k = 0; k < n; ++k) num += __shfl_sync(0xffffffffu, w, k) * __ldcg(piece(c + k) + d);
     }
-    static_cast<T*>(a.out)[static_cast<size_t>(g.tok) * a.out_stride + (g.kvh * G + r) * kD + d] = from_float<T>(sum.value());
+    if (lane < W)
+      static_cast<T*>(a.out)[static_cast<size_t>(g.tok) * a.out_stride + (g.kvh * G + r) * kD + d] = from_float<T>(num * exp2f(dtop) / den);
   }
 }
 
@@ -367,7 +383,7 @@ kv8_decode_kernel(const Kv8Args a) {
   for (int u = begin; u < end;) {
     const Kv8Segment g = kv8_segment(a, start, u, end);
     const int32_t* bt = a.block_table + static_cast<size_t>(g.seq) * a.max_blocks;
-    float* piece = a.part + (static_cast<size_t>(blockIdx.x) * 2 + (u == begin ? 0 : 1)) * (G * (kD + 3));
+    float* piece = a.part + (static_cast<size_t>(blockIdx.x) * 2 + (u == begin ? 0 : 1)) * (G * (kD + 4));
     for (int g0 = 0; g0 < G; g0 += kGenHeads) {
       const int ng = min(kGenHeads, G - g0);
       float q[kGenHeads][16], acc[kGenHeads][16], m[kGenHeads], l[kGenHeads];
@@ -486,12 +502,8 @@ kv8_decode_kernel(const Kv8Args a) {
         if (g.whole) {
           static_cast<T*>(a.out)[static_cast<size_t>(g.tok) * a.out_stride + (g.kvh * G + r) * kD + d] = from_float<T>(num / den);
         } else {
-          Kv8Piece x;
-          x.m = mx;
-          x.d = 0.f;
-          x.den = den;
-          x.num = num;
-          kv8_leave(piece + r * (kD + 3), kD, d, x);
+          piece[r * (kD + 4) + d] = num;
+          if (d == 0) *reinterpret_cast<float4*>(piece + r * (kD + 4) + kD) = make_float4(0.f, mx, den, 0.f);
         }
       }
       __syncthreads();
@@ -508,7 +520,7 @@ kv8_decode_kernel(const Kv8Args a) {
       __syncthreads();
       if (last) {
         __threadfence();
-        kv8_merge<T>(a, g, units, shares, threadIdx.x, kGenThreads);
+        kv8_merge<T>(a, g, units, shares, warp, kGenThreads / 32);
       }
       __syncthreads();
     }
@@ -766,7 +778,7 @@ struct TcDevice {
 };
 
 size_t tc_smem(int csize, int G) {
-  return static_cast<size_t>(kTcWarps) * (kRingBytes + kHeadBytes) + (csize > 1 ? sizeof(float) * csize * G * (kD + 3) : 0);
+  return static_cast<size_t>(kTcWarps) * kRingBytes + (csize > 1 ? sizeof(float) * csize * G * kPartLd : 0);
 }
 
 // What is asked of the device once.
@@ -870,7 +882,7 @@ int launch_decode_tc(Kv8Args a, int max_ctx, long long sum_ctx, int impl, cudaSt
 extern "C" {
 
 // The floats of the workspace for groups of G heads (kv8.cuh: Kv8Args::part).
-long long rl_kv8_part_floats(int G) { return static_cast<long long>(kMaxShares) * 2 * G * (kD + 3); }
+long long rl_kv8_part_floats(int G) { return static_cast<long long>(kMaxShares) * 2 * G * (kD + 4); }
 
 int rl_kv8_write(int dtype, const void* qkv, int qkv_stride, const int32_t* positions, const int32_t* slots,
                  const float* cos, const float* sin, void* kc, void* vc, void* ks, void* vs, void* q_out, int q_stride,
@@ -891,7 +903,14 @@ int rl_kv8_attn_decode(int dtype, const void* q, int q_stride, void* kc, void* v
   int sms = 0;
   int e = device_sms(&sms);
   if (e) return e;
-  if (store) {
+#ifdef RL_KV8_TC
+  const bool tc = dtype == 1 && hq / hkv <= 16 && impl != 1;
+#else
+  const bool tc = false;
+#endif
+  // (pages of 64 tokens reach over two sub-blocks, which may be two warps': their tokens are stored by a kernel of its own)
+  const bool fused = store && tc && page_size <= 32;
+  if (store && !fused) {
     auto run = dtype == 0 ? launch_write<float> : launch_write<bf16>;
     e = run(q, q_stride, nullptr, nullptr, static_cast<const int4*>(items), bt, max_blocks, cos, sin, static_cast<uint8_t*>(kc),
             static_cast<uint8_t*>(vc), static_cast<uint8_t*>(ks), static_cast<uint8_t*>(vs), nullptr, 0, nitems, hq, hkv, page_size,
@@ -919,6 +938,7 @@ int rl_kv8_attn_decode(int dtype, const void* q, int q_stride, void* kc, void* v
   a.window = window;
   a.scale = scale;
   a.cos = store ? cos : nullptr;
+  a.store = fused ? 1 : 0;
   a.sin = sin;
   a.max_pos = max_pos;
   a.status = status;
@@ -926,7 +946,7 @@ int rl_kv8_attn_decode(int dtype, const void* q, int q_stride, void* kc, void* v
     a.items = static_cast<const int4*>(items) + i0;
     a.nitems = nitems - i0 < kMaxItems ? nitems - i0 : kMaxItems;
 #ifdef RL_KV8_TC
-    if (dtype == 1 && hq / hkv <= 16 && impl != 1) {
+    if (tc) {
       e = launch_decode_tc(a, max_ctx, sum_ctx, impl, stream);
       if (e) return e;
       continue;

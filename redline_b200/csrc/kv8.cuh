@@ -84,7 +84,7 @@ struct Kv8Args {
   int max_blocks;
   const int4* items;           // (token index of the query, sequence index, context length, 0)
   int nitems;
-  float* part;                 // [shares, 2, G, D + 3] pieces: numerators, d, m, denominator (Kv8Piece)
+  float* part;                 // [shares, 2, G, D + 4] pieces: numerators, d, m, denominator
   int* counters;               // [items * Hkv], zero between launches
   void* out;                   // [tokens, out_stride]
   int out_stride;
@@ -93,35 +93,12 @@ struct Kv8Args {
   const float* cos;            // q is rotated by the kernel if given (position: context - 1)
   const float* sin;
   int max_pos;
+  int store;                   // q holds rows [q | k | v]: the tokens' keys and values are stored by the attention's kernel
   int* status;
 };
 
-// What a part of a row's keys comes to, for one head and one entry of its result (log2 units): the denominator times 2^m and
-// the numerator times 2^(m + d).  Two references, because a numerator's terms carry the scales of their pages; the second as a
-// distance from the first, so that it keeps its bits when the scores are large.
-struct Kv8Piece {
-  float m = -INFINITY, d = -INFINITY, den = 0.f, num = 0.f;
-  __device__ __forceinline__ void add(float od, float om, float oden, float onum) {
-    if (om == -INFINITY && oden == 0.f) return;          // (a part without keys)
-    const float t = fmaxf(m, om);
-    const float a = m == -INFINITY ? -INFINITY : m - t, b = om == -INFINITY ? 0.f : om - t;
-    const float td = fmaxf(d + a, od + b);
-    const float wa = a == -INFINITY ? 0.f : exp2f(d + a - td);
-    num = num * wa + onum * exp2f(od + b - td);
-    den = den * exp2f(a) + oden * exp2f(b);
-    m = t;
-    d = td;
-  }
-  __device__ __forceinline__ float value() const { return num / den * exp2f(d); }
-};
-// Entry d of a piece into its place (all entries of a head are left by somebody).
-__device__ __forceinline__ void kv8_leave(float* place, int dim, int d, const Kv8Piece& x) {
-  place[d] = x.num;
-  if (d == 0) {
-    place[dim] = x.d;
-    place[dim + 1] = x.m;
-    place[dim + 2] = x.den;
-  }
-}
+// What a part of a row's keys comes to, for one head, is left as D numerators times 2^(m + d) and a denominator times 2^m (log2
+// units).  Two references, because a numerator's terms carry the scales of their pages; the second as a distance from
+// the first, so that it keeps its bits when the scores are large.  A part without keys has m = -inf and denominator 0.
 
 }  // namespace rl

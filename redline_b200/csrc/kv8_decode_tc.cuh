@@ -4,17 +4,23 @@
 // are cut into as many equal runs of sub-blocks (32 keys) as the group has warps.  Every warp is a pipeline of its own:
 // the sub-blocks of its run come by 16-byte asynchronous copies into a private ring, 8 to 16 KB on their way while one is worked on
 // (44 KB an SM cover the way from DRAM at full rate).  A sub-block:
-//   S = Q K^T    mma.sync.m16n8k16 on halves: an e4m3 number is a half exactly (one conversion for two); q is scaled by a power of
-//                two per row to at most 256 and rounded to 11 bits.  (The same instruction on e4m3 bytes is put together from
-//                conversions, two products on halves and sums on this machine; it took 1.5 times as long.)  Which entries of the head a
-//                k index of the product stands for is free, so a lane's 16 bytes of a key are four k steps of the B
-//                fragment as they lie.
-//   softmax      online, in log2 units: the denominator sums 2^(x - m), m the largest score; the weights for the product are
-//                2^(x - m + e - d), e the exponent of the page's value scale and d the largest x - m + e, so that they keep
-//                their bits whatever scales lie side by side (pages of zeros among them) and O needs no factor a page
-//   O += P V     P as halves, scaled to at most 2^14: 11 bits down to 2^-28 of the run's largest weight.  ldmatrix transposes 16 x 16
-//                bytes of V: four keys of an entry in a word
-// Page ids and scales are fetched a window of 32 pages at a time, a page to a lane, and the window after it behind that.
+//   S = K Q^T    mma.sync.m16n8k16 on halves, 16 keys x 8 query heads: an e4m3 number is a half exactly (one conversion for two); q is
+//                scaled by a power of two per row to at most 256 and rounded to 11 bits.  (The instruction on e4m3 bytes is put together
+//                from conversions, products on halves and sums on this machine and was slower; with the heads as the wide side, half
+//                of its rows empty, there were twice as many products.)  Which entries of the head a k index of the product
+//                stands for is free, so a lane's 16 bytes of a key are four k steps of the A fragment as they lie.
+//   softmax      online, in log2 units, against a reference that moves only when some score exceeds it by 2^10: one vote a sub-block
+//                instead of shuffles.  The weights are halves, 2^5 at the reference: 11 bits down to 2^-19 of it, steps of 2^-29 below.
+//                For the product they carry the value scale of their page relative to the largest so far (2^-28 of that loses bits)
+//   O^T += V^T P^T   ldmatrix transposes 16 x 16 bytes of V: four keys of an entry in a word; movmatrix transposes P
+// With the rotation in the kernel (a.store) the warp that has a row's newest page also stores the token's key and value there: it
+// takes that sub-block first, puts the token over what the copy brought, rescales the page if its scale rises, and goes on
+// with the bytes as they are stored.
+// Page ids and scales are fetched a window of 32 pages at a time, a page to a lane, ahead of their use.
+//
+// A launch of few keys is a chain of trips to memory (item, page ids, keys; then the results' way to their row), so whatever does not
+// depend on one another is asked for together, and results meet in two steps: weights by a warp a head, then sums of 16 bytes a
+// thread.
 //
 // Where rows are shared out (see launch_decode_tc for the choice):
 //   rows    a cluster of up to 8 CTAs to a row, whose partial results meet in the first one's shared memory; or, with more rows
@@ -29,7 +35,6 @@ constexpr int kSub = 32;                                 // keys of a sub-block
 constexpr int kSubBytes = kSub * kD;                     // K (or V) of one
 constexpr int kRing = kD == 64 ? 4 : 3;                  // (192 KB for all warps either way)
 constexpr int kRingBytes = kRing * 2 * kSubBytes;
-constexpr int kHeadBytes = kRing * 16;                   // the scales of a warp's stages: (K, log2 of V) of the first 16 keys and of the second
 constexpr int kMaxCluster = 8;
 constexpr int kPartLd = kD + 4;                          // floats to a head in a warp's partial result: kd numerators, d, m, denominator
 static_assert(16 * kPartLd * 4 <= kRingBytes, "a warp's partial result lies in its own ring");
@@ -65,6 +70,18 @@ __device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// An 8 x 8 tile of halves, a row's two to a lane, transposed.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+// (volatile: asked for where it stands)
+__device__ __forceinline__ uint4 ldg16(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
 __device__ __forceinline__ void mma_f16_first(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
       : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
@@ -95,136 +112,258 @@ __device__ __forceinline__ uint32_t cluster_size() {
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
   return r;
 }
+// (nothing to be seen yet: only that the others have begun)
+__device__ __forceinline__ void cluster_arrive_begun() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-// A float to this CTA's address p in CTA `rank` of the cluster.
-__device__ __forceinline__ void store_cluster(float* p, uint32_t rank, float v) {
+// Four floats to this CTA's address p in CTA `rank` of the cluster.
+__device__ __forceinline__ void store_cluster(float* p, uint32_t rank, float4 v) {
   uint32_t remote;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_addr(p)), "r"(rank));
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v) : "memory");
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(remote), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
 
-// One warp's result for its run; thread (g, t) holds, of head g, entries 8 j + 2 t + e at o[j][e], and of head g + 8 (HI)
-// at o[j][2 + e].
+constexpr float kTcGrow = 10.f;        // log2 of how far a score may exceed the reference
+constexpr int kTcBase = 5;             // log2 of a weight at the reference: 2^15 at most
+
+// One warp's result for its run.  Thread (g, t) holds entries 16 c + g (o[c][i][0 and 1]) and 16 c + 8 + g (2 and 3) of the heads
+// 8 i + 2 t and 8 i + 2 t + 1, and those heads' references and denominators (of its own keys until the end).
+template <bool HI>
 struct TcState {
-  float o[kD / 8][4];
-  float m[2], d[2], l[2];        // (the same for a row's four lanes, but for the denominator of the lane's own keys)
+  float o[kD / 16][HI ? 2 : 1][4];
+  float m[HI ? 2 : 1][2], l[HI ? 2 : 1][2];
+  int vref;                            // the exponent that the numerators' values are relative to (the same for the warp)
 };
 
-// q of the segment's token as A fragments (k step by k step; the rows g and g + 8, and both once more for the step's second
-// half), rotated on the way if the tables are given, and the factor of the exponent.
+// What q needs from memory: asked for first, used when the copies are on their way.
 template <bool HI>
-__device__ __forceinline__ void tc_load_q(const Kv8Args& a, const Kv8Segment& s, int lane, uint32_t (*qf)[HI ? 4 : 2], float* factor) {
-  constexpr float kLog2e = 1.4426950408889634f;
-  constexpr int NC = kD / 64;                            // 16-entry pieces of a head to a lane: entries 64 c + 16 t ..
+struct TcQ {
+  uint4 raw[HI ? 2 : 1][kD / 32];                        // entries 64 c + 16 t .. + 15 of the heads g (and g + 8)
+  uint4 cs[4], sn[4];
+};
+template <bool HI>
+__device__ __forceinline__ void tc_fetch_q(const Kv8Args& a, const Kv8Segment& s, int lane, TcQ<HI>& q) {
   const int g = lane >> 2, t = lane & 3, G = a.hq / a.hkv;
 #pragma unroll
   for (int h = 0; h < (HI ? 2 : 1); ++h) {
     const int r = g + 8 * h;
+    const uint4* row = reinterpret_cast<const uint4*>(static_cast<const bf16*>(a.q) + static_cast<size_t>(s.tok) * a.q_stride +
+                                                      (s.kvh * G + r) * kD + t * 16);
+#pragma unroll
+    for (int c = 0; c < kD / 32; ++c) {
+      q.raw[h][c] = make_uint4(0, 0, 0, 0);
+      if (r < G) q.raw[h][c] = ldg16(row + (c >> 1) * 8 + (c & 1));
+    }
+  }
+  if (a.cos != nullptr) {
+    int pos = s.ctx - 1;
+    if (pos >= a.max_pos) {
+      if (lane == 0) atomicOr(a.status, 2);
+      pos = 0;
+    }
+    // entry i turns with i + D/2: at head size 64 that is lane t ^ 2's, at 128 the lane's own other piece
+    const size_t at = static_cast<size_t>(pos) * (kD / 2) + (kD == 64 ? t & 1 : t) * 16;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      q.cs[e] = ldg16(a.cos + at + 4 * e);
+      q.sn[e] = ldg16(a.sin + at + 4 * e);
+    }
+  }
+}
+
+// q as B fragments (k step by k step: the column of head g, and of g + 8), rotated on the way if the tables are given, and
+// the factors of the exponents of the heads whose scores the lane has.
+template <bool HI>
+__device__ __forceinline__ void tc_make_q(const Kv8Args& a, const TcQ<HI>& q, int lane, uint32_t (*qf)[kD / 16][2], float (*factor)[2]) {
+  constexpr float kLog2e = 1.4426950408889634f;
+  constexpr int NC = kD / 64;
+  float cs[16], sn[16];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t c[4] = {q.cs[e].x, q.cs[e].y, q.cs[e].z, q.cs[e].w}, s[4] = {q.sn[e].x, q.sn[e].y, q.sn[e].z, q.sn[e].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      cs[4 * e + i] = __uint_as_float(c[i]);
+      sn[4 * e + i] = kD == 64 && (lane & 2) == 0 ? -__uint_as_float(s[i]) : __uint_as_float(s[i]);
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < (HI ? 2 : 1); ++h) {
     float x[NC][16];
-    if (r < G) {
-      const bf16* row = static_cast<const bf16*>(a.q) + static_cast<size_t>(s.tok) * a.q_stride + (s.kvh * G + r) * kD + t * 16;
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        load16(row + c * 64, x[c]);
-        load16(row + c * 64 + 8, x[c] + 8);
+    for (int c = 0; c < kD / 32; ++c) {
+      const uint32_t w[4] = {q.raw[h][c].x, q.raw[h][c].y, q.raw[h][c].z, q.raw[h][c].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[c >> 1][(c & 1) * 8 + 2 * i] = __uint_as_float(w[i] << 16);
+        x[c >> 1][(c & 1) * 8 + 2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
       }
-    } else {
-#pragma unroll
-      for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) x[c][e] = 0.f;
     }
     if (a.cos != nullptr) {
-      int pos = s.ctx - 1;
-      if (pos >= a.max_pos) {
-        if (lane == 0) atomicOr(a.status, 2);
-        pos = 0;
-      }
-      // entry i turns with i + D/2: at head size 64 that is lane t ^ 2's, at 128 the lane's own other piece
-      const int d0 = (kD == 64 ? t & 1 : t) * 16;
 #pragma unroll
-      for (int e0 = 0; e0 < 16; e0 += 4) {
-        float cs[4], sn[4];
-        load16(a.cos + static_cast<size_t>(pos) * (kD / 2) + d0 + e0, cs);
-        load16(a.sin + static_cast<size_t>(pos) * (kD / 2) + d0 + e0, sn);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int e = e0 + i;
-          if constexpr (kD == 64) {
-            const float other = __shfl_xor_sync(0xffffffffu, x[0][e], 2);
-            x[0][e] = t < 2 ? x[0][e] * cs[i] - other * sn[i] : x[0][e] * cs[i] + other * sn[i];
-          } else {
-            const float lo = x[0][e], hi = x[NC - 1][e];
-            x[0][e] = lo * cs[i] - hi * sn[i];
-            x[NC - 1][e] = hi * cs[i] + lo * sn[i];
-          }
+      for (int e = 0; e < 16; ++e) {
+        if constexpr (kD == 64) {
+          const float other = __shfl_xor_sync(0xffffffffu, x[0][e], 2);
+          x[0][e] = x[0][e] * cs[e] + other * sn[e];
+        } else {
+          const float lo = x[0][e], hi = x[NC - 1][e];
+          x[0][e] = lo * cs[e] - hi * sn[e];
+          x[NC - 1][e] = hi * cs[e] + lo * sn[e];
         }
       }
     }
-    float most = 0.f;
-    bool odd = false;                                    // (a row that is not finite is not a number, not a large one)
+    // (the largest of the bits of the magnitudes is that of the magnitudes, and beyond the finite ones for what is not)
+    uint32_t most = 0;
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        most = fmaxf(most, fabsf(x[c][e]));
-        odd |= !(fabsf(x[c][e]) < INFINITY);
-      }
-    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    odd = ((__ballot_sync(0xffffffffu, odd) >> (g * 4)) & 15u) != 0;
-    const int ex = static_cast<int>(__float_as_uint(most) >> 23);        // the largest entry is 1.m * 2^(ex - 127)
-    const int up = ex == 0 ? 0 : min(134 - ex, 127);                     // ... and is scaled to 1.m * 2^7
+      for (int e = 0; e < 16; ++e) most = max(most, __float_as_uint(x[c][e]) & 0x7fffffffu);
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    const int ex = static_cast<int>(most >> 23);         // the largest entry is 1.m * 2^(ex - 127)
+    const int up = ex == 0 ? 0 : min(134 - ex, 127);     // ... and is scaled to 1.m * 2^7
     const float mul = kv8_exp2i(max(up, -126));
-    factor[h] = odd ? __uint_as_float(0x7fc00000u) : a.scale * kLog2e * kv8_exp2i(-up);
+    // (a row that is not finite is not a number, not a large one)
+    const float f = ex == 255 ? __uint_as_float(0x7fc00000u) : a.scale * kLog2e * kv8_exp2i(-up);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) factor[h][e] = __shfl_sync(0xffffffffu, f, ((lane & 3) * 2 + e) * 4);
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        float y[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = odd ? 0.f : x[c][4 * k + e] * mul;
-        qf[c * 4 + k][h] = pack_halves(y[0], y[1]);
-        qf[c * 4 + k][h + (HI ? 2 : 1)] = pack_halves(y[2], y[3]);
+        qf[h][c * 4 + k][0] = pack_halves(x[c][4 * k] * mul, x[c][4 * k + 1] * mul);
+        qf[h][c * 4 + k][1] = pack_halves(x[c][4 * k + 2] * mul, x[c][4 * k + 3] * mul);
       }
   }
 }
 
-// The run of sub-blocks [sb0, sb0 + n) of the segment through the warp's ring (`ring`, its stages' scales at `head`).
-// `waited`: the kernels before this one are done; if they are not, the first copies are those of pages that the one before
-// does not write.
-template <bool HI>
-__device__ __forceinline__ void tc_run(const Kv8Args& a, const Kv8Segment& s, int sb0, int n, uint32_t ring, uint32_t head, int lane,
-                                       bool& waited, TcState& st) {
-  constexpr int KS = kD / 16, NJ = kD / 8, NR = HI ? 2 : 1;
-  constexpr int CPR = kD / 16;                           // 16-byte pieces of a key
-  const int g = lane >> 2, t = lane & 3;
-  const int shift = a.page_shift, ps = 1 << shift;
-  const int32_t* bt = a.block_table + static_cast<size_t>(s.seq) * a.max_blocks;
-#pragma unroll
-  for (int j = 0; j < NJ; ++j)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) st.o[j][e] = 0.f;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    st.m[h] = st.d[h] = -INFINITY;
-    st.l[h] = 0.f;
+// The token's own key (lanes 0 .. D/16 - 1) and value (the next D/16): entries 8 c .. + 7 and those D/2 further, and the angles.
+struct TcToken {
+  uint4 x0, x1;
+  float cs[8], sn[8];
+};
+__device__ __forceinline__ void tc_fetch_token(const Kv8Args& a, const Kv8Segment& s, int lane, TcToken& x) {
+  constexpr int CH = kD / 16;
+  if (lane >= 2 * CH) return;
+  const int c = lane % CH;
+  const bf16* p = static_cast<const bf16*>(a.q) + static_cast<size_t>(s.tok) * a.q_stride +
+                  (a.hq + (lane < CH ? 0 : a.hkv) + s.kvh) * kD + c * 8;
+  x.x0 = ldg16(p);
+  x.x1 = ldg16(p + kD / 2);
+  const size_t at = static_cast<size_t>(s.ctx - 1 < a.max_pos ? s.ctx - 1 : 0) * (kD / 2) + c * 8;
+  load8(a.cos + at, x.cs);
+  load8(a.sin + at, x.sn);
+}
+// Where 16-byte piece ch of row r of a sub-block lies in its stage (K, V): the fragment reads are free of bank conflicts.
+__device__ __forceinline__ uint32_t tc_place(bool is_v, int r, int ch) {
+  const int sw = kD == 64 ? (is_v ? (r >> 1) & 3 : 0) : (is_v ? r & 7 : (r & 1) << 2);
+  return static_cast<uint32_t>((is_v ? kSubBytes : 0) + r * kD + ((ch ^ sw) << 4));
+}
+// Stores the token into its page, in the cache (if `mine`) and in the stage that holds the page.  codes: the bytes of the
+// page's scales (K, then V); they come back as they are now.
+__device__ __forceinline__ uint32_t tc_store_token(const Kv8Args& a, const Kv8Segment& s, int page, uint32_t stage, int lane, bool mine,
+                                                   const TcToken& token, uint32_t codes) {
+  constexpr int CH = kD / 16;
+  const int ps = 1 << a.page_shift, pos = s.ctx - 1, off = pos & (ps - 1), row = pos % kSub, row0 = row - off;
+  float amax = 0.f, x0[8] = {}, x1[8] = {};
+  if (lane < 2 * CH) {
+    load16(reinterpret_cast<const bf16*>(&token.x0), x0);
+    load16(reinterpret_cast<const bf16*>(&token.x1), x1);
+    if (lane < CH) kv8_rotate8(x0, x1, token.cs, token.sn);
   }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float u = fabsf(x0[e]), v = fabsf(x1[e]);
+    amax = fmaxf(amax, fmaxf(u < INFINITY ? u : 0.f, v < INFINITY ? v : 0.f));
+  }
+#pragma unroll
+  for (int o = 1; o < CH; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  const size_t block = static_cast<size_t>(page) * a.hkv + s.kvh;
+  uint32_t now = 0;
+#pragma unroll
+  for (int is_v = 0; is_v < 2; ++is_v) {
+    uint8_t* base = const_cast<uint8_t*>(is_v ? a.vcache : a.kcache) + block * ps * kD;
+    const int old = min(static_cast<int>((codes >> (8 * is_v)) & 255), 254);
+    int code = kv8_code(__shfl_sync(0xffffffffu, amax, is_v * CH));
+    if (off > 0) {
+      if (code > old) {                          // what is in the page goes over to the larger scale
+        const float f = kv8_exp2i(max(old - code, -127));
+        for (int c = lane; c < off * CH; c += 32) {
+          const uint32_t at = stage + tc_place(is_v, row0 + c / CH, c % CH);
+          float y[16];
+          kv8_f16(lds16(at), y);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) y[e] *= f;
+          const uint4 w = make_uint4(kv8_pack4(y), kv8_pack4(y + 4), kv8_pack4(y + 8), kv8_pack4(y + 12));
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
+          if (mine) *(reinterpret_cast<uint4*>(base) + c) = w;
+        }
+      } else {
+        code = old;
+      }
+    }
+    if (mine && lane == 0) const_cast<uint8_t*>(is_v ? a.vscale : a.kscale)[block] = static_cast<uint8_t>(code);
+    if (lane >= is_v * CH && lane < (is_v + 1) * CH) {
+      const int c = lane - is_v * CH;
+      const float inv = kv8_exp2i(127 - code);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x0[e] = fabsf(x0[e]) < INFINITY ? x0[e] * inv : __uint_as_float(0x7fc00000u);
+        x1[e] = fabsf(x1[e]) < INFINITY ? x1[e] * inv : __uint_as_float(0x7fc00000u);
+      }
+      const uint2 lo = make_uint2(kv8_pack4(x0), kv8_pack4(x0 + 4)), hi = make_uint2(kv8_pack4(x1), kv8_pack4(x1 + 4));
+      const uint32_t p0 = stage + tc_place(is_v, row, c >> 1) + (c & 1) * 8;
+      const uint32_t p1 = stage + tc_place(is_v, row, (c + CH) >> 1) + (c & 1) * 8;
+      asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(p0), "r"(lo.x), "r"(lo.y) : "memory");
+      asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(p1), "r"(hi.x), "r"(hi.y) : "memory");
+      if (mine) {
+        *reinterpret_cast<uint2*>(base + off * kD + c * 8) = lo;
+        *reinterpret_cast<uint2*>(base + off * kD + kD / 2 + c * 8) = hi;
+      }
+    }
+    now |= static_cast<uint32_t>(code) << (8 * is_v);
+  }
+  __syncwarp();
+  return now;
+}
+
+// The run of sub-blocks [sb0, sb0 + n) of the segment, the last one first, through the warp's ring.
+template <bool HI>
+__device__ __forceinline__ void tc_run(const Kv8Args& a, const Kv8Segment& s, int sb0, int n, uint32_t ring, int lane, TcState<HI>& st) {
+  constexpr int KS = kD / 16, NC = kD / 16, NR = HI ? 2 : 1;
+  constexpr int CPR = kD / 16;                           // 16-byte pieces of a key
+  const int shift = a.page_shift, ps = 1 << shift;
+#pragma unroll
+  for (int h = 0; h < NR; ++h) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) st.o[c][h][e] = 0.f;
+    st.m[h][0] = st.m[h][1] = -INFINITY;
+    st.l[h][0] = st.l[h][1] = 0.f;
+  }
+  st.vref = -1000;
+  if (n <= 0) return;
+  const int32_t* bt = a.block_table + static_cast<size_t>(s.seq) * a.max_blocks;
   // (a sub-block may reach over either end of the live keys, into pages that need not be there any more: their places are
   // filled from the nearest live page)
-  const int page_first = s.key_lo >> shift, page_last = (s.key_hi - 1) >> shift;
-  const int page0 = n > 0 ? max((sb0 * kSub) >> shift, page_first) : 0;
-  // a window of 32 pages, a page to a lane: its id and its scales; and the next window's
-  int window = 0, my_page = 0, next_page = 0;
-  float my_kf = 0.f, my_ve = 0.f, next_kf = 0.f, next_ve = 0.f;
-  auto fetch = [&](int w, int& page, float& kf, float& ve) {
-    page = bt[min(page0 + w * 32 + lane, page_last)];
+  const int page_first = s.key_lo >> shift, page_last = min(s.key_hi - 1, (sb0 + n) * kSub - 1) >> shift;
+  auto page_of = [&](int key) { return page_last - min(max(key >> shift, page_first), page_last); };     // counted from the last
+  // a window of 32 pages, a page to a lane: its id and the bytes of its scales (K, V), those of the window before, and the
+  // ids of the next; and the scales of the window that the sums are in
+  int window = 0, my_page = bt[max(page_last - lane, page_first)], next_page = 0;
+  const int top = sb0 + n - 1;
+  const bool store = a.store && s.key_hi == s.ctx && top == (s.ctx - 1) / kSub;      // the newest page is this warp's
+  TcQ<HI> q;
+  tc_fetch_q<HI>(a, s, lane, q);
+  TcToken token;
+  if (store) tc_fetch_token(a, s, lane, token);
+  auto codes_of = [&](int page) -> uint32_t {
     const size_t at = static_cast<size_t>(page) * a.hkv + s.kvh;
-    const int kc = __ldcg(a.kscale + at), vc = __ldcg(a.vscale + at);
-    kf = kv8_scale(kc);
-    ve = vc == 255 ? __uint_as_float(0x7fc00000u) : static_cast<float>(vc - 127);
+    return static_cast<uint32_t>(__ldcg(a.kscale + at)) | static_cast<uint32_t>(__ldcg(a.vscale + at)) << 8;
   };
+  uint32_t my_codes = codes_of(my_page), old_codes = 0;
+  if (page_last - 32 >= page_first) next_page = bt[max(page_last - 32 - lane, page_first)];
   // Copies sub-block sb into stage `stage`.  16 keys of a page are contiguous; the places in shared memory are swizzled so that
   // the fragment reads are free of bank conflicts.  Bytes behind the segment's last key are copied too (they lie in the page).
   const uint32_t ch = lane % CPR, in = lane / CPR;       // this lane's piece of a row, its row of a round
@@ -237,15 +376,15 @@ __device__ __forceinline__ void tc_run(const Kv8Args& a, const Kv8Segment& s, in
   auto issue = [&](int sb, int stage) {
     const uint32_t kdst = ring + stage * (2 * kSubBytes) + koff, vdst = ring + stage * (2 * kSubBytes) + kSubBytes + voff;
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 1; b >= 0; --b) {
       const int key = sb * kSub + b * 16;
-      const int idx = min(max(key >> shift, page_first), page_last) - page0;
+      const int idx = page_of(key);
       if ((idx >> 5) != window) {
         window = idx >> 5;
         my_page = next_page;
-        my_kf = next_kf;
-        my_ve = next_ve;
-        fetch(window + 1, next_page, next_kf, next_ve);
+        old_codes = my_codes;
+        my_codes = codes_of(my_page);
+        next_page = bt[max(page_last - window * 32 - 32 - lane, page_first)];
       }
       const int page = __shfl_sync(0xffffffffu, my_page, idx & 31);
       const size_t at = page * page_bytes + (key & (ps - 1)) * kD;
@@ -256,54 +395,49 @@ __device__ __forceinline__ void tc_run(const Kv8Args& a, const Kv8Segment& s, in
         // (a round is 4 rows of 128 bytes or 8 of 64: only the first changes the swizzle, by bit 2 of the row)
         copy16((kD == 64 ? vdst : vdst ^ ((i & 1) << 6)) + b * (16 * kD) + i * 512, vp + i * 512);
       }
-      if (lane == (idx & 31))
-        asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(head + stage * 16 + b * 8), "f"(my_kf), "f"(my_ve) : "memory");
     }
   };
-  int loaded = 0;
-  if (n > 0) {
-    fetch(0, my_page, my_kf, my_ve);
-    if (page0 + 32 <= page_last) fetch(1, next_page, next_kf, next_ve);
-  }
-  if (!waited) {
-    const int newest = (s.ctx - 1) >> shift;             // the page that the kernel before this one may be writing to
 #pragma unroll 1
-    for (; loaded < min(n, kRing - 1) && (((sb0 + loaded) * kSub + kSub - 1) >> shift) < newest; ++loaded) {
-      issue(sb0 + loaded, loaded);
-      copies_commit();
-    }
-    pdl_wait();
-    waited = true;
-    if (n > 0 && page0 + window * 32 + 63 >= newest) {   // its scales are there now
-      fetch(window, my_page, my_kf, my_ve);
-      if (page0 + 32 <= page_last) fetch(window + 1, next_page, next_kf, next_ve);
-    }
-  }
-  if (n <= 0) return;
-#pragma unroll 1
-  for (; loaded < kRing - 1; ++loaded) {
-    if (loaded < n) issue(sb0 + loaded, loaded);
+  for (int i = 0; i < kRing - 1; ++i) {
+    if (i < n) issue(top - i, i);
     copies_commit();                                     // (a group to a sub-block, empty behind the last)
   }
-  uint32_t qf[KS][HI ? 4 : 2];
-  float factor[NR];
-  tc_load_q<HI>(a, s, lane, qf, factor);
+  const int token_page = __shfl_sync(0xffffffffu, my_page, 0);
+  bool mine = true;
+  if (store) {                                           // (of several items that name one page the first stores: see kv8_write_kernel)
+    for (int i = lane; i < s.item; i += 32) {
+      const int4 other = a.items[i];
+      if (other.z > 0 && a.block_table[static_cast<size_t>(other.y) * a.max_blocks + ((other.z - 1) >> shift)] == token_page) mine = false;
+    }
+    mine = __all_sync(0xffffffffu, mine);
+    if (!mine && token_page != 0 && lane == 0) atomicOr(a.status, 8);
+  }
+  uint32_t qf[NR][KS][2];
+  float factor[NR][2];
+  tc_make_q<HI>(a, q, lane, qf, factor);
+  if (store) {
+    copies_wait<kRing - 2>();
+    __syncwarp();
+    const uint32_t codes = tc_store_token(a, s, token_page, ring, lane, mine, token, __shfl_sync(0xffffffffu, my_codes, 0));
+    if (lane == 0) my_codes = codes;
+  }
 
-  // lane addresses: key 4 (g / 2) + g % 2 of K (so that a lane's scores are those of keys 4 t .. 4 t + 3), key lane of V
-  const uint32_t kr = 4 * (g >> 1) + (g & 1);
-  const uint32_t krow = kr * kD + (kD == 64 ? t : t ^ ((kr & 1) << 2)) * 16;
+  // lane addresses: key 4 (g / 2) + g % 2 of K and the one 2 further (so that the weights of keys 4 t .. 4 t + 3 meet in a lane
+  // once they are transposed), key lane of V
+  const uint32_t kr = 4 * (lane >> 3) + ((lane >> 2) & 1);
+  const uint32_t krow = kr * kD + (kD == 64 ? lane & 3 : (lane & 3) ^ ((kr & 1) << 2)) * 16;
   const uint32_t vrow = lane * kD, vsw = kD == 64 ? (lane >> 1) & 3 : lane & 7;
   int stage = 0, ahead = kRing - 1;
 #pragma unroll 1
   for (int i = 0; i < n; ++i) {
-    const int k0 = (sb0 + i) * kSub;
+    const int k0 = (top - i) * kSub;
     copies_wait<kRing - 2>();
     __syncwarp();                                        // (every lane's copies; and every lane is through with the sub-block before)
-    if (i + kRing - 1 < n) issue(sb0 + i + kRing - 1, ahead);
+    if (i + kRing - 1 < n) issue(top - i - (kRing - 1), ahead);
     copies_commit();
     const uint32_t kst = ring + stage * (2 * kSubBytes) + krow, vst = ring + stage * (2 * kSubBytes) + kSubBytes + vrow;
-    const uint4 hd = lds16(head + stage * 16);
-    const float kf[2] = {__uint_as_float(hd.x), __uint_as_float(hd.z)}, ve[2] = {__uint_as_float(hd.y), __uint_as_float(hd.w)};
+    ahead = stage;
+    stage = stage + 1 == kRing ? 0 : stage + 1;
     const bool whole = k0 >= s.key_lo && k0 + kSub <= s.key_hi;
     if (!whole) {
       // a key that is not seen may hold anything, what is not a number included: its weight of 0 does not cover that
@@ -315,134 +449,195 @@ __device__ __forceinline__ void tc_run(const Kv8Args& a, const Kv8Segment& s, in
       }
       __syncwarp();
     }
-    ahead = stage;
-    stage = stage + 1 == kRing ? 0 : stage + 1;
-    // ---- S: rows g (and g + 8), keys 16 (nt / 2) + 4 t + 2 (nt % 2) + e
-    float sv[4][4];
+    // ---- S: 16 keys b (rows 4 (g / 2) + g % 2, and 2 further: c0 and c2), heads 8 h + 2 t (c0) and 8 h + 2 t + 1
+    float sv[2][NR][4];
 #pragma unroll
-    for (int nt = 0; nt < 4; ++nt) {
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int c = 0; c < KS / 4; ++c) {
-        const uint4 kw = lds16((c ? kst ^ 64u : kst) + ((nt >> 1) * 16 + (nt & 1) * 2) * kD);
-        const uint32_t w[4] = {kw.x, kw.y, kw.z, kw.w};
+        const uint4 k0w = lds16((c ? kst ^ 64u : kst) + b * 16 * kD), k1w = lds16((c ? kst ^ 64u : kst) + (b * 16 + 2) * kD);
+        const uint32_t w0[4] = {k0w.x, k0w.y, k0w.z, k0w.w}, w1[4] = {k1w.x, k1w.y, k1w.z, k1w.w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const uint32_t* q = qf[c * 4 + k];
-          uint32_t b0, b1;
-          halves4(w[k], b0, b1);
-          if (c == 0 && k == 0) mma_f16_first(sv[nt], q[0], HI ? q[1] : 0u, q[HI ? 2 : 1], HI ? q[HI ? 3 : 0] : 0u, b0, b1);
-          else mma_f16(sv[nt], q[0], HI ? q[1] : 0u, q[HI ? 2 : 1], HI ? q[HI ? 3 : 0] : 0u, b0, b1);
+          uint32_t a0, a1, a2, a3;
+          halves4(w0[k], a0, a2);
+          halves4(w1[k], a1, a3);
+#pragma unroll
+          for (int h = 0; h < NR; ++h) {
+            const uint32_t* q2 = qf[h][c * 4 + k];
+            if (c == 0 && k == 0) mma_f16_first(sv[b][h], a0, a1, a2, a3, q2[0], q2[1]);
+            else mma_f16(sv[b][h], a0, a1, a2, a3, q2[0], q2[1]);
+          }
         }
       }
-    }
-    // ---- V as B fragments: entries 16 c + g and 16 c + 8 + g, keys 4 t .. + 3 and 16 further
-    uint32_t v[kD / 16][4];
+    // ---- V^T as A fragments: entries 16 c + g and 16 c + 8 + g, keys 4 t .. + 3 and 16 further
+    uint32_t v[NC][4];
 #pragma unroll
-    for (int c = 0; c < kD / 16; ++c) ldmatrix_trans(v[c], vst + ((c ^ vsw) << 4));
+    for (int c = 0; c < NC; ++c) ldmatrix_trans(v[c], vst + ((c ^ vsw) << 4));
+    // the scales of the first and the second 16 keys (the copies are at most one window ahead)
+    float kf[2];
+    int ve[2];
+    bool odd = false;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int idx = page_of(k0 + b * 16);
+      const uint32_t c = __shfl_sync(0xffffffffu, (idx >> 5) == window ? my_codes : old_codes, idx & 31);
+      kf[b] = kv8_scale(c & 255);
+      ve[b] = static_cast<int>(c >> 8) - 127;
+      odd |= ve[b] == 128;
+    }
+    const int vref = max(st.vref, max(ve[0], ve[1]));
+    if (vref != st.vref) {                               // (the same for the warp)
+      const float f = kv8_exp2i(max(st.vref - vref, -127));
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int h = 0; h < NR; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) st.o[c][h][e] *= f;
+      st.vref = vref;
+    }
     if (!whole) {
 #pragma unroll
-      for (int nt = 0; nt < 4; ++nt)
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int key = k0 + b * 16 + static_cast<int>(kr) + 2 * r;
+          if (key < s.key_lo || key >= s.key_hi)
+#pragma unroll
+            for (int h = 0; h < NR; ++h) sv[b][h][2 * r] = sv[b][h][2 * r + 1] = -INFINITY;
+        }
+    }
+    float f[2][NR][2], y[2][NR][4];
+    bool grown = false;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int h = 0; h < NR; ++h) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int key = k0 + (nt >> 1) * 16 + t * 4 + (nt & 1) * 2 + e;
-          if (key < s.key_lo || key >= s.key_hi) {
-            sv[nt][e] = -INFINITY;
-            if (HI) sv[nt][2 + e] = -INFINITY;
+          f[b][h][e] = factor[h][e] * kf[b];
+          // (times -inf it has to be -inf; so small a factor makes every score 0)
+          if (f[b][h][e] < 1.2e-38f) f[b][h][e] = 1.2e-38f;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          y[b][h][e] = fmaf(sv[b][h][e], f[b][h][e & 1], -st.m[h][e & 1]);
+          grown |= y[b][h][e] > kTcGrow;
+        }
+      }
+    if (__any_sync(0xffffffffu, grown)) {                // (the first sub-block among them: the reference is -inf)
+#pragma unroll
+      for (int h = 0; h < NR; ++h)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float m = st.m[h][e];
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              y[b][h][2 * r + e] = sv[b][h][2 * r + e] * f[b][h][e];
+              m = fmaxf(m, y[b][h][2 * r + e]);
+            }
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+          const float alpha = m == st.m[h][e] ? 1.f : exp2_fast(st.m[h][e] - m);
+          st.m[h][e] = m;
+          st.l[h][e] *= alpha;
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            st.o[c][h][e] *= alpha;
+            st.o[c][h][2 + e] *= alpha;
           }
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) y[b][h][2 * r + e] -= m;
         }
     }
-    float alpha[NR];
-    uint32_t pf[2][4] = {};                              // the weights as A fragments of 16 keys each
+    // ---- the weights as B fragments: keys 4 t, 4 t + 1 and 4 t + 2, 4 t + 3 of head 8 h + g
+    uint32_t pf[2][NR][2];
 #pragma unroll
-    for (int h = 0; h < NR; ++h) {
-      float mx[2];
+    for (int b = 0; b < 2; ++b) {
+      float w = kv8_exp2i(max(ve[b] - vref + kTcBase, -127));
+      if (odd && ve[b] == 128) w = __uint_as_float(0x7fc00000u);
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        float f = factor[h] * kf[b];
-        f = f < 1.2e-38f ? 1.2e-38f : f;                 // (times -inf it has to be -inf; so small a factor makes every score 0)
+      for (int h = 0; h < NR; ++h)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) sv[2 * b + u][2 * h + e] *= f;
-        mx[b] = fmaxf(fmaxf(sv[2 * b][2 * h], sv[2 * b][2 * h + 1]), fmaxf(sv[2 * b + 1][2 * h], sv[2 * b + 1][2 * h + 1]));
-        mx[b] = fmaxf(mx[b], __shfl_xor_sync(0xffffffffu, mx[b], 1));
-        mx[b] = fmaxf(mx[b], __shfl_xor_sync(0xffffffffu, mx[b], 2));
-      }
-      const float m = fmaxf(st.m[h], fmaxf(mx[0], mx[1]));
-      const float dm = st.m[h] - m;                      // -inf the first time
-      const float d = fmaxf(st.d[h] + dm, fmaxf(mx[0] - m + ve[0], mx[1] - m + ve[1]));
-      alpha[h] = exp2_fast(st.d[h] + dm - d);
-      float sum = 0.f;
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        // (a block whose best score is 2^-112 of the row's best and whose scale is as many times larger would need more)
-        const float w = exp2_fast(fminf(ve[b] - d + 14.f, 126.f));
-        float p[4];
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float x = exp2_fast(sv[2 * b + u][2 * h + e] - m);
-            sum += x;
-            p[2 * u + e] = x * w;
-          }
-        pf[b][h] = pack_halves(p[0], p[1]);
-        pf[b][2 + h] = pack_halves(p[2], p[3]);
-      }
-      st.l[h] = st.l[h] * exp2_fast(dm) + sum;
-      st.m[h] = m;
-      st.d[h] = d;
-    }
-    if (__any_sync(0xffffffffu, alpha[0] != 1.f || (HI && alpha[NR - 1] != 1.f))) {
-#pragma unroll
-      for (int j = 0; j < NJ; ++j)
-#pragma unroll
-        for (int e = 0; e < (HI ? 4 : 2); ++e) st.o[j][e] *= alpha[HI ? e >> 1 : 0];
-    }
-    // ---- O += P V
-#pragma unroll
-    for (int c = 0; c < kD / 16; ++c)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        float* o = st.o[2 * c + u];
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          uint32_t b0, b1;
-          halves4(v[c][2 * b + u], b0, b1);
-          mma_f16(o, pf[b][0], pf[b][1], pf[b][2], pf[b][3], b0, b1);
+        for (int r = 0; r < 2; ++r) {
+          const float p0 = exp2_fast(y[b][h][2 * r]), p1 = exp2_fast(y[b][h][2 * r + 1]);
+          st.l[h][0] += p0;
+          st.l[h][1] += p1;
+          pf[b][h][r] = transposed(pack_halves(p0 * w, p1 * w));
         }
+    }
+    // ---- O^T += V^T P^T
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        uint32_t a0, a1, a2, a3;
+        halves4(v[c][2 * b], a0, a2);
+        halves4(v[c][2 * b + 1], a1, a3);
+#pragma unroll
+        for (int h = 0; h < NR; ++h) mma_f16(st.o[c][h], a0, a1, a2, a3, pf[b][h][0], pf[b][h][1]);
       }
   }
   copies_wait<0>();
 #pragma unroll
-  for (int h = 0; h < NR; ++h) {                         // the row's four lanes
-    st.l[h] += __shfl_xor_sync(0xffffffffu, st.l[h], 1);
-    st.l[h] += __shfl_xor_sync(0xffffffffu, st.l[h], 2);
-  }
+  for (int h = 0; h < NR; ++h)                           // the eight lanes of a head
 #pragma unroll
-  for (int j = 0; j < NJ; ++j)
+    for (int e = 0; e < 2; ++e)
 #pragma unroll
-    for (int e = 0; e < (HI ? 4 : 2); ++e) st.o[j][e] *= 6.103515625e-5f;        // 2^-14
+      for (int o = 4; o < 32; o <<= 1) st.l[h][e] += __shfl_xor_sync(0xffffffffu, st.l[h][e], o);
   __syncwarp();
 }
 
-// Adds up the partial results of warps [w0, w0 + nw) for head r, entry d (they are in the warps' rings).
-__device__ __forceinline__ Kv8Piece tc_fold(const unsigned char* smem, int w0, int nw, int r, int d) {
-  Kv8Piece sum;
-  for (int w = w0; w < w0 + nw; ++w)
-    sum.m = fmaxf(sum.m, (reinterpret_cast<const float*>(smem + w * kRingBytes) + r * kPartLd)[kD + 1]);
-  for (int w = w0; w < w0 + nw; ++w) {
-    const float* p = reinterpret_cast<const float*>(smem + w * kRingBytes) + r * kPartLd;
-    sum.d = fmaxf(sum.d, p[kD] + (p[kD + 1] - sum.m));
+// The partial results of a group's warps (in their rings: `first` is the first one's), added up in order.  The group's `gsize` warps
+// call it together, after a barrier; `bar` is its named barrier.  put(r, d, sums of entries d .. d + 3, m, d, denominator).
+__device__ __forceinline__ void tc_group_barrier(int bar, int gsize) {
+  asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(gsize * 32) : "memory");
+}
+template <typename Put>
+__device__ __forceinline__ void tc_fold(unsigned char* first, int gsize, int wg, int lane, int bar, int G, Put put) {
+  // weights: a warp to a head, a lane to a partial result
+  for (int r = wg; r < G; r += gsize) {
+    float* p = reinterpret_cast<float*>(first + min(lane, gsize - 1) * kRingBytes) + r * kPartLd + kD;
+    const float d = p[0], m = p[1], l = lane < gsize ? p[2] : 0.f;
+    const bool none = m == -INFINITY && l == 0.f;        // (a warp without keys)
+    const float top = warp_max(m), dm = none ? 0.f : m - top;
+    const float dtop = warp_max(none ? -INFINITY : d + dm);
+    const float den = warp_sum(none ? 0.f : l * exp2f(dm));
+    __syncwarp();
+    if (lane < gsize) p[0] = none ? 0.f : exp2f(d + dm - dtop);
+    if (lane == 0) {
+      p[1] = top;
+      p[2] = dtop;
+      p[3] = den;
+    }
   }
-  for (int w = w0; w < w0 + nw; ++w) {
-    const float* p = reinterpret_cast<const float*>(smem + w * kRingBytes) + r * kPartLd;
-    if (p[kD + 1] == -INFINITY && p[kD + 2] == 0.f) continue;        // (a warp without keys)
-    const float dm = p[kD + 1] - sum.m;
-    sum.num += exp2f(p[kD] + dm - sum.d) * p[d];
-    sum.den += exp2f(dm) * p[kD + 2];
+  tc_group_barrier(bar, gsize);
+  for (int i = wg * 32 + lane; i < G * (kD / 4); i += gsize * 32) {
+    const int r = i / (kD / 4), d = (i - r * (kD / 4)) * 4;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int w = 0; w < gsize; ++w) {
+      const float* p = reinterpret_cast<const float*>(first + w * kRingBytes) + r * kPartLd;
+      const float f = p[kD];
+      const float4 x = *reinterpret_cast<const float4*>(p + d);
+      sum.x += f * x.x;
+      sum.y += f * x.y;
+      sum.z += f * x.z;
+      sum.w += f * x.w;
+    }
+    const float* p = reinterpret_cast<const float*>(first) + r * kPartLd + kD;
+    put(r, d, sum, p[1], p[2], p[3]);
   }
-  return sum;
+}
+// Four entries of a row's result.
+__device__ __forceinline__ void tc_put(const Kv8Args& a, const Kv8Segment& s, int r, int d, float4 num, float dd, float den) {
+  const float f = exp2f(dd) / den;
+  const float v[4] = {num.x * f, num.y * f, num.z * f, num.w * f};
+  store4(static_cast<bf16*>(a.out) + static_cast<size_t>(s.tok) * a.out_stride + (s.kvh * (a.hq / a.hkv) + r) * kD + d, v);
 }
 
 // groups: of the CTA's warps, a divisor of their number.  shares: the keys in equal shares (else: rows).
@@ -456,17 +651,11 @@ kv8_decode_tc_kernel(const Kv8Args a, int groups, int by_shares) {
   const int G = a.hq / a.hkv;
   const int csize = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_rank());
   const int gsize = kTcWarps / groups, gi = warp / gsize, wg = warp - gi * gsize;
-  const int gthreads = gsize * 32, gtid = wg * 32 + lane;
+  const int gtid = wg * 32 + lane;
   const int nclusters = gridDim.x / csize;
-  float* slots = reinterpret_cast<float*>(smem + kTcWarps * (kRingBytes + kHeadBytes));      // [csize][G][kD + 3], of the first CTA of a cluster
-  // With the rotation in this kernel the one before it is the write of the tokens' keys (launch_decode_tc), and what came
-  // before that is done: only the newest pages have to wait.  Without, anything may be under way.
-  if (csize > 1) cluster_arrive();                       // (met before the first store into another CTA: it has begun by then)
-  bool waited = false;
-  if (a.cos == nullptr) {
-    pdl_wait();
-    waited = true;
-  }
+  float* slots = reinterpret_cast<float*>(smem + kTcWarps * kRingBytes);      // [csize][G][kPartLd], of the first CTA of a cluster
+  if (csize > 1) cluster_arrive_begun();                       // (met before the first store into another CTA: it has begun by then)
+  pdl_wait();
   int units = 0, shares = 0, u = 0, end = 0;
   if (by_shares) {
     units = kv8_units(a, start);
@@ -507,68 +696,74 @@ kv8_decode_tc_kernel(const Kv8Args a, int groups, int by_shares) {
     const int W = csize * gsize, wi = rank * gsize + wg;
     const int first = s.key_lo / kSub, all = (s.key_hi - 1) / kSub - first + 1;
     const int per = all / W, rem = all - per * W;
-    TcState st;
-    tc_run<HI>(a, s, first + wi * per + min(wi, rem), per + (wi < rem ? 1 : 0), smem_addr(smem) + warp * kRingBytes,
-                      smem_addr(smem) + kTcWarps * kRingBytes + warp * kHeadBytes, lane, waited, st);
+    TcState<HI> st;
+    tc_run<HI>(a, s, first + wi * per + min(wi, rem), per + (wi < rem ? 1 : 0), smem_addr(smem) + warp * kRingBytes, lane, st);
     // ---- its partial result into its ring
     float* mine = reinterpret_cast<float*>(smem + warp * kRingBytes);
     const int g = lane >> 2, t = lane & 3;
 #pragma unroll
-    for (int h = 0; h < (HI ? 2 : 1); ++h) {
-      const int r = g + 8 * h;
-      if (r < G) {
+    for (int h = 0; h < (HI ? 2 : 1); ++h)
 #pragma unroll
-        for (int j = 0; j < kD / 8; ++j)
-          *reinterpret_cast<float2*>(mine + r * kPartLd + 8 * j + 2 * t) = make_float2(st.o[j][2 * h], st.o[j][2 * h + 1]);
-        if (t == 0) {
-          mine[r * kPartLd + kD] = st.d[h];
-          mine[r * kPartLd + kD + 1] = st.m[h];
-          mine[r * kPartLd + kD + 2] = st.l[h];
+      for (int e = 0; e < 2; ++e) {
+        const int r = 8 * h + 2 * t + e;
+        if (r >= G) continue;
+#pragma unroll
+        for (int c = 0; c < kD / 16; ++c) {
+          mine[r * kPartLd + 16 * c + g] = st.o[c][h][e];
+          mine[r * kPartLd + 16 * c + 8 + g] = st.o[c][h][2 + e];
         }
+        if (g == 0) *reinterpret_cast<float4*>(mine + r * kPartLd + kD) = make_float4(static_cast<float>(st.vref - kTcBase), st.m[h][e], st.l[h][e], 0.f);
       }
-    }
     if (csize > 1) {
       // ---- the CTA's sums into a slot of the cluster's first CTA, which adds the slots in order
       __syncthreads();
       cluster_wait();
-      for (int i = threadIdx.x; i < G * kD; i += kTcThreads) {
-        const int r = i / kD, d = i - r * kD;
-        const Kv8Piece x = tc_fold(smem, 0, kTcWarps, r, d);
-        float* slot = slots + (rank * G + r) * (kD + 3);
-        store_cluster(slot + d, 0, x.num);
-        if (d == 0) {
-          store_cluster(slot + kD, 0, x.d);
-          store_cluster(slot + kD + 1, 0, x.m);
-          store_cluster(slot + kD + 2, 0, x.den);
-        }
-      }
+      tc_fold(smem, kTcWarps, warp, lane, 1, G, [&](int r, int d, float4 num, float m, float dd, float den) {
+        float* slot = slots + (rank * G + r) * kPartLd;
+        store_cluster(slot + d, 0, num);
+        if (d == 0) store_cluster(slot + kD, 0, make_float4(dd, m, den, 0.f));
+      });
       cluster_arrive();
       cluster_wait();
       if (rank == 0)
-        for (int i = threadIdx.x; i < G * kD; i += kTcThreads) {
-          const int r = i / kD, d = i - r * kD;
-          Kv8Piece x;
+        for (int i = threadIdx.x; i < G * (kD / 4); i += kTcThreads) {
+          const int r = i / (kD / 4), d = (i - r * (kD / 4)) * 4;
+          float top = -INFINITY, dtop = -INFINITY, den = 0.f;
+          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int c = 0; c < csize; ++c) top = fmaxf(top, slots[(c * G + r) * kPartLd + kD + 1]);
           for (int c = 0; c < csize; ++c) {
-            const float* p = slots + (c * G + r) * (kD + 3);
-            x.add(p[kD], p[kD + 1], p[kD + 2], p[d]);
+            const float* p = slots + (c * G + r) * kPartLd + kD;
+            if (p[2] != 0.f) dtop = fmaxf(dtop, p[0] + (p[1] - top));
           }
-          static_cast<bf16*>(a.out)[static_cast<size_t>(s.tok) * a.out_stride + (s.kvh * G + r) * kD + d] = __float2bfloat16_rn(x.value());
+          for (int c = 0; c < csize; ++c) {
+            const float* p = slots + (c * G + r) * kPartLd;
+            if (p[kD + 2] == 0.f) continue;              // (a CTA without keys)
+            const float dm = p[kD + 1] - top, f = exp2f(p[kD] + dm - dtop);
+            den += p[kD + 2] * exp2f(dm);
+            const float4 x = *reinterpret_cast<const float4*>(p + d);
+            sum.x += f * x.x;
+            sum.y += f * x.y;
+            sum.z += f * x.z;
+            sum.w += f * x.w;
+          }
+          tc_put(a, s, r, d, sum, dtop, den);
         }
       continue;                                          // (one row to a cluster: see the launch)
     }
-    asm volatile("bar.sync %0, %1;" ::"r"(1 + gi), "r"(gthreads) : "memory");
-    float* piece = by_shares && !s.whole ? a.part + (static_cast<size_t>(share) * 2 + (u == share_first ? 0 : 1)) * (G * (kD + 3)) : nullptr;
-    for (int i = gtid; i < G * kD; i += gthreads) {
-      const int r = i / kD, d = i - r * kD;
-      const Kv8Piece x = tc_fold(smem, gi * gsize, gsize, r, d);
-      if (piece == nullptr)
-        static_cast<bf16*>(a.out)[static_cast<size_t>(s.tok) * a.out_stride + (s.kvh * G + r) * kD + d] = __float2bfloat16_rn(x.value());
-      else
-        kv8_leave(piece + r * (kD + 3), kD, d, x);
-    }
+    tc_group_barrier(1 + gi, gsize);
+    float* piece = by_shares && !s.whole ? a.part + (static_cast<size_t>(share) * 2 + (u == share_first ? 0 : 1)) * (G * (kD + 4)) : nullptr;
+    tc_fold(smem + gi * gsize * kRingBytes, gsize, wg, lane, 1 + gi, G, [&](int r, int d, float4 num, float m, float dd, float den) {
+      if (piece == nullptr) {
+        tc_put(a, s, r, d, num, dd, den);
+      } else {
+        float* p = piece + r * (kD + 4);
+        *reinterpret_cast<float4*>(p + d) = num;
+        if (d == 0) *reinterpret_cast<float4*>(p + kD) = make_float4(dd, m, den, 0.f);
+      }
+    });
     if (piece != nullptr) {
       __threadfence();                                   // the piece, before it is counted
-      asm volatile("bar.sync %0, %1;" ::"r"(1 + gi), "r"(gthreads) : "memory");
+      tc_group_barrier(1 + gi, gsize);
       if (gtid == 0) {
         const int pieces = kv8_share_of(s.row_end - 1, units, shares) - kv8_share_of(s.row_begin, units, shares) + 1;
         int* c = a.counters + static_cast<size_t>(s.item) * a.hkv + s.kvh;
@@ -576,16 +771,15 @@ kv8_decode_tc_kernel(const Kv8Args a, int groups, int by_shares) {
         if (done) *c = 0;
         last[gi] = done;
       }
-      asm volatile("bar.sync %0, %1;" ::"r"(1 + gi), "r"(gthreads) : "memory");
+      tc_group_barrier(1 + gi, gsize);
       if (last[gi]) {
         __threadfence();
-        kv8_merge<bf16>(a, s, units, shares, gtid, gthreads);
+        kv8_merge<bf16>(a, s, units, shares, wg, gsize);
       }
     }
-    asm volatile("bar.sync %0, %1;" ::"r"(1 + gi), "r"(gthreads) : "memory");      // before the rings are used again
+    tc_group_barrier(1 + gi, gsize);                     // before the rings are used again
     if (by_shares) u = s.next;
   }
-  if (!waited) pdl_wait();                               // (nothing of this launch ends before what it follows)
 }
 
 }  // namespace rl

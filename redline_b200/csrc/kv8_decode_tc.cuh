@@ -135,196 +135,165 @@ struct TcState {
   int vref;                            // the exponent that the numerators' values are relative to (the same for the warp)
 };
 
-// What q needs from memory: asked for first, used when the copies are on their way.
-template <bool HI>
-struct TcQ {
-  uint4 raw[HI ? 2 : 1][kD / 32];                        // entries 64 c + 16 t .. + 15 of the heads g (and g + 8)
-  uint4 cs[4], sn[4];
+// A row of the token (a query head's, or its own key or value) is taken by 8 lanes, kRowPart entries d .. and as many D/2 further to a
+// lane, so that both entries of a rotated pair are there; four rows at a time.  What it takes is asked for before the first
+// copies and used when those are on their way.
+constexpr int kRowPart = kD / 16;
+struct TcRaw {
+  uint32_t lo[kRowPart / 2], hi[kRowPart / 2];
 };
-template <bool HI>
-__device__ __forceinline__ void tc_fetch_q(const Kv8Args& a, const Kv8Segment& s, int lane, TcQ<HI>& q) {
-  const int g = lane >> 2, t = lane & 3, G = a.hq / a.hkv;
+struct TcAngles {
+  float c[kRowPart], n[kRowPart];
+};
+template <int N>
+__device__ __forceinline__ void ldg_words(const void* p, uint32_t* v) {      // (volatile: asked for where it stands)
+  if constexpr (N == 2) {
+    asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "l"(p));
+  } else {
 #pragma unroll
-  for (int h = 0; h < (HI ? 2 : 1); ++h) {
-    const int r = g + 8 * h;
-    const uint4* row = reinterpret_cast<const uint4*>(static_cast<const bf16*>(a.q) + static_cast<size_t>(s.tok) * a.q_stride +
-                                                      (s.kvh * G + r) * kD + t * 16);
-#pragma unroll
-    for (int c = 0; c < kD / 32; ++c) {
-      q.raw[h][c] = make_uint4(0, 0, 0, 0);
-      if (r < G) q.raw[h][c] = ldg16(row + (c >> 1) * 8 + (c & 1));
+    for (int i = 0; i < N; i += 4) {
+      const uint4 x = ldg16(static_cast<const char*>(p) + i * 4);
+      v[i] = x.x;
+      v[i + 1] = x.y;
+      v[i + 2] = x.z;
+      v[i + 3] = x.w;
     }
   }
-  if (a.cos != nullptr) {
-    int pos = s.ctx - 1;
-    if (pos >= a.max_pos) {
-      if (lane == 0) atomicOr(a.status, 2);
-      pos = 0;
-    }
-    // entry i turns with i + D/2: at head size 64 that is lane t ^ 2's, at 128 the lane's own other piece
-    const size_t at = static_cast<size_t>(pos) * (kD / 2) + (kD == 64 ? t & 1 : t) * 16;
+}
+__device__ __forceinline__ void tc_fetch_row(const Kv8Args& a, const Kv8Segment& s, int head, int lane, TcRaw& r) {
+  const bf16* p = static_cast<const bf16*>(a.q) + static_cast<size_t>(s.tok) * a.q_stride + head * kD + (lane & 7) * kRowPart;
+  ldg_words<kRowPart / 2>(p, r.lo);
+  ldg_words<kRowPart / 2>(p + kD / 2, r.hi);
+}
+__device__ __forceinline__ void tc_fetch_angles(const Kv8Args& a, const Kv8Segment& s, int lane, TcAngles& t) {
+  const size_t at = static_cast<size_t>(s.ctx - 1 < a.max_pos ? s.ctx - 1 : 0) * (kD / 2) + (lane & 7) * kRowPart;
+  ldg_words<kRowPart>(a.cos + at, reinterpret_cast<uint32_t*>(t.c));
+  ldg_words<kRowPart>(a.sin + at, reinterpret_cast<uint32_t*>(t.n));
+}
+// (rounded as the write rounds them: kv8_rotate8)
+__device__ __forceinline__ void tc_make_row(const TcRaw& r, const TcAngles& t, bool turn, float* x0, float* x1) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      q.cs[e] = ldg16(a.cos + at + 4 * e);
-      q.sn[e] = ldg16(a.sin + at + 4 * e);
+  for (int e = 0; e < kRowPart; e += 2) {
+    x0[e] = __uint_as_float(r.lo[e / 2] << 16);
+    x0[e + 1] = __uint_as_float(r.lo[e / 2] & 0xffff0000u);
+    x1[e] = __uint_as_float(r.hi[e / 2] << 16);
+    x1[e + 1] = __uint_as_float(r.hi[e / 2] & 0xffff0000u);
+  }
+  if (turn) {
+#pragma unroll
+    for (int e = 0; e < kRowPart; ++e) {
+      const float lo = x0[e], hi = x1[e];
+      x0[e] = __fsub_rn(__fmul_rn(lo, t.c[e]), __fmul_rn(hi, t.n[e]));
+      x1[e] = __fadd_rn(__fmul_rn(hi, t.c[e]), __fmul_rn(lo, t.n[e]));
     }
   }
 }
 
-// q as B fragments (k step by k step: the column of head g, and of g + 8), rotated on the way if the tables are given, and
-// the factors of the exponents of the heads whose scores the lane has.
+// q of the segment's token as halves into `area` (shared memory, [heads][D]), scaled by a power of two per row to at most 256, and
+// the factors of the exponents behind them.  `row` is the lane's first row.
 template <bool HI>
-__device__ __forceinline__ void tc_make_q(const Kv8Args& a, const TcQ<HI>& q, int lane, uint32_t (*qf)[kD / 16][2], float (*factor)[2]) {
+__device__ __forceinline__ void tc_make_q(const Kv8Args& a, const Kv8Segment& s, int lane, uint32_t area, TcRaw& row, const TcAngles& t) {
   constexpr float kLog2e = 1.4426950408889634f;
-  constexpr int NC = kD / 64;
-  float cs[16], sn[16];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const uint32_t c[4] = {q.cs[e].x, q.cs[e].y, q.cs[e].z, q.cs[e].w}, s[4] = {q.sn[e].x, q.sn[e].y, q.sn[e].z, q.sn[e].w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      cs[4 * e + i] = __uint_as_float(c[i]);
-      sn[4 * e + i] = kD == 64 && (lane & 2) == 0 ? -__uint_as_float(s[i]) : __uint_as_float(s[i]);
-    }
-  }
-#pragma unroll
-  for (int h = 0; h < (HI ? 2 : 1); ++h) {
-    float x[NC][16];
-#pragma unroll
-    for (int c = 0; c < kD / 32; ++c) {
-      const uint32_t w[4] = {q.raw[h][c].x, q.raw[h][c].y, q.raw[h][c].z, q.raw[h][c].w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[c >> 1][(c & 1) * 8 + 2 * i] = __uint_as_float(w[i] << 16);
-        x[c >> 1][(c & 1) * 8 + 2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-      }
-    }
-    if (a.cos != nullptr) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        if constexpr (kD == 64) {
-          const float other = __shfl_xor_sync(0xffffffffu, x[0][e], 2);
-          x[0][e] = x[0][e] * cs[e] + other * sn[e];
-        } else {
-          const float lo = x[0][e], hi = x[NC - 1][e];
-          x[0][e] = lo * cs[e] - hi * sn[e];
-          x[NC - 1][e] = hi * cs[e] + lo * sn[e];
-        }
-      }
-    }
+  const int G = a.hq / a.hkv;
+  if (a.cos != nullptr && s.ctx > a.max_pos && lane == 0) atomicOr(a.status, 2);
+#pragma unroll 1
+  for (int r0 = 0; r0 < G; r0 += 4) {
+    const int r = min(r0 + (lane >> 3), G - 1);          // (lanes without a row of their own repeat the last)
+    float x0[kRowPart], x1[kRowPart];
+    tc_make_row(row, t, a.cos != nullptr, x0, x1);
+    if (r0 + 4 < G) tc_fetch_row(a, s, s.kvh * G + min(r + 4, G - 1), lane, row);
     // (the largest of the bits of the magnitudes is that of the magnitudes, and beyond the finite ones for what is not)
     uint32_t most = 0;
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
+    for (int e = 0; e < kRowPart; ++e)
+      most = max(most, max(__float_as_uint(x0[e]) & 0x7fffffffu, __float_as_uint(x1[e]) & 0x7fffffffu));
 #pragma unroll
-      for (int e = 0; e < 16; ++e) most = max(most, __float_as_uint(x[c][e]) & 0x7fffffffu);
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    for (int o = 1; o < 8; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
     const int ex = static_cast<int>(most >> 23);         // the largest entry is 1.m * 2^(ex - 127)
     const int up = ex == 0 ? 0 : min(134 - ex, 127);     // ... and is scaled to 1.m * 2^7
     const float mul = kv8_exp2i(max(up, -126));
     // (a row that is not finite is not a number, not a large one)
     const float f = ex == 255 ? __uint_as_float(0x7fc00000u) : a.scale * kLog2e * kv8_exp2i(-up);
+    const uint32_t at = area + r * (kD * 2) + (lane & 7) * (kRowPart * 2);
 #pragma unroll
-    for (int e = 0; e < 2; ++e) factor[h][e] = __shfl_sync(0xffffffffu, f, ((lane & 3) * 2 + e) * 4);
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        qf[h][c * 4 + k][0] = pack_halves(x[c][4 * k] * mul, x[c][4 * k + 1] * mul);
-        qf[h][c * 4 + k][1] = pack_halves(x[c][4 * k + 2] * mul, x[c][4 * k + 3] * mul);
-      }
+    for (int e = 0; e < kRowPart; e += 4) {
+      asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at + 2 * e), "r"(pack_halves(x0[e] * mul, x0[e + 1] * mul)),
+                   "r"(pack_halves(x0[e + 2] * mul, x0[e + 3] * mul)) : "memory");
+      asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at + kD + 2 * e), "r"(pack_halves(x1[e] * mul, x1[e + 1] * mul)),
+                   "r"(pack_halves(x1[e + 2] * mul, x1[e + 3] * mul)) : "memory");
+    }
+    asm volatile("st.shared.f32 [%0], %1;" ::"r"(area + (HI ? 16 : 8) * (kD * 2) + r * 4), "f"(f) : "memory");
   }
+  __syncwarp();
 }
 
-// The token's own key (lanes 0 .. D/16 - 1) and value (the next D/16): entries 8 c .. + 7 and those D/2 further, and the angles.
-struct TcToken {
-  uint4 x0, x1;
-  float cs[8], sn[8];
-};
-__device__ __forceinline__ void tc_fetch_token(const Kv8Args& a, const Kv8Segment& s, int lane, TcToken& x) {
-  constexpr int CH = kD / 16;
-  if (lane >= 2 * CH) return;
-  const int c = lane % CH;
-  const bf16* p = static_cast<const bf16*>(a.q) + static_cast<size_t>(s.tok) * a.q_stride +
-                  (a.hq + (lane < CH ? 0 : a.hkv) + s.kvh) * kD + c * 8;
-  x.x0 = ldg16(p);
-  x.x1 = ldg16(p + kD / 2);
-  const size_t at = static_cast<size_t>(s.ctx - 1 < a.max_pos ? s.ctx - 1 : 0) * (kD / 2) + c * 8;
-  load8(a.cos + at, x.cs);
-  load8(a.sin + at, x.sn);
-}
 // Where 16-byte piece ch of row r of a sub-block lies in its stage (K, V): the fragment reads are free of bank conflicts.
 __device__ __forceinline__ uint32_t tc_place(bool is_v, int r, int ch) {
   const int sw = kD == 64 ? (is_v ? (r >> 1) & 3 : 0) : (is_v ? r & 7 : (r & 1) << 2);
   return static_cast<uint32_t>((is_v ? kSubBytes : 0) + r * kD + ((ch ^ sw) << 4));
 }
-// Stores the token into its page, in the cache (if `mine`) and in the stage that holds the page.  codes: the bytes of the
-// page's scales (K, then V); they come back as they are now.
+// Stores the token's key (lanes 0 .. 7) and value (8 .. 15; the others repeat) into its page, in the cache (if `mine`) and in the stage that
+// holds the page.  codes: the bytes of the page's scales (K, then V); they come back as they are now.
 __device__ __forceinline__ uint32_t tc_store_token(const Kv8Args& a, const Kv8Segment& s, int page, uint32_t stage, int lane, bool mine,
-                                                   const TcToken& token, uint32_t codes) {
+                                                   const TcRaw& token, const TcAngles& t, uint32_t codes) {
   constexpr int CH = kD / 16;
   const int ps = 1 << a.page_shift, pos = s.ctx - 1, off = pos & (ps - 1), row = pos % kSub, row0 = row - off;
-  float amax = 0.f, x0[8] = {}, x1[8] = {};
-  if (lane < 2 * CH) {
-    load16(reinterpret_cast<const bf16*>(&token.x0), x0);
-    load16(reinterpret_cast<const bf16*>(&token.x1), x1);
-    if (lane < CH) kv8_rotate8(x0, x1, token.cs, token.sn);
-  }
+  const int which = (lane >> 3) & 1;
+  float x0[kRowPart], x1[kRowPart], amax = 0.f;
+  tc_make_row(token, t, which == 0, x0, x1);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
+  for (int e = 0; e < kRowPart; ++e) {
     const float u = fabsf(x0[e]), v = fabsf(x1[e]);
     amax = fmaxf(amax, fmaxf(u < INFINITY ? u : 0.f, v < INFINITY ? v : 0.f));
   }
 #pragma unroll
-  for (int o = 1; o < CH; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  for (int o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
   const size_t block = static_cast<size_t>(page) * a.hkv + s.kvh;
-  uint32_t now = 0;
+  const int old = min(static_cast<int>((codes >> (8 * which)) & 255), 254);
+  int code = kv8_code(amax);
+  if (off > 0) code = max(code, old);
+  const int kcode = __shfl_sync(0xffffffffu, code, 0), vcode = __shfl_sync(0xffffffffu, code, 8);
+  if (off > 0) {                                         // what is in the page goes over to a larger scale
+#pragma unroll 1
+    for (int is_v = 0; is_v < 2; ++is_v) {
+      const int was = min(static_cast<int>((codes >> (8 * is_v)) & 255), 254), now = is_v ? vcode : kcode;
+      if (now == was) continue;
+      uint4* base = reinterpret_cast<uint4*>(const_cast<uint8_t*>(is_v ? a.vcache : a.kcache) + block * ps * kD);
+      const float f = kv8_exp2i(max(was - now, -127));
+#pragma unroll 1
+      for (int c = lane; c < off * CH; c += 32) {
+        const uint32_t at = stage + tc_place(is_v, row0 + c / CH, c % CH);
+        float y[16];
+        kv8_f16(lds16(at), y);
 #pragma unroll
-  for (int is_v = 0; is_v < 2; ++is_v) {
-    uint8_t* base = const_cast<uint8_t*>(is_v ? a.vcache : a.kcache) + block * ps * kD;
-    const int old = min(static_cast<int>((codes >> (8 * is_v)) & 255), 254);
-    int code = kv8_code(__shfl_sync(0xffffffffu, amax, is_v * CH));
-    if (off > 0) {
-      if (code > old) {                          // what is in the page goes over to the larger scale
-        const float f = kv8_exp2i(max(old - code, -127));
-        for (int c = lane; c < off * CH; c += 32) {
-          const uint32_t at = stage + tc_place(is_v, row0 + c / CH, c % CH);
-          float y[16];
-          kv8_f16(lds16(at), y);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) y[e] *= f;
-          const uint4 w = make_uint4(kv8_pack4(y), kv8_pack4(y + 4), kv8_pack4(y + 8), kv8_pack4(y + 12));
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
-          if (mine) *(reinterpret_cast<uint4*>(base) + c) = w;
-        }
-      } else {
-        code = old;
+        for (int e = 0; e < 16; ++e) y[e] *= f;
+        const uint4 w = make_uint4(kv8_pack4(y), kv8_pack4(y + 4), kv8_pack4(y + 8), kv8_pack4(y + 12));
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
+        if (mine) base[c] = w;
       }
     }
-    if (mine && lane == 0) const_cast<uint8_t*>(is_v ? a.vscale : a.kscale)[block] = static_cast<uint8_t>(code);
-    if (lane >= is_v * CH && lane < (is_v + 1) * CH) {
-      const int c = lane - is_v * CH;
-      const float inv = kv8_exp2i(127 - code);
+  }
+  if (lane < 16) {
+    const float inv = kv8_exp2i(127 - code);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x0[e] = fabsf(x0[e]) < INFINITY ? x0[e] * inv : __uint_as_float(0x7fc00000u);
-        x1[e] = fabsf(x1[e]) < INFINITY ? x1[e] * inv : __uint_as_float(0x7fc00000u);
-      }
-      const uint2 lo = make_uint2(kv8_pack4(x0), kv8_pack4(x0 + 4)), hi = make_uint2(kv8_pack4(x1), kv8_pack4(x1 + 4));
-      const uint32_t p0 = stage + tc_place(is_v, row, c >> 1) + (c & 1) * 8;
-      const uint32_t p1 = stage + tc_place(is_v, row, (c + CH) >> 1) + (c & 1) * 8;
-      asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(p0), "r"(lo.x), "r"(lo.y) : "memory");
-      asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(p1), "r"(hi.x), "r"(hi.y) : "memory");
-      if (mine) {
-        *reinterpret_cast<uint2*>(base + off * kD + c * 8) = lo;
-        *reinterpret_cast<uint2*>(base + off * kD + kD / 2 + c * 8) = hi;
-      }
+    for (int e = 0; e < kRowPart; ++e) {
+      x0[e] = fabsf(x0[e]) < INFINITY ? x0[e] * inv : __uint_as_float(0x7fc00000u);
+      x1[e] = fabsf(x1[e]) < INFINITY ? x1[e] * inv : __uint_as_float(0x7fc00000u);
     }
-    now |= static_cast<uint32_t>(code) << (8 * is_v);
+    uint8_t* dst = const_cast<uint8_t*>(which ? a.vcache : a.kcache) + (block * ps + off) * kD;
+#pragma unroll
+    for (int e = 0; e < kRowPart; e += 4)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int d = (lane & 7) * kRowPart + e + half * (kD / 2);
+        const uint32_t w = kv8_pack4((half ? x1 : x0) + e);
+        asm volatile("st.shared.u32 [%0], %1;" ::"r"(stage + tc_place(which, row, d >> 4) + (d & 15)), "r"(w) : "memory");
+        if (mine) *reinterpret_cast<uint32_t*>(dst + d) = w;
+      }
+    if (mine && (lane & 7) == 0) const_cast<uint8_t*>(which ? a.vscale : a.kscale)[block] = static_cast<uint8_t>(code);
   }
   __syncwarp();
-  return now;
+  return static_cast<uint32_t>(kcode) | static_cast<uint32_t>(vcode) << 8;
 }
 
 // The run of sub-blocks [sb0, sb0 + n) of the segment, the last one first, through the warp's ring.
@@ -354,10 +323,11 @@ __device__ __forceinline__ void tc_run(const Kv8Args& a, const Kv8Segment& s, in
   int window = 0, my_page = bt[max(page_last - lane, page_first)], next_page = 0;
   const int top = sb0 + n - 1;
   const bool store = a.store && s.key_hi == s.ctx && top == (s.ctx - 1) / kSub;      // the newest page is this warp's
-  TcQ<HI> q;
-  tc_fetch_q<HI>(a, s, lane, q);
-  TcToken token;
-  if (store) tc_fetch_token(a, s, lane, token);
+  TcRaw row, token;
+  TcAngles angles;
+  tc_fetch_row(a, s, s.kvh * (a.hq / a.hkv) + min(lane >> 3, a.hq / a.hkv - 1), lane, row);
+  if (a.cos != nullptr) tc_fetch_angles(a, s, lane, angles);
+  if (store) tc_fetch_row(a, s, a.hq + ((lane >> 3) & 1) * a.hkv + s.kvh, lane, token);
   auto codes_of = [&](int page) -> uint32_t {
     const size_t at = static_cast<size_t>(page) * a.hkv + s.kvh;
     return static_cast<uint32_t>(__ldcg(a.kscale + at)) | static_cast<uint32_t>(__ldcg(a.vscale + at)) << 8;
@@ -397,14 +367,10 @@ __device__ __forceinline__ void tc_run(const Kv8Args& a, const Kv8Segment& s, in
       }
     }
   };
-#pragma unroll 1
-  for (int i = 0; i < kRing - 1; ++i) {
-    if (i < n) issue(top - i, i);
-    copies_commit();                                     // (a group to a sub-block, empty behind the last)
-  }
   const int token_page = __shfl_sync(0xffffffffu, my_page, 0);
   bool mine = true;
   if (store) {                                           // (of several items that name one page the first stores: see kv8_write_kernel)
+#pragma unroll 1
     for (int i = lane; i < s.item; i += 32) {
       const int4 other = a.items[i];
       if (other.z > 0 && a.block_table[static_cast<size_t>(other.y) * a.max_blocks + ((other.z - 1) >> shift)] == token_page) mine = false;
@@ -412,31 +378,56 @@ __device__ __forceinline__ void tc_run(const Kv8Args& a, const Kv8Segment& s, in
     mine = __all_sync(0xffffffffu, mine);
     if (!mine && token_page != 0 && lane == 0) atomicOr(a.status, 8);
   }
-  uint32_t qf[NR][KS][2];
-  float factor[NR][2];
-  tc_make_q<HI>(a, q, lane, qf, factor);
-  if (store) {
-    copies_wait<kRing - 2>();
-    __syncwarp();
-    const uint32_t codes = tc_store_token(a, s, token_page, ring, lane, mine, token, __shfl_sync(0xffffffffu, my_codes, 0));
-    if (lane == 0) my_codes = codes;
-  }
-
   // lane addresses: key 4 (g / 2) + g % 2 of K and the one 2 further (so that the weights of keys 4 t .. 4 t + 3 meet in a lane
   // once they are transposed), key lane of V
   const uint32_t kr = 4 * (lane >> 3) + ((lane >> 2) & 1);
   const uint32_t krow = kr * kD + (kD == 64 ? lane & 3 : (lane & 3) ^ ((kr & 1) << 2)) * 16;
   const uint32_t vrow = lane * kD, vsw = kD == 64 ? (lane >> 1) & 3 : lane & 7;
-  int stage = 0, ahead = kRing - 1;
+  uint32_t qf[NR][KS][2];
+  float factor[NR][2];
+  int stage = 0, ahead = 0;
 #pragma unroll 1
-  for (int i = 0; i < n; ++i) {
+  for (int i = 1 - kRing; i < n; ++i) {
     const int k0 = (top - i) * kSub;
-    copies_wait<kRing - 2>();
-    __syncwarp();                                        // (every lane's copies; and every lane is through with the sub-block before)
+    if (i == 0) {                                        // the first copies are on their way: q, by way of the stage that is still free
+      const uint32_t area = ring + (kRing - 1) * (2 * kSubBytes);
+      tc_make_q<HI>(a, s, lane, area, row, angles);
+#pragma unroll
+      for (int h = 0; h < NR; ++h) {
+        const int r = (lane >> 2) + 8 * h;
+        const bool has = r < a.hq / a.hkv;
+#pragma unroll
+        for (int c = 0; c < KS / 4; ++c)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const uint4 x = lds16(area + r * (kD * 2) + c * 128 + (lane & 3) * 32 + u * 16);
+            qf[h][c * 4 + 2 * u][0] = has ? x.x : 0u;
+            qf[h][c * 4 + 2 * u][1] = has ? x.y : 0u;
+            qf[h][c * 4 + 2 * u + 1][0] = has ? x.z : 0u;
+            qf[h][c * 4 + 2 * u + 1][1] = has ? x.w : 0u;
+          }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int hd = 8 * h + (lane & 3) * 2 + e;
+          float f;
+          asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(area + (HI ? 16 : 8) * (kD * 2) + hd * 4));
+          factor[h][e] = hd < a.hq / a.hkv ? f : 0.f;
+        }
+      }
+    }
+    if (i >= 0) {
+      copies_wait<kRing - 2>();
+      __syncwarp();                                      // (every lane's copies; and every lane is through with the sub-block before)
+    }
+    if (i == 0 && store) {
+      const uint32_t codes = tc_store_token(a, s, token_page, ring, lane, mine, token, angles, __shfl_sync(0xffffffffu, my_codes, 0));
+      if (lane == 0) my_codes = codes;
+    }
     if (i + kRing - 1 < n) issue(top - i - (kRing - 1), ahead);
-    copies_commit();
+    ahead = ahead + 1 == kRing ? 0 : ahead + 1;
+    copies_commit();                                     // (a group to a sub-block, empty behind the last)
+    if (i < 0) continue;
     const uint32_t kst = ring + stage * (2 * kSubBytes) + krow, vst = ring + stage * (2 * kSubBytes) + kSubBytes + vrow;
-    ahead = stage;
     stage = stage + 1 == kRing ? 0 : stage + 1;
     const bool whole = k0 >= s.key_lo && k0 + kSub <= s.key_hi;
     if (!whole) {
@@ -593,23 +584,26 @@ __device__ __forceinline__ void tc_run(const Kv8Args& a, const Kv8Segment& s, in
   __syncwarp();
 }
 
-// The partial results of a group's warps (in their rings: `first` is the first one's), added up in order.  The group's `gsize` warps
-// call it together, after a barrier; `bar` is its named barrier.  put(r, d, sums of entries d .. d + 3, m, d, denominator).
 __device__ __forceinline__ void tc_group_barrier(int bar, int gsize) {
   asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(gsize * 32) : "memory");
 }
-template <typename Put>
-__device__ __forceinline__ void tc_fold(unsigned char* first, int gsize, int wg, int lane, int bar, int G, Put put) {
+// Adds up `n` partial results ([G][kPartLd] floats, `stride` bytes apart in shared memory; the first one's references are
+// overwritten) in order and leaves the sums: as the row's result (`out`; to == nullptr), as a partial result in global memory, or (rank >= 0)
+// in the shared memory of CTA `rank` of the cluster.  The `gsize` warps that call it meet at barrier `bar`.
+// (One piece of code for all of them, and little of it: code that a launch runs once comes from L2 or memory, a microsecond for some
+// hundreds of instructions.)
+__device__ __noinline__ void tc_fold(unsigned char* parts, int stride, int n, int wg, int gsize, int bar, int G, bf16* out, float* to, int rank) {
+  const int lane = threadIdx.x & 31;
   // weights: a warp to a head, a lane to a partial result
+#pragma unroll 1
   for (int r = wg; r < G; r += gsize) {
-    float* p = reinterpret_cast<float*>(first + min(lane, gsize - 1) * kRingBytes) + r * kPartLd + kD;
-    const float d = p[0], m = p[1], l = lane < gsize ? p[2] : 0.f;
-    const bool none = m == -INFINITY && l == 0.f;        // (a warp without keys)
-    const float top = warp_max(m), dm = none ? 0.f : m - top;
-    const float dtop = warp_max(none ? -INFINITY : d + dm);
-    const float den = warp_sum(none ? 0.f : l * exp2f(dm));
-    __syncwarp();
-    if (lane < gsize) p[0] = none ? 0.f : exp2f(d + dm - dtop);
+    float* p = reinterpret_cast<float*>(parts + min(lane, n - 1) * stride) + r * kPartLd + kD;
+    const float4 x = *reinterpret_cast<const float4*>(p);                // d, m, denominator
+    const bool none = lane >= n || (x.y == -INFINITY && x.z == 0.f);     // (a part without keys)
+    const float top = warp_max(x.y), dm = none ? 0.f : x.y - top;
+    const float dtop = warp_max(none ? -INFINITY : x.x + dm);
+    const float den = warp_sum(none ? 0.f : x.z * exp2_fast(dm));
+    if (lane < n) p[0] = none ? 0.f : exp2_fast(x.x + dm - dtop);
     if (lane == 0) {
       p[1] = top;
       p[2] = dtop;
@@ -617,27 +611,38 @@ __device__ __forceinline__ void tc_fold(unsigned char* first, int gsize, int wg,
     }
   }
   tc_group_barrier(bar, gsize);
+#pragma unroll 1
   for (int i = wg * 32 + lane; i < G * (kD / 4); i += gsize * 32) {
     const int r = i / (kD / 4), d = (i - r * (kD / 4)) * 4;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int w = 0; w < gsize; ++w) {
-      const float* p = reinterpret_cast<const float*>(first + w * kRingBytes) + r * kPartLd;
+    const float* p = reinterpret_cast<const float*>(parts) + r * kPartLd;
+    const float4 ref = *reinterpret_cast<const float4*>(p + kD);         // weight, m, d, denominator
+#pragma unroll 1
+    for (int w = 0; w < n; ++w) {
       const float f = p[kD];
       const float4 x = *reinterpret_cast<const float4*>(p + d);
+      p += stride / 4;
       sum.x += f * x.x;
       sum.y += f * x.y;
       sum.z += f * x.z;
       sum.w += f * x.w;
     }
-    const float* p = reinterpret_cast<const float*>(first) + r * kPartLd + kD;
-    put(r, d, sum, p[1], p[2], p[3]);
+    if (to == nullptr) {
+      const float f = __fdividef(exp2_fast(ref.z), ref.w);
+      const float v[4] = {sum.x * f, sum.y * f, sum.z * f, sum.w * f};
+      store4(out + r * kD + d, v);
+    } else {
+      float* q = to + r * kPartLd;
+      const float4 refs = make_float4(ref.z, ref.y, ref.w, 0.f);
+      if (rank >= 0) {
+        store_cluster(q + d, rank, sum);
+        if (d == 0) store_cluster(q + kD, rank, refs);
+      } else {
+        *reinterpret_cast<float4*>(q + d) = sum;
+        if (d == 0) *reinterpret_cast<float4*>(q + kD) = refs;
+      }
+    }
   }
-}
-// Four entries of a row's result.
-__device__ __forceinline__ void tc_put(const Kv8Args& a, const Kv8Segment& s, int r, int d, float4 num, float dd, float den) {
-  const float f = exp2f(dd) / den;
-  const float v[4] = {num.x * f, num.y * f, num.z * f, num.w * f};
-  store4(static_cast<bf16*>(a.out) + static_cast<size_t>(s.tok) * a.out_stride + (s.kvh * (a.hq / a.hkv) + r) * kD + d, v);
 }
 
 // groups: of the CTA's warps, a divisor of their number.  shares: the keys in equal shares (else: rows).
@@ -698,6 +703,7 @@ kv8_decode_tc_kernel(const Kv8Args a, int groups, int by_shares) {
     const int per = all / W, rem = all - per * W;
     TcState<HI> st;
     tc_run<HI>(a, s, first + wi * per + min(wi, rem), per + (wi < rem ? 1 : 0), smem_addr(smem) + warp * kRingBytes, lane, st);
+    bf16* out = static_cast<bf16*>(a.out) + static_cast<size_t>(s.tok) * a.out_stride + s.kvh * G * kD;
     // ---- its partial result into its ring
     float* mine = reinterpret_cast<float*>(smem + warp * kRingBytes);
     const int g = lane >> 2, t = lane & 3;
@@ -718,49 +724,15 @@ kv8_decode_tc_kernel(const Kv8Args a, int groups, int by_shares) {
       // ---- the CTA's sums into a slot of the cluster's first CTA, which adds the slots in order
       __syncthreads();
       cluster_wait();
-      tc_fold(smem, kTcWarps, warp, lane, 1, G, [&](int r, int d, float4 num, float m, float dd, float den) {
-        float* slot = slots + (rank * G + r) * kPartLd;
-        store_cluster(slot + d, 0, num);
-        if (d == 0) store_cluster(slot + kD, 0, make_float4(dd, m, den, 0.f));
-      });
+      tc_fold(smem, kRingBytes, kTcWarps, warp, kTcWarps, 1, G, nullptr, slots + rank * G * kPartLd, 0);
       cluster_arrive();
       cluster_wait();
-      if (rank == 0)
-        for (int i = threadIdx.x; i < G * (kD / 4); i += kTcThreads) {
-          const int r = i / (kD / 4), d = (i - r * (kD / 4)) * 4;
-          float top = -INFINITY, dtop = -INFINITY, den = 0.f;
-          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int c = 0; c < csize; ++c) top = fmaxf(top, slots[(c * G + r) * kPartLd + kD + 1]);
-          for (int c = 0; c < csize; ++c) {
-            const float* p = slots + (c * G + r) * kPartLd + kD;
-            if (p[2] != 0.f) dtop = fmaxf(dtop, p[0] + (p[1] - top));
-          }
-          for (int c = 0; c < csize; ++c) {
-            const float* p = slots + (c * G + r) * kPartLd;
-            if (p[kD + 2] == 0.f) continue;              // (a CTA without keys)
-            const float dm = p[kD + 1] - top, f = exp2f(p[kD] + dm - dtop);
-            den += p[kD + 2] * exp2f(dm);
-            const float4 x = *reinterpret_cast<const float4*>(p + d);
-            sum.x += f * x.x;
-            sum.y += f * x.y;
-            sum.z += f * x.z;
-            sum.w += f * x.w;
-          }
-          tc_put(a, s, r, d, sum, dtop, den);
-        }
+      if (rank == 0) tc_fold(reinterpret_cast<unsigned char*>(slots), G * kPartLd * 4, csize, warp, kTcWarps, 1, G, out, nullptr, -1);
       continue;                                          // (one row to a cluster: see the launch)
     }
     tc_group_barrier(1 + gi, gsize);
     float* piece = by_shares && !s.whole ? a.part + (static_cast<size_t>(share) * 2 + (u == share_first ? 0 : 1)) * (G * (kD + 4)) : nullptr;
-    tc_fold(smem + gi * gsize * kRingBytes, gsize, wg, lane, 1 + gi, G, [&](int r, int d, float4 num, float m, float dd, float den) {
-      if (piece == nullptr) {
-        tc_put(a, s, r, d, num, dd, den);
-      } else {
-        float* p = piece + r * (kD + 4);
-        *reinterpret_cast<float4*>(p + d) = num;
-        if (d == 0) *reinterpret_cast<float4*>(p + kD) = make_float4(dd, m, den, 0.f);
-      }
-    });
+    tc_fold(smem + gi * gsize * kRingBytes, kRingBytes, gsize, wg, gsize, 1 + gi, G, out, piece, -1);
     if (piece != nullptr) {
       __threadfence();                                   // the piece, before it is counted
       tc_group_barrier(1 + gi, gsize);

@@ -641,6 +641,7 @@ constexpr int kBQ = 32, kBK = 32, kPreThreads = 128;
 
 template <typename T>
 struct PrefillArgs {
+  static constexpr bool kEightBit = false;     // (what the kernel of prefill_tc.cuh goes by)
   const T* q;
   int q_stride;
   const T* kcache;
@@ -1343,7 +1344,7 @@ int launch_prefill(const void* q, int q_stride, const void* kc, const void* vc, 
         int n = 0;
         e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
         if (e == cudaSuccess)
-          e = cudaFuncSetAttribute(prefill_attn_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+          e = cudaFuncSetAttribute(prefill_attn_tc_kernel<PrefillArgs<bf16>>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                    static_cast<int>(kPrefillTcSmem));
         if (e != cudaSuccess) return static_cast<int>(e);
         tsms_of[dev] = n > 0 ? n : 1;
@@ -1351,7 +1352,7 @@ int launch_prefill(const void* q, int q_stride, const void* kc, const void* vc, 
       const int tsms = tsms_of[dev];
       const long long items = static_cast<long long>(tiles) * hkv * ((hq / hkv + 1) / 2);   // (tile, kv head, pair of heads)
       const int ctas = static_cast<int>(items < tsms ? items : tsms);      // persistent: one CTA per SM
-      launch_kernel(prefill_attn_tc_kernel, dim3(ctas), dim3(kTcThreads), kPrefillTcSmem, stream, a, tiles, status);
+      launch_kernel(prefill_attn_tc_kernel<PrefillArgs<bf16>>, dim3(ctas), dim3(kTcThreads), kPrefillTcSmem, stream, a, tiles, status);
       return static_cast<int>(cudaGetLastError());
     }
   }

@@ -528,19 +528,9 @@ kv8_decode_kernel(const Kv8Args a) {
   }
 }
 
-}  // namespace rl
-
-#if RL_HEAD_DIM == 64 || RL_HEAD_DIM == 128
-#include "kv8_decode_tc.cuh"
-#define RL_KV8_TC 1
-#endif
-
-namespace rl {
-
-// ------------------------------------------------------------------------------------------------ portions of prompts
-
 template <typename T>
 struct Kv8PrefillArgs {
+  static constexpr bool kEightBit = true;      // (what the kernel of prefill_tc.cuh goes by)
   const T* q;
   int q_stride;
   const uint8_t* kcache;
@@ -558,6 +548,18 @@ struct Kv8PrefillArgs {
   int hq, hkv, page_shift, window;
   float scale;
 };
+
+}  // namespace rl
+
+#if RL_HEAD_DIM == 64 || RL_HEAD_DIM == 128
+#include "kv8_decode_tc.cuh"
+#include "prefill_tc.cuh"
+#define RL_KV8_TC 1
+#endif
+
+namespace rl {
+
+// ------------------------------------------------------------------------------------------------ portions of prompts
 
 constexpr int kPR = 64, kPK = 64, kPreThreads = 256;      // query rows and keys of a tile
 constexpr int kPLd = 68;                                  // floats to a row of 64 in shared memory
@@ -778,7 +780,7 @@ struct TcDevice {
 };
 
 size_t tc_smem(int csize, int G) {
-  return static_cast<size_t>(kTcWarps) * kRingBytes + (csize > 1 ? sizeof(float) * csize * G * kPartLd : 0);
+  return static_cast<size_t>(kDecWarps) * kRingBytes + (csize > 1 ? sizeof(float) * csize * G * kPartLd : 0);
 }
 
 // What is asked of the device once.
@@ -807,7 +809,7 @@ int tc_device(const TcDevice** out) {
     for (int c = 1; c <= kMaxCluster; ++c) {
       cudaLaunchConfig_t q = {};
       q.gridDim = dim3(c);
-      q.blockDim = dim3(kTcThreads);
+      q.blockDim = dim3(kDecThreads);
       q.dynamicSmemBytes = tc_smem(c, 1);
       cudaLaunchAttribute at[1];
       at[0].id = cudaLaunchAttributeClusterDimension;
@@ -846,9 +848,9 @@ int launch_decode_tc(Kv8Args a, int max_ctx, long long sum_ctx, int impl, cudaSt
   // as few groups (a divisor of the warps) as give every row one at once, else a warp to a row
   int groups = 1;
   if (rows > resident) {
-    groups = kTcWarps;
-    for (int k = 2; k < kTcWarps; ++k)
-      if (kTcWarps % k == 0 && static_cast<long long>(resident) * k >= rows) {
+    groups = kDecWarps;
+    for (int k = 2; k < kDecWarps; ++k)
+      if (kDecWarps % k == 0 && static_cast<long long>(resident) * k >= rows) {
         groups = k;
         break;
       }
@@ -859,7 +861,7 @@ int launch_decode_tc(Kv8Args a, int max_ctx, long long sum_ctx, int impl, cudaSt
   const int clusters = static_cast<int>(wanted < resident || csize > 1 ? wanted : resident);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(clusters * csize);
-  cfg.blockDim = dim3(kTcThreads);
+  cfg.blockDim = dim3(kDecThreads);
   cfg.dynamicSmemBytes = tc_smem(csize, G);
   cfg.stream = stream;
   cudaLaunchAttribute at[2];
@@ -975,7 +977,7 @@ template <typename T>
 int launch_prefill(const void* q, int q_stride, const void* kc, const void* vc, const void* ks, const void* vs, const int32_t* bt,
                    int max_blocks, const int32_t* tile_seq, const int32_t* tile_tok, const int32_t* tile_rows,
                    const int32_t* positions, void* out, int out_stride, int tiles, int hq, int hkv, int page_size, int window,
-                   float scale, cudaStream_t stream) {
+                   float scale, int impl, int* status, cudaStream_t stream) {
   Kv8PrefillArgs<T> a;
   a.q = static_cast<const T*>(q);
   a.q_stride = q_stride;
@@ -1001,6 +1003,28 @@ int launch_prefill(const void* q, int q_stride, const void* kc, const void* vc, 
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return static_cast<int>(e);
   if (dev < 0 || dev >= kMaxDevices) return static_cast<int>(cudaErrorInvalidDevice);
+#ifdef RL_KV8_TC
+  if constexpr (sizeof(T) == 2) {
+    if (impl != 1) {
+      int sms = 0;
+      const int err = device_sms(&sms);
+      if (err) return err;
+      if (!attr_set[dev]) {
+        e = cudaFuncSetAttribute(prefill_attn_tc_kernel<Kv8PrefillArgs<bf16>>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 static_cast<int>(kPrefillTcSmem));
+        if (e == cudaSuccess)
+          e = cudaFuncSetAttribute(kv8_prefill_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kPreSmem));
+        if (e != cudaSuccess) return static_cast<int>(e);
+        attr_set[dev] = true;
+      }
+      const long long work = static_cast<long long>(tiles) * hkv * ((hq / hkv + 1) / 2);     // (tile, kv head, pair of heads)
+      launch_kernel(prefill_attn_tc_kernel<Kv8PrefillArgs<bf16>>, dim3(static_cast<unsigned>(work < sms ? work : sms)), dim3(kTcThreads),
+                    kPrefillTcSmem, stream, a, tiles, status);
+      return static_cast<int>(cudaGetLastError());
+    }
+  }
+#endif
+  if (impl > 1) return static_cast<int>(cudaErrorInvalidValue);
   if (!attr_set[dev]) {
     e = cudaFuncSetAttribute(kv8_prefill_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kPreSmem));
     if (e != cudaSuccess) return static_cast<int>(e);
@@ -1015,9 +1039,9 @@ int launch_prefill(const void* q, int q_stride, const void* kc, const void* vc, 
 extern "C" int rl_kv8_attn_prefill(int dtype, const void* q, int q_stride, const void* kc, const void* vc, const void* ks,
                                    const void* vs, const int32_t* bt, int max_blocks, const int32_t* tile_seq,
                                    const int32_t* tile_tok, const int32_t* tile_rows, const int32_t* positions, void* out,
-                                   int out_stride, int tiles, int hq, int hkv, int page_size, int window, float scale,
-                                   void* stream) {
+                                   int out_stride, int tiles, int hq, int hkv, int page_size, int window, float scale, int impl,
+                                   int* status, void* stream) {
   auto run = dtype == 0 ? launch_prefill<float> : launch_prefill<bf16>;
   return run(q, q_stride, kc, vc, ks, vs, bt, max_blocks, tile_seq, tile_tok, tile_rows, positions, out, out_stride, tiles, hq,
-             hkv, page_size, window, scale, static_cast<cudaStream_t>(stream));
+             hkv, page_size, window, scale, impl, status, static_cast<cudaStream_t>(stream));
 }

@@ -28,9 +28,11 @@
 //   shares  the launch's keys in equal shares, one to a group (kv8.cuh): for rows of very different lengths
 #pragma once
 
+#include "tma.cuh"
+
 namespace rl {
 
-constexpr int kTcWarps = kD == 64 ? 12 : 8, kTcThreads = kTcWarps * 32;
+constexpr int kDecWarps = kD == 64 ? 12 : 8, kDecThreads = kDecWarps * 32;
 constexpr int kSub = 32;                                 // keys of a sub-block
 constexpr int kSubBytes = kSub * kD;                     // K (or V) of one
 constexpr int kRing = kD == 64 ? 4 : 3;                  // (192 KB for all warps either way)
@@ -39,13 +41,16 @@ constexpr int kMaxCluster = 8;
 constexpr int kPartLd = kD + 4;                          // floats to a head in a warp's partial result: kd numerators, d, m, denominator
 static_assert(16 * kPartLd * 4 <= kRingBytes, "a warp's partial result lies in its own ring");
 
-__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-__device__ __forceinline__ void copy16(uint32_t smem, const void* gmem) {
+__device__ __forceinline__ void cp_async16_s(uint32_t smem, const void* gmem) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(smem), "l"(gmem));
 }
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+__device__ __forceinline__ void cp_async16_s(uint32_t smem, const void* gmem, bool pred) {
+  const int bytes = pred ? 16 : 0;   // src-size 0: the 16 bytes are zero-filled
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem), "l"(gmem), "r"(bytes));
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
 template <int N>
-__device__ __forceinline__ void copies_wait() {
+__device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ uint4 lds16(uint32_t addr) {
@@ -53,7 +58,7 @@ __device__ __forceinline__ uint4 lds16(uint32_t addr) {
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
   return v;
 }
-__device__ __forceinline__ float exp2_fast(float x) {
+__device__ __forceinline__ float ex2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
@@ -119,12 +124,12 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 // Four floats to this CTA's address p in CTA `rank` of the cluster.
 __device__ __forceinline__ void store_cluster(float* p, uint32_t rank, float4 v) {
   uint32_t remote;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_addr(p)), "r"(rank));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(p)), "r"(rank));
   asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(remote), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
 
-constexpr float kTcGrow = 10.f;        // log2 of how far a score may exceed the reference
-constexpr int kTcBase = 5;             // log2 of a weight at the reference: 2^15 at most
+constexpr float kDecGrow = 10.f;        // log2 of how far a score may exceed the reference
+constexpr int kDecBase = 5;             // log2 of a weight at the reference: 2^15 at most
 
 // One warp's result for its run.  Thread (g, t) holds entries 16 c + g (o[c][i][0 and 1]) and 16 c + 8 + g (2 and 3) of the heads
 // 8 i + 2 t and 8 i + 2 t + 1, and those heads' references and denominators (of its own keys until the end).
@@ -361,9 +366,9 @@ __device__ __forceinline__ void tc_run(const Kv8Args& a, const Kv8Segment& s, in
       const uint8_t *kp = kbase + at, *vp = vbase + at;
 #pragma unroll
       for (int i = 0; i < CPR / 2; ++i) {
-        copy16(kdst + b * (16 * kD) + i * 512, kp + i * 512);
+        cp_async16_s(kdst + b * (16 * kD) + i * 512, kp + i * 512);
         // (a round is 4 rows of 128 bytes or 8 of 64: only the first changes the swizzle, by bit 2 of the row)
-        copy16((kD == 64 ? vdst : vdst ^ ((i & 1) << 6)) + b * (16 * kD) + i * 512, vp + i * 512);
+        cp_async16_s((kD == 64 ? vdst : vdst ^ ((i & 1) << 6)) + b * (16 * kD) + i * 512, vp + i * 512);
       }
     }
   };
@@ -416,7 +421,7 @@ __device__ __forceinline__ void tc_run(const Kv8Args& a, const Kv8Segment& s, in
       }
     }
     if (i >= 0) {
-      copies_wait<kRing - 2>();
+      cp_async_wait<kRing - 2>();
       __syncwarp();                                      // (every lane's copies; and every lane is through with the sub-block before)
     }
     if (i == 0 && store) {
@@ -425,7 +430,7 @@ __device__ __forceinline__ void tc_run(const Kv8Args& a, const Kv8Segment& s, in
     }
     if (i + kRing - 1 < n) issue(top - i - (kRing - 1), ahead);
     ahead = ahead + 1 == kRing ? 0 : ahead + 1;
-    copies_commit();                                     // (a group to a sub-block, empty behind the last)
+    cp_async_commit();                                     // (a group to a sub-block, empty behind the last)
     if (i < 0) continue;
     const uint32_t kst = ring + stage * (2 * kSubBytes) + krow, vst = ring + stage * (2 * kSubBytes) + kSubBytes + vrow;
     stage = stage + 1 == kRing ? 0 : stage + 1;
@@ -514,7 +519,7 @@ __device__ __forceinline__ void tc_run(const Kv8Args& a, const Kv8Segment& s, in
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           y[b][h][e] = fmaf(sv[b][h][e], f[b][h][e & 1], -st.m[h][e & 1]);
-          grown |= y[b][h][e] > kTcGrow;
+          grown |= y[b][h][e] > kDecGrow;
         }
       }
     if (__any_sync(0xffffffffu, grown)) {                // (the first sub-block among them: the reference is -inf)
@@ -532,7 +537,7 @@ __device__ __forceinline__ void tc_run(const Kv8Args& a, const Kv8Segment& s, in
             }
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-          const float alpha = m == st.m[h][e] ? 1.f : exp2_fast(st.m[h][e] - m);
+          const float alpha = m == st.m[h][e] ? 1.f : ex2_approx(st.m[h][e] - m);
           st.m[h][e] = m;
           st.l[h][e] *= alpha;
 #pragma unroll
@@ -550,13 +555,13 @@ __device__ __forceinline__ void tc_run(const Kv8Args& a, const Kv8Segment& s, in
     uint32_t pf[2][NR][2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      float w = kv8_exp2i(max(ve[b] - vref + kTcBase, -127));
+      float w = kv8_exp2i(max(ve[b] - vref + kDecBase, -127));
       if (odd && ve[b] == 128) w = __uint_as_float(0x7fc00000u);
 #pragma unroll
       for (int h = 0; h < NR; ++h)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const float p0 = exp2_fast(y[b][h][2 * r]), p1 = exp2_fast(y[b][h][2 * r + 1]);
+          const float p0 = ex2_approx(y[b][h][2 * r]), p1 = ex2_approx(y[b][h][2 * r + 1]);
           st.l[h][0] += p0;
           st.l[h][1] += p1;
           pf[b][h][r] = transposed(pack_halves(p0 * w, p1 * w));
@@ -574,7 +579,7 @@ __device__ __forceinline__ void tc_run(const Kv8Args& a, const Kv8Segment& s, in
         for (int h = 0; h < NR; ++h) mma_f16(st.o[c][h], a0, a1, a2, a3, pf[b][h][0], pf[b][h][1]);
       }
   }
-  copies_wait<0>();
+  cp_async_wait<0>();
 #pragma unroll
   for (int h = 0; h < NR; ++h)                           // the eight lanes of a head
 #pragma unroll
@@ -602,8 +607,8 @@ __device__ __noinline__ void tc_fold(unsigned char* parts, int stride, int n, in
     const bool none = lane >= n || (x.y == -INFINITY && x.z == 0.f);     // (a part without keys)
     const float top = warp_max(x.y), dm = none ? 0.f : x.y - top;
     const float dtop = warp_max(none ? -INFINITY : x.x + dm);
-    const float den = warp_sum(none ? 0.f : x.z * exp2_fast(dm));
-    if (lane < n) p[0] = none ? 0.f : exp2_fast(x.x + dm - dtop);
+    const float den = warp_sum(none ? 0.f : x.z * ex2_approx(dm));
+    if (lane < n) p[0] = none ? 0.f : ex2_approx(x.x + dm - dtop);
     if (lane == 0) {
       p[1] = top;
       p[2] = dtop;
@@ -628,7 +633,7 @@ __device__ __noinline__ void tc_fold(unsigned char* parts, int stride, int n, in
       sum.w += f * x.w;
     }
     if (to == nullptr) {
-      const float f = __fdividef(exp2_fast(ref.z), ref.w);
+      const float f = __fdividef(ex2_approx(ref.z), ref.w);
       const float v[4] = {sum.x * f, sum.y * f, sum.z * f, sum.w * f};
       store4(out + r * kD + d, v);
     } else {
@@ -647,18 +652,18 @@ __device__ __noinline__ void tc_fold(unsigned char* parts, int stride, int n, in
 
 // groups: of the CTA's warps, a divisor of their number.  shares: the keys in equal shares (else: rows).
 template <bool HI>
-__global__ void __launch_bounds__(kTcThreads, 1)
+__global__ void __launch_bounds__(kDecThreads, 1)
 kv8_decode_tc_kernel(const Kv8Args a, int groups, int by_shares) {
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ int start[kMaxItems + 1];
-  __shared__ int last[kTcWarps];
+  __shared__ int last[kDecWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int G = a.hq / a.hkv;
   const int csize = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_rank());
-  const int gsize = kTcWarps / groups, gi = warp / gsize, wg = warp - gi * gsize;
+  const int gsize = kDecWarps / groups, gi = warp / gsize, wg = warp - gi * gsize;
   const int gtid = wg * 32 + lane;
   const int nclusters = gridDim.x / csize;
-  float* slots = reinterpret_cast<float*>(smem + kTcWarps * kRingBytes);      // [csize][G][kPartLd], of the first CTA of a cluster
+  float* slots = reinterpret_cast<float*>(smem + kDecWarps * kRingBytes);      // [csize][G][kPartLd], of the first CTA of a cluster
   if (csize > 1) cluster_arrive_begun();                       // (met before the first store into another CTA: it has begun by then)
   pdl_wait();
   int units = 0, shares = 0, u = 0, end = 0;
@@ -702,7 +707,7 @@ kv8_decode_tc_kernel(const Kv8Args a, int groups, int by_shares) {
     const int first = s.key_lo / kSub, all = (s.key_hi - 1) / kSub - first + 1;
     const int per = all / W, rem = all - per * W;
     TcState<HI> st;
-    tc_run<HI>(a, s, first + wi * per + min(wi, rem), per + (wi < rem ? 1 : 0), smem_addr(smem) + warp * kRingBytes, lane, st);
+    tc_run<HI>(a, s, first + wi * per + min(wi, rem), per + (wi < rem ? 1 : 0), smem_u32(smem) + warp * kRingBytes, lane, st);
     bf16* out = static_cast<bf16*>(a.out) + static_cast<size_t>(s.tok) * a.out_stride + s.kvh * G * kD;
     // ---- its partial result into its ring
     float* mine = reinterpret_cast<float*>(smem + warp * kRingBytes);
@@ -718,16 +723,16 @@ kv8_decode_tc_kernel(const Kv8Args a, int groups, int by_shares) {
           mine[r * kPartLd + 16 * c + g] = st.o[c][h][e];
           mine[r * kPartLd + 16 * c + 8 + g] = st.o[c][h][2 + e];
         }
-        if (g == 0) *reinterpret_cast<float4*>(mine + r * kPartLd + kD) = make_float4(static_cast<float>(st.vref - kTcBase), st.m[h][e], st.l[h][e], 0.f);
+        if (g == 0) *reinterpret_cast<float4*>(mine + r * kPartLd + kD) = make_float4(static_cast<float>(st.vref - kDecBase), st.m[h][e], st.l[h][e], 0.f);
       }
     if (csize > 1) {
       // ---- the CTA's sums into a slot of the cluster's first CTA, which adds the slots in order
       __syncthreads();
       cluster_wait();
-      tc_fold(smem, kRingBytes, kTcWarps, warp, kTcWarps, 1, G, nullptr, slots + rank * G * kPartLd, 0);
+      tc_fold(smem, kRingBytes, kDecWarps, warp, kDecWarps, 1, G, nullptr, slots + rank * G * kPartLd, 0);
       cluster_arrive();
       cluster_wait();
-      if (rank == 0) tc_fold(reinterpret_cast<unsigned char*>(slots), G * kPartLd * 4, csize, warp, kTcWarps, 1, G, out, nullptr, -1);
+      if (rank == 0) tc_fold(reinterpret_cast<unsigned char*>(slots), G * kPartLd * 4, csize, warp, kDecWarps, 1, G, out, nullptr, -1);
       continue;                                          // (one row to a cluster: see the launch)
     }
     tc_group_barrier(1 + gi, gsize);

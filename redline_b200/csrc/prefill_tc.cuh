@@ -1,6 +1,8 @@
 // Prompt-portion attention on the fifth-generation tensor cores (bfloat16, head size 64 or 128).
 //
-// Included by attention.cu.  An item of work is a tile of up to 128 consecutive query rows of one
+// Included by attention.cu, and by kv8.cu for a cache in 8 bits (the arguments' type says which: kEightBit; the loaders then bring
+// a tile's bytes through registers and leave them as bfloat16 times their page's scale, a power of two, so exactly).  Before it come
+// cp_async16_s, cp_async_commit, cp_async_wait and ex2_approx.  An item of work is a tile of up to 128 consecutive query rows of one
 // sequence for TWO query heads of one kv head (the last pair of an odd group has one): the two
 // heads are the CTA's two "slots", they attend to the same keys and values, so a K tile and a V
 // tile are brought into shared memory once for both.  Persistent CTAs (one per SM) take items
@@ -82,7 +84,8 @@ struct TcItem {
 };
 
 // Item `rem` of a tile of query rows: kv head rem / pairs, pair of heads rem % pairs.
-__device__ __forceinline__ TcItem tc_item(const PrefillArgs<bf16>& a, int tile, int rem, int pairs) {
+template <typename Args>
+__device__ __forceinline__ TcItem tc_item(const Args& a, int tile, int rem, int pairs) {
   TcItem w;
   const int G = a.hq / a.hkv;
   w.kvh = rem / pairs;
@@ -226,14 +229,16 @@ struct TcWalk {
   int round = 0, item = -1;
   int it = 0, g = 0, it1 = 0, g1 = 0;
   TcItem w;
-  __device__ __forceinline__ bool first(const PrefillArgs<bf16>& a, int n_items, int pairs, int tiles) {
+  template <typename Args>
+  __device__ __forceinline__ bool first(const Args& a, int n_items, int pairs, int tiles) {
     item = tc_next_item(round, n_items);
     if (item < 0) return false;
     w = load(a, item, pairs, tiles);
     return true;
   }
   // moves to the CTA's next item; false when there is none
-  __device__ __forceinline__ bool next(const PrefillArgs<bf16>& a, int n_items, int pairs, int tiles) {
+  template <typename Args>
+  __device__ __forceinline__ bool next(const Args& a, int n_items, int pairs, int tiles) {
     ++it;
     g += w.nt;
     if (w.two) {
@@ -244,15 +249,136 @@ struct TcWalk {
   }
   // Items are numbered longest first (a later tile of a sequence attends to more keys), the kv heads and
   // pairs of a tile next to each other, so that CTAs that run together share K and V in L2.
-  static __device__ __forceinline__ TcItem load(const PrefillArgs<bf16>& a, int item, int pairs, int tiles) {
+  template <typename Args>
+  static __device__ __forceinline__ TcItem load(const Args& a, int item, int pairs, int tiles) {
     const int per_tile = a.hkv * pairs;
     const int t = item / per_tile;
     return tc_item(a, tiles - 1 - t, item - t * per_tile, pairs);
   }
 };
 
+// The loaders of a cache in 8 bits: one warp K (and both Q), one V.  A tile's 16-byte pieces come through registers in batches of
+// eight a lane, the next batch on its way while one is converted (e4m3 to half, to float, times the scale, the upper 16 bits:
+// 6.5 instructions for two numbers) and stored where the copies of a 16-bit cache would have put it.  A page's scale comes with
+// its id, a tile ahead.
+template <typename Args>
+__device__ __forceinline__ void tc_load_eight_bit(const Args& a, PrefillTcShared* sh, unsigned char* q_s, unsigned char* k_s,
+                                                  unsigned char* v_s, bool is_v, int lane, int n_items, int pairs, int tiles) {
+  constexpr int P = kD / 16, RPI = 32 / P;               // pieces of a row; rows that the warp's lanes cover at once
+  constexpr int kBatch = 8, kBatches = kTcKeys / (RPI * kBatch), kBatchRows = RPI * kBatch;
+  const uint8_t* cache = is_v ? a.vcache : a.kcache;
+  const uint8_t* scales = is_v ? a.vscale : a.kscale;
+  unsigned char* stage0 = is_v ? v_s : k_s;
+  uint64_t* full = is_v ? sh->v_full : sh->k_full;
+  uint64_t* freed = is_v ? sh->v_free : sh->k_free;
+  const int shift = a.page_shift, ps_mask = (1 << shift) - 1;
+  const int piece = lane % P, rr = lane / P;             // piece of a row, row within a round
+  // the piece's two 16-byte chunks (2 piece and 2 piece + 1) lie in half chunk / 8 at place (chunk % 8) ^ (row % 8)
+  const uint32_t c_half = static_cast<uint32_t>(piece >> 2) * kTcHalfBytes;
+  const int c7 = (2 * piece) & 7;
+  bool ok = true;
+  TcWalk wk;
+  for (bool more = wk.first(a, n_items, pairs, tiles); more && ok; more = wk.next(a, n_items, pairs, tiles)) {
+    const TcItem& w = wk.w;
+    const int32_t* bt = a.block_table + static_cast<size_t>(w.seq) * a.max_blocks;
+    const int first = w.lo0 >> shift, last = (w.k_end - 1) >> shift;
+    // a tile's pages (at most eight: pages of 16 keys or more), one to a lane: its id and its scale
+    auto page_of = [&](int i) {
+      return bt[min(max(((w.k_begin + i * kTcKeys) >> shift) + (lane & 7), first), last)];
+    };
+    auto scale_of = [&](int page) { return scales[static_cast<size_t>(page) * a.hkv + w.kvh]; };
+    int page = page_of(0);
+    int next_page = w.nt > 1 ? page_of(1) : 0;
+    int code = scale_of(page);
+    bool q_pending = false;
+    if (!is_v) {
+      for (int s = 0; s < (w.two ? 2 : 1) && ok; ++s) {
+        const int n = s == 0 ? wk.it : wk.it1;           // the slot's items so far
+        ok = mbar_wait(&sh->q_free[s], (n & 1) ^ 1, &sh->abort);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        constexpr int CPR = kD / 8, QRI = 32 / CPR;
+        const int c = lane % CPR, qr = lane / CPR;
+        const uint32_t dst = smem_u32(q_s) + s * kTcTileBytes + static_cast<uint32_t>(c >> 3) * kTcHalfBytes;
+        for (int j = 0; j < kTcRows / QRI; ++j) {
+          const int r = j * QRI + qr;
+          const bool live = r < w.rows;
+          const bf16* src = a.q + static_cast<size_t>(w.tok0 + (live ? r : 0)) * a.q_stride + (w.head0 + s) * kD + c * 8;
+          cp_async16_s(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4), src, live);
+        }
+      }
+      if (!ok) break;
+      cp_async_commit();
+      q_pending = true;
+    }
+    uint4 raw[2][kBatch];
+    // asks for batch b of the tile that begins at key k0 (pages and scales of that tile in `pg`)
+    auto ask = [&](int k0, int b, int pg, uint4* v) {
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int row = b * kBatchRows + j * RPI + rr, key = k0 + row;
+        const size_t id = static_cast<size_t>(__shfl_sync(0xffffffffu, pg, ((k0 & ps_mask) + row) >> shift));
+        v[j] = make_uint4(0, 0, 0, 0);
+        if (key < w.k_end && key >= w.lo0)
+          v[j] = *reinterpret_cast<const uint4*>(cache + (((id * a.hkv + w.kvh) << shift) + (key & ps_mask)) * kD + piece * 16);
+      }
+    };
+    ask(w.k_begin, 0, page, raw[0]);
+    for (int i = 0; i < w.nt && ok; ++i) {
+      const int g = wk.g + i, b = g % kTcStages;
+      const int k0 = w.k_begin + i * kTcKeys;
+      const int next_code = i + 1 < w.nt ? scale_of(next_page) : 0;
+      const int after_page = i + 2 < w.nt ? page_of(i + 2) : 0;
+      ok = mbar_wait(&freed[b], ((g / kTcStages) & 1) ^ 1, &sh->abort);      // (a fresh barrier passes a wait on parity 1)
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      unsigned char* dst = stage0 + b * kTcTileBytes + c_half;
+      const float my_scale = kv8_scale(code);
+#pragma unroll
+      for (int n = 0; n < kBatches; ++n) {
+        if (n + 1 < kBatches) ask(k0, n + 1, page, raw[(n + 1) & 1]);
+        else if (i + 1 < w.nt) ask(k0 + kTcKeys, 0, next_page, raw[(n + 1) & 1]);
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          const int row = n * kBatchRows + j * RPI + rr;
+          const float f = __shfl_sync(0xffffffffu, my_scale, ((k0 & ps_mask) + row) >> shift);
+          const uint4 v = raw[n & 1][j];
+          const uint32_t in[4] = {v.x, v.y, v.z, v.w};
+          uint32_t out[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float x[4];
+            kv8_f4(in[e], x);
+            out[2 * e] = __byte_perm(__float_as_uint(x[0] * f), __float_as_uint(x[1] * f), 0x7632);
+            out[2 * e + 1] = __byte_perm(__float_as_uint(x[2] * f), __float_as_uint(x[3] * f), 0x7632);
+          }
+          *reinterpret_cast<uint4*>(dst + row * 128 + ((c7 ^ (row & 7)) << 4)) = make_uint4(out[0], out[1], out[2], out[3]);
+          *reinterpret_cast<uint4*>(dst + row * 128 + (((c7 + 1) ^ (row & 7)) << 4)) = make_uint4(out[4], out[5], out[6], out[7]);
+        }
+      }
+      if (q_pending) cp_async_wait<0>();
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) {
+        if (q_pending) {
+          mbar_arrive(&sh->q_full[0]);
+          if (w.two) mbar_arrive(&sh->q_full[1]);
+        }
+        mbar_arrive(&full[b]);
+      }
+      q_pending = false;
+      page = next_page;
+      next_page = after_page;
+      code = next_code;
+    }
+    if (q_pending) cp_async_wait<0>();                   // (left on an abort: no copy may outlive the CTA)
+  }
+  cp_async_wait<0>();
+}
+
+template <typename Args>
 __global__ void __launch_bounds__(kTcThreads, 1)
-prefill_attn_tc_kernel(const PrefillArgs<bf16> a, int tiles, int* status) {
+prefill_attn_tc_kernel(const Args a, int tiles, int* status) {
   static_assert(kD == 64 || kD == 128, "this kernel is written for head sizes 64 and 128");
   constexpr float kLog2e = 1.4426950408889634f;
   extern __shared__ unsigned char smem_raw[];
@@ -298,7 +424,10 @@ prefill_attn_tc_kernel(const PrefillArgs<bf16> a, int tiles, int* status) {
   pdl_launch();
   pdl_wait();        // q and the newest keys come from the kernels before this one
 
-  if (warp == kTcRowWarps || warp == kTcRowWarps + 1) {
+  if (Args::kEightBit && (warp == kTcRowWarps || warp == kTcRowWarps + 1)) {
+    if constexpr (Args::kEightBit) tc_load_eight_bit(a, sh, q_s, k_s, v_s, warp == kTcRowWarps + 1, lane, n_items, pairs, tiles);
+  } else if (warp == kTcRowWarps || warp == kTcRowWarps + 1) {
+    if constexpr (!Args::kEightBit) {
     // ------------------------------------------------------------------ loaders: one warp K (and both Q), one V
     const bool is_v = warp == kTcRowWarps + 1;
     const int ps_shift = __ffs(a.page_size) - 1, ps_mask = a.page_size - 1;
@@ -404,6 +533,7 @@ prefill_attn_tc_kernel(const PrefillArgs<bf16> a, int tiles, int* status) {
       }
     }
     hand_over(true);
+    }
   } else if (warp >= kTcRowWarps + 2) {
     // ------------------------------------------------------------------ MMA issue: lane 0 of one warp per slot
     // Each slot has an issuing thread of its own, so that neither slot's products ever wait for the

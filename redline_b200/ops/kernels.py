@@ -858,9 +858,10 @@ _kv8_part: Dict[Tuple[int, int], int] = {}
 def kv8_attn_prefill(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch.Tensor,
                      vscale: torch.Tensor, block_table: torch.Tensor, tile_seq: torch.Tensor, tile_tok: torch.Tensor,
                      tile_rows: torch.Tensor, positions: torch.Tensor, out: torch.Tensor, tiles: int, num_heads: int,
-                     num_kv_heads: int, head_dim: int, page_size: int, window: int, scale: float) -> None:
+                     num_kv_heads: int, head_dim: int, page_size: int, window: int, scale: float, impl: int = 0) -> None:
     """``attn_prefill`` over a cache in 8 bits (kv8_write): tiles of up to 128 consecutive query tokens of one sequence
-    (tile_seq, tile_tok, tile_rows); rows of ``out`` that no tile names are left as they were."""
+    (tile_seq, tile_tok, tile_rows); rows of ``out`` that no tile names are left as they were.  impl 0: the best kernel that
+    applies (bfloat16 at head sizes 64 and 128: tcgen05; else CUDA cores); 1: CUDA cores; 3: the tcgen05 kernel or an error."""
     what = "kv8_attn_prefill"
     _kv8_check(what, kcache, vcache, kscale, vscale, num_heads, num_kv_heads, head_dim, page_size)
     _kv8_rows(what, "q", q, q_stride, num_heads * head_dim, kcache)
@@ -879,12 +880,12 @@ def kv8_attn_prefill(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, vcach
         return
     f = _fn(_kv8(head_dim), "rl_kv8_attn_prefill",
             [c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
-             c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p])
+             c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p])
     with _on(kcache):
         _check(f(_code(q.dtype), q.data_ptr(), q_stride, kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(), vscale.data_ptr(),
                  block_table.data_ptr(), block_table.shape[1], tile_seq.data_ptr(), tile_tok.data_ptr(), tile_rows.data_ptr(),
                  positions.data_ptr(), out.data_ptr(), out.stride(0), tiles, num_heads, num_kv_heads, page_size, window,
-                 float(scale), _stream()), what)
+                 float(scale), impl, tc_status(q.device).data_ptr(), _stream()), what)
 
 
 # ------------------------------------------- row-wise kernels of blocks with norms on both sides

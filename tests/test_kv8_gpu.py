@@ -401,7 +401,8 @@ def tiles_of(segments):
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
 @pytest.mark.parametrize("heads,kv_heads,dim,page,window,segments", PROMPT)
-def test_prefill(heads, kv_heads, dim, page, window, segments, dtype):
+@pytest.mark.parametrize("impl", [0, 1])
+def test_prefill(heads, kv_heads, dim, page, window, segments, dtype, impl):
     lengths = [a + n for a, n in segments]
     cache, table = filled(lengths, heads, kv_heads, dim, page, seed=dim)
     g = torch.Generator().manual_seed(7)
@@ -413,7 +414,7 @@ def test_prefill(heads, kv_heads, dim, page, window, segments, dtype):
     scale = 1.0 / math.sqrt(dim)
     qg = q.to(DEV)
     kernels.kv8_attn_prefill(qg, qg.stride(0), *on_gpu(cache), table.to(DEV), seq, tok, rows, positions, out, len(seq), heads,
-                             kv_heads, dim, page, window, scale)
+                             kv_heads, dim, page, window, scale, impl=impl)
     assert kernels.tc_status(out.device).item() == 0
     k, v = P.values(cache[0], cache[2]), P.values(cache[1], cache[3])
     row = 0

@@ -1018,7 +1018,7 @@ int launch_prefill(const void* q, int q_stride, const void* kc, const void* vc, 
         attr_set[dev] = true;
       }
       const long long work = static_cast<long long>(tiles) * hkv * ((hq / hkv + 1) / 2);     // (tile, kv head, pair of heads)
-      launch_kernel(prefill_attn_tc_kernel<Kv8PrefillArgs<bf16>>, dim3(static_cast<unsigned>(work < sms ? work : sms)), dim3(kTcThreads),
+      launch_kernel(prefill_attn_tc_kernel<Kv8PrefillArgs<bf16>>, dim3(static_cast<unsigned>(work < sms ? work : sms)), dim3(kTcThreads8),
                     kPrefillTcSmem, stream, a, tiles, status);
       return static_cast<int>(cudaGetLastError());
     }

@@ -61,6 +61,14 @@ constexpr int kTcTmemCols = 512;
 constexpr int kTcColO = 256;                            // O of slot s at kTcColO + s * kD
 constexpr bool kTcOwnP = kD == 64;                      // P has tensor-memory columns of its own (else: over S)
 constexpr int kTcColP = 384;                            // with columns of its own: P of slot s at kTcColP + s * 64
+// A cache in 8 bits: as many loaders for K, and for V, as there are stages (one warp alone takes twice as long over a tile as the
+// rows).  A loader's tiles then all lie in one stage, and its waits for that stage see every phase: with more loaders than stages one
+// could be two phases ahead, which a wait on a parity does not tell from none.  Warps 8 .. 11, 14 and 15 load, 12 and 13 issue the
+// MMAs.  Sixteen warps begin with 128 registers a thread; the two warpgroups of rows take 160, the other two leave them 96:
+// 256 x (160 + 96) = 512 x 128.
+constexpr int kTcThreads8 = 512, kTcRowRegs8 = 160, kTcOtherRegs8 = 96, kTcLoaders8 = kTcStages;
+static_assert(kTcLoaders8 <= 3, "six warps load");
+static_assert(256 * (kTcRowRegs8 + kTcOtherRegs8) <= 512 * 128, "the launch's registers");
 constexpr float kTcGrow = 8.f;                          // log2 of the growth of a row's maximum that moves the reference
 
 struct PrefillTcShared {
@@ -257,15 +265,15 @@ struct TcWalk {
   }
 };
 
-// The loaders of a cache in 8 bits: one warp K (and both Q), one V.  A tile's 16-byte pieces come through registers in batches of
-// eight a lane, the next batch on its way while one is converted (e4m3 to half, to float, times the scale, the upper 16 bits:
+// The loaders of a cache in 8 bits: some warps K (the first of them both Q, too), as many V, a tile to each in turn.  A tile's
+// 16-byte pieces come through registers in batches of four a lane, the next batch on its way while one is converted (e4m3 to half, to float, times the scale, the upper 16 bits:
 // 6.5 instructions for two numbers) and stored where the copies of a 16-bit cache would have put it.  A page's scale comes with
 // its id, a tile ahead.
 template <typename Args>
 __device__ __forceinline__ void tc_load_eight_bit(const Args& a, PrefillTcShared* sh, unsigned char* q_s, unsigned char* k_s,
-                                                  unsigned char* v_s, bool is_v, int lane, int n_items, int pairs, int tiles) {
+                                                  unsigned char* v_s, bool is_v, int turn, int lane, int n_items, int pairs, int tiles) {
   constexpr int P = kD / 16, RPI = 32 / P;               // pieces of a row; rows that the warp's lanes cover at once
-  constexpr int kBatch = 8, kBatches = kTcKeys / (RPI * kBatch), kBatchRows = RPI * kBatch;
+  constexpr int kBatch = 4, kBatches = kTcKeys / (RPI * kBatch), kBatchRows = RPI * kBatch;
   const uint8_t* cache = is_v ? a.vcache : a.kcache;
   const uint8_t* scales = is_v ? a.vscale : a.kscale;
   unsigned char* stage0 = is_v ? v_s : k_s;
@@ -287,11 +295,12 @@ __device__ __forceinline__ void tc_load_eight_bit(const Args& a, PrefillTcShared
       return bt[min(max(((w.k_begin + i * kTcKeys) >> shift) + (lane & 7), first), last)];
     };
     auto scale_of = [&](int page) { return scales[static_cast<size_t>(page) * a.hkv + w.kvh]; };
-    int page = page_of(0);
-    int next_page = w.nt > 1 ? page_of(1) : 0;
-    int code = scale_of(page);
+    int i = (turn + kTcLoaders8 - wk.g % kTcLoaders8) % kTcLoaders8;     // the warp's first tile of the item
+    int page = i < w.nt ? page_of(i) : 0;
+    int next_page = i + kTcLoaders8 < w.nt ? page_of(i + kTcLoaders8) : 0;
+    int code = i < w.nt ? scale_of(page) : 0;
     bool q_pending = false;
-    if (!is_v) {
+    if (!is_v && turn == 0) {
       for (int s = 0; s < (w.two ? 2 : 1) && ok; ++s) {
         const int n = s == 0 ? wk.it : wk.it1;           // the slot's items so far
         ok = mbar_wait(&sh->q_free[s], (n & 1) ^ 1, &sh->abort);
@@ -311,6 +320,18 @@ __device__ __forceinline__ void tc_load_eight_bit(const Args& a, PrefillTcShared
       cp_async_commit();
       q_pending = true;
     }
+    auto hand_over_q = [&]() {
+      cp_async_wait<0>();
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&sh->q_full[0]);
+        if (w.two) mbar_arrive(&sh->q_full[1]);
+      }
+      q_pending = false;
+    };
+    if (q_pending && i >= w.nt) hand_over_q();           // (no tile of this item is the warp's)
+    if (i >= w.nt) continue;
     uint4 raw[2][kBatch];
     // asks for batch b of the tile that begins at key k0 (pages and scales of that tile in `pg`)
     auto ask = [&](int k0, int b, int pg, uint4* v) {
@@ -323,12 +344,13 @@ __device__ __forceinline__ void tc_load_eight_bit(const Args& a, PrefillTcShared
           v[j] = *reinterpret_cast<const uint4*>(cache + (((id * a.hkv + w.kvh) << shift) + (key & ps_mask)) * kD + piece * 16);
       }
     };
-    ask(w.k_begin, 0, page, raw[0]);
-    for (int i = 0; i < w.nt && ok; ++i) {
+    ask(w.k_begin + i * kTcKeys, 0, page, raw[0]);
+    if (q_pending) hand_over_q();
+    for (; i < w.nt && ok; i += kTcLoaders8) {
       const int g = wk.g + i, b = g % kTcStages;
       const int k0 = w.k_begin + i * kTcKeys;
-      const int next_code = i + 1 < w.nt ? scale_of(next_page) : 0;
-      const int after_page = i + 2 < w.nt ? page_of(i + 2) : 0;
+      const int next_code = i + kTcLoaders8 < w.nt ? scale_of(next_page) : 0;
+      const int after_page = i + 2 * kTcLoaders8 < w.nt ? page_of(i + 2 * kTcLoaders8) : 0;
       ok = mbar_wait(&freed[b], ((g / kTcStages) & 1) ^ 1, &sh->abort);      // (a fresh barrier passes a wait on parity 1)
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
@@ -337,7 +359,7 @@ __device__ __forceinline__ void tc_load_eight_bit(const Args& a, PrefillTcShared
 #pragma unroll
       for (int n = 0; n < kBatches; ++n) {
         if (n + 1 < kBatches) ask(k0, n + 1, page, raw[(n + 1) & 1]);
-        else if (i + 1 < w.nt) ask(k0 + kTcKeys, 0, next_page, raw[(n + 1) & 1]);
+        else if (i + kTcLoaders8 < w.nt) ask(k0 + kTcLoaders8 * kTcKeys, 0, next_page, raw[(n + 1) & 1]);
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
           const int row = n * kBatchRows + j * RPI + rr;
@@ -356,28 +378,19 @@ __device__ __forceinline__ void tc_load_eight_bit(const Args& a, PrefillTcShared
           *reinterpret_cast<uint4*>(dst + row * 128 + (((c7 + 1) ^ (row & 7)) << 4)) = make_uint4(out[4], out[5], out[6], out[7]);
         }
       }
-      if (q_pending) cp_async_wait<0>();
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) {
-        if (q_pending) {
-          mbar_arrive(&sh->q_full[0]);
-          if (w.two) mbar_arrive(&sh->q_full[1]);
-        }
-        mbar_arrive(&full[b]);
-      }
-      q_pending = false;
+      if (lane == 0) mbar_arrive(&full[b]);
       page = next_page;
       next_page = after_page;
       code = next_code;
     }
-    if (q_pending) cp_async_wait<0>();                   // (left on an abort: no copy may outlive the CTA)
   }
-  cp_async_wait<0>();
+  cp_async_wait<0>();                                    // (left on an abort: no copy may outlive the CTA)
 }
 
 template <typename Args>
-__global__ void __launch_bounds__(kTcThreads, 1)
+__global__ void __launch_bounds__(Args::kEightBit ? kTcThreads8 : kTcThreads, 1)
 prefill_attn_tc_kernel(const Args a, int tiles, int* status) {
   static_assert(kD == 64 || kD == 128, "this kernel is written for head sizes 64 and 128");
   constexpr float kLog2e = 1.4426950408889634f;
@@ -388,6 +401,7 @@ prefill_attn_tc_kernel(const Args a, int tiles, int* status) {
   unsigned char* k_s = base + 2 * kTcTileBytes;                     // kTcStages tiles
   unsigned char* v_s = base + (2 + kTcStages) * kTcTileBytes;       // kTcStages tiles
   PrefillTcShared* sh = reinterpret_cast<PrefillTcShared*>(base + (2 + 2 * kTcStages) * kTcTileBytes);
+  constexpr int kMma = Args::kEightBit ? 12 : kTcRowWarps + 2;      // the first of the two MMA warps
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int pairs = (a.hq / a.hkv + 1) / 2;
   const int n_items = tiles * a.hkv * pairs;
@@ -411,7 +425,7 @@ prefill_attn_tc_kernel(const Args a, int tiles, int* status) {
     sh->abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == kTcRowWarps + 2) {   // TMEM allocation is a whole-warp operation
+  if (warp == kMma) {   // TMEM allocation is a whole-warp operation
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh->tmem_base)),
                  "r"(kTcTmemCols)
                  : "memory");
@@ -424,9 +438,14 @@ prefill_attn_tc_kernel(const Args a, int tiles, int* status) {
   pdl_launch();
   pdl_wait();        // q and the newest keys come from the kernels before this one
 
-  if (Args::kEightBit && (warp == kTcRowWarps || warp == kTcRowWarps + 1)) {
-    if constexpr (Args::kEightBit) tc_load_eight_bit(a, sh, q_s, k_s, v_s, warp == kTcRowWarps + 1, lane, n_items, pairs, tiles);
-  } else if (warp == kTcRowWarps || warp == kTcRowWarps + 1) {
+  if (warp >= kTcRowWarps) {
+  if constexpr (Args::kEightBit) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTcOtherRegs8));
+  if (Args::kEightBit && warp != kMma && warp != kMma + 1) {
+    if constexpr (Args::kEightBit) {
+      const int l = warp < kMma ? warp - kTcRowWarps : warp - kTcRowWarps - 2;      // first K's loaders, then V's
+      if (l < 2 * kTcLoaders8) tc_load_eight_bit(a, sh, q_s, k_s, v_s, l >= kTcLoaders8, l % kTcLoaders8, lane, n_items, pairs, tiles);
+    }
+  } else if (!Args::kEightBit && (warp == kTcRowWarps || warp == kTcRowWarps + 1)) {
     if constexpr (!Args::kEightBit) {
     // ------------------------------------------------------------------ loaders: one warp K (and both Q), one V
     const bool is_v = warp == kTcRowWarps + 1;
@@ -534,13 +553,13 @@ prefill_attn_tc_kernel(const Args a, int tiles, int* status) {
     }
     hand_over(true);
     }
-  } else if (warp >= kTcRowWarps + 2) {
+  } else {
     // ------------------------------------------------------------------ MMA issue: lane 0 of one warp per slot
     // Each slot has an issuing thread of its own, so that neither slot's products ever wait for the
     // other slot's rows.  With columns of its own for P a slot's products go  S(0), S(1), O += P(0) V,
     // S(2), O += P(1) V, ...: the S product runs one key tile ahead of the rows; with P over S:
     // S(0), O += P(0) V, S(1), O += P(1) V, ...
-    const int s = warp - (kTcRowWarps + 2);
+    const int s = warp - kMma;
     if (lane == 0 && blockIdx.x < n_items) {
       const uint32_t idesc_qk = umma_idesc(kTcRows, kTcKeys);
       const uint32_t idesc_pv = umma_idesc(kTcRows, 64) | (1u << 16);          // B (V) is MN-major; 64 columns of O at a time
@@ -624,7 +643,9 @@ prefill_attn_tc_kernel(const Args a, int tiles, int* status) {
         }
       }
     }
+  }
   } else {
+    if constexpr (Args::kEightBit) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTcRowRegs8));
     // ------------------------------------------------------------------ the row threads, one to a row
     // Warp w < 8: slot w / 4, rows 32 (w % 4) .. + 32 of the slot's tile (the TMEM lanes a warp may touch).  A thread
     // reads its row of S in four pieces of 32 keys: 2 and 3 for the maximum alone, then 0 and 1, which stay in
@@ -805,7 +826,7 @@ prefill_attn_tc_kernel(const Args a, int tiles, int* status) {
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == kTcRowWarps + 2) {
+  if (warp == kMma) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTcTmemCols) : "memory");
   }

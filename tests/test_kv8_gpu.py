@@ -425,6 +425,33 @@ def test_prefill(heads, kv_heads, dim, page, window, segments, dtype, impl):
     assert (out[T:] == 9.0).all()                     # rows behind the last sequence stay as they were
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim,page,window,segments", [
+    (32, 8, 64, 16, 0, ((900, 1500), (0, 700), (10, 1))), (32, 8, 128, 16, 0, ((700, 1400), (0, 900))),
+    (24, 8, 128, 64, 300, ((0, 1300), (2000, 1000))), (8, 8, 64, 32, 0, ((0, 2600), (300, 1500)))])
+def test_prefill_of_more_items_than_sms(heads, kv_heads, dim, page, window, segments):
+    """Several items to a CTA, of one key tile and of many, groups of one, three and four heads; some rows of every tile looked at."""
+    lengths = [a + n for a, n in segments]
+    cache, table = filled(lengths, heads, kv_heads, dim, page, seed=1)
+    g = torch.Generator().manual_seed(8)
+    T = sum(n for _, n in segments)
+    q = torch.randn(T, heads * dim, generator=g).bfloat16()
+    positions = torch.tensor([p for a, n in segments for p in range(a, a + n)], dtype=torch.int32, device=DEV)
+    seq, tok, rows = tiles_of(segments)
+    out = torch.full((T, heads * dim), 9.0, dtype=q.dtype, device=DEV)
+    scale = 1.0 / math.sqrt(dim)
+    qg = q.to(DEV)
+    kernels.kv8_attn_prefill(qg, qg.stride(0), *on_gpu(cache), table.to(DEV), seq, tok, rows, positions, out, len(seq), heads,
+                             kv_heads, dim, page, window, scale)
+    assert kernels.tc_status(out.device).item() == 0
+    k, v = P.values(cache[0], cache[2]), P.values(cache[1], cache[3])
+    row = 0
+    for s, (a, n) in enumerate(segments):
+        for i in sorted({*range(0, n, 128), *range(77, n, 128), n - 1}):
+            ref = P.attend(q[row + i:row + i + 1].view(1, heads, dim), k, v, table[s], [a + i], window, scale)
+            near(out[row + i:row + i + 1].view(1, heads, dim), ref, v[table[s][:-(-lengths[s] // page)].long()], "bfloat16")
+        row += n
+
+
 @pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
 @pytest.mark.parametrize("heads,kv_heads,dim,page", [(4, 2, 64, 16), (4, 1, 128, 32), (10, 2, 80, 64)])
 def test_a_run_of_steps(heads, kv_heads, dim, page, dtype):

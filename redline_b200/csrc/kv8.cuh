@@ -41,6 +41,21 @@ __device__ __forceinline__ uint32_t kv8_h2(uint32_t two) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(two)));
   return h;
 }
+// Four e4m3 bytes as two words of two halves.
+__device__ __forceinline__ void halves4(uint32_t four, uint32_t& lo, uint32_t& hi) {
+  asm("{\n"
+      ".reg .b16 a, b;\n"
+      "mov.b32 {a, b}, %2;\n"
+      "cvt.rn.f16x2.e4m3x2 %0, a;\n"
+      "cvt.rn.f16x2.e4m3x2 %1, b;\n"
+      "}\n"
+      : "=r"(lo), "=r"(hi)
+      : "r"(four));
+}
+__device__ __forceinline__ uint32_t pack_halves(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
 // Four e4m3 bytes as floats.
 __device__ __forceinline__ void kv8_f4(uint32_t four, float* f) {
   const uint32_t a = kv8_h2(four), b = kv8_h2(four >> 16);

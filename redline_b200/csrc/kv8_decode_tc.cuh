@@ -92,21 +92,6 @@ __device__ __forceinline__ void mma_f16_first(float* c, uint32_t a0, uint32_t a1
       : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
-// Four e4m3 bytes as two words of two halves.
-__device__ __forceinline__ void halves4(uint32_t four, uint32_t& lo, uint32_t& hi) {
-  asm("{\n"
-      ".reg .b16 a, b;\n"
-      "mov.b32 {a, b}, %2;\n"
-      "cvt.rn.f16x2.e4m3x2 %0, a;\n"
-      "cvt.rn.f16x2.e4m3x2 %1, b;\n"
-      "}\n"
-      : "=r"(lo), "=r"(hi)
-      : "r"(four));
-}
-__device__ __forceinline__ uint32_t pack_halves(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));

@@ -1,8 +1,12 @@
 // Prompt-portion attention on the fifth-generation tensor cores (bfloat16, head size 64 or 128).
 //
-// Included by attention.cu, and by kv8.cu for a cache in 8 bits (the arguments' type says which: kEightBit; the loaders then bring
-// a tile's bytes through registers and leave them as bfloat16 times their page's scale, a power of two, so exactly).  Before it come
-// cp_async16_s, cp_async_commit, cp_async_wait and ex2_approx.  An item of work is a tile of up to 128 consecutive query rows of one
+// Included by attention.cu, and by kv8.cu for a cache in 8 bits (the arguments' type says which: kEightBit).  Before it come
+// cp_async16_s, cp_async_commit, cp_async_wait and ex2_approx.  With eight bits the products are of halves: the loaders bring a tile's
+// bytes through registers and convert them (one conversion and one product for two numbers; to bfloat16 it was four times as
+// many instructions, and a portion of 2,048 behind 6,144 keys took 419 us).  A page's scale goes in relative to the largest of the
+// item's pages, so that no half overflows: exact for pages down to 2^-15 of that, and rounded to 2^-25 of its unit below; the largest
+// goes into the exponent's factor (keys) and the epilogue's (values).  Queries are rounded to halves, so they are finite up to
+// 65,504 and exact from 2^-14 on.  P is a half too.  An item of work is a tile of up to 128 consecutive query rows of one
 // sequence for TWO query heads of one kv head (the last pair of an odd group has one): the two
 // heads are the CTA's two "slots", they attend to the same keys and values, so a K tile and a V
 // tile are brought into shared memory once for both.  Persistent CTAs (one per SM) take items
@@ -46,6 +50,7 @@
 // loops, the copies in flight are waited for, TMEM is freed and bit 2 of *status is set.
 #pragma once
 
+#include "kv8.cuh"
 #include "umma.cuh"
 
 namespace rl {
@@ -81,6 +86,7 @@ struct PrefillTcShared {
   uint64_t o_free[2];                             // per slot: its four row warps have read the item's O
   uint32_t tmem_base;
   volatile int abort;
+  float item_k[8], item_v[8];                     // eight bits: an item's largest scales, by it % 8 (loaders are at most six items ahead)
 };
 constexpr size_t kPrefillTcSmem = 1024 + (2 + 2 * kTcStages) * kTcTileBytes + sizeof(PrefillTcShared);
 
@@ -265,15 +271,22 @@ struct TcWalk {
   }
 };
 
-// The loaders of a cache in 8 bits: some warps K (the first of them both Q, too), as many V, a tile to each in turn.  A tile's
-// 16-byte pieces come through registers in batches of four a lane, the next batch on its way while one is converted (e4m3 to half, to float, times the scale, the upper 16 bits:
-// 6.5 instructions for two numbers) and stored where the copies of a 16-bit cache would have put it.  A page's scale comes with
-// its id, a tile ahead.
+// 2^e as a pair of halves, for e <= 0 (0 below the halves' range).
+__device__ __forceinline__ __half2 tc_half_power(int e) {
+  const uint32_t b = e >= -14 ? static_cast<uint32_t>(e + 15) << 10 : (e >= -24 ? 1u << (e + 24) : 0u);
+  const uint32_t two = b | b << 16;
+  return *reinterpret_cast<const __half2*>(&two);
+}
+
+// The loaders of a cache in 8 bits: some warps K (and the first of them both Q), as many V, a tile to each in turn.  A tile's
+// 16-byte pieces come through registers in batches of 16 or 32 keys, the next batch on its way while one is converted and stored where
+// the copies of a 16-bit cache would have put it.  Page ids and scales come a tile ahead, a page to a lane.
 template <typename Args>
 __device__ __forceinline__ void tc_load_eight_bit(const Args& a, PrefillTcShared* sh, unsigned char* q_s, unsigned char* k_s,
                                                   unsigned char* v_s, bool is_v, int turn, int lane, int n_items, int pairs, int tiles) {
   constexpr int P = kD / 16, RPI = 32 / P;               // pieces of a row; rows that the warp's lanes cover at once
-  constexpr int kBatch = 4, kBatches = kTcKeys / (RPI * kBatch), kBatchRows = RPI * kBatch;
+  constexpr int kPer16 = 16 / RPI;                       // pieces of a lane in 16 keys (of one page)
+  constexpr int kBatch = 4, kBlocks = kBatch / kPer16, kBatches = 8 / kBlocks;      // a batch: kBlocks times 16 keys
   const uint8_t* cache = is_v ? a.vcache : a.kcache;
   const uint8_t* scales = is_v ? a.vscale : a.kscale;
   unsigned char* stage0 = is_v ? v_s : k_s;
@@ -281,71 +294,87 @@ __device__ __forceinline__ void tc_load_eight_bit(const Args& a, PrefillTcShared
   uint64_t* freed = is_v ? sh->v_free : sh->k_free;
   const int shift = a.page_shift, ps_mask = (1 << shift) - 1;
   const int piece = lane % P, rr = lane / P;             // piece of a row, row within a round
-  // the piece's two 16-byte chunks (2 piece and 2 piece + 1) lie in half chunk / 8 at place (chunk % 8) ^ (row % 8)
+  // the piece's two 16-byte chunks (2 piece and 2 piece + 1) lie in half chunk / 8 at place (chunk % 8) ^ (row % 8); a row's
+  // place % 8 is the lane's own, or with rounds of four rows the lane's own and another 4 in every second
   const uint32_t c_half = static_cast<uint32_t>(piece >> 2) * kTcHalfBytes;
-  const int c7 = (2 * piece) & 7;
+  const uint32_t at0 = c_half + rr * 128 + ((((2 * piece) & 7) ^ rr) << 4), at1 = c_half + rr * 128 + ((((2 * piece + 1) & 7) ^ rr) << 4);
   bool ok = true;
   TcWalk wk;
   for (bool more = wk.first(a, n_items, pairs, tiles); more && ok; more = wk.next(a, n_items, pairs, tiles)) {
     const TcItem& w = wk.w;
     const int32_t* bt = a.block_table + static_cast<size_t>(w.seq) * a.max_blocks;
     const int first = w.lo0 >> shift, last = (w.k_end - 1) >> shift;
-    // a tile's pages (at most eight: pages of 16 keys or more), one to a lane: its id and its scale
-    auto page_of = [&](int i) {
-      return bt[min(max(((w.k_begin + i * kTcKeys) >> shift) + (lane & 7), first), last)];
-    };
-    auto scale_of = [&](int page) { return scales[static_cast<size_t>(page) * a.hkv + w.kvh]; };
+    // the item's largest scale
+    int most = 0;
+#pragma unroll 4
+    for (int pg = first + lane; pg <= last; pg += 32) most = max(most, static_cast<int>(scales[static_cast<size_t>(bt[pg]) * a.hkv + w.kvh]));
+    most = __reduce_max_sync(0xffffffffu, most);
     int i = (turn + kTcLoaders8 - wk.g % kTcLoaders8) % kTcLoaders8;     // the warp's first tile of the item
+    if (i == 0 && lane == 0) (is_v ? sh->item_v : sh->item_k)[wk.it & 7] = kv8_scale(most);
+    // a tile's pages (at most eight: pages of 16 keys or more), one to a lane: its id and its scale
+    auto page_of = [&](int t) {
+      return bt[min(max(((w.k_begin + t * kTcKeys) >> shift) + (lane & 7), first), last)];
+    };
+    auto scale_of = [&](int page) { return static_cast<int>(scales[static_cast<size_t>(page) * a.hkv + w.kvh]); };
     int page = i < w.nt ? page_of(i) : 0;
     int next_page = i + kTcLoaders8 < w.nt ? page_of(i + kTcLoaders8) : 0;
     int code = i < w.nt ? scale_of(page) : 0;
-    bool q_pending = false;
     if (!is_v && turn == 0) {
+      constexpr int CPR = kD / 8, QRI = 32 / CPR;
+      const int c = lane % CPR, qr = lane / CPR;
       for (int s = 0; s < (w.two ? 2 : 1) && ok; ++s) {
         const int n = s == 0 ? wk.it : wk.it1;           // the slot's items so far
+        const bf16* src = a.q + static_cast<size_t>(w.tok0) * a.q_stride + (w.head0 + s) * kD + c * 8;
+        unsigned char* dst = q_s + s * kTcTileBytes + static_cast<uint32_t>(c >> 3) * kTcHalfBytes;
         ok = mbar_wait(&sh->q_free[s], (n & 1) ^ 1, &sh->abort);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        constexpr int CPR = kD / 8, QRI = 32 / CPR;
-        const int c = lane % CPR, qr = lane / CPR;
-        const uint32_t dst = smem_u32(q_s) + s * kTcTileBytes + static_cast<uint32_t>(c >> 3) * kTcHalfBytes;
-        for (int j = 0; j < kTcRows / QRI; ++j) {
-          const int r = j * QRI + qr;
-          const bool live = r < w.rows;
-          const bf16* src = a.q + static_cast<size_t>(w.tok0 + (live ? r : 0)) * a.q_stride + (w.head0 + s) * kD + c * 8;
-          cp_async16_s(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4), src, live);
+#pragma unroll 1
+        for (int j = 0; j < kTcRows; j += 8 * QRI) {
+          uint4 x[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            const int r = j + u * QRI + qr;
+            x[u] = make_uint4(0, 0, 0, 0);
+            if (r < w.rows) x[u] = *reinterpret_cast<const uint4*>(src + static_cast<size_t>(r) * a.q_stride);
+          }
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            const int r = j + u * QRI + qr;
+            uint32_t in[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const __half2 h = __floats2half2_rn(__uint_as_float(in[e] << 16), __uint_as_float(in[e] & 0xffff0000u));
+              in[e] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+            *reinterpret_cast<uint4*>(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(in[0], in[1], in[2], in[3]);
+          }
         }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->q_full[s]);
       }
       if (!ok) break;
-      cp_async_commit();
-      q_pending = true;
     }
-    auto hand_over_q = [&]() {
-      cp_async_wait<0>();
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&sh->q_full[0]);
-        if (w.two) mbar_arrive(&sh->q_full[1]);
-      }
-      q_pending = false;
-    };
-    if (q_pending && i >= w.nt) hand_over_q();           // (no tile of this item is the warp's)
     if (i >= w.nt) continue;
     uint4 raw[2][kBatch];
-    // asks for batch b of the tile that begins at key k0 (pages and scales of that tile in `pg`)
+    // asks for batch b of the tile that begins at key k0 (its pages in `pg`)
     auto ask = [&](int k0, int b, int pg, uint4* v) {
+      const bool whole = k0 >= w.lo0 && k0 + kTcKeys <= w.k_end;
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        const int row = b * kBatchRows + j * RPI + rr, key = k0 + row;
-        const size_t id = static_cast<size_t>(__shfl_sync(0xffffffffu, pg, ((k0 & ps_mask) + row) >> shift));
-        v[j] = make_uint4(0, 0, 0, 0);
-        if (key < w.k_end && key >= w.lo0)
-          v[j] = *reinterpret_cast<const uint4*>(cache + (((id * a.hkv + w.kvh) << shift) + (key & ps_mask)) * kD + piece * 16);
+      for (int j = 0; j < kBlocks; ++j) {
+        const int key = k0 + (b * kBlocks + j) * 16;
+        const int id = __shfl_sync(0xffffffffu, pg, ((k0 & ps_mask) + (b * kBlocks + j) * 16) >> shift);
+        const uint8_t* p = cache + (((static_cast<size_t>(id) * a.hkv + w.kvh) << shift) + (key & ps_mask)) * kD + lane * 16;
+#pragma unroll
+        for (int u = 0; u < kPer16; ++u) {
+          const int mine = key + u * RPI + rr;
+          v[j * kPer16 + u] = make_uint4(0, 0, 0, 0);
+          if (whole || (mine < w.k_end && mine >= w.lo0)) v[j * kPer16 + u] = *reinterpret_cast<const uint4*>(p + u * 512);
+        }
       }
     };
     ask(w.k_begin + i * kTcKeys, 0, page, raw[0]);
-    if (q_pending) hand_over_q();
     for (; i < w.nt && ok; i += kTcLoaders8) {
       const int g = wk.g + i, b = g % kTcStages;
       const int k0 = w.k_begin + i * kTcKeys;
@@ -354,28 +383,34 @@ __device__ __forceinline__ void tc_load_eight_bit(const Args& a, PrefillTcShared
       ok = mbar_wait(&freed[b], ((g / kTcStages) & 1) ^ 1, &sh->abort);      // (a fresh barrier passes a wait on parity 1)
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      unsigned char* dst = stage0 + b * kTcTileBytes + c_half;
-      const float my_scale = kv8_scale(code);
+      unsigned char* dst = stage0 + b * kTcTileBytes;
 #pragma unroll
       for (int n = 0; n < kBatches; ++n) {
         if (n + 1 < kBatches) ask(k0, n + 1, page, raw[(n + 1) & 1]);
         else if (i + kTcLoaders8 < w.nt) ask(k0 + kTcLoaders8 * kTcKeys, 0, next_page, raw[(n + 1) & 1]);
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-          const int row = n * kBatchRows + j * RPI + rr;
-          const float f = __shfl_sync(0xffffffffu, my_scale, ((k0 & ps_mask) + row) >> shift);
-          const uint4 v = raw[n & 1][j];
-          const uint32_t in[4] = {v.x, v.y, v.z, v.w};
-          uint32_t out[8];
+        for (int j = 0; j < kBlocks; ++j) {
+          const int c = __shfl_sync(0xffffffffu, code, ((k0 & ps_mask) + (n * kBlocks + j) * 16) >> shift);
+          const __half2 f = tc_half_power(c - most);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float x[4];
-            kv8_f4(in[e], x);
-            out[2 * e] = __byte_perm(__float_as_uint(x[0] * f), __float_as_uint(x[1] * f), 0x7632);
-            out[2 * e + 1] = __byte_perm(__float_as_uint(x[2] * f), __float_as_uint(x[3] * f), 0x7632);
+          for (int u = 0; u < kPer16; ++u) {
+            const uint4 v = raw[n & 1][j * kPer16 + u];
+            const uint32_t in[4] = {v.x, v.y, v.z, v.w};
+            uint32_t out[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              halves4(in[e], out[2 * e], out[2 * e + 1]);
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&out[2 * e + x]), f);
+                out[2 * e + x] = *reinterpret_cast<const uint32_t*>(&h);
+              }
+            }
+            const int row = (n * kBlocks + j) * 16 + u * RPI;            // (+ rr)
+            const uint32_t sw = RPI == 4 && (u & 1) ? 64u : 0u;
+            *reinterpret_cast<uint4*>(dst + (at0 ^ sw) + row * 128) = make_uint4(out[0], out[1], out[2], out[3]);
+            *reinterpret_cast<uint4*>(dst + (at1 ^ sw) + row * 128) = make_uint4(out[4], out[5], out[6], out[7]);
           }
-          *reinterpret_cast<uint4*>(dst + row * 128 + ((c7 ^ (row & 7)) << 4)) = make_uint4(out[0], out[1], out[2], out[3]);
-          *reinterpret_cast<uint4*>(dst + row * 128 + (((c7 + 1) ^ (row & 7)) << 4)) = make_uint4(out[4], out[5], out[6], out[7]);
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -386,7 +421,6 @@ __device__ __forceinline__ void tc_load_eight_bit(const Args& a, PrefillTcShared
       code = next_code;
     }
   }
-  cp_async_wait<0>();                                    // (left on an abort: no copy may outlive the CTA)
 }
 
 template <typename Args>
@@ -561,8 +595,9 @@ prefill_attn_tc_kernel(const Args a, int tiles, int* status) {
     // S(0), O += P(0) V, S(1), O += P(1) V, ...
     const int s = warp - kMma;
     if (lane == 0 && blockIdx.x < n_items) {
-      const uint32_t idesc_qk = umma_idesc(kTcRows, kTcKeys);
-      const uint32_t idesc_pv = umma_idesc(kTcRows, 64) | (1u << 16);          // B (V) is MN-major; 64 columns of O at a time
+      constexpr uint32_t kHalves = Args::kEightBit ? (1u << 7) | (1u << 10) : 0u;      // (clear: both operands are halves)
+      const uint32_t idesc_qk = umma_idesc(kTcRows, kTcKeys) & ~kHalves;
+      const uint32_t idesc_pv = (umma_idesc(kTcRows, 64) & ~kHalves) | (1u << 16);          // B (V) is MN-major; 64 columns of O at a time
       const uint32_t q_u = smem_u32(q_s) + s * kTcTileBytes, k_u = smem_u32(k_s), v_u = smem_u32(v_s);
       const uint32_t s_col = tmem + s * kTcKeys, o_col = tmem + kTcColO + s * kD;
       const uint32_t p_col = kTcOwnP ? tmem + kTcColP + s * 64 : s_col;
@@ -658,7 +693,7 @@ prefill_attn_tc_kernel(const Args a, int tiles, int* status) {
     const uint32_t s_addr = tmem + lane_addr + s * kTcKeys;           // S
     const uint32_t p_addr = kTcOwnP ? tmem + lane_addr + kTcColP + s * 64 : s_addr;      // 64 columns of P
     const uint32_t o_addr = tmem + lane_addr + kTcColO + s * kD;
-    const float sc = a.scale * kLog2e;
+    float sc = a.scale * kLog2e;
     bool ok = true;
     TcWalk wk;
     for (bool more = wk.first(a, n_items, pairs, tiles); more && ok; more = wk.next(a, n_items, pairs, tiles)) {
@@ -679,6 +714,11 @@ prefill_attn_tc_kernel(const Args a, int tiles, int* status) {
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
+        if constexpr (Args::kEightBit)      // (once there is a tile of the item, its loader has left the scale)
+          if (i == 0) {
+            sc = a.scale * kLog2e * sh->item_k[wk.it & 7];
+            if (sc < 1.2e-38f) sc = 1.2e-38f;              // (times -inf it has to be -inf; so small a factor makes every score 0)
+          }
         // only tiles that reach past the first row's position, before the last row's window or past the
         // tile's rows need the masks (the same for the whole CTA)
         const bool masked = (t0 + kTcKeys - 1 > pos0) || (a.window > 0 && t0 < pos0 + kTcRows - a.window) || (rows < kTcRows);
@@ -744,9 +784,14 @@ prefill_attn_tc_kernel(const Args a, int tiles, int* status) {
             const float p0 = ex2_approx(x0), p1 = ex2_approx(x1), p2 = ex2_approx(x2), p3 = ex2_approx(x3);
             sum_a = add_f32x2(sum_a, f32x2(p0, p1));
             sum_b = add_f32x2(sum_b, f32x2(p2, p3));
-            const __nv_bfloat162 lo = __floats2bfloat162_rn(p0, p1), hi = __floats2bfloat162_rn(p2, p3);
-            v[j >> 1] = *reinterpret_cast<const uint32_t*>(&lo);       // (columns j / 2: behind the ones still to be read)
-            v[(j >> 1) + 1] = *reinterpret_cast<const uint32_t*>(&hi);
+            if constexpr (Args::kEightBit) {
+              v[j >> 1] = pack_halves(p0, p1);
+              v[(j >> 1) + 1] = pack_halves(p2, p3);
+            } else {
+              const __nv_bfloat162 lo = __floats2bfloat162_rn(p0, p1), hi = __floats2bfloat162_rn(p2, p3);
+              v[j >> 1] = *reinterpret_cast<const uint32_t*>(&lo);       // (columns j / 2: behind the ones still to be read)
+              v[(j >> 1) + 1] = *reinterpret_cast<const uint32_t*>(&hi);
+            }
           }
         };
         exponentials(va);
@@ -802,7 +847,8 @@ prefill_attn_tc_kernel(const Args a, int tiles, int* status) {
       if (!ok) break;
       tc_fence_after();
       const float l_all = l[0] + l[1];
-      const float inv = l_all > 0.f ? 1.f / l_all : 0.f;
+      float inv = l_all > 0.f ? 1.f / l_all : 0.f;
+      if constexpr (Args::kEightBit) inv *= sh->item_v[wk.it & 7];
       bf16* dst = a.out + static_cast<size_t>(w.tok0 + (r < rows ? r : 0)) * a.out_stride + (w.head0 + s) * kD;
 #pragma unroll
       for (int c0 = 0; c0 < kD; c0 += 32) {

@@ -82,153 +82,168 @@ __device__ __forceinline__ int kv8_position(const Kv8WriteArgs<T>& a, int pos) {
   return 0;
 }
 
-constexpr int kWriteThreads = 512;
+constexpr int kWriteThreads = 256, kWriteWarps = kWriteThreads / 32;
+constexpr int kWriteTokens = 32 / (kD / 16);       // tokens that a warp takes at once: each D/16 lanes, 8 entries of either half of the head
+// Rounds of them that stay in registers between the two passes over a run: a page of 16 tokens at head sizes up to 128.
+constexpr int kWriteRounds = kD <= 64 ? 2 : 4;
 
-// The first `kv_blocks` CTAs are one to a token (or item): where a RUN begins there, the tokens that follow one another in
-// one page, the CTA stores the run, a warp to the keys or the values of a kv head; the others have nothing to do.  (A
-// warp to 16 tokens of a head: 32 bytes of each lane's asked for at once.  With one CTA to a fixed window of tokens, single
-// tokens would queue in one CTA, and where a prompt's pages begin among the tokens is not known to the host.)  The CTAs
-// behind them rotate q, eight pairs of entries to a thread.
-// The scale needs the block's largest magnitude before the first byte can be written: two passes over the run, the
-// second of which finds it in L1.
+// gridDim.y = tasks + 1.  CTAs (x, y < tasks) store: where a RUN begins among the `span` tokens from x * span, the tokens that follow one
+// another in one page, a warp takes the keys or the values of one kv head of the run.  CTAs (x, tasks) rotate the q of those
+// tokens, eight pairs of entries to a thread.
+// Where runs begin is not known to the host.  One token to a CTA as long as all are resident at once: each of a decode batch is a
+// run of its own, and four runs one after another take four times as long.  Four to a CTA beyond: most tokens of a prompt
+// begin no run, and the CTAs are handed out one by one.
+// What bounds it is the way from the slots to the rows to the block's largest magnitude to the bytes; what does not depend on one
+// another is asked for together.
 template <typename T>
-__global__ void __launch_bounds__(kWriteThreads)
-kv8_write_kernel(const Kv8WriteArgs<T> a, int kv_blocks) {
+__global__ void __launch_bounds__(kWriteThreads, 3)
+kv8_write_kernel(const Kv8WriteArgs<T> a, int span, int tasks) {
   pdl_wait();
   pdl_launch();
-  constexpr int CH = kD / 16;                    // lanes to a token: each has 8 entries of either half of the head
-  if (static_cast<int>(blockIdx.x) >= kv_blocks) {
-    const int per = a.hq * CH;
-    const long long idx = static_cast<long long>(blockIdx.x - kv_blocks) * kWriteThreads + threadIdx.x;
-    if (idx >= static_cast<long long>(a.tokens) * per) return;
-    const int t = static_cast<int>(idx / per), rest = static_cast<int>(idx - static_cast<long long>(t) * per);
-    const int col = rest / CH * kD + rest % CH * 8;
-    const T* src = a.qkv + static_cast<size_t>(t) * a.qkv_stride + col;
-    float x0[8], x1[8];
-    load8(src, x0);
-    load8(src + kD / 2, x1);
-    if (a.cos != nullptr) {
-      const size_t at = static_cast<size_t>(kv8_position(a, a.positions[t])) * (kD / 2) + rest % CH * 8;
-      float c[8], s[8];
-      load8(a.cos + at, c);
-      load8(a.sin + at, s);
-      kv8_rotate8(x0, x1, c, s);
-    }
-    T* dst = a.q_out + static_cast<size_t>(t) * a.q_stride + col;
-    store8(dst, x0);
-    store8(dst + kD / 2, x1);
-    return;
-  }
-  const int t = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int ps = 1 << a.page_shift;
-  // (asked for together: the slots of the token before, of this one and of 30 more, and those of all before it)
-  const int near = t - 1 + lane;
-  const long long theirs = near >= 0 && near < a.tokens ? kv8_slot(a, near) : -1;
-  const long long slot = __shfl_sync(0xffffffffu, theirs, 1);
-  if (slot < 0) return;
-  if (slot >= a.num_slots) {
-    if (threadIdx.x == 0) atomicOr(a.status, 4);
-    return;
-  }
-  const int off = static_cast<int>(slot & (ps - 1));
-  const long long page = slot >> a.page_shift;
-  if (off > 0 && __shfl_sync(0xffffffffu, theirs, 0) == slot - 1) return;      // not the first of its run
-  // Two runs of one page in one call would each set its scale without the other's: only the first is stored.  (Page 0
-  // is the reserved one that padding rows write to: nothing to tell of there.)
-  bool before = false;
-  for (int i = threadIdx.x; i < t; i += blockDim.x) {
-    const long long s = kv8_slot(a, i);
-    before |= s >= 0 && (s >> a.page_shift) == page;
-  }
-  if (__syncthreads_or(before)) {
-    if (threadIdx.x == 0 && page != 0) atomicOr(a.status, 8);
-    return;
-  }
-  int n;                                         // tokens of the run
-  {
-    // (lane l has token t - 1 + l; lane 0 stands for itself)
-    unsigned m = __ballot_sync(0xffffffffu, lane == 0 || (off + lane - 1 < ps && theirs == slot + lane - 1));
-    n = m == 0xffffffffu ? 31 : __ffs(~m) - 2;
-    while (n >= 31 && off + n < ps) {
-      const int i = n + lane;
-      m = __ballot_sync(0xffffffffu, t + i < a.tokens && off + i < ps && kv8_slot(a, t + i) == slot + i);
-      if (m != 0xffffffffu) {
-        n += __ffs(~m) - 1;
-        break;
+  constexpr int CH = kD / 16, TPR = kWriteTokens;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int t0 = blockIdx.x * span, ps = 1 << a.page_shift;
+  if (static_cast<int>(blockIdx.y) == tasks) {
+    if (a.q_out == nullptr) return;
+    const int per = a.hq * CH, n = min(span, a.tokens - t0) * per;
+#pragma unroll 2
+    for (int i = threadIdx.x; i < n; i += kWriteThreads) {
+      const int t = t0 + i / per, rest = i % per, col = rest / CH * kD + rest % CH * 8;
+      const T* src = a.qkv + static_cast<size_t>(t) * a.qkv_stride + col;
+      float x0[8], x1[8];
+      load8(src, x0);
+      load8(src + kD / 2, x1);
+      if (a.cos != nullptr) {
+        const size_t at = static_cast<size_t>(kv8_position(a, a.positions[t])) * (kD / 2) + rest % CH * 8;
+        float c[8], s[8];
+        load8(a.cos + at, c);
+        load8(a.sin + at, s);
+        kv8_rotate8(x0, x1, c, s);
       }
-      n += 32;
+      T* dst = a.q_out + static_cast<size_t>(t) * a.q_stride + col;
+      store8(dst, x0);
+      store8(dst + kD / 2, x1);
     }
+    return;
   }
-  constexpr int TPR = 32 / CH;                   // tokens that a warp takes at once
+  // the slots of the token before, of the CTA's and of those after them (lane l: token t0 - 1 + l)
+  long long theirs = -1;
+  if (t0 - 1 + lane >= 0 && t0 - 1 + lane < a.tokens) theirs = kv8_slot(a, t0 - 1 + lane);
+  const int w = blockIdx.y * kWriteWarps + warp;           // keys of kv head w, or values of kv head w - hkv
+  const bool busy = w < 2 * a.hkv, is_v = w >= a.hkv;
+  const int h = is_v ? w - a.hkv : w;
   const int tl = lane / CH, ch = lane - tl * CH;
-  for (int w = warp; w < 2 * a.hkv; w += blockDim.x >> 5) {
-    const bool is_v = w >= a.hkv;
-    const int h = is_v ? w - a.hkv : w;
+  for (int l = 1; l <= span; ++l) {                        // (the same for the whole CTA)
+    const int t = t0 + l - 1;
+    const long long slot = __shfl_sync(0xffffffffu, theirs, l);
+    if (slot < 0) continue;
+    if (slot >= a.num_slots) {
+      if (threadIdx.x == 0) atomicOr(a.status, 4);
+      continue;
+    }
+    const int off = static_cast<int>(slot & (ps - 1));
+    const long long page = slot >> a.page_shift;
+    if (off > 0 && __shfl_sync(0xffffffffu, theirs, l - 1) == slot - 1) continue;      // not the first of its run
+    int n;                                                 // tokens of the run
+    {
+      // (lane l has its first token; those before stand for themselves)
+      unsigned m = __ballot_sync(0xffffffffu, lane < l || (off + lane - l < ps && theirs == slot + lane - l));
+      n = m == 0xffffffffu ? 32 - l : __ffs(~m) - 1 - l;
+      while (n >= 32 - l && off + n < ps) {
+        const int i = n + lane;
+        m = __ballot_sync(0xffffffffu, t + i < a.tokens && off + i < ps && kv8_slot(a, t + i) == slot + i);
+        if (m != 0xffffffffu) {
+          n += __ffs(~m) - 1;
+          break;
+        }
+        n += 32;
+      }
+    }
     const T* src = a.qkv + static_cast<size_t>(t) * a.qkv_stride + static_cast<size_t>(a.hq + w) * kD + ch * 8;
     const bool turn = !is_v && a.cos != nullptr;
-    auto load = [&](int i, float* x0, float* x1) {
+    auto load = [&](int i, float* x) {                     // token i of the run
       const T* p = src + static_cast<size_t>(i) * a.qkv_stride;
-      load8(p, x0);
-      load8(p + kD / 2, x1);
+      load8(p, x);
+      load8(p + kD / 2, x + 8);
       if (turn) {
         const int pos = a.items != nullptr ? a.items[t + i].z - 1 : a.positions[t + i];
         const size_t at = static_cast<size_t>(kv8_position(a, pos)) * (kD / 2) + ch * 8;
         float c[8], s[8];
         load8(a.cos + at, c);
         load8(a.sin + at, s);
-        kv8_rotate8(x0, x1, c, s);
+        kv8_rotate8(x, x + 8, c, s);
       }
     };
-    float amax = 0.f;
-#pragma unroll 2
-    for (int i = tl; i < n; i += TPR) {
-      if (tl >= TPR) break;
-      float x0[8], x1[8];
-      load(i, x0, x1);
+    const bool lanes = busy && tl < TPR;
+    float kept[kWriteRounds][16];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float u = fabsf(x0[e]), v = fabsf(x1[e]);
-        amax = fmaxf(amax, fmaxf(u < INFINITY ? u : 0.f, v < INFINITY ? v : 0.f));
-      }
+    for (int r = 0; r < kWriteRounds; ++r)
+      if (lanes && tl + r * TPR < n) load(tl + r * TPR, kept[r]);
+    uint8_t* scale = (is_v ? a.vscale : a.kscale) + static_cast<size_t>(page) * a.hkv + h;
+    const int old = busy && off > 0 ? min(static_cast<int>(*scale), 254) : 0;
+    // Two runs of one page in one call would each set its scale without the other's: only the first is stored.  (Page 0
+    // is the reserved one that padding rows write to: nothing to tell of there.)
+    bool before = false;
+    for (int i = threadIdx.x; i < t; i += kWriteThreads) {
+      const long long s = kv8_slot(a, i);
+      before |= s >= 0 && (s >> a.page_shift) == page;
     }
+    if (__syncthreads_or(before)) {                        // (every thread has read its scale)
+      if (threadIdx.x == 0 && page != 0) atomicOr(a.status, 8);
+      continue;
+    }
+    if (!busy) continue;
+    float amax = 0.f;
+    auto largest = [&](const float* x) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float u = fabsf(x[e]);
+        amax = fmaxf(amax, u < INFINITY ? u : 0.f);
+      }
+    };
+#pragma unroll
+    for (int r = 0; r < kWriteRounds; ++r)
+      if (lanes && tl + r * TPR < n) largest(kept[r]);
+    if (lanes)
+      for (int i = tl + kWriteRounds * TPR; i < n; i += TPR) {
+        float x[16];
+        load(i, x);
+        largest(x);
+      }
     amax = warp_max(amax);
     uint8_t* cache = is_v ? a.vcache : a.kcache;
-    uint8_t* scale = (is_v ? a.vscale : a.kscale) + static_cast<size_t>(page) * a.hkv + h;
     uint8_t* base = cache + (static_cast<size_t>(page) * a.hkv + h) * (static_cast<size_t>(ps) * kD);
-    int code = kv8_code(amax);
-    if (off > 0) {
-      const int old = min(static_cast<int>(*scale), 254);
-      if (code > old) {                          // what is in the page goes over to the larger scale
-        const float f = kv8_exp2i(max(old - code, -127));
-        for (int c = lane; c < off * (kD / 16); c += 32) {
-          uint4* p = reinterpret_cast<uint4*>(base) + c;
-          float x[16];
-          kv8_f16(*p, x);
+    const int code = max(kv8_code(amax), old);
+    if (off > 0 && code > old) {                           // what is in the page goes over to the larger scale
+      const float f = kv8_exp2i(max(old - code, -127));
+      for (int c = lane; c < off * (kD / 16); c += 32) {
+        uint4* p = reinterpret_cast<uint4*>(base) + c;
+        float x[16];
+        kv8_f16(*p, x);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) x[e] *= f;
-          *p = make_uint4(kv8_pack4(x), kv8_pack4(x + 4), kv8_pack4(x + 8), kv8_pack4(x + 12));
-        }
-      } else {
-        code = old;
+        for (int e = 0; e < 16; ++e) x[e] *= f;
+        *p = make_uint4(kv8_pack4(x), kv8_pack4(x + 4), kv8_pack4(x + 8), kv8_pack4(x + 12));
       }
-      __syncwarp();                              // (every lane has read the scale)
     }
     if (lane == 0) *scale = static_cast<uint8_t>(code);
     const float inv = kv8_exp2i(127 - code);
-#pragma unroll 2
-    for (int i = tl; i < n; i += TPR) {
-      if (tl >= TPR) break;
-      float x0[8], x1[8];
-      load(i, x0, x1);
+    auto put = [&](int i, float* x) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {              // (what is not finite is stored as not a number, and left out of the scale)
-        x0[e] = fabsf(x0[e]) < INFINITY ? x0[e] * inv : __uint_as_float(0x7fc00000u);
-        x1[e] = fabsf(x1[e]) < INFINITY ? x1[e] * inv : __uint_as_float(0x7fc00000u);
-      }
+      for (int e = 0; e < 16; ++e)                         // (what is not finite is stored as not a number, and left out of the scale)
+        x[e] = fabsf(x[e]) < INFINITY ? x[e] * inv : __uint_as_float(0x7fc00000u);
       uint8_t* dst = base + static_cast<size_t>(off + i) * kD + ch * 8;
-      *reinterpret_cast<uint2*>(dst) = make_uint2(kv8_pack4(x0), kv8_pack4(x0 + 4));
-      *reinterpret_cast<uint2*>(dst + kD / 2) = make_uint2(kv8_pack4(x1), kv8_pack4(x1 + 4));
-    }
+      *reinterpret_cast<uint2*>(dst) = make_uint2(kv8_pack4(x), kv8_pack4(x + 4));
+      *reinterpret_cast<uint2*>(dst + kD / 2) = make_uint2(kv8_pack4(x + 8), kv8_pack4(x + 12));
+    };
+#pragma unroll
+    for (int r = 0; r < kWriteRounds; ++r)
+      if (lanes && tl + r * TPR < n) put(tl + r * TPR, kept[r]);
+    if (lanes)
+      for (int i = tl + kWriteRounds * TPR; i < n; i += TPR) {
+        float x[16];
+        load(i, x);
+        put(i, x);
+      }
   }
 }
 
@@ -755,12 +770,14 @@ int launch_write(const void* qkv, int qkv_stride, const int32_t* positions, cons
   a.max_pos = max_pos;
   a.num_slots = num_slots;
   a.status = status;
-  const int kv_blocks = slots != nullptr || items != nullptr ? tokens : 0;
-  const long long pairs = q_out != nullptr ? static_cast<long long>(tokens) * hq * (kD / 16) : 0;
-  const long long blocks = kv_blocks + (pairs + kWriteThreads - 1) / kWriteThreads;
-  if (blocks == 0) return 0;
-  if (blocks > 0x7fffffffLL) return static_cast<int>(cudaErrorInvalidValue);
-  launch_kernel(kv8_write_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(kWriteThreads), 0, stream, a, kv_blocks);
+  if (tokens == 0 || (slots == nullptr && items == nullptr && q_out == nullptr)) return 0;
+  int sms = 0;
+  const int e = device_sms(&sms);
+  if (e) return e;
+  const int tasks = slots != nullptr || items != nullptr ? (2 * hkv + kWriteWarps - 1) / kWriteWarps : 0;
+  const int span = static_cast<long long>(tokens) * (tasks + 1) <= 4 * sms ? 1 : 4;
+  launch_kernel(kv8_write_kernel<T>, dim3((tokens + span - 1) / span, tasks + (q_out != nullptr ? 1 : 0)), dim3(kWriteThreads), 0, stream, a,
+                span, tasks);
   return static_cast<int>(cudaGetLastError());
 }
 

@@ -299,16 +299,20 @@ struct Kv8Segment {
   bool whole;
 };
 
-// The units of share s of `shares`: [s U / shares, (s + 1) U / shares).
-__device__ __forceinline__ int kv8_share_begin(int s, int units, int shares) {
-  return static_cast<int>(static_cast<long long>(units) * s / shares);
-}
-// The share that unit u lies in.
-__device__ __forceinline__ int kv8_share_of(int u, int units, int shares) {
-  int s = static_cast<int>((static_cast<long long>(u) * shares) / units);
-  while (kv8_share_begin(s + 1, units, shares) <= u) ++s;
-  return s;
-}
+// The shares: of q + 1 units the first `rem`, of q the others (never more shares than units).
+struct Kv8Cut {
+  int shares, q, rem;
+  __device__ __forceinline__ Kv8Cut(int units, int most) {
+    shares = min(most, units);
+    q = shares > 0 ? units / shares : 0;
+    rem = units - q * shares;
+  }
+  __device__ __forceinline__ int begin(int s) const { return s * q + min(s, rem); }
+  __device__ __forceinline__ int of(int u) const {         // the share that unit u lies in
+    const int big = rem * (q + 1);
+    return u < big ? u / (q + 1) : rem + (u - big) / q;
+  }
+};
 
 __device__ __forceinline__ Kv8Segment kv8_segment(const Kv8Args& a, const int* start, int u, int end) {
   int lo = 0, hi = a.nitems - 1;            // the largest i with start[i] <= u (items without keys have no units)
@@ -334,21 +338,21 @@ __device__ __forceinline__ Kv8Segment kv8_segment(const Kv8Args& a, const int* s
   return g;
 }
 
-// The pieces of a cut row, added in the order of the keys and written out, by `nwarps` warps: a warp to 32 (or 16) entries of a
-// head.  First a lane to a piece, for the references and the weights, then an entry to a lane, the pieces' loads in flight together.
+// The pieces of a cut row, which shares s0 .. s1 have left, added in the order of the keys and written out, by `nwarps` warps: a warp to
+// 32 (or 16) entries of a head.  First a lane to a piece, for the references and the weights, then an entry to a lane, the pieces' loads in
+// flight together.  (place: of the first share, which ends with the row unless it begins with it; the others' is 0.)
 template <typename T>
-__device__ __forceinline__ void kv8_merge(const Kv8Args& a, const Kv8Segment& g, int units, int shares, int warp, int nwarps) {
+__device__ __noinline__ void kv8_merge(const float* part, int G, int s0, int s1, int place, T* out, int warp, int nwarps) {
   constexpr int W = kD % 32 == 0 ? 32 : 16, NB = kD / W;
-  const int lane = threadIdx.x & 31, G = a.hq / a.hkv;
-  const int s0 = kv8_share_of(g.row_begin, units, shares), s1 = kv8_share_of(g.row_end - 1, units, shares);
+  const int lane = threadIdx.x & 31;
   const int row = G * (kD + 4);
-  // (the first piece ends its share unless it begins it: its place is 0 then, as everybody else's)
-  const int first = kv8_share_begin(s0, units, shares) != g.row_begin ? 1 : 0;
+#pragma unroll 1
   for (int i = warp; i < G * NB; i += nwarps) {
     const int r = i / NB, d = (i - r * NB) * W + lane % W;
-    const float* base = a.part + r * (kD + 4);
-    auto piece = [&](int s) { return base + (static_cast<size_t>(s) * 2 + (s == s0 ? first : 0)) * row; };
+    const float* base = part + r * (kD + 4);
+    auto piece = [&](int s) { return base + (static_cast<size_t>(s) * 2 + (s == s0 ? place : 0)) * row; };
     float top = -INFINITY, dtop = -INFINITY, den = 0.f, num = 0.f;
+#pragma unroll 1
     for (int c = s0; c <= s1; c += 32) {                 // (32 pieces at a time; the sums so far are carried over)
       const bool in = c + lane <= s1;
       const float4 x = in ? __ldcg(reinterpret_cast<const float4*>(piece(c + lane) + kD)) : make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
@@ -366,7 +370,7 @@ __device__ __forceinline__ void kv8_merge(const Kv8Args& a, const Kv8Segment& g,
       for (int k = 0; k < n; ++k) num += __shfl_sync(0xffffffffu, w, k) * __ldcg(piece(c + k) + d);
     }
     if (lane < W)
-      static_cast<T*>(a.out)[static_cast<size_t>(g.tok) * a.out_stride + (g.kvh * G + r) * kD + d] = from_float<T>(num * exp2f(dtop) / den);
+      out[r * kD + d] = from_float<T>(num * exp2f(dtop) / den);
   }
 }
 
@@ -390,11 +394,9 @@ kv8_decode_kernel(const Kv8Args a) {
   const int G = a.hq / a.hkv, ps = 1 << a.page_shift;
   const int ch = lane % kGenLanes, slot = lane / kGenLanes;
   const bool in_head = ch * 16 < kD;
-  const int units = kv8_units(a, start);
-  const int shares = min(static_cast<int>(gridDim.x), units);      // every share has a unit
-  if (static_cast<int>(blockIdx.x) >= shares) return;
-  const int end = kv8_share_begin(blockIdx.x + 1, units, shares);
-  const int begin = kv8_share_begin(blockIdx.x, units, shares);
+  const Kv8Cut cut(kv8_units(a, start), gridDim.x);
+  if (static_cast<int>(blockIdx.x) >= cut.shares) return;
+  const int begin = cut.begin(blockIdx.x), end = cut.begin(blockIdx.x + 1);
   for (int u = begin; u < end;) {
     const Kv8Segment g = kv8_segment(a, start, u, end);
     const int32_t* bt = a.block_table + static_cast<size_t>(g.seq) * a.max_blocks;
@@ -527,15 +529,16 @@ kv8_decode_kernel(const Kv8Args a) {
       __threadfence();                       // the piece, before it is counted
       __syncthreads();
       if (threadIdx.x == 0) {
-        const int pieces = kv8_share_of(g.row_end - 1, units, shares) - kv8_share_of(g.row_begin, units, shares) + 1;
         int* c = a.counters + static_cast<size_t>(g.item) * a.hkv + g.kvh;
-        last = atomicAdd(c, 1) == pieces - 1;
+        last = atomicAdd(c, 1) == cut.of(g.row_end - 1) - cut.of(g.row_begin);
         if (last) *c = 0;
       }
       __syncthreads();
       if (last) {
         __threadfence();
-        kv8_merge<T>(a, g, units, shares, warp, kGenThreads / 32);
+        const int s0 = cut.of(g.row_begin);
+        kv8_merge<T>(a.part, G, s0, cut.of(g.row_end - 1), cut.begin(s0) != g.row_begin ? 1 : 0,
+                     static_cast<T*>(a.out) + static_cast<size_t>(g.tok) * a.out_stride + g.kvh * G * kD, warp, kGenThreads / 32);
       }
       __syncthreads();
     }
@@ -789,6 +792,11 @@ constexpr int kMaxShares = 1776;
 typedef void (*TcKernel)(Kv8Args, int, int);
 const TcKernel kTcKernels[2] = {kv8_decode_tc_kernel<false>, kv8_decode_tc_kernel<true>};      // (true: groups of more than 8 heads)
 
+// Which of rows (2), shares (3) and pieces (4) a launch goes by.
+int kv8_choice(long long rows, int resident, int dim, int max_ctx, double mean_ctx) {
+  return 2;
+}
+
 struct TcDevice {
   bool ready;
   int sms;
@@ -848,36 +856,63 @@ int tc_device(const TcDevice** out) {
   return 0;
 }
 
-// impl 2: by rows; 3: by shares; 0: the one that is expected to be faster.
-int launch_decode_tc(Kv8Args a, int max_ctx, long long sum_ctx, int impl, cudaStream_t stream) {
+// How a launch's rows are shared out; see kv8_decode_tc_kernel.
+struct TcPlan {
+  int csize, groups, ctas, parts;      // parts: 0 rows, > 0 pieces of a row, -1 shares
+};
+
+// impl 2: rows; 3: shares; 4: every row in as many pieces as there are CTAs for; 0: the one that is expected to be the
+// fastest, from the longest context and the sum of all as the host knows them (sum_ctx 0: unknown).
+int tc_plan(int nitems, int hq, int hkv, int max_ctx, long long sum_ctx, int impl, TcPlan* plan) {
   const TcDevice* d = nullptr;
   const int err = tc_device(&d);
   if (err) return err;
-  const int G = a.hq / a.hkv;
-  const long long rows = static_cast<long long>(a.nitems) * a.hkv;
-  int csize = 1;
-  for (int c = kMaxCluster; c > 1; --c)
-    if (d->resident[c] >= rows && tc_smem(c, G) <= static_cast<size_t>(d->smem_most)) {
-      csize = c;
-      break;
-    }
+  const int G = hq / hkv;
+  const long long rows = static_cast<long long>(nitems) * hkv;
   const int resident = d->resident[1] > 0 ? d->resident[1] : d->sms;
+  plan->csize = 1;
+  plan->groups = 1;
+  plan->parts = 0;
+  if (impl == 0) impl = kv8_choice(rows, resident, kD, max_ctx, nitems > 0 ? static_cast<double>(sum_ctx) / nitems : 0.0);
+  if (impl == 4 && rows > resident) impl = 2;
+  if (impl == 2) {
+    for (int c = kMaxCluster; c > 1; --c)
+      if (d->resident[c] >= rows && tc_smem(c, G) <= static_cast<size_t>(d->smem_most)) {
+        plan->csize = c;
+        break;
+      }
+  } else if (impl == 4) {
+    plan->parts = static_cast<int>(resident / rows);
+    plan->ctas = static_cast<int>(rows * plan->parts);
+    return 0;
+  } else {
+    plan->parts = -1;
+  }
   // as few groups (a divisor of the warps) as give every row one at once, else a warp to a row
-  int groups = 1;
   if (rows > resident) {
-    groups = kDecWarps;
+    plan->groups = kDecWarps;
     for (int k = 2; k < kDecWarps; ++k)
       if (kDecWarps % k == 0 && static_cast<long long>(resident) * k >= rows) {
-        groups = k;
+        plan->groups = k;
         break;
       }
   }
-  const bool by_shares = impl == 3;
-  if (by_shares) csize = 1;
-  const long long wanted = by_shares ? resident : (csize > 1 ? rows : (rows + groups - 1) / groups);
-  const int clusters = static_cast<int>(wanted < resident || csize > 1 ? wanted : resident);
+  if (plan->parts < 0) {
+    plan->ctas = resident;
+  } else {
+    const long long wanted = plan->csize > 1 ? rows : (rows + plan->groups - 1) / plan->groups;
+    plan->ctas = static_cast<int>((wanted < resident || plan->csize > 1 ? wanted : resident) * plan->csize);
+  }
+  return 0;
+}
+
+int launch_decode_tc(Kv8Args a, int max_ctx, long long sum_ctx, int impl, cudaStream_t stream) {
+  TcPlan plan;
+  const int err = tc_plan(a.nitems, a.hq, a.hkv, max_ctx, sum_ctx, impl, &plan);
+  if (err) return err;
+  const int G = a.hq / a.hkv, csize = plan.csize;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(clusters * csize);
+  cfg.gridDim = dim3(plan.ctas);
   cfg.blockDim = dim3(kDecThreads);
   cfg.dynamicSmemBytes = tc_smem(csize, G);
   cfg.stream = stream;
@@ -890,8 +925,7 @@ int launch_decode_tc(Kv8Args a, int max_ctx, long long sum_ctx, int impl, cudaSt
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  const int shares_flag = by_shares ? 1 : 0;
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, kTcKernels[G > 8 ? 1 : 0], a, groups, shares_flag));
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, kTcKernels[G > 8 ? 1 : 0], a, plan.groups, plan.parts));
 }
 
 #endif
@@ -899,6 +933,20 @@ int launch_decode_tc(Kv8Args a, int max_ctx, long long sum_ctx, int impl, cudaSt
 }  // namespace
 
 extern "C" {
+
+// Which way of sharing out (2, 3 or 4; 0: the CUDA cores) a launch on the tensor cores would go by impl 0, or an error as a negative number.
+int rl_kv8_decode_choice(int dtype, int nitems, int hq, int hkv, int max_ctx, long long sum_ctx) {
+#ifdef RL_KV8_TC
+  if (dtype == 1 && hq / hkv <= 16 && nitems > 0) {
+    const TcDevice* d = nullptr;
+    const int err = tc_device(&d);
+    if (err) return -err;
+    return kv8_choice(static_cast<long long>(nitems) * hkv, d->resident[1] > 0 ? d->resident[1] : d->sms, kD, max_ctx,
+                      static_cast<double>(sum_ctx) / nitems);
+  }
+#endif
+  return 0;
+}
 
 // The floats of the workspace for groups of G heads (kv8.cuh: Kv8Args::part).
 long long rl_kv8_part_floats(int G) { return static_cast<long long>(kMaxShares) * 2 * G * (kD + 4); }

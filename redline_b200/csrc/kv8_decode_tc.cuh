@@ -25,6 +25,7 @@
 // Where rows are shared out (see launch_decode_tc for the choice):
 //   rows    a cluster of up to 8 CTAs to a row, whose partial results meet in the first one's shared memory; or, with more rows
 //           than clusters can be resident, CTAs whose warps form groups that take a row each, one after another
+//   pieces  every row in as many pieces as there are CTAs for, which meet in global memory: few rows, and long ones
 //   shares  the launch's keys in equal shares, one to a group (kv8.cuh): for rows of very different lengths
 #pragma once
 
@@ -635,10 +636,10 @@ __device__ __noinline__ void tc_fold(unsigned char* parts, int stride, int n, in
   }
 }
 
-// groups: of the CTA's warps, a divisor of their number.  shares: the keys in equal shares (else: rows).
+// groups: of the CTA's warps, a divisor of their number.  parts: 0 rows, > 0 pieces of a row (one to a CTA), -1 shares.
 template <bool HI>
 __global__ void __launch_bounds__(kDecThreads, 1)
-kv8_decode_tc_kernel(const Kv8Args a, int groups, int by_shares) {
+kv8_decode_tc_kernel(const Kv8Args a, int groups, int parts) {
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ int start[kMaxItems + 1];
   __shared__ int last[kDecWarps];
@@ -651,19 +652,13 @@ kv8_decode_tc_kernel(const Kv8Args a, int groups, int by_shares) {
   float* slots = reinterpret_cast<float*>(smem + kDecWarps * kRingBytes);      // [csize][G][kPartLd], of the first CTA of a cluster
   if (csize > 1) cluster_arrive_begun();                       // (met before the first store into another CTA: it has begun by then)
   pdl_wait();
-  int units = 0, shares = 0, u = 0, end = 0;
-  if (by_shares) {
-    units = kv8_units(a, start);
-    shares = min(nclusters * groups, units);
-    const int mine = gi * nclusters + blockIdx.x;        // (neighbouring shares lie on different SMs)
-    if (mine < shares) {
-      u = kv8_share_begin(mine, units, shares);
-      end = kv8_share_begin(mine + 1, units, shares);
-    }
-  }
-  const int share = gi * nclusters + blockIdx.x, share_first = u;
+  const bool by_shares = parts < 0;
+  const Kv8Cut cut(by_shares ? kv8_units(a, start) : 0, nclusters * groups);
+  const int share = gi * nclusters + blockIdx.x;          // (neighbouring shares lie on different SMs)
+  int u = by_shares && share < cut.shares ? cut.begin(share) : 0;
+  const int share_first = u, end = by_shares && share < cut.shares ? cut.begin(share + 1) : 0;
   const int nrows = a.nitems * a.hkv;
-  int rowi = gi * nclusters + blockIdx.x / csize;
+  int rowi = parts > 0 ? blockIdx.x / parts : gi * nclusters + blockIdx.x / csize;
 #pragma unroll 1
   for (;;) {
     Kv8Segment s;
@@ -680,16 +675,23 @@ kv8_decode_tc_kernel(const Kv8Args a, int groups, int by_shares) {
       s.ctx = info.z;
       s.key_lo = a.window > 0 && s.ctx > a.window ? s.ctx - a.window : 0;
       s.key_hi = s.ctx;
-      s.whole = true;
-      rowi += groups * nclusters;
+      s.whole = parts == 0;
+      rowi = parts > 0 ? nrows : rowi + groups * nclusters;
       if (s.ctx <= 0) {                                  // (the same for the whole cluster)
         if (csize > 1) cluster_wait();
         continue;
       }
+      if (parts > 0) {                                   // this CTA's piece, in whole sub-blocks
+        const int j = blockIdx.x % parts, first = s.key_lo / kSub, all = (s.key_hi - 1) / kSub - first + 1;
+        const int b0 = first + static_cast<int>(static_cast<long long>(all) * j / parts);
+        const int b1 = first + static_cast<int>(static_cast<long long>(all) * (j + 1) / parts);
+        s.key_lo = max(s.key_lo, b0 * kSub);
+        s.key_hi = min(s.key_hi, b1 * kSub);
+      }
     }
     // ---- this warp's run of sub-blocks
     const int W = csize * gsize, wi = rank * gsize + wg;
-    const int first = s.key_lo / kSub, all = (s.key_hi - 1) / kSub - first + 1;
+    const int first = s.key_lo / kSub, all = s.key_hi > s.key_lo ? (s.key_hi - 1) / kSub - first + 1 : 0;
     const int per = all / W, rem = all - per * W;
     TcState<HI> st;
     tc_run<HI>(a, s, first + wi * per + min(wi, rem), per + (wi < rem ? 1 : 0), smem_u32(smem) + warp * kRingBytes, lane, st);
@@ -721,22 +723,24 @@ kv8_decode_tc_kernel(const Kv8Args a, int groups, int by_shares) {
       continue;                                          // (one row to a cluster: see the launch)
     }
     tc_group_barrier(1 + gi, gsize);
-    float* piece = by_shares && !s.whole ? a.part + (static_cast<size_t>(share) * 2 + (u == share_first ? 0 : 1)) * (G * (kD + 4)) : nullptr;
+    // (with pieces CTA x leaves the piece of share x)
+    float* piece = !s.whole ? a.part + (static_cast<size_t>(share) * 2 + (u == share_first ? 0 : 1)) * (G * (kD + 4)) : nullptr;
     tc_fold(smem + gi * gsize * kRingBytes, kRingBytes, gsize, wg, gsize, 1 + gi, G, out, piece, -1);
     if (piece != nullptr) {
       __threadfence();                                   // the piece, before it is counted
       tc_group_barrier(1 + gi, gsize);
+      const int s0 = parts > 0 ? blockIdx.x / parts * parts : cut.of(s.row_begin);
+      const int s1 = parts > 0 ? s0 + parts - 1 : cut.of(s.row_end - 1);
       if (gtid == 0) {
-        const int pieces = kv8_share_of(s.row_end - 1, units, shares) - kv8_share_of(s.row_begin, units, shares) + 1;
         int* c = a.counters + static_cast<size_t>(s.item) * a.hkv + s.kvh;
-        const int done = atomicAdd(c, 1) == pieces - 1;
+        const int done = atomicAdd(c, 1) == s1 - s0;
         if (done) *c = 0;
         last[gi] = done;
       }
       tc_group_barrier(1 + gi, gsize);
       if (last[gi]) {
         __threadfence();
-        kv8_merge<bf16>(a, s, units, shares, wg, gsize);
+        kv8_merge<bf16>(a.part, G, s0, s1, parts < 0 && cut.begin(s0) != s.row_begin ? 1 : 0, out, wg, gsize);
       }
     }
     tc_group_barrier(1 + gi, gsize);                     // before the rings are used again

@@ -236,7 +236,7 @@ DECODE = [  # heads, kv heads, head size, page, window, contexts
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
 @pytest.mark.parametrize("heads,kv_heads,dim,page,window,ctxs", DECODE)
-@pytest.mark.parametrize("impl", [0, 1, 2, 3])
+@pytest.mark.parametrize("impl", [0, 1, 2, 3, 4])
 def test_decode(heads, kv_heads, dim, page, window, ctxs, dtype, impl):
     if impl >= 2 and (dtype == "float32" or dim not in (64, 128) or heads > 16 * kv_heads):
         with pytest.raises(kernels.KernelError):
@@ -274,7 +274,7 @@ def test_decode_of_many_and_of_very_different_lengths(dim, dtype):
             near(out[s].view(1, heads, dim), ref, v[table[s][:-(-ctxs[s] // page)].long()], dtype)
         again = decode(qg, gpu, table, ctxs, heads, kv_heads, dim, page, 0, scale)
         assert torch.equal(out, again)
-        for kw in (dict(max_ctx=max(ctxs), sum_ctx=sum(ctxs)), dict(impl=1)) + ((dict(impl=2), dict(impl=3)) if dtype == "bfloat16" else ()):
+        for kw in (dict(max_ctx=max(ctxs), sum_ctx=sum(ctxs)), dict(impl=1)) + ((dict(impl=2), dict(impl=3), dict(impl=4)) if dtype == "bfloat16" else ()):
             told = decode(qg, gpu, table, ctxs, heads, kv_heads, dim, page, 0, scale, **kw)
             for s in range(len(ctxs)):      # (another way to share the work out: other last bits)
                 mine = v[table[s][:-(-ctxs[s] // page)].long()]
@@ -327,9 +327,13 @@ def test_decode_leaves_rows_without_keys(dim):
 
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
-@pytest.mark.parametrize("heads,kv_heads,dim,page,window", [(4, 2, 64, 16, 0), (32, 8, 64, 32, 0), (4, 1, 128, 64, 40), (10, 2, 80, 16, 0)])
-def test_decode_with_the_tokens_own_keys(heads, kv_heads, dim, page, window, dtype):
+@pytest.mark.parametrize("heads,kv_heads,dim,page,window", [(4, 2, 64, 16, 0), (32, 8, 64, 32, 0), (4, 1, 128, 64, 40), (10, 2, 80, 16, 0),
+                                                            (12, 1, 128, 16, 0), (20, 2, 64, 16, 35), (8, 1, 128, 32, 0)])
+@pytest.mark.parametrize("impl", [0, 2, 3, 4])
+def test_decode_with_the_tokens_own_keys(heads, kv_heads, dim, page, window, dtype, impl):
     """Rows [q | k | v] as the projection leaves them: stored and attended, against the write and the attention one after another."""
+    if impl and (dtype == "float32" or dim == 80):
+        pytest.skip("one way only")
     ctxs = (1, 2, 16, 17, 32, 64, 65, 200, 333)
     cache, table = filled([max(n - 1, 1) for n in ctxs], heads, kv_heads, dim, page, seed=8, poison=False)
     spare = int(table.max()) + 1
@@ -358,7 +362,7 @@ def test_decode_with_the_tokens_own_keys(heads, kv_heads, dim, page, window, dty
         out = torch.empty(len(ctxs), heads * dim, dtype=x.dtype, device=DEV)
         xg = x.to(DEV)
         kernels.kv8_attn_decode_rope(xg, xg.stride(0), *gpu, table.to(DEV), items, work, out, len(ctxs), heads, kv_heads, dim, page,
-                                     window, scale, cos.to(DEV), sin.to(DEV), status, max_ctx=max(ctxs), sum_ctx=sum(ctxs))
+                                     window, scale, cos.to(DEV), sin.to(DEV), status, max_ctx=max(ctxs), sum_ctx=sum(ctxs), impl=impl)
         assert torch.equal(xg.cpu(), x) and status.item() == 0
         positions = [n - 1 for n in ctxs]
         slots = [int(table[s, p // page]) * page + p % page for s, p in enumerate(positions)]

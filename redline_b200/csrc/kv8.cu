@@ -792,11 +792,6 @@ constexpr int kMaxShares = 1776;
 typedef void (*TcKernel)(Kv8Args, int, int);
 const TcKernel kTcKernels[2] = {kv8_decode_tc_kernel<false>, kv8_decode_tc_kernel<true>};      // (true: groups of more than 8 heads)
 
-// Which of rows (2), shares (3) and pieces (4) a launch goes by.
-int kv8_choice(long long rows, int resident, int dim, int max_ctx, double mean_ctx) {
-  return 2;
-}
-
 struct TcDevice {
   bool ready;
   int sms;
@@ -850,6 +845,7 @@ int tc_device(const TcDevice** out) {
       }
       d.resident[c] = k;
     }
+    if (d.resident[1] < 1) return static_cast<int>(cudaErrorNotSupported);
     d.ready = true;
   }
   *out = &d;
@@ -861,48 +857,84 @@ struct TcPlan {
   int csize, groups, ctas, parts;      // parts: 0 rows, > 0 pieces of a row, -1 shares
 };
 
+// The CTAs of a row's cluster, and as few groups (a divisor of the warps) as give every row one at once, else a warp to a row.
+void tc_rows(const TcDevice* d, long long rows, int G, int* csize, int* groups) {
+  *csize = *groups = 1;
+  for (int c = kMaxCluster; c > 1; --c)
+    if (d->resident[c] >= rows && tc_smem(c, G) <= static_cast<size_t>(d->smem_most)) {
+      *csize = c;
+      return;
+    }
+  if (rows > d->resident[1]) {
+    *groups = kDecWarps;
+    for (int k = 2; k < kDecWarps; ++k)
+      if (kDecWarps % k == 0 && static_cast<long long>(d->resident[1]) * k >= rows) {
+        *groups = k;
+        break;
+      }
+  }
+}
+
+// The pieces of a row where there is a CTA for each; the last to arrive adds them up, which takes some 0.2 us a piece.
+int tc_pieces(const TcDevice* d, long long rows) {
+  const long long k = d->resident[1] / rows;
+  return static_cast<int>(k < 48 ? k : 48);
+}
+
+// Which of rows (2), shares (3) and pieces (4) is expected to take the shortest, in us: a start; then the longest of a warp's
+// run of sub-blocks, what the busiest SM reads and what all bytes take.  Fitted to 1017 launches (kv heads 1, 2 and 8, groups of
+// four, 1 to 128 sequences of 256 to 131,072 keys, all equal or spread over L / 8 or L / 64 to L), over which the choice is 0.2 % longer
+// than the best (1.19 times at the worst).  Rows / shares / pieces, us, with 8 kv heads: one sequence of 65,536 keys 33 / 34 / 25 at head
+// size 64 and 47 / 48 / 38 at 128; 8 of 4,096 at head size 64 16 / 26 / 20; 24 of 1,024 to 8,192 at 128 76 / 62 / -.
+int kv8_choice(const TcDevice* d, int nitems, int hq, int hkv, int max_ctx, double mean) {
+  if (mean <= 0.0) return 2;
+  const long long rows = static_cast<long long>(nitems) * hkv;
+  int csize, groups;
+  tc_rows(d, rows, hq / hkv, &csize, &groups);
+  const bool narrow = kD == 64;
+  const double lat = narrow ? 0.81 : 1.20, sm_rate = narrow ? 42e3 : 58e3, rate = narrow ? 20e6 : 6.4e6;
+  const double key = kD * 2.0, bytes = rows * mean * key;
+  auto longest = [](double a, double b, double c) { return a > b ? (a > c ? a : c) : (b > c ? b : c); };
+  const double turns = csize == 1 ? (rows + static_cast<long long>(d->resident[1]) * groups - 1) / (static_cast<long long>(d->resident[1]) * groups) : 1;
+  const int per_row = csize * (kDecWarps / groups);
+  const double run = (max_ctx / kSub + per_row) / per_row + (turns - 1) * mean / kSub / per_row;
+  const double by_rows = (narrow ? 6.5 : 7.4) + longest(run * lat, (max_ctx + (groups * turns - 1) * mean) * key / csize / sm_rate, bytes / rate);
+  const double by_shares = (narrow ? 17.1 : 21.5) + bytes / (narrow ? 4.12e6 : 5.09e6);
+  double by_pieces = 1e30;
+  if (rows <= d->resident[1]) {
+    const int k = tc_pieces(d, rows);
+    by_pieces = (narrow ? 11.7 : 14.6) + longest((max_ctx / kSub + k * kDecWarps) / (k * kDecWarps) * lat, max_ctx * key / k / sm_rate, bytes / (narrow ? 7.1e6 : 7.8e6));
+  }
+  return by_rows <= by_shares && by_rows <= by_pieces ? 2 : (by_pieces <= by_shares ? 4 : 3);
+}
+
 // impl 2: rows; 3: shares; 4: every row in as many pieces as there are CTAs for; 0: the one that is expected to be the
 // fastest, from the longest context and the sum of all as the host knows them (sum_ctx 0: unknown).
 int tc_plan(int nitems, int hq, int hkv, int max_ctx, long long sum_ctx, int impl, TcPlan* plan) {
   const TcDevice* d = nullptr;
   const int err = tc_device(&d);
   if (err) return err;
-  const int G = hq / hkv;
   const long long rows = static_cast<long long>(nitems) * hkv;
-  const int resident = d->resident[1] > 0 ? d->resident[1] : d->sms;
+  const int resident = d->resident[1];
   plan->csize = 1;
   plan->groups = 1;
   plan->parts = 0;
-  if (impl == 0) impl = kv8_choice(rows, resident, kD, max_ctx, nitems > 0 ? static_cast<double>(sum_ctx) / nitems : 0.0);
+  if (impl == 0) impl = kv8_choice(d, nitems, hq, hkv, max_ctx, static_cast<double>(sum_ctx) / nitems);
   if (impl == 4 && rows > resident) impl = 2;
-  if (impl == 2) {
-    for (int c = kMaxCluster; c > 1; --c)
-      if (d->resident[c] >= rows && tc_smem(c, G) <= static_cast<size_t>(d->smem_most)) {
-        plan->csize = c;
-        break;
-      }
-  } else if (impl == 4) {
-    plan->parts = static_cast<int>(resident / rows);
+  if (impl == 4) {
+    plan->parts = tc_pieces(d, rows);
     plan->ctas = static_cast<int>(rows * plan->parts);
     return 0;
-  } else {
+  }
+  tc_rows(d, rows, hq / hkv, &plan->csize, &plan->groups);
+  if (impl == 3) {
+    plan->csize = 1;
     plan->parts = -1;
-  }
-  // as few groups (a divisor of the warps) as give every row one at once, else a warp to a row
-  if (rows > resident) {
-    plan->groups = kDecWarps;
-    for (int k = 2; k < kDecWarps; ++k)
-      if (kDecWarps % k == 0 && static_cast<long long>(resident) * k >= rows) {
-        plan->groups = k;
-        break;
-      }
-  }
-  if (plan->parts < 0) {
     plan->ctas = resident;
-  } else {
-    const long long wanted = plan->csize > 1 ? rows : (rows + plan->groups - 1) / plan->groups;
-    plan->ctas = static_cast<int>((wanted < resident || plan->csize > 1 ? wanted : resident) * plan->csize);
+    return 0;
   }
+  const long long wanted = plan->csize > 1 ? rows : (rows + plan->groups - 1) / plan->groups;
+  plan->ctas = static_cast<int>((wanted < resident || plan->csize > 1 ? wanted : resident) * plan->csize);
   return 0;
 }
 
@@ -941,8 +973,7 @@ int rl_kv8_decode_choice(int dtype, int nitems, int hq, int hkv, int max_ctx, lo
     const TcDevice* d = nullptr;
     const int err = tc_device(&d);
     if (err) return -err;
-    return kv8_choice(static_cast<long long>(nitems) * hkv, d->resident[1] > 0 ? d->resident[1] : d->sms, kD, max_ctx,
-                      static_cast<double>(sum_ctx) / nitems);
+    return kv8_choice(d, nitems, hq, hkv, max_ctx, static_cast<double>(sum_ctx) / nitems);
   }
 #endif
   return 0;

@@ -12,6 +12,7 @@ import math
 import os
 from concurrent.futures import ThreadPoolExecutor
 from ctypes import c_float, c_int, c_longlong, c_uint, c_void_p
+from functools import lru_cache
 from typing import Dict, Optional, Tuple
 
 import torch
@@ -674,10 +675,12 @@ def _kv8(head_dim: int) -> ctypes.CDLL:
     return _lib(f"kv8_d{head_dim}", "kv8.cu", {"RL_HEAD_DIM": head_dim})
 
 
+# (A step of single tokens makes one of these calls per layer, and its GPU time is a few us: every attribute of a tensor is asked
+# for once, since each costs 0.1 to 0.3 us: kv8_write's call with its launch went from 15.7 to 12.9 us of one core.)
 def _kv8_check(what: str, kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch.Tensor, vscale: torch.Tensor, num_heads: int,
                num_kv_heads: int, head_dim: int, page_size: int) -> None:
     """The cache's tensors have the types and shapes that the kernels take."""
-    shape = kcache.shape
+    shape, scales = kcache.shape, kscale.shape
     if (kcache.dtype is not KV8_DTYPE or vcache.dtype is not KV8_DTYPE or kscale.dtype is not KV8_SCALE_DTYPE
             or vscale.dtype is not KV8_SCALE_DTYPE):
         raise KernelError(f"{what}: the cache is float8_e4m3fn and its scales float8_e8m0fnu; got {kcache.dtype}, "
@@ -686,41 +689,55 @@ def _kv8_check(what: str, kcache: torch.Tensor, vcache: torch.Tensor, kscale: to
         raise KernelError(f"{what}: pages of 16, 32 or 64 tokens; got {page_size}")
     if num_kv_heads <= 0 or num_heads <= 0 or num_heads % num_kv_heads:
         raise KernelError(f"{what}: {num_heads} query heads are no multiple of {num_kv_heads} kv heads")
-    if (len(shape) != 4 or shape[1] != num_kv_heads or shape[2] != page_size or shape[3] != head_dim
-            or vcache.shape != shape or kscale.shape != shape[:2] or vscale.shape != shape[:2]):
+    if (len(shape) != 4 or shape[1] != num_kv_heads or shape[2] != page_size or shape[3] != head_dim or vcache.shape != shape
+            or len(scales) != 2 or scales[0] != shape[0] or scales[1] != num_kv_heads or vscale.shape != scales):
         raise KernelError(f"{what}: caches [pages, {num_kv_heads}, {page_size}, {head_dim}] and scales [pages, {num_kv_heads}]; "
                           f"got {tuple(shape)}, {tuple(vcache.shape)}, {tuple(kscale.shape)}, {tuple(vscale.shape)}")
     if not (kcache.is_contiguous() and vcache.is_contiguous() and kscale.is_contiguous() and vscale.is_contiguous()):
         raise KernelError(f"{what}: the cache and its scales must be contiguous")
     if (kcache.data_ptr() | vcache.data_ptr()) % 16:
         raise KernelError(f"{what}: the cache must start on a 16-byte boundary")
-    if not kcache.is_cuda or not (kcache.device == vcache.device == kscale.device == vscale.device):
+    at = kcache.get_device()
+    if at < 0 or vcache.get_device() != at or kscale.get_device() != at or vscale.get_device() != at:
         raise KernelError("redline_b200 kernels run on CUDA tensors only; there is no CPU fallback")
 
 
-def _kv8_rows(what: str, name: str, x: torch.Tensor, stride: int, columns: int, cache: torch.Tensor) -> None:
-    """``x``: rows of at least ``columns`` elements, ``stride`` apart, in 16-byte pieces, on the cache's device."""
-    piece = 8 if x.dtype is torch.bfloat16 else 4
-    if x.device != cache.device:
-        raise KernelError(f"{what}: {name} is on {x.device}, the cache on {cache.device}")
-    if x.dim() != 2 or x.stride(1) != 1 or x.stride(0) != stride or x.shape[1] < columns or (x.shape[0] > 1 and stride < columns):
-        raise KernelError(f"{what}: {name} must be rows of {columns} contiguous elements, {stride} apart; got "
-                          f"{tuple(x.shape)} with strides {x.stride()}")
-    if stride % piece or x.data_ptr() % 16:
+def _kv8_rows(what: str, name: str, x: torch.Tensor, stride: Optional[int], columns: int, at: int) -> int:
+    """``x``: rows of at least ``columns`` elements, ``stride`` apart (None: as they are), in 16-byte pieces, on the cache's device.
+    Returns the stride."""
+    shape, strides = x.shape, x.stride()
+    if x.get_device() != at:
+        raise KernelError(f"{what}: {name} is on {x.device}, the cache is not")
+    if (len(shape) != 2 or strides[1] != 1 or (stride is not None and strides[0] != stride) or shape[1] < columns
+            or (shape[0] > 1 and strides[0] < columns)):
+        raise KernelError(f"{what}: {name} must be rows of {columns} contiguous elements, {stride or strides[0]} apart; got "
+                          f"{tuple(shape)} with strides {strides}")
+    if strides[0] % (8 if x.dtype is torch.bfloat16 else 4) or x.data_ptr() % 16:
         raise KernelError(f"{what}: the rows of {name} must start on 16-byte boundaries")
+    return strides[0]
 
 
-def _kv8_ints(what: str, cache: torch.Tensor, **tensors: torch.Tensor) -> None:
+def _kv8_ints(what: str, at: int, **tensors: torch.Tensor) -> None:
     for name, t in tensors.items():
-        if t.dtype is not torch.int32 or t.device != cache.device or not t.is_contiguous():
-            raise KernelError(f"{what}: {name} must be a contiguous int32 tensor on {cache.device}; got {t.dtype} on {t.device}")
+        if t.dtype is not torch.int32 or t.get_device() != at or not t.is_contiguous():
+            raise KernelError(f"{what}: {name} must be a contiguous int32 tensor on the cache's device; got {t.dtype} on {t.device}")
 
 
-def _kv8_tables(what: str, cos: torch.Tensor, sin: torch.Tensor, head_dim: int, cache: torch.Tensor) -> None:
-    if (cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or cos.dim() != 2 or cos.shape[1] != head_dim // 2
-            or sin.shape != cos.shape or not cos.is_contiguous() or not sin.is_contiguous() or cos.device != cache.device
-            or sin.device != cache.device or (cos.data_ptr() | sin.data_ptr()) % 16):
+def _kv8_tables(what: str, cos: torch.Tensor, sin: torch.Tensor, head_dim: int, at: int) -> int:
+    """Returns the number of positions."""
+    shape = cos.shape
+    if (cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or len(shape) != 2 or shape[1] != head_dim // 2
+            or sin.shape != shape or not cos.is_contiguous() or not sin.is_contiguous() or cos.get_device() != at
+            or sin.get_device() != at or (cos.data_ptr() | sin.data_ptr()) % 16):
         raise KernelError(f"{what}: cos / sin must be contiguous float32 [positions, {head_dim // 2}] on the cache's device")
+    return shape[0]
+
+
+def _kv8_scale(what: str, window: int, scale: float) -> None:
+    if window < 0:
+        raise KernelError(f"{what}: a window of {window} keys")
+    if not 0.0 < scale < math.inf:
+        raise KernelError(f"{what}: the scores' scale must be positive; got {scale}")
 
 
 def kv8_write(qkv: torch.Tensor, positions: torch.Tensor, slots: Optional[torch.Tensor], cos: Optional[torch.Tensor],
@@ -738,33 +755,42 @@ def kv8_write(qkv: torch.Tensor, positions: torch.Tensor, slots: Optional[torch.
     left out of the scale.  The tokens of a page follow one another in a call: of several runs in one page the first is
     stored, and the others set bit 8 of ``status`` (not in page 0, which belongs to the padding rows)."""
     what = "kv8_write"
-    T = tokens if tokens is not None else qkv.shape[0]
+    rows = qkv.shape[0]
+    T = tokens if tokens is not None else rows
     _kv8_check(what, kcache, vcache, kscale, vscale, num_heads, num_kv_heads, head_dim, page_size)
-    _kv8_rows(what, "qkv", qkv, qkv.stride(0), (num_heads + 2 * num_kv_heads) * head_dim, kcache)
-    _kv8_ints(what, kcache, positions=positions, status=status)
-    if not 0 <= T <= qkv.shape[0] or positions.numel() < T:
-        raise KernelError(f"{what}: {T} tokens of {qkv.shape[0]} rows and {positions.numel()} positions")
+    at = kcache.get_device()
+    stride = _kv8_rows(what, "qkv", qkv, None, (num_heads + 2 * num_kv_heads) * head_dim, at)
+    _kv8_ints(what, at, positions=positions, status=status)
+    if not 0 <= T <= rows or positions.numel() < T:
+        raise KernelError(f"{what}: {T} tokens of {rows} rows and {positions.numel()} positions")
     if slots is not None:
-        _kv8_ints(what, kcache, slots=slots)
+        _kv8_ints(what, at, slots=slots)
         if slots.numel() < T:
             raise KernelError(f"{what}: {slots.numel()} slots for {T} tokens")
     if (cos is None) != (sin is None):
         raise KernelError(f"{what}: cos and sin come together")
-    if cos is not None:
-        _kv8_tables(what, cos, sin, head_dim, kcache)
+    max_pos = _kv8_tables(what, cos, sin, head_dim, at) if cos is not None else 2 ** 31 - 1
+    q_stride = 0
     if q_out is not None:
-        _kv8_rows(what, "q_out", q_out, q_out.stride(0), num_heads * head_dim, kcache)
+        q_stride = _kv8_rows(what, "q_out", q_out, None, num_heads * head_dim, at)
         if q_out.dtype is not qkv.dtype or q_out.shape[0] < T:
             raise KernelError(f"{what}: q_out must be {qkv.dtype} with {T} rows")
     f = _fn(_kv8(head_dim), "rl_kv8_write",
             [c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
              c_int, c_int, c_int, c_int, c_int, c_int, c_longlong, c_void_p, c_void_p])
     with _on(kcache):
-        _check(f(_code(qkv.dtype), qkv.data_ptr(), qkv.stride(0), positions.data_ptr(), _ptr(slots), _ptr(cos), _ptr(sin),
+        _check(f(_code(qkv.dtype), qkv.data_ptr(), stride, positions.data_ptr(), _ptr(slots), _ptr(cos), _ptr(sin),
                  kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(), vscale.data_ptr(), _ptr(q_out),
-                 0 if q_out is None else q_out.stride(0), T, num_heads, num_kv_heads, page_size,
-                 cos.shape[0] if cos is not None else 2 ** 31 - 1, kcache.shape[0] * page_size, status.data_ptr(), _stream()),
+                 q_stride, T, num_heads, num_kv_heads, page_size, max_pos, kcache.shape[0] * page_size, status.data_ptr(), _stream()),
                what)
+
+
+@lru_cache(maxsize=None)
+def kv8_part_floats(num_heads: int, num_kv_heads: int, head_dim: int) -> int:
+    """The floats of the first tensor of ``kv8_decode_workspace``, whatever the number of items."""
+    f = _kv8(head_dim).rl_kv8_part_floats
+    f.restype, f.argtypes = c_longlong, [c_int]
+    return f(num_heads // num_kv_heads)
 
 
 def kv8_decode_workspace(nitems: int, num_heads: int, num_kv_heads: int, head_dim: int,
@@ -772,9 +798,7 @@ def kv8_decode_workspace(nitems: int, num_heads: int, num_kv_heads: int, head_di
     """What ``kv8_attn_decode`` and ``kv8_attn_decode_rope`` need beside their arguments for up to ``nitems`` items: room for
     the pieces of rows that are shared out, and counters, which launches leave zero.  One stream uses a workspace at a time
     (two graphs that may run side by side need one each)."""
-    f = _kv8(head_dim).rl_kv8_part_floats
-    f.restype, f.argtypes = c_longlong, [c_int]
-    return (torch.empty(f(num_heads // num_kv_heads), dtype=torch.float32, device=device),
+    return (torch.empty(kv8_part_floats(num_heads, num_kv_heads, head_dim), dtype=torch.float32, device=device),
             torch.zeros(max(nitems, 1) * num_kv_heads, dtype=torch.int32, device=device))
 
 
@@ -782,41 +806,39 @@ def _kv8_decode(what: str, q, q_stride, kcache, vcache, kscale, vscale, block_ta
                 num_kv_heads, head_dim, page_size, window, scale, cos, sin, status, max_ctx, sum_ctx, impl) -> None:
     store = cos is not None
     _kv8_check(what, kcache, vcache, kscale, vscale, num_heads, num_kv_heads, head_dim, page_size)
-    _kv8_rows(what, "qkv" if store else "q", q, q_stride, (num_heads + (2 * num_kv_heads if store else 0)) * head_dim, kcache)
-    _kv8_rows(what, "out", out, out.stride(0), num_heads * head_dim, kcache)
+    at = kcache.get_device()
+    _kv8_rows(what, "qkv" if store else "q", q, q_stride, (num_heads + (2 * num_kv_heads if store else 0)) * head_dim, at)
+    out_stride = _kv8_rows(what, "out", out, None, num_heads * head_dim, at)
     part, counters = workspace
-    _kv8_ints(what, kcache, block_table=block_table, items=items, counters=counters)
+    _kv8_ints(what, at, block_table=block_table, items=items, counters=counters)
     if out.dtype is not q.dtype:
         raise KernelError(f"{what}: out must be {q.dtype}")
     if nitems < 0 or items.numel() < 4 * nitems or items.data_ptr() % 16:
         raise KernelError(f"{what}: items must be int32 [{nitems}, 4] on a 16-byte boundary")
     if block_table.dim() != 2:
         raise KernelError(f"{what}: block_table must be [sequences, blocks]")
-    if window < 0:
-        raise KernelError(f"{what}: a window of {window} keys")
-    lib = _kv8(head_dim)
-    need = _kv8_part.get((head_dim, num_heads // num_kv_heads))
-    if need is None:
-        g = lib.rl_kv8_part_floats
-        g.restype, g.argtypes = c_longlong, [c_int]
-        need = _kv8_part[(head_dim, num_heads // num_kv_heads)] = g(num_heads // num_kv_heads)
-    if part.numel() < need or part.dtype is not torch.float32 or part.device != kcache.device or counters.numel() < nitems * num_kv_heads:
+    blocks = block_table.shape[1]
+    _kv8_scale(what, window, scale)
+    need = kv8_part_floats(num_heads, num_kv_heads, head_dim)
+    if part.numel() < need or part.dtype is not torch.float32 or part.get_device() != at or counters.numel() < nitems * num_kv_heads:
         raise KernelError(f"{what}: the workspace is too small (kv8_decode_workspace)")
+    max_pos = 0
     if store:
-        _kv8_tables(what, cos, sin, head_dim, kcache)
-        _kv8_ints(what, kcache, status=status)
-    capacity = block_table.shape[1] * page_size
-    max_ctx = min(max_ctx, capacity) if max_ctx > 0 else capacity
-    seen = min(max_ctx, window) if window > 0 else max_ctx
-    f = _fn(lib, "rl_kv8_attn_decode",
+        max_pos = _kv8_tables(what, cos, sin, head_dim, at)
+        _kv8_ints(what, at, status=status)
+    capacity = blocks * page_size
+    seen = min(max_ctx, capacity) if max_ctx > 0 else capacity
+    if window > 0:
+        seen, sum_ctx = min(seen, window), min(sum_ctx, nitems * window)
+    f = _fn(_kv8(head_dim), "rl_kv8_attn_decode",
             [c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p,
              c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_int, c_int, c_longlong, c_void_p,
              c_int, c_longlong, c_int, c_void_p])
     with _on(kcache):
         _check(f(_code(q.dtype), q.data_ptr(), q_stride, kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(),
-                 vscale.data_ptr(), block_table.data_ptr(), block_table.shape[1], items.data_ptr(), nitems, part.data_ptr(),
-                 counters.data_ptr(), out.data_ptr(), out.stride(0), num_heads, num_kv_heads, page_size, window, float(scale),
-                 _ptr(cos), _ptr(sin), cos.shape[0] if store else 0, 1 if store else 0, kcache.shape[0] * page_size,
+                 vscale.data_ptr(), block_table.data_ptr(), blocks, items.data_ptr(), nitems, part.data_ptr(),
+                 counters.data_ptr(), out.data_ptr(), out_stride, num_heads, num_kv_heads, page_size, window, scale,
+                 _ptr(cos), _ptr(sin), max_pos, 1 if store else 0, kcache.shape[0] * page_size,
                  status.data_ptr() if store else None, seen, sum_ctx, impl, _stream()),
                what, 2 if store else 1)
 
@@ -852,7 +874,18 @@ def kv8_attn_decode_rope(qkv: torch.Tensor, q_stride: int, kcache: torch.Tensor,
                 num_heads, num_kv_heads, head_dim, page_size, window, scale, cos, sin, status, max_ctx, sum_ctx, impl)
 
 
-_kv8_part: Dict[Tuple[int, int], int] = {}
+def kv8_decode_choice(dtype: torch.dtype, nitems: int, num_heads: int, num_kv_heads: int, head_dim: int, max_ctx: int, sum_ctx: int,
+                      window: int, device: torch.device) -> int:
+    """Which way ``kv8_attn_decode`` with impl 0 would share out a launch of ``nitems`` rows of at most ``max_ctx`` and together
+    ``sum_ctx`` keys (its impl 2, 3 or 4; 0: the CUDA cores): for callers that capture launches and replay them at other lengths."""
+    if window > 0:
+        max_ctx, sum_ctx = min(max_ctx, window), min(sum_ctx, nitems * window)
+    f = _fn(_kv8(head_dim), "rl_kv8_decode_choice", [c_int, c_int, c_int, c_int, c_int, c_longlong])
+    with torch.cuda.device(device):
+        got = f(_code(dtype), nitems, num_heads, num_kv_heads, max_ctx, sum_ctx)
+    if got < 0:
+        raise KernelError(f"kv8_decode_choice: CUDA error {-got}")
+    return got
 
 
 def kv8_attn_prefill(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch.Tensor,
@@ -864,18 +897,17 @@ def kv8_attn_prefill(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, vcach
     applies (bfloat16 at head sizes 64 and 128: tcgen05; else CUDA cores); 1: CUDA cores; 3: the tcgen05 kernel or an error."""
     what = "kv8_attn_prefill"
     _kv8_check(what, kcache, vcache, kscale, vscale, num_heads, num_kv_heads, head_dim, page_size)
-    _kv8_rows(what, "q", q, q_stride, num_heads * head_dim, kcache)
-    _kv8_rows(what, "out", out, out.stride(0), num_heads * head_dim, kcache)
-    _kv8_ints(what, kcache, block_table=block_table, tile_seq=tile_seq, tile_tok=tile_tok, tile_rows=tile_rows,
-              positions=positions)
+    at = kcache.get_device()
+    _kv8_rows(what, "q", q, q_stride, num_heads * head_dim, at)
+    out_stride = _kv8_rows(what, "out", out, None, num_heads * head_dim, at)
+    _kv8_ints(what, at, block_table=block_table, tile_seq=tile_seq, tile_tok=tile_tok, tile_rows=tile_rows, positions=positions)
     if out.dtype is not q.dtype:
         raise KernelError(f"{what}: out must be {q.dtype}")
     if tiles < 0 or min(tile_seq.numel(), tile_tok.numel(), tile_rows.numel()) < tiles:
         raise KernelError(f"{what}: lists of {tile_seq.numel()}, {tile_tok.numel()} and {tile_rows.numel()} for {tiles} tiles")
     if block_table.dim() != 2:
         raise KernelError(f"{what}: block_table must be [sequences, blocks]")
-    if window < 0:
-        raise KernelError(f"{what}: a window of {window} keys")
+    _kv8_scale(what, window, scale)
     if tiles == 0:
         return
     f = _fn(_kv8(head_dim), "rl_kv8_attn_prefill",
@@ -884,8 +916,8 @@ def kv8_attn_prefill(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, vcach
     with _on(kcache):
         _check(f(_code(q.dtype), q.data_ptr(), q_stride, kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(), vscale.data_ptr(),
                  block_table.data_ptr(), block_table.shape[1], tile_seq.data_ptr(), tile_tok.data_ptr(), tile_rows.data_ptr(),
-                 positions.data_ptr(), out.data_ptr(), out.stride(0), tiles, num_heads, num_kv_heads, page_size, window,
-                 float(scale), impl, tc_status(q.device).data_ptr(), _stream()), what)
+                 positions.data_ptr(), out.data_ptr(), out_stride, tiles, num_heads, num_kv_heads, page_size, window,
+                 scale, impl, tc_status(q.device).data_ptr(), _stream()), what)
 
 
 # ------------------------------------------- row-wise kernels of blocks with norms on both sides

@@ -25,6 +25,8 @@ def add_engine_options(ap: argparse.ArgumentParser) -> None:
     g.add_argument("--max-logit-rows", type=int, default=0)
     g.add_argument("--block-size", type=int, default=16, help="tokens per cache page")
     g.add_argument("--kv-cache-tokens", type=int, default=0, help="cache capacity in tokens (default: from memory)")
+    g.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "fp8"],
+                   help="what the cache holds keys and values in: the type of --dtype (default), or 8 bits")
     g.add_argument("--gpu-memory-utilization", type=float, default=None, help="device memory fraction to use")
     g.add_argument("--no-cuda-graphs", action="store_true", help="disable CUDA graph replay for decode")
     g.add_argument("--no-async", action="store_true", help="disable asynchronous (pipelined) scheduling")
@@ -39,7 +41,7 @@ def engine_options(args: argparse.Namespace, default_utilization: float = 0.9) -
     return dict(
         dtype=args.dtype, max_seqs=args.max_seqs, max_batched_tokens=args.max_batched_tokens,
         max_seq_len=args.max_seq_len, max_logit_rows=args.max_logit_rows, block_size=args.block_size,
-        kv_cache_tokens=args.kv_cache_tokens, gpu_memory_utilization=util,
+        kv_cache_tokens=args.kv_cache_tokens, kv_cache_dtype=args.kv_cache_dtype, gpu_memory_utilization=util,
         cuda_graphs=not args.no_cuda_graphs, async_scheduling=not args.no_async,
         mix_prefill_decode=not args.no_mixed_batches, nvtx_layers=args.nvtx_layers,
         track_memory=args.track_memory, device=args.device)

@@ -2,7 +2,8 @@
 layer call that owns a cache and every tensor its mixer caches, a view
 [pages, *leading axes, page_size, last axis] (for attention: K and V
 [pages, heads, page_size, head_dim], so that a (page, head) is one contiguous
-[page_size, head_dim] box); and per state-keeping layer call one pool [slots, *state shape]
+[page_size, head_dim] box; for a tensor kept per page [pages, *axes]); and per
+state-keeping layer call one pool [slots, *state shape]
 (reference layout of the pages: src/cuda/model/kv_cache.cpp:17-52, src/cuda/kernels/kernels.h:15-27)."""
 
 from __future__ import annotations
@@ -12,12 +13,17 @@ from typing import Dict, List, Optional, Sequence
 import torch
 
 from ..parts.base import LayerCache
-from ..parts.spec import StateSpec
+from ..parts.spec import CacheTensor, StateSpec
 from .manager import GroupInfo
 
 
 def bytes_per_page(groups: Sequence[GroupInfo], page_size: int, elem_size: int) -> List[int]:
-    return [len(g.owners) * g.spec.elements_per_token() * page_size * elem_size for g in groups]
+    def of(t: CacheTensor) -> int:
+        return t.page_elements(page_size) * (elem_size if t.dtype is None else getattr(torch, t.dtype).itemsize)
+    return [len(g.owners) * sum(of(t) for t in g.spec.tensors) for g in groups]
+
+
+ALIGN = 256        # bytes: where the tensors of a group that mixes types start
 
 
 class CacheStorage:
@@ -27,6 +33,9 @@ class CacheStorage:
         self.pools: List[torch.Tensor] = []
         self._by_owner: Dict[int, LayerCache] = {}
         for gi, (g, n) in enumerate(zip(groups, pages_per_group)):
+            if g.spec.typed():
+                self._add_typed(gi, g, n, dtype, device)
+                continue
             per_owner = n * page_size * g.spec.elements_per_token()
             pool = torch.zeros(max(len(g.owners), 1) * per_owner, dtype=dtype, device=device)
             self.pools.append(pool)
@@ -38,6 +47,22 @@ class CacheStorage:
                     views[t.name] = pool[off:off + size].view((n,) + tuple(t.shape[:-1]) + (page_size, t.shape[-1]))
                     off += size
                 self._by_owner[owner] = LayerCache(gi, views, True)
+
+    def _add_typed(self, gi: int, g: GroupInfo, n: int, dtype: torch.dtype, device: torch.device) -> None:
+        """A group whose tensors name their types: one allocation of bytes."""
+        parts = []                  # (name, type, first byte, bytes, shape) within an owner's share
+        per_owner = 0
+        for t in g.spec.tensors:
+            dt = dtype if t.dtype is None else getattr(torch, t.dtype)
+            size = n * t.page_elements(self.page_size) * dt.itemsize
+            parts.append((t.name, dt, per_owner, size, (n,) + t.page_shape(self.page_size)))
+            per_owner += (size + ALIGN - 1) // ALIGN * ALIGN
+        pool = torch.zeros(max(len(g.owners), 1) * per_owner, dtype=torch.uint8, device=device)
+        self.pools.append(pool)
+        for j, owner in enumerate(g.owners):
+            first = j * per_owner
+            self._by_owner[owner] = LayerCache(gi, {name: pool[first + at:first + at + size].view(dt).view(shape)
+                                                    for name, dt, at, size, shape in parts}, True)
 
     def of_owner(self, owner: int, write: bool) -> LayerCache:
         c = self._by_owner[owner]

@@ -10,6 +10,7 @@ from typing import Any, Dict
 import torch
 
 DTYPES = {"bfloat16": torch.bfloat16, "bf16": torch.bfloat16, "float32": torch.float32, "fp32": torch.float32}
+KV_CACHE_DTYPES = {"auto": None, "fp8": torch.float8_e4m3fn}
 
 
 @dataclass
@@ -22,6 +23,7 @@ class EngineConfig:
     max_logit_rows: int = 0            # 0: max(max_num_seqs, 64)
     block_size: int = 16               # tokens per cache page
     kv_cache_tokens: int = 0           # 0: from the memory budget
+    kv_cache_dtype: str = "auto"       # "auto": the cache holds keys and values in dtype; "fp8": in 8 bits
     gpu_memory_utilization: float = 0.90
     cuda_graphs: bool = True
     async_scheduling: bool = True
@@ -52,6 +54,8 @@ class EngineConfig:
     def validate(self) -> None:
         if self.dtype not in DTYPES:
             raise ValueError(f"dtype must be one of {sorted(DTYPES)}, got {self.dtype}")
+        if self.kv_cache_dtype not in KV_CACHE_DTYPES:
+            raise ValueError(f"kv_cache_dtype must be one of {sorted(KV_CACHE_DTYPES)}, got {self.kv_cache_dtype}")
         if self.block_size not in (16, 32, 64):
             raise ValueError(f"block_size must be 16, 32 or 64, got {self.block_size}")
         if self.max_num_seqs <= 0 or self.max_num_batched_tokens <= 0 or self.max_seq_len <= 1:
@@ -62,6 +66,10 @@ class EngineConfig:
     @property
     def torch_dtype(self) -> torch.dtype:
         return DTYPES[self.dtype]
+
+    @property
+    def torch_cache_dtype(self) -> torch.dtype:
+        return KV_CACHE_DTYPES[self.kv_cache_dtype] or self.torch_dtype
 
     @property
     def logit_rows(self) -> int:

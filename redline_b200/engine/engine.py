@@ -455,7 +455,7 @@ class Engine:
             "architecture": self.model_config.architecture,
             "dtype": self.cfg.dtype,
             "config": {k: getattr(self.cfg, k) for k in (
-                "max_num_seqs", "max_num_batched_tokens", "max_seq_len", "block_size", "kv_cache_tokens",
+                "max_num_seqs", "max_num_batched_tokens", "max_seq_len", "block_size", "kv_cache_tokens", "kv_cache_dtype",
                 "gpu_memory_utilization", "cuda_graphs", "async_scheduling", "mix_prefill_decode", "nvtx_layers",
                 "track_memory")},
             "cache_groups": [{"kind": g.spec.kind, "window": g.spec.window, "layers": len(g.owners),

@@ -134,18 +134,20 @@ def linear_work(rows: int, w: torch.Tensor, act_elem: int, out_elem: int) -> tup
     return (float(w.numel() * w.element_size() + rows * k * act_elem + rows * n * out_elem), 2.0 * rows * n * k)
 
 
-def attention_work(host, num_heads: int, num_kv_heads: int, head_dim: int, window: int, elem: int, chunk: int = 0) -> dict:
+def attention_work(host, num_heads: int, num_kv_heads: int, head_dim: int, window: int, elem: int, chunk: int = 0,
+                   kv_elem: int = 0) -> dict:
     """What the attention of a step has to read and compute, from the step's host-side description
     (``host.q_len`` / ``host.start_pos`` per sequence): {"decode": (bytes, flops), "prefill": (bytes, flops)}.
     A single token reads the keys and values of its context once per kv head; a portion of n tokens
     after p earlier ones reads its p + n keys and values once and computes over the causal part.  ``window`` > 0 or
-    ``chunk`` > 0: only the last so many keys, or those of the token's chunk of so many positions, are seen."""
+    ``chunk`` > 0: only the last so many keys, or those of the token's chunk of so many positions, are seen.  ``elem``: bytes of
+    a number, in the cache ``kv_elem`` (0: the same)."""
 
     def seen(pos: int) -> int:
         return min(pos + 1, window) if window > 0 else (pos % chunk + 1 if chunk > 0 else pos + 1)
 
     dec_b = dec_f = pre_b = pre_f = 0.0
-    kv_row = 2.0 * num_kv_heads * head_dim * elem            # K and V of one token
+    kv_row = 2.0 * num_kv_heads * head_dim * (kv_elem or elem)      # K and V of one token
     q_row = 2.0 * num_heads * head_dim * elem                # q read, output written
     for n, p in zip(host.q_len, host.start_pos):
         if n == 1:

@@ -35,7 +35,7 @@ GRAPH_MAX_ROWS = 1024          # no graph is captured for more rows than this
 # head is then bound by its products and not by reading its table for every 64 rows).
 SCORE_LOGITS_BYTES = 256 << 20
 STATUS_MESSAGES = {1: "a token id outside the vocabulary", 2: "a position beyond the rotary table",
-                   4: "a cache slot beyond the pool"}
+                   4: "a cache slot beyond the pool", 8: "a second run of tokens in one page of a cache in 8 bits"}
 
 
 class EngineError(RuntimeError):
@@ -71,8 +71,14 @@ class ModelRunner:
         self.dtype = cfg.torch_dtype
         self.max_seq_len = cfg.max_seq_len
         self.rt = Runtime(device=self.device, dtype=self.dtype, max_tokens=cfg.max_num_batched_tokens,
-                          max_seqs=cfg.max_num_seqs, max_seq_len=cfg.max_seq_len, page_size=cfg.block_size)
+                          max_seqs=cfg.max_num_seqs, max_seq_len=cfg.max_seq_len, page_size=cfg.block_size,
+                          cache_dtype=cfg.torch_cache_dtype)
         self.model = DecoderModel(self.spec, self.rt)
+        if self.rt.cache_dtype != self.dtype:
+            for kind, cs in {b.mixer.spec.kind: b.mixer.cache_spec() for b in self.model.blocks}.items():
+                if cs is not None and not cs.typed():
+                    raise EngineError(f"kv_cache_dtype '{cfg.kv_cache_dtype}': layers of kind '{kind}' keep their caches in "
+                                      f"{cfg.dtype} only")
         self.model.load_weights(CheckpointReader(cfg.model))
         self.vocab_size = self.spec.vocab_size
 

@@ -51,10 +51,12 @@ class GQAttention(Mixer):
         self.q_size = p.num_heads * p.head_dim
         self.kv_size = p.num_kv_heads * p.head_dim
         self.qkv_size = self.q_size + 2 * self.kv_size
+        self.eight_bit = rt.cache_dtype == kernels.KV8_DTYPE       # keys and values in 8 bits (kernels.kv8_write)
 
     def cache_spec(self) -> CacheSpec:
         p = self.params
-        return CacheSpec.keys_values("window" if p.window > 0 else "full", p.num_kv_heads, p.head_dim, p.window)
+        make = CacheSpec.keys_values_eight_bit if self.eight_bit else CacheSpec.keys_values
+        return make("window" if p.window > 0 else "full", p.num_kv_heads, p.head_dim, p.window)
 
     def tiling(self):
         return kernels.PREFILL_TILE_ROWS, kernels.DECODE_PARTITION
@@ -173,8 +175,15 @@ class GQAttention(Mixer):
     def decode_variant(self, ctx) -> int:
         """4 where the decode kernel of one cluster per (sequence, kv head) is expected to be the fastest
         (kernels.attn_decode_rows_pays) and takes the layer (groups of at most 16 heads), else 0 (the kernels choose among
-        themselves)."""
+        themselves).  For a cache in 8 bits the way in which its kernel shares out the rows (kernels.kv8_decode_choice)."""
         p, rt = self.params, self.rt
+        if self.eight_bit and ctx.num_decode > 0:
+            memo = ctx.__dict__.setdefault("_decode_variants", {})
+            key = (8, p.num_heads, p.num_kv_heads, p.head_dim, p.window)
+            if key not in memo:
+                memo[key] = kernels.kv8_decode_choice(rt.dtype, ctx.num_decode, p.num_heads, p.num_kv_heads, p.head_dim,
+                                                      ctx.decode_max_ctx, ctx.decode_sum_ctx, p.window, rt.device)
+            return memo[key]
         if (rt.dtype != torch.bfloat16 or ctx.num_decode <= 0 or p.num_heads > 16 * p.num_kv_heads
                 or os.environ.get("REDLINE_DECODE_ROWS", "1") == "0"):
             return 0
@@ -205,6 +214,9 @@ class GQAttention(Mixer):
         tables = self.position.rotary_tables()
         g = ctx.groups[cache.group]
         attn = ws.get("attn.out", (rt.max_tokens, self.q_size), rt.dtype)[:T]
+        if self.eight_bit:
+            self._attend_eight_bit(qkv, ctx, cache, g, tables, attn)
+            return attn
         part_o = part_ml = None
         variant = self.decode_variant(ctx) if ctx.num_decode > 0 else 0
         if ctx.num_decode > 0:
@@ -247,11 +259,45 @@ class GQAttention(Mixer):
             self._mark_attention(ctx, "attention_prefill", "prefill")
         return attn
 
+    def _attend_eight_bit(self, qkv, ctx, cache: LayerCache, g, tables, attn) -> None:
+        """``_attend`` from the position encoding on, over a cache in 8 bits."""
+        p, rt = self.params, self.rt
+        T = ctx.T
+        held = cache.eight_bit
+        sizes = (p.num_heads, p.num_kv_heads, p.head_dim, rt.page_size)
+        cos, sin = tables if tables is not None else (None, None)
+        variant, work = 0, None
+        if ctx.num_decode > 0:
+            variant = self.decode_variant(ctx)
+            work = (rt.workspace.get("attn.kv8_part", (kernels.kv8_part_floats(*sizes[:3]),), torch.float32),
+                    self._counters(ctx.max_items))
+            if tables is not None and cache.write and ctx.num_decode == T and ctx.num_tiles == 0:
+                kernels.kv8_attn_decode_rope(qkv, self.qkv_size, *held, g.block_table, ctx.decode_info, work, attn,
+                                             ctx.num_decode, *sizes, p.window, self.scale, cos, sin, ctx.status, impl=variant)
+                self._mark_attention(ctx, "rope+kv_write+attention_decode", "decode")
+                return
+        if tables is None:
+            self.position.apply(qkv, p.num_heads, p.num_kv_heads, p.head_dim, ctx)
+        kernels.kv8_write(qkv, ctx.positions, g.slots if cache.write else None, cos, sin, *held,
+                          None if tables is None else qkv[:, :self.q_size], *sizes, ctx.status, tokens=T)
+        if ctx.profiler is not None:
+            elem = qkv.element_size()
+            ctx.profiler.mark("rope+kv_write", T * (2.0 * self.q_size * elem + 2.0 * self.kv_size * (elem + 1)), 0.0)
+        if ctx.num_decode > 0:
+            kernels.kv8_attn_decode(qkv, self.qkv_size, *held, g.block_table, ctx.decode_info, work, attn, ctx.num_decode,
+                                    *sizes, p.window, self.scale, impl=variant)
+            self._mark_attention(ctx, "attention_decode", "decode")
+        if ctx.num_tiles > 0:
+            kernels.kv8_attn_prefill(qkv, self.qkv_size, *held, g.block_table, ctx.tile_seq, ctx.tile_tok, ctx.tile_rows,
+                                     ctx.positions, attn, ctx.num_tiles, *sizes, p.window, self.scale)
+            self._mark_attention(ctx, "attention_prefill", "prefill")
+
     def _mark_attention(self, ctx, op: str, which: str) -> None:
         if ctx.profiler is None:
             return
         from ..engine.profiler import attention_work
         p = self.params
         elem = 2 if self.rt.dtype == torch.bfloat16 else 4
-        nbytes, flops = attention_work(ctx.host, p.num_heads, p.num_kv_heads, p.head_dim, p.window, elem)[which]
+        nbytes, flops = attention_work(ctx.host, p.num_heads, p.num_kv_heads, p.head_dim, p.window, elem,
+                                       kv_elem=1 if self.eight_bit else elem)[which]
         ctx.profiler.mark(op, nbytes, flops)

@@ -95,14 +95,17 @@ class Runtime:
     """What a part may know of the engine it runs in."""
 
     device: torch.device
-    dtype: torch.dtype            # activation / cache type: float32 or bfloat16
+    dtype: torch.dtype            # activation type (and the cache's, unless cache_dtype says otherwise): float32 or bfloat16
     max_tokens: int               # most tokens in one step
     max_seqs: int                 # most sequences in one step
     max_seq_len: int              # longest sequence
     page_size: int
     workspace: Workspace = None   # type: ignore[assignment]
+    cache_dtype: Optional[torch.dtype] = None    # None: dtype; float8_e4m3fn: mixers that can keep keys and values in 8 bits do
 
     def __post_init__(self):
+        if self.cache_dtype is None:
+            self.cache_dtype = self.dtype
         if self.workspace is None:
             self.workspace = Workspace(self.device)
 
@@ -111,7 +114,7 @@ class Runtime:
 class LayerCache:
     """The cache one call of a layer works on: the tensors its mixer's ``CacheSpec`` names, each
     [pages, *leading axes, page_size, last axis] in the pages of its cache group (for attention
-    ``k`` and ``v`` [pages, heads, page_size, D]), and whether this call writes its tokens there."""
+    ``k`` and ``v`` [pages, heads, page_size, D], in 8 bits with their scales [pages, heads]), and whether this call writes its tokens there."""
 
     group: int
     tensors: Dict[str, torch.Tensor]
@@ -124,6 +127,12 @@ class LayerCache:
     @property
     def v(self) -> torch.Tensor:
         return self.tensors["v"]
+
+    @property
+    def eight_bit(self) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+        """Keys, values and their scales of a cache in 8 bits."""
+        t = self.tensors
+        return t["k"], t["v"], t["k_scale"], t["v_scale"]
 
 
 class Watched:

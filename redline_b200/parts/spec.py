@@ -92,16 +92,26 @@ class CacheTensor:
     shape  of one token, for instance (heads, head_dim).  The last axis is kept contiguous; the pool
            lays a tensor out as [pages, *shape[:-1], page_size, shape[-1]], so that the tokens of a page
            under one index of the leading axes (a head's keys) are one contiguous box.
+    dtype  name of the elements' type (None: the engine's activation type)
+    per_page  one entry of ``shape`` for a page and not for each of its tokens: the pool is [pages, *shape]
     """
 
     name: str
     shape: Tuple[int, ...]
+    dtype: Optional[str] = None
+    per_page: bool = False
 
     def elements(self) -> int:
         n = 1
         for x in self.shape:
             n *= int(x)
         return n
+
+    def page_elements(self, page_size: int) -> int:
+        return self.elements() * (1 if self.per_page else page_size)
+
+    def page_shape(self, page_size: int) -> Tuple[int, ...]:
+        return tuple(self.shape) if self.per_page else tuple(self.shape[:-1]) + (page_size, self.shape[-1])
 
 
 @dataclass(frozen=True)
@@ -127,8 +137,20 @@ class CacheSpec:
         """Keys "k" and values "v" of [heads, head_dim] per token: what grouped-query attention caches."""
         return CacheSpec(kind, (CacheTensor("k", (heads, head_dim)), CacheTensor("v", (heads, head_dim))), window)
 
+    @staticmethod
+    def keys_values_eight_bit(kind: str, heads: int, head_dim: int, window: int = 0) -> "CacheSpec":
+        """The same in 8 bits, with a scale for every page of a head (``kernels.kv8_write``)."""
+        eight, scale = "float8_e4m3fn", "float8_e8m0fnu"
+        return CacheSpec(kind, (CacheTensor("k", (heads, head_dim), eight), CacheTensor("v", (heads, head_dim), eight),
+                                CacheTensor("k_scale", (heads,), scale, True), CacheTensor("v_scale", (heads,), scale, True)),
+                         window)
+
+    def typed(self) -> bool:
+        """Whether the tensors name their types."""
+        return any(t.dtype is not None for t in self.tensors)
+
     def elements_per_token(self) -> int:
-        return sum(t.elements() for t in self.tensors)
+        return sum(t.elements() for t in self.tensors if not t.per_page)
 
     def group_key(self) -> Tuple:
         return (self.kind, self.tensors, self.window, self.keep_first)

@@ -5,7 +5,7 @@
     outs = engine.generate([[1, 2, 3]], max_new_tokens=32, temperature=0.8, seed=1)
 
 Options carry the names of the command-line flags: ``max_seqs``, ``max_batched_tokens``,
-``max_seq_len``, ``max_logit_rows``, ``block_size``, ``kv_cache_tokens``,
+``max_seq_len``, ``max_logit_rows``, ``block_size``, ``kv_cache_tokens``, ``kv_cache_dtype``,
 ``gpu_memory_utilization``, ``cuda_graphs``, ``async_scheduling``, ``mix_prefill_decode``,
 ``device``, plus ``dtype``.  The reference also has a subprocess engine around its
 compiled programs for installs without the extension module; this package is

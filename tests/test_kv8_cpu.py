@@ -86,6 +86,9 @@ def test_rows_that_are_refused(monkeypatch):
         (prefill, dict(out=torch.zeros(3, HEADS * DIM, dtype=torch.bfloat16)), "out must be"),
         (prefill, dict(tiles=2), "for 2 tiles"),
         (prefill, dict(window=-1), "window"),
+        (prefill, dict(scale=0.0), "scale must be positive"),
+        (prefill, dict(scale=-1.0), "scale must be positive"),
+        (prefill, dict(scale=float("nan")), "scale must be positive"),
         (prefill, dict(block_table=ints(8)), "block_table"),
         (prefill, dict(block_table=torch.zeros(2, 4, dtype=torch.int64)), "block_table"),
     ]
@@ -132,3 +135,61 @@ def test_a_page_filled_in_pieces_is_the_page_filled_at_once():
     assert ((a - b).abs() <= unit * 2.0 ** -9).all()
     normal = x.transpose(0, 1)[None].abs().double() >= unit * 2.0 ** -5
     assert torch.equal(a[normal], b[normal])
+
+
+def test_the_engines_option(tmp_path):
+    import argparse
+    from redline_b200.apps.cli_common import add_engine_options, engine_options
+    from redline_b200.config import EngineConfig
+    assert EngineConfig.from_options("m", {}).torch_cache_dtype == torch.bfloat16
+    assert EngineConfig.from_options("m", dict(dtype="float32")).torch_cache_dtype == torch.float32
+    assert EngineConfig.from_options("m", dict(kv_cache_dtype="fp8")).torch_cache_dtype == kernels.KV8_DTYPE
+    with pytest.raises(ValueError, match="kv_cache_dtype"):
+        EngineConfig.from_options("m", dict(kv_cache_dtype="int8"))
+    ap = argparse.ArgumentParser()
+    add_engine_options(ap)
+    assert engine_options(ap.parse_args([]))["kv_cache_dtype"] == "auto"
+    assert engine_options(ap.parse_args(["--kv-cache-dtype", "fp8"]))["kv_cache_dtype"] == "fp8"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_the_engines_pools(dtype):
+    """A group in 8 bits beside one in the activations' type: types, shapes, starts on 16 bytes, no byte shared, sizes."""
+    from redline_b200.cache.manager import GroupInfo
+    from redline_b200.cache.storage import CacheStorage, bytes_per_page
+    from redline_b200.parts.spec import CacheSpec
+    groups = [GroupInfo(CacheSpec.keys_values_eight_bit("full", 3, 80), [0, 2, 5]), GroupInfo(CacheSpec.keys_values("full", 3, 80), [1])]
+    assert groups[0].spec.typed() and not groups[1].spec.typed() and groups[0].spec.elements_per_token() == 2 * 3 * 80
+    assert bytes_per_page(groups, 16, dtype.itemsize) == [3 * (2 * 3 * 80 * 16 + 2 * 3), 2 * 3 * 80 * 16 * dtype.itemsize]
+    store = CacheStorage(groups, [7, 5], 16, dtype, torch.device("cpu"))
+    spans = []
+    for owner in (0, 2, 5):
+        c = store.of_owner(owner, True)
+        k, v, ks, vs = c.eight_bit
+        assert k.dtype == v.dtype == kernels.KV8_DTYPE and ks.dtype == vs.dtype == kernels.KV8_SCALE_DTYPE
+        assert k.shape == v.shape == (7, 3, 16, 80) and ks.shape == vs.shape == (7, 3) and c.group == 0
+        for t in c.eight_bit:
+            assert t.is_contiguous() and t.data_ptr() % 16 == 0 and not t.view(torch.uint8).any()
+            spans.append((t.data_ptr(), t.data_ptr() + t.numel()))
+    spans.sort()
+    assert all(a[1] <= b[0] for a, b in zip(spans, spans[1:]))
+    assert store.pools[0].data_ptr() <= spans[0][0] and spans[-1][1] <= store.pools[0].data_ptr() + store.pools[0].numel()
+    plain = store.of_owner(1, True)
+    assert plain.k.dtype == dtype and plain.k.shape == (5, 3, 16, 80)
+    assert sum(b - a for a, b in spans) <= 7 * bytes_per_page(groups, 16, dtype.itemsize)[0] <= store.pools[0].numel()
+
+
+def test_the_mixers_cache():
+    from redline_b200.config import RopeScaling
+    from redline_b200.parts import PartSpec, build_part
+    from redline_b200.parts.attention import AttentionParams
+    from redline_b200.parts.base import Runtime
+    from redline_b200.parts.rope import RotaryParams
+    position = PartSpec("rope", RotaryParams(16, 10000.0, RopeScaling(), 64))
+    spec = PartSpec("gqa_attention", AttentionParams(64, 4, 2, 16, position, window=24))
+    cpu = torch.device("cpu")
+    plain = build_part("mixer", spec, Runtime(cpu, torch.bfloat16, 8, 2, 64, 16)).cache_spec()
+    eight = build_part("mixer", spec, Runtime(cpu, torch.bfloat16, 8, 2, 64, 16, cache_dtype=kernels.KV8_DTYPE)).cache_spec()
+    assert [(t.name, t.shape, t.dtype) for t in plain.tensors] == [("k", (2, 16), None), ("v", (2, 16), None)]
+    assert [t.name for t in eight.tensors] == ["k", "v", "k_scale", "v_scale"] and (eight.kind, eight.window) == ("window", 24)
+    assert plain.group_key() != eight.group_key()

@@ -1045,7 +1045,7 @@ int rl_kv8_attn_decode(int dtype, const void* q, int q_stride, void* kc, void* v
     a.nitems = nitems - i0 < kMaxItems ? nitems - i0 : kMaxItems;
 #ifdef RL_KV8_TC
     if (tc) {
-      e = launch_decode_tc(a, max_ctx, sum_ctx, impl, stream);
+      e = launch_decode_tc(a, max_ctx, sum_ctx / nitems * a.nitems, impl, stream);
       if (e) return e;
       continue;
     }
@@ -1094,7 +1094,7 @@ int launch_prefill(const void* q, int q_stride, const void* kc, const void* vc, 
   a.page_shift = shift_of(page_size);
   a.window = window;
   a.scale = scale;
-  static bool attr_set[kMaxDevices];
+  static bool tc_set[kMaxDevices], simt_set[kMaxDevices];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return static_cast<int>(e);
@@ -1105,13 +1105,11 @@ int launch_prefill(const void* q, int q_stride, const void* kc, const void* vc, 
       int sms = 0;
       const int err = device_sms(&sms);
       if (err) return err;
-      if (!attr_set[dev]) {
+      if (!tc_set[dev]) {
         e = cudaFuncSetAttribute(prefill_attn_tc_kernel<Kv8PrefillArgs<bf16>>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  static_cast<int>(kPrefillTcSmem));
-        if (e == cudaSuccess)
-          e = cudaFuncSetAttribute(kv8_prefill_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kPreSmem));
         if (e != cudaSuccess) return static_cast<int>(e);
-        attr_set[dev] = true;
+        tc_set[dev] = true;
       }
       const long long work = static_cast<long long>(tiles) * hkv * ((hq / hkv + 1) / 2);     // (tile, kv head, pair of heads)
       launch_kernel(prefill_attn_tc_kernel<Kv8PrefillArgs<bf16>>, dim3(static_cast<unsigned>(work < sms ? work : sms)), dim3(kTcThreads8),
@@ -1121,10 +1119,10 @@ int launch_prefill(const void* q, int q_stride, const void* kc, const void* vc, 
   }
 #endif
   if (impl > 1) return static_cast<int>(cudaErrorInvalidValue);
-  if (!attr_set[dev]) {
+  if (!simt_set[dev]) {
     e = cudaFuncSetAttribute(kv8_prefill_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kPreSmem));
     if (e != cudaSuccess) return static_cast<int>(e);
-    attr_set[dev] = true;
+    simt_set[dev] = true;
   }
   launch_kernel(kv8_prefill_kernel<T>, dim3(tiles * 2, hq), dim3(kPreThreads), kPreSmem, stream, a);
   return static_cast<int>(cudaGetLastError());

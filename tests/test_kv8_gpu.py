@@ -7,6 +7,9 @@ The write is compared bit for bit.  Attention, with E the largest magnitude amon
             their roundings weigh the values, so their sum is at most half a step of E)"""
 
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -560,3 +563,26 @@ def test_on_another_stream():
         there = decode(q, gpu, table, ctxs, heads, kv_heads, dim, page, 0, 0.125)
     side.synchronize()
     assert torch.equal(here, there)
+
+
+def test_the_cuda_core_kernel_first():
+    """A process whose first portion goes to the CUDA cores, and its second to the tensor cores: each kernel's shared memory is asked for."""
+    code = """
+import sys, torch
+sys.path.insert(0, "tests")
+import test_kv8_gpu as T
+from redline_b200.ops import kernels
+cache, table = T.filled([130], 4, 2, 64, 16, seed=1)
+gpu = T.on_gpu(cache)
+q = torch.randn(130, 256, dtype=torch.bfloat16, device="cuda")
+seq, tok, rows = T.tiles_of([(0, 130)])
+pos = torch.arange(130, dtype=torch.int32, device="cuda")
+outs = []
+for impl in (1, 3, 0):
+    outs.append(torch.empty_like(q))
+    kernels.kv8_attn_prefill(q, 256, *gpu, table.to("cuda"), seq, tok, rows, pos, outs[-1], len(seq), 4, 2, 64, 16, 0, 0.125, impl=impl)
+torch.cuda.synchronize()
+assert all(torch.isfinite(o).all() for o in outs) and torch.equal(outs[1], outs[2])
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    subprocess.run([sys.executable, "-c", code], cwd=root, check=True, timeout=300)

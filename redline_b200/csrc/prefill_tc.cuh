@@ -66,13 +66,11 @@ constexpr int kTcTmemCols = 512;
 constexpr int kTcColO = 256;                            // O of slot s at kTcColO + s * kD
 constexpr bool kTcOwnP = kD == 64;                      // P has tensor-memory columns of its own (else: over S)
 constexpr int kTcColP = 384;                            // with columns of its own: P of slot s at kTcColP + s * 64
-// A cache in 8 bits: as many loaders for K, and for V, as there are stages (one warp alone takes twice as long over a tile as the
-// rows).  A loader's tiles then all lie in one stage, and its waits for that stage see every phase: with more loaders than stages one
-// could be two phases ahead, which a wait on a parity does not tell from none.  Warps 8 .. 11, 14 and 15 load, 12 and 13 issue the
+// A cache in 8 bits: teams of three warps load K and V (one warp alone takes twice as long over a tile as the rows).  Every warp of a
+// team works on every tile, so its waits for a stage see every phase.  Warps 8 .. 11, 14 and 15 load, 12 and 13 issue the
 // MMAs.  Sixteen warps begin with 128 registers a thread; the two warpgroups of rows take 160, the other two leave them 96:
 // 256 x (160 + 96) = 512 x 128.
-constexpr int kTcThreads8 = 512, kTcRowRegs8 = 160, kTcOtherRegs8 = 96, kTcLoaders8 = kTcStages;
-static_assert(kTcLoaders8 <= 3, "six warps load");
+constexpr int kTcThreads8 = 512, kTcRowRegs8 = 160, kTcOtherRegs8 = 96, kTcLoaders8 = 3;
 static_assert(256 * (kTcRowRegs8 + kTcOtherRegs8) <= 512 * 128, "the launch's registers");
 constexpr float kTcGrow = 8.f;                          // log2 of the growth of a row's maximum that moves the reference
 
@@ -278,15 +276,19 @@ __device__ __forceinline__ __half2 tc_half_power(int e) {
   return *reinterpret_cast<const __half2*>(&two);
 }
 
-// The loaders of a cache in 8 bits: some warps K (and the first of them both Q), as many V, a tile to each in turn.  A tile's
-// 16-byte pieces come through registers in batches of 16 or 32 keys, the next batch on its way while one is converted and stored where
-// the copies of a 16-bit cache would have put it.  Page ids and scales come a tile ahead, a page to a lane.
+// The loaders of a cache in 8 bits: three warps K, three V (the first two of them a slot's Q as well).  The UNITS of a CTA's tiles, 16 or 32
+// keys each (four 16-byte pieces to a lane), go to a team's warps in turn, so all of them work on one tile.  (With a tile to a warp, each
+// with a stage of its own, a stage was empty for the whole time that one warp takes over a tile: OLDUS)  A unit's
+// bytes come through registers, the next unit's on their way while one is converted and stored where the copies of a 16-bit cache would
+// have put it.  Page ids and scales come 32 units at a time, a unit to a lane, a window ahead.
 template <typename Args>
 __device__ __forceinline__ void tc_load_eight_bit(const Args& a, PrefillTcShared* sh, unsigned char* q_s, unsigned char* k_s,
                                                   unsigned char* v_s, bool is_v, int turn, int lane, int n_items, int pairs, int tiles) {
+  constexpr int L = kTcLoaders8;
   constexpr int P = kD / 16, RPI = 32 / P;               // pieces of a row; rows that the warp's lanes cover at once
   constexpr int kPer16 = 16 / RPI;                       // pieces of a lane in 16 keys (of one page)
-  constexpr int kBatch = 4, kBlocks = kBatch / kPer16, kBatches = 8 / kBlocks;      // a batch: kBlocks times 16 keys
+  constexpr int kPieces = 4, kBlocks = kPieces / kPer16, kUnits = 8 / kBlocks;      // a unit: kBlocks times 16 keys; units of a tile
+  static_assert(kUnits >= L, "every warp of a team has a unit in every tile");
   const uint8_t* cache = is_v ? a.vcache : a.kcache;
   const uint8_t* scales = is_v ? a.vscale : a.kscale;
   unsigned char* stage0 = is_v ? v_s : k_s;
@@ -298,128 +300,154 @@ __device__ __forceinline__ void tc_load_eight_bit(const Args& a, PrefillTcShared
   // place % 8 is the lane's own, or with rounds of four rows the lane's own and another 4 in every second
   const uint32_t c_half = static_cast<uint32_t>(piece >> 2) * kTcHalfBytes;
   const uint32_t at0 = c_half + rr * 128 + ((((2 * piece) & 7) ^ rr) << 4), at1 = c_half + rr * 128 + ((((2 * piece + 1) & 7) ^ rr) << 4);
+  struct Unit {
+    uint4 raw[kPieces];
+    int code[kBlocks];
+  };
   bool ok = true;
   TcWalk wk;
   for (bool more = wk.first(a, n_items, pairs, tiles); more && ok; more = wk.next(a, n_items, pairs, tiles)) {
     const TcItem& w = wk.w;
     const int32_t* bt = a.block_table + static_cast<size_t>(w.seq) * a.max_blocks;
     const int first = w.lo0 >> shift, last = (w.k_end - 1) >> shift;
+    const int units = w.nt * kUnits;
+    int x = (turn + L - (wk.g * kUnits) % L) % L;        // the warp's first unit of the item
+    auto pages_of = [&](int u, int* id) {                // a lane's unit of the 32 from u on
+#pragma unroll
+      for (int j = 0; j < kBlocks; ++j)
+        id[j] = bt[min(max((w.k_begin + ((u + L * lane) * kBlocks + j) * 16) >> shift, first), last)];
+    };
+    auto codes_of = [&](const int* id, int* code) {
+#pragma unroll
+      for (int j = 0; j < kBlocks; ++j) code[j] = scales[static_cast<size_t>(id[j]) * a.hkv + w.kvh];
+    };
+    int id[kBlocks], code[kBlocks], next_id[kBlocks], next_code[kBlocks];
+    pages_of(x, id);
+    pages_of(x + 32 * L, next_id);
+    codes_of(id, code);
     // the item's largest scale
     int most = 0;
 #pragma unroll 4
     for (int pg = first + lane; pg <= last; pg += 32) most = max(most, static_cast<int>(scales[static_cast<size_t>(bt[pg]) * a.hkv + w.kvh]));
     most = __reduce_max_sync(0xffffffffu, most);
-    int i = (turn + kTcLoaders8 - wk.g % kTcLoaders8) % kTcLoaders8;     // the warp's first tile of the item
-    if (i == 0 && lane == 0) (is_v ? sh->item_v : sh->item_k)[wk.it & 7] = kv8_scale(most);
-    // a tile's pages (at most eight: pages of 16 keys or more), one to a lane: its id and its scale
-    auto page_of = [&](int t) {
-      return bt[min(max(((w.k_begin + t * kTcKeys) >> shift) + (lane & 7), first), last)];
-    };
-    auto scale_of = [&](int page) { return static_cast<int>(scales[static_cast<size_t>(page) * a.hkv + w.kvh]); };
-    int page = i < w.nt ? page_of(i) : 0;
-    int next_page = i + kTcLoaders8 < w.nt ? page_of(i + kTcLoaders8) : 0;
-    int code = i < w.nt ? scale_of(page) : 0;
-    if (!is_v && turn == 0) {
+    if (turn == 0 && lane == 0) (is_v ? sh->item_v : sh->item_k)[wk.it & 7] = kv8_scale(most);
+    if (is_v && turn < (w.two ? 2 : 1)) {
       constexpr int CPR = kD / 8, QRI = 32 / CPR;
-      const int c = lane % CPR, qr = lane / CPR;
-      for (int s = 0; s < (w.two ? 2 : 1) && ok; ++s) {
-        const int n = s == 0 ? wk.it : wk.it1;           // the slot's items so far
-        const bf16* src = a.q + static_cast<size_t>(w.tok0) * a.q_stride + (w.head0 + s) * kD + c * 8;
-        unsigned char* dst = q_s + s * kTcTileBytes + static_cast<uint32_t>(c >> 3) * kTcHalfBytes;
-        ok = mbar_wait(&sh->q_free[s], (n & 1) ^ 1, &sh->abort);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-#pragma unroll 1
-        for (int j = 0; j < kTcRows; j += 8 * QRI) {
-          uint4 x[8];
-#pragma unroll
-          for (int u = 0; u < 8; ++u) {
-            const int r = j + u * QRI + qr;
-            x[u] = make_uint4(0, 0, 0, 0);
-            if (r < w.rows) x[u] = *reinterpret_cast<const uint4*>(src + static_cast<size_t>(r) * a.q_stride);
-          }
-#pragma unroll
-          for (int u = 0; u < 8; ++u) {
-            const int r = j + u * QRI + qr;
-            uint32_t in[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const __half2 h = __floats2half2_rn(__uint_as_float(in[e] << 16), __uint_as_float(in[e] & 0xffff0000u));
-              in[e] = *reinterpret_cast<const uint32_t*>(&h);
-            }
-            *reinterpret_cast<uint4*>(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(in[0], in[1], in[2], in[3]);
-          }
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh->q_full[s]);
-      }
-      if (!ok) break;
-    }
-    if (i >= w.nt) continue;
-    uint4 raw[2][kBatch];
-    // asks for batch b of the tile that begins at key k0 (its pages in `pg`)
-    auto ask = [&](int k0, int b, int pg, uint4* v) {
-      const bool whole = k0 >= w.lo0 && k0 + kTcKeys <= w.k_end;
-#pragma unroll
-      for (int j = 0; j < kBlocks; ++j) {
-        const int key = k0 + (b * kBlocks + j) * 16;
-        const int id = __shfl_sync(0xffffffffu, pg, ((k0 & ps_mask) + (b * kBlocks + j) * 16) >> shift);
-        const uint8_t* p = cache + (((static_cast<size_t>(id) * a.hkv + w.kvh) << shift) + (key & ps_mask)) * kD + lane * 16;
-#pragma unroll
-        for (int u = 0; u < kPer16; ++u) {
-          const int mine = key + u * RPI + rr;
-          v[j * kPer16 + u] = make_uint4(0, 0, 0, 0);
-          if (whole || (mine < w.k_end && mine >= w.lo0)) v[j * kPer16 + u] = *reinterpret_cast<const uint4*>(p + u * 512);
-        }
-      }
-    };
-    ask(w.k_begin + i * kTcKeys, 0, page, raw[0]);
-    for (; i < w.nt && ok; i += kTcLoaders8) {
-      const int g = wk.g + i, b = g % kTcStages;
-      const int k0 = w.k_begin + i * kTcKeys;
-      const int next_code = i + kTcLoaders8 < w.nt ? scale_of(next_page) : 0;
-      const int after_page = i + 2 * kTcLoaders8 < w.nt ? page_of(i + 2 * kTcLoaders8) : 0;
-      ok = mbar_wait(&freed[b], ((g / kTcStages) & 1) ^ 1, &sh->abort);      // (a fresh barrier passes a wait on parity 1)
+      const int c = lane % CPR, qr = lane / CPR, s = turn;
+      const int n = s == 0 ? wk.it : wk.it1;             // the slot's items so far
+      const bf16* src = a.q + static_cast<size_t>(w.tok0) * a.q_stride + (w.head0 + s) * kD + c * 8;
+      unsigned char* dst = q_s + s * kTcTileBytes + static_cast<uint32_t>(c >> 3) * kTcHalfBytes;
+      ok = mbar_wait(&sh->q_free[s], (n & 1) ^ 1, &sh->abort);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      unsigned char* dst = stage0 + b * kTcTileBytes;
+#pragma unroll 1
+      for (int j = 0; j < kTcRows; j += 8 * QRI) {
+        uint4 v[8];
 #pragma unroll
-      for (int n = 0; n < kBatches; ++n) {
-        if (n + 1 < kBatches) ask(k0, n + 1, page, raw[(n + 1) & 1]);
-        else if (i + kTcLoaders8 < w.nt) ask(k0 + kTcLoaders8 * kTcKeys, 0, next_page, raw[(n + 1) & 1]);
+        for (int u = 0; u < 8; ++u) {
+          const int row = j + u * QRI + qr;
+          v[u] = make_uint4(0, 0, 0, 0);
+          if (row < w.rows) v[u] = *reinterpret_cast<const uint4*>(src + static_cast<size_t>(row) * a.q_stride);
+        }
 #pragma unroll
-        for (int j = 0; j < kBlocks; ++j) {
-          const int c = __shfl_sync(0xffffffffu, code, ((k0 & ps_mask) + (n * kBlocks + j) * 16) >> shift);
-          const __half2 f = tc_half_power(c - most);
+        for (int u = 0; u < 8; ++u) {
+          const int row = j + u * QRI + qr;
+          uint32_t in[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
 #pragma unroll
-          for (int u = 0; u < kPer16; ++u) {
-            const uint4 v = raw[n & 1][j * kPer16 + u];
-            const uint32_t in[4] = {v.x, v.y, v.z, v.w};
-            uint32_t out[8];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              halves4(in[e], out[2 * e], out[2 * e + 1]);
-#pragma unroll
-              for (int x = 0; x < 2; ++x) {
-                const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&out[2 * e + x]), f);
-                out[2 * e + x] = *reinterpret_cast<const uint32_t*>(&h);
-              }
-            }
-            const int row = (n * kBlocks + j) * 16 + u * RPI;            // (+ rr)
-            const uint32_t sw = RPI == 4 && (u & 1) ? 64u : 0u;
-            *reinterpret_cast<uint4*>(dst + (at0 ^ sw) + row * 128) = make_uint4(out[0], out[1], out[2], out[3]);
-            *reinterpret_cast<uint4*>(dst + (at1 ^ sw) + row * 128) = make_uint4(out[4], out[5], out[6], out[7]);
+          for (int e = 0; e < 4; ++e) {
+            const __half2 h = __floats2half2_rn(__uint_as_float(in[e] << 16), __uint_as_float(in[e] & 0xffff0000u));
+            in[e] = *reinterpret_cast<const uint32_t*>(&h);
           }
+          *reinterpret_cast<uint4*>(dst + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = make_uint4(in[0], in[1], in[2], in[3]);
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(&full[b]);
-      page = next_page;
-      next_page = after_page;
-      code = next_code;
+      if (lane == 0) mbar_arrive(&sh->q_full[s]);
     }
+    // asks for unit u, the r-th of the window
+    int r = 0;
+    auto ask = [&](int u, Unit& to) {
+      if (r == 16) codes_of(next_id, next_code);
+      if (r == 32) {
+#pragma unroll
+        for (int j = 0; j < kBlocks; ++j) {
+          id[j] = next_id[j];
+          code[j] = next_code[j];
+        }
+        pages_of(u + 32 * L, next_id);
+        r = 0;
+      }
+      const int k0 = w.k_begin + u * (16 * kBlocks);
+      const bool whole = k0 >= w.lo0 && k0 + 16 * kBlocks <= w.k_end;
+#pragma unroll
+      for (int j = 0; j < kBlocks; ++j) {
+        const int key = k0 + j * 16;
+        const int page = __shfl_sync(0xffffffffu, id[j], r);
+        to.code[j] = __shfl_sync(0xffffffffu, code[j], r);
+        const uint8_t* p = cache + (((static_cast<size_t>(page) * a.hkv + w.kvh) << shift) + (key & ps_mask)) * kD + lane * 16;
+#pragma unroll
+        for (int i = 0; i < kPer16; ++i) {
+          const int mine = key + i * RPI + rr;
+          to.raw[j * kPer16 + i] = make_uint4(0, 0, 0, 0);
+          if (whole || (mine < w.k_end && mine >= w.lo0)) to.raw[j * kPer16 + i] = *reinterpret_cast<const uint4*>(p + i * 512);
+        }
+      }
+      ++r;
+    };
+    int tile = -1;                                       // the item's tile that the warp is at
+    auto hand_over = [&]() {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[(wk.g + tile) % kTcStages]);
+    };
+    auto put = [&](int u, const Unit& from) {
+      if (u / kUnits != tile) {
+        if (tile >= 0) hand_over();
+        tile = u / kUnits;
+        const int g = wk.g + tile;
+        ok = mbar_wait(&freed[g % kTcStages], ((g / kTcStages) & 1) ^ 1, &sh->abort);      // (a fresh barrier passes a wait on parity 1)
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) return;
+      }
+      unsigned char* dst = stage0 + ((wk.g + tile) % kTcStages) * kTcTileBytes + (u % kUnits) * (kBlocks * 16 * 128);
+#pragma unroll
+      for (int j = 0; j < kBlocks; ++j) {
+        const __half2 f = tc_half_power(from.code[j] - most);
+#pragma unroll
+        for (int i = 0; i < kPer16; ++i) {
+          const uint4 v = from.raw[j * kPer16 + i];
+          const uint32_t in[4] = {v.x, v.y, v.z, v.w};
+          uint32_t out[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            halves4(in[e], out[2 * e], out[2 * e + 1]);
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&out[2 * e + y]), f);
+              out[2 * e + y] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+          }
+          const int row = j * 16 + i * RPI;              // (+ rr)
+          const uint32_t sw = RPI == 4 && (i & 1) ? 64u : 0u;
+          *reinterpret_cast<uint4*>(dst + (at0 ^ sw) + row * 128) = make_uint4(out[0], out[1], out[2], out[3]);
+          *reinterpret_cast<uint4*>(dst + (at1 ^ sw) + row * 128) = make_uint4(out[4], out[5], out[6], out[7]);
+        }
+      }
+    };
+    Unit even, odd;
+    ask(x, even);
+#pragma unroll 1
+    for (; x < units; x += 2 * L) {
+      if (x + L < units) ask(x + L, odd);
+      put(x, even);
+      if (!ok) break;
+      if (x + L >= units) break;
+      if (x + 2 * L < units) ask(x + 2 * L, even);
+      put(x + L, odd);
+      if (!ok) break;
+    }
+    if (ok) hand_over();
   }
 }
 
@@ -451,9 +479,9 @@ prefill_attn_tc_kernel(const Args a, int tiles, int* status) {
       mbar_init(&sh->o_free[s], 4);
     }
     for (int b = 0; b < kTcStages; ++b) {
-      mbar_init(&sh->k_full[b], 1);
+      mbar_init(&sh->k_full[b], Args::kEightBit ? kTcLoaders8 : 1);
       mbar_init(&sh->k_free[b], 2);       // one commit per slot (a lone slot commits twice)
-      mbar_init(&sh->v_full[b], 1);
+      mbar_init(&sh->v_full[b], Args::kEightBit ? kTcLoaders8 : 1);
       mbar_init(&sh->v_free[b], 2);
     }
     sh->abort = 0;
@@ -477,7 +505,7 @@ prefill_attn_tc_kernel(const Args a, int tiles, int* status) {
   if (Args::kEightBit && warp != kMma && warp != kMma + 1) {
     if constexpr (Args::kEightBit) {
       const int l = warp < kMma ? warp - kTcRowWarps : warp - kTcRowWarps - 2;      // first K's loaders, then V's
-      if (l < 2 * kTcLoaders8) tc_load_eight_bit(a, sh, q_s, k_s, v_s, l >= kTcLoaders8, l % kTcLoaders8, lane, n_items, pairs, tiles);
+      tc_load_eight_bit(a, sh, q_s, k_s, v_s, l >= kTcLoaders8, l % kTcLoaders8, lane, n_items, pairs, tiles);
     }
   } else if (!Args::kEightBit && (warp == kTcRowWarps || warp == kTcRowWarps + 1)) {
     if constexpr (!Args::kEightBit) {

@@ -94,7 +94,8 @@ constexpr int kWriteRounds = kD <= 64 ? 2 : 4;
 // run of its own, and four runs one after another take four times as long.  Four to a CTA beyond: most tokens of a prompt
 // begin no run, and the CTAs are handed out one by one.
 // What bounds it is the way from the slots to the rows to the block's largest magnitude to the bytes; what does not depend on one
-// another is asked for together.
+// another is asked for together.  32 / 8 heads of 64: 8 single tokens 3.7 us, a prompt of 2,048 tokens 11.4 us (2.0 TB/s); nine portions
+// of 1 to 700 tokens at head size 128 26.6 us (2.3 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(kWriteThreads, 3)
 kv8_write_kernel(const Kv8WriteArgs<T> a, int span, int tasks) {
@@ -379,7 +380,9 @@ constexpr int kGenHeads = 4;               // query heads in one pass over the k
 constexpr int kGenLanes = kD <= 16 ? 1 : kD <= 32 ? 2 : kD <= 64 ? 4 : kD <= 128 ? 8 : 16;     // lanes to a key: 16 entries each
 
 // Single tokens on the CUDA cores.  A CTA to a share; a key to kGenLanes lanes of a warp, each with 16 entries of four
-// query heads and their numerators in registers and a running (max, denominator) of its own keys.
+// query heads and their numerators in registers and a running (max, denominator) of its own keys.  For float32 and the head sizes and groups
+// that the tensor-core kernel does not take; what bounds it is the conversions and products, 0.5 to 0.9 TB/s of the cache (32 / 8 heads in
+// bfloat16: 8 x 4,096 keys at head size 64 69 us against 16.6, 1 x 131,072 at 128 353 against 58).
 template <typename T>
 __global__ void __launch_bounds__(kGenThreads)
 kv8_decode_kernel(const Kv8Args a) {
@@ -585,7 +588,9 @@ constexpr size_t kPreSmem = sizeof(float) * (2 * kD * kPLd + kPK * kD + kPK * kP
 
 // Portions of prompts on the CUDA cores: a CTA to 64 consecutive query rows (half a tile of the launch) of one head;
 // keys in tiles of 64.  Thread (ty, tx) has rows 4 ty .. + 3; of S their keys 4 tx .. + 3 (operands as four rows and four
-// keys side by side: two 16-byte reads for 16 products), of O their columns tx + 16 j.
+// keys side by side: two 16-byte reads for 16 products), of O their columns tx + 16 j.  For float32 and the head sizes that the tcgen05
+// kernel does not take (bfloat16 at 64: 2,048 tokens behind 6,144 keys 5,520 us against 276); float32, four portions of 33 to 129 tokens, 3 / 1
+// heads of 128: 45 us.  What bounds it is the FFMA pipe and the reads of its operands from shared memory; few items do not fill the SMs.
 template <typename T>
 __global__ void __launch_bounds__(kPreThreads)
 kv8_prefill_kernel(const Kv8PrefillArgs<T> a) {
@@ -966,6 +971,61 @@ int launch_decode_tc(Kv8Args a, int max_ctx, long long sum_ctx, int impl, cudaSt
 
 extern "C" {
 
+// The arguments of the entry points: fields of eight bytes, packed by the caller.  (A foreign call with 30 arguments of its own
+// took 8 us of one core, one with a packed argument takes 2.)
+struct Kv8WriteCall {
+  int64_t dtype;
+  const void* qkv;
+  int64_t qkv_stride;
+  const int32_t *positions, *slots;
+  const float *cos, *sin;
+  uint8_t *kc, *vc, *ks, *vs;
+  void* q_out;
+  int64_t q_stride, tokens, hq, hkv, page_size, max_pos, num_slots;
+  int* status;
+  cudaStream_t stream;
+};
+
+// store: q holds the unrotated rows [q | k | v]; the tokens' keys and values are stored first (by the attention's kernel itself or a launch of
+// their own), and the attention rotates q on its way in.
+struct Kv8DecodeCall {
+  int64_t dtype;
+  const void* q;
+  int64_t q_stride;
+  uint8_t *kc, *vc, *ks, *vs;
+  const int32_t* block_table;
+  int64_t max_blocks;
+  const int4* items;
+  int64_t nitems;
+  float* part;
+  int* counters;
+  void* out;
+  int64_t out_stride, hq, hkv, page_size, window;
+  double scale;
+  const float *cos, *sin;
+  int64_t max_pos, store, num_slots;
+  int* status;
+  int64_t max_ctx, sum_ctx, impl;
+  cudaStream_t stream;
+};
+
+struct Kv8PrefillCall {
+  int64_t dtype;
+  const void* q;
+  int64_t q_stride;
+  const uint8_t *kc, *vc, *ks, *vs;
+  const int32_t* block_table;
+  int64_t max_blocks;
+  const int32_t *tile_seq, *tile_tok, *tile_rows, *positions;
+  void* out;
+  int64_t out_stride, tiles, hq, hkv, page_size, window;
+  double scale;
+  int64_t impl;
+  int* status;
+  cudaStream_t stream;
+};
+static_assert(sizeof(Kv8WriteCall) == 21 * 8 && sizeof(Kv8DecodeCall) == 30 * 8 && sizeof(Kv8PrefillCall) == 24 * 8, "as they are packed");
+
 // Which way of sharing out (2, 3 or 4; 0: the CUDA cores) a launch on the tensor cores would go by impl 0, or an error as a negative number.
 int rl_kv8_decode_choice(int dtype, int nitems, int hq, int hkv, int max_ctx, long long sum_ctx) {
 #ifdef RL_KV8_TC
@@ -982,70 +1042,65 @@ int rl_kv8_decode_choice(int dtype, int nitems, int hq, int hkv, int max_ctx, lo
 // The floats of the workspace for groups of G heads (kv8.cuh: Kv8Args::part).
 long long rl_kv8_part_floats(int G) { return static_cast<long long>(kMaxShares) * 2 * G * (kD + 4); }
 
-int rl_kv8_write(int dtype, const void* qkv, int qkv_stride, const int32_t* positions, const int32_t* slots,
-                 const float* cos, const float* sin, void* kc, void* vc, void* ks, void* vs, void* q_out, int q_stride,
-                 int tokens, int hq, int hkv, int page_size, int max_pos, long long num_slots, int* status, void* stream) {
-  auto run = dtype == 0 ? launch_write<float> : launch_write<bf16>;
-  return run(qkv, qkv_stride, positions, slots, nullptr, nullptr, 0, cos, sin, static_cast<uint8_t*>(kc),
-             static_cast<uint8_t*>(vc), static_cast<uint8_t*>(ks), static_cast<uint8_t*>(vs), q_out, q_stride, tokens, hq, hkv,
-             page_size, max_pos, num_slots, status, static_cast<cudaStream_t>(stream));
+int rl_kv8_write(const Kv8WriteCall* c) {
+  auto run = c->dtype == 0 ? launch_write<float> : launch_write<bf16>;
+  return run(c->qkv, static_cast<int>(c->qkv_stride), c->positions, c->slots, nullptr, nullptr, 0, c->cos, c->sin, c->kc, c->vc, c->ks,
+             c->vs, c->q_out, static_cast<int>(c->q_stride), static_cast<int>(c->tokens), static_cast<int>(c->hq),
+             static_cast<int>(c->hkv), static_cast<int>(c->page_size), static_cast<int>(c->max_pos), c->num_slots, c->status, c->stream);
 }
 
-// Single tokens.  store: q holds the unrotated rows [q | k | v]; the tokens' keys and values are stored first, in a
-// launch of their own, and the attention rotates q on its way in.
-int rl_kv8_attn_decode(int dtype, const void* q, int q_stride, void* kc, void* vc, void* ks, void* vs, const int32_t* bt,
-                       int max_blocks, const void* items, int nitems, float* part, int* counters, void* out, int out_stride,
-                       int hq, int hkv, int page_size, int window, float scale, const float* cos, const float* sin, int max_pos,
-                       int store, long long num_slots, int* status, int max_ctx, long long sum_ctx, int impl, void* stream_) {
-  const cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+int rl_kv8_attn_decode(const Kv8DecodeCall* c) {
+  const int nitems = static_cast<int>(c->nitems), hq = static_cast<int>(c->hq), hkv = static_cast<int>(c->hkv);
+  const int page_size = static_cast<int>(c->page_size), impl = static_cast<int>(c->impl), max_pos = static_cast<int>(c->max_pos);
+  const int max_ctx = static_cast<int>(c->max_ctx), q_stride = static_cast<int>(c->q_stride);
+  const bool store = c->store != 0, single = c->dtype == 0;
   int sms = 0;
   int e = device_sms(&sms);
   if (e) return e;
 #ifdef RL_KV8_TC
-  const bool tc = dtype == 1 && hq / hkv <= 16 && impl != 1;
+  const bool tc = !single && hq / hkv <= 16 && impl != 1;
 #else
   const bool tc = false;
 #endif
   // (pages of 64 tokens reach over two sub-blocks, which may be two warps': their tokens are stored by a kernel of its own)
   const bool fused = store && tc && page_size <= 32;
   if (store && !fused) {
-    auto run = dtype == 0 ? launch_write<float> : launch_write<bf16>;
-    e = run(q, q_stride, nullptr, nullptr, static_cast<const int4*>(items), bt, max_blocks, cos, sin, static_cast<uint8_t*>(kc),
-            static_cast<uint8_t*>(vc), static_cast<uint8_t*>(ks), static_cast<uint8_t*>(vs), nullptr, 0, nitems, hq, hkv, page_size,
-            max_pos, num_slots, status, stream);
+    auto run = single ? launch_write<float> : launch_write<bf16>;
+    e = run(c->q, q_stride, nullptr, nullptr, c->items, c->block_table, static_cast<int>(c->max_blocks), c->cos, c->sin, c->kc, c->vc,
+            c->ks, c->vs, nullptr, 0, nitems, hq, hkv, page_size, max_pos, c->num_slots, c->status, c->stream);
     if (e) return e;
   }
   Kv8Args a;
-  a.q = q;
+  a.q = c->q;
   a.q_stride = q_stride;
-  a.kcache = static_cast<const uint8_t*>(kc);
-  a.vcache = static_cast<const uint8_t*>(vc);
-  a.kscale = static_cast<const uint8_t*>(ks);
-  a.vscale = static_cast<const uint8_t*>(vs);
-  a.block_table = bt;
-  a.max_blocks = max_blocks;
-  a.items = static_cast<const int4*>(items);
+  a.kcache = c->kc;
+  a.vcache = c->vc;
+  a.kscale = c->ks;
+  a.vscale = c->vs;
+  a.block_table = c->block_table;
+  a.max_blocks = static_cast<int>(c->max_blocks);
+  a.items = c->items;
   a.nitems = nitems;
-  a.part = part;
-  a.counters = counters;
-  a.out = out;
-  a.out_stride = out_stride;
+  a.part = c->part;
+  a.counters = c->counters;
+  a.out = c->out;
+  a.out_stride = static_cast<int>(c->out_stride);
   a.hq = hq;
   a.hkv = hkv;
   a.page_shift = shift_of(page_size);
-  a.window = window;
-  a.scale = scale;
-  a.cos = store ? cos : nullptr;
+  a.window = static_cast<int>(c->window);
+  a.scale = static_cast<float>(c->scale);
+  a.cos = store ? c->cos : nullptr;
   a.store = fused ? 1 : 0;
-  a.sin = sin;
+  a.sin = c->sin;
   a.max_pos = max_pos;
-  a.status = status;
+  a.status = c->status;
   for (int i0 = 0; i0 < nitems; i0 += kMaxItems) {         // (one launch unless there are very many items)
-    a.items = static_cast<const int4*>(items) + i0;
+    a.items = c->items + i0;
     a.nitems = nitems - i0 < kMaxItems ? nitems - i0 : kMaxItems;
 #ifdef RL_KV8_TC
     if (tc) {
-      e = launch_decode_tc(a, max_ctx, sum_ctx / nitems * a.nitems, impl, stream);
+      e = launch_decode_tc(a, max_ctx, c->sum_ctx / nitems * a.nitems, impl, c->stream);
       if (e) return e;
       continue;
     }
@@ -1055,10 +1110,10 @@ int rl_kv8_attn_decode(int dtype, const void* q, int q_stride, void* kc, void* v
     const long long max_units = static_cast<long long>(a.nitems) * hkv * (max_ctx / kUnit + 2);
     const int most = sms * 2 < kMaxShares ? sms * 2 : kMaxShares;
     const int ctas = static_cast<int>(max_units < most ? max_units : most);
-    if (dtype == 0)
-      launch_kernel(kv8_decode_kernel<float>, dim3(ctas), dim3(kGenThreads), 0, stream, a);
+    if (single)
+      launch_kernel(kv8_decode_kernel<float>, dim3(ctas), dim3(kGenThreads), 0, c->stream, a);
     else
-      launch_kernel(kv8_decode_kernel<bf16>, dim3(ctas), dim3(kGenThreads), 0, stream, a);
+      launch_kernel(kv8_decode_kernel<bf16>, dim3(ctas), dim3(kGenThreads), 0, c->stream, a);
     e = static_cast<int>(cudaGetLastError());
     if (e) return e;
   }
@@ -1130,12 +1185,10 @@ int launch_prefill(const void* q, int q_stride, const void* kc, const void* vc, 
 
 }  // namespace
 
-extern "C" int rl_kv8_attn_prefill(int dtype, const void* q, int q_stride, const void* kc, const void* vc, const void* ks,
-                                   const void* vs, const int32_t* bt, int max_blocks, const int32_t* tile_seq,
-                                   const int32_t* tile_tok, const int32_t* tile_rows, const int32_t* positions, void* out,
-                                   int out_stride, int tiles, int hq, int hkv, int page_size, int window, float scale, int impl,
-                                   int* status, void* stream) {
-  auto run = dtype == 0 ? launch_prefill<float> : launch_prefill<bf16>;
-  return run(q, q_stride, kc, vc, ks, vs, bt, max_blocks, tile_seq, tile_tok, tile_rows, positions, out, out_stride, tiles, hq,
-             hkv, page_size, window, scale, impl, status, static_cast<cudaStream_t>(stream));
+extern "C" int rl_kv8_attn_prefill(const Kv8PrefillCall* c) {
+  auto run = c->dtype == 0 ? launch_prefill<float> : launch_prefill<bf16>;
+  return run(c->q, static_cast<int>(c->q_stride), c->kc, c->vc, c->ks, c->vs, c->block_table, static_cast<int>(c->max_blocks), c->tile_seq,
+             c->tile_tok, c->tile_rows, c->positions, c->out, static_cast<int>(c->out_stride), static_cast<int>(c->tiles),
+             static_cast<int>(c->hq), static_cast<int>(c->hkv), static_cast<int>(c->page_size), static_cast<int>(c->window),
+             static_cast<float>(c->scale), static_cast<int>(c->impl), c->status, c->stream);
 }

@@ -22,7 +22,11 @@
 // depend on one another is asked for together, and results meet in two steps: weights by a warp a head, then sums of 16 bytes a
 // thread.
 //
-// Where rows are shared out (see launch_decode_tc for the choice):
+// What bounds a long launch is the copies' rate; a short one its chain of trips (0.7 us each) and the one fetch of every
+// instruction.  32 / 8 heads, the token's own write included at head size 64: one sequence of 513 keys 8.8 us, 8 of 4,096 16.6 us (2.0 TB/s),
+// 64 of 516 to 768 19.0; head size 128: one of 131,072 keys 58 us (4.6 TB/s), 24 of 64 to 8,192 62 us (3.6 TB/s).
+//
+// Where rows are shared out (see kv8_choice in kv8.cu for which):
 //   rows    a cluster of up to 8 CTAs to a row, whose partial results meet in the first one's shared memory; or, with more rows
 //           than clusters can be resident, CTAs whose warps form groups that take a row each, one after another
 //   pieces  every row in as many pieces as there are CTAs for, which meet in global memory: few rows, and long ones

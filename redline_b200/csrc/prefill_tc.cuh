@@ -41,6 +41,9 @@
 // head size 128, 333 tokens 21.9 (26.4), 2,048 70.4 (79.5), 8,192 834 (918), 16,384 3,146 (3,464), 2,048 behind 12,288
 // 724 (795).  So long rows at head size 64 are 1 to 2 % slower: half the row warps hide less of the hand-overs.
 // The two give the same bits: a row's denominator is summed in the two threads' chains still.
+// With eight bits, 32 / 8 heads of 64: 333 tokens behind 1,000 keys 35 us (16 bits 36), 2,048 behind 6,144 276 us, 436 TFLOP/s (227); three
+// portions of 300 to 900 tokens behind up to 2,000 at head size 128 169 us, 289 TFLOP/s.  The loaders' instructions are what it takes
+// longer: without them the long portion takes 249 us, without the conversions alone 280 of 284.
 // Warp roles: warps 0-3 rows of slot 0, warps 4-7 rows of slot 1 (warp w owns TMEM lanes
 // 32 (w % 4) ..), warp 8 brings both Q tiles once per item and the K tiles, warp 9 the V tiles,
 // from the paged cache with 16-byte cp.async copies (zero-filled outside the live keys), lane 0
@@ -68,9 +71,9 @@ constexpr bool kTcOwnP = kD == 64;                      // P has tensor-memory c
 constexpr int kTcColP = 384;                            // with columns of its own: P of slot s at kTcColP + s * 64
 // A cache in 8 bits: teams of three warps load K and V (one warp alone takes twice as long over a tile as the rows).  Every warp of a
 // team works on every tile, so its waits for a stage see every phase.  Warps 8 .. 11, 14 and 15 load, 12 and 13 issue the
-// MMAs.  Sixteen warps begin with 128 registers a thread; the two warpgroups of rows take 160, the other two leave them 96:
-// 256 x (160 + 96) = 512 x 128.
-constexpr int kTcThreads8 = 512, kTcRowRegs8 = 160, kTcOtherRegs8 = 96, kTcLoaders8 = 3;
+// MMAs.  Sixteen warps begin with 128 registers a thread; the two warpgroups of rows take 152, the other two leave them 104:
+// 256 x (152 + 104) = 512 x 128.  (160 and 96: 1 to 6 % longer.)
+constexpr int kTcThreads8 = 512, kTcRowRegs8 = 152, kTcOtherRegs8 = 104, kTcLoaders8 = 3;
 static_assert(256 * (kTcRowRegs8 + kTcOtherRegs8) <= 512 * 128, "the launch's registers");
 constexpr float kTcGrow = 8.f;                          // log2 of the growth of a row's maximum that moves the reference
 
@@ -270,15 +273,15 @@ struct TcWalk {
 };
 
 // 2^e as a pair of halves, for e <= 0 (0 below the halves' range).
-__device__ __forceinline__ __half2 tc_half_power(int e) {
+__device__ __forceinline__ uint32_t tc_half_power(int e) {
   const uint32_t b = e >= -14 ? static_cast<uint32_t>(e + 15) << 10 : (e >= -24 ? 1u << (e + 24) : 0u);
-  const uint32_t two = b | b << 16;
-  return *reinterpret_cast<const __half2*>(&two);
+  return b | b << 16;
 }
 
 // The loaders of a cache in 8 bits: three warps K, three V (the first two of them a slot's Q as well).  The UNITS of a CTA's tiles, 16 or 32
 // keys each (four 16-byte pieces to a lane), go to a team's warps in turn, so all of them work on one tile.  (With a tile to a warp, each
-// with a stage of its own, a stage was empty for the whole time that one warp takes over a tile: OLDUS)  A unit's
+// with a stage of its own, a stage was empty for the whole time that one warp takes over a tile: 2,048 tokens behind 6,144 keys
+// 322 us, three portions at head size 128 212; with teams 276 and 169.  A ring of bytes in shared memory instead of registers: 357.)  A unit's
 // bytes come through registers, the next unit's on their way while one is converted and stored where the copies of a 16-bit cache would
 // have put it.  Page ids and scales come 32 units at a time, a unit to a lane, a window ahead.
 template <typename Args>
@@ -300,9 +303,11 @@ __device__ __forceinline__ void tc_load_eight_bit(const Args& a, PrefillTcShared
   // place % 8 is the lane's own, or with rounds of four rows the lane's own and another 4 in every second
   const uint32_t c_half = static_cast<uint32_t>(piece >> 2) * kTcHalfBytes;
   const uint32_t at0 = c_half + rr * 128 + ((((2 * piece) & 7) ^ rr) << 4), at1 = c_half + rr * 128 + ((((2 * piece + 1) & 7) ^ rr) << 4);
+  const uint8_t* const cache_lane = cache + lane * 16;
+  const uint32_t page_bytes = static_cast<uint32_t>(kD) << shift;
   struct Unit {
     uint4 raw[kPieces];
-    int code[kBlocks];
+    uint32_t factor[kBlocks];
   };
   bool ok = true;
   TcWalk wk;
@@ -312,19 +317,19 @@ __device__ __forceinline__ void tc_load_eight_bit(const Args& a, PrefillTcShared
     const int first = w.lo0 >> shift, last = (w.k_end - 1) >> shift;
     const int units = w.nt * kUnits;
     int x = (turn + L - (wk.g * kUnits) % L) % L;        // the warp's first unit of the item
-    auto pages_of = [&](int u, int* id) {                // a lane's unit of the 32 from u on
+    auto pages_of = [&](int u, int* page) {              // a lane's unit of the 32 from u on: its blocks' (page, head)
 #pragma unroll
       for (int j = 0; j < kBlocks; ++j)
-        id[j] = bt[min(max((w.k_begin + ((u + L * lane) * kBlocks + j) * 16) >> shift, first), last)];
+        page[j] = bt[min(max((w.k_begin + ((u + L * lane) * kBlocks + j) * 16) >> shift, first), last)] * a.hkv + w.kvh;
     };
-    auto codes_of = [&](const int* id, int* code) {
+    auto codes_of = [&](const int* page, int* code) {
 #pragma unroll
-      for (int j = 0; j < kBlocks; ++j) code[j] = scales[static_cast<size_t>(id[j]) * a.hkv + w.kvh];
+      for (int j = 0; j < kBlocks; ++j) code[j] = scales[page[j]];
     };
-    int id[kBlocks], code[kBlocks], next_id[kBlocks], next_code[kBlocks];
-    pages_of(x, id);
-    pages_of(x + 32 * L, next_id);
-    codes_of(id, code);
+    int page[kBlocks], next_page[kBlocks], next_code[kBlocks];
+    pages_of(x, page);
+    codes_of(page, next_code);
+    pages_of(x + 32 * L, next_page);
     // the item's largest scale
     int most = 0;
 #pragma unroll 4
@@ -365,55 +370,67 @@ __device__ __forceinline__ void tc_load_eight_bit(const Args& a, PrefillTcShared
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->q_full[s]);
     }
+    uint32_t factor[kBlocks];
+    auto factors_of = [&](const int* code) {
+#pragma unroll
+      for (int j = 0; j < kBlocks; ++j) factor[j] = tc_half_power(code[j] - most);
+    };
+    factors_of(next_code);
     // asks for unit u, the r-th of the window
     int r = 0;
     auto ask = [&](int u, Unit& to) {
-      if (r == 16) codes_of(next_id, next_code);
+      if (r == 16) codes_of(next_page, next_code);
       if (r == 32) {
 #pragma unroll
-        for (int j = 0; j < kBlocks; ++j) {
-          id[j] = next_id[j];
-          code[j] = next_code[j];
-        }
-        pages_of(u + 32 * L, next_id);
+        for (int j = 0; j < kBlocks; ++j) page[j] = next_page[j];
+        factors_of(next_code);
+        pages_of(u + 32 * L, next_page);
         r = 0;
       }
       const int k0 = w.k_begin + u * (16 * kBlocks);
-      const bool whole = k0 >= w.lo0 && k0 + 16 * kBlocks <= w.k_end;
+      const uint8_t* from[kBlocks];
 #pragma unroll
       for (int j = 0; j < kBlocks; ++j) {
-        const int key = k0 + j * 16;
-        const int page = __shfl_sync(0xffffffffu, id[j], r);
-        to.code[j] = __shfl_sync(0xffffffffu, code[j], r);
-        const uint8_t* p = cache + (((static_cast<size_t>(page) * a.hkv + w.kvh) << shift) + (key & ps_mask)) * kD + lane * 16;
+        from[j] = cache_lane + static_cast<size_t>(static_cast<uint32_t>(__shfl_sync(0xffffffffu, page[j], r))) * page_bytes
+                  + ((k0 + j * 16) & ps_mask) * kD;
+        to.factor[j] = __shfl_sync(0xffffffffu, factor[j], r);
+      }
+      if (k0 >= w.lo0 && k0 + 16 * kBlocks <= w.k_end) {
 #pragma unroll
-        for (int i = 0; i < kPer16; ++i) {
-          const int mine = key + i * RPI + rr;
-          to.raw[j * kPer16 + i] = make_uint4(0, 0, 0, 0);
-          if (whole || (mine < w.k_end && mine >= w.lo0)) to.raw[j * kPer16 + i] = *reinterpret_cast<const uint4*>(p + i * 512);
+        for (int i = 0; i < kPieces; ++i) to.raw[i] = *reinterpret_cast<const uint4*>(from[i / kPer16] + i % kPer16 * 512);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+          const int key = k0 + i / kPer16 * 16 + i % kPer16 * RPI + rr;
+          to.raw[i] = make_uint4(0, 0, 0, 0);
+          if (key < w.k_end && key >= w.lo0) to.raw[i] = *reinterpret_cast<const uint4*>(from[i / kPer16] + i % kPer16 * 512);
         }
       }
       ++r;
     };
     int tile = -1;                                       // the item's tile that the warp is at
+    int stage = 0;
+    unsigned char* tile_at = stage0;
     auto hand_over = [&]() {
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(&full[(wk.g + tile) % kTcStages]);
+      if (lane == 0) mbar_arrive(&full[stage]);
     };
     auto put = [&](int u, const Unit& from) {
       if (u / kUnits != tile) {
         if (tile >= 0) hand_over();
         tile = u / kUnits;
         const int g = wk.g + tile;
-        ok = mbar_wait(&freed[g % kTcStages], ((g / kTcStages) & 1) ^ 1, &sh->abort);      // (a fresh barrier passes a wait on parity 1)
+        stage = g % kTcStages;
+        tile_at = stage0 + stage * kTcTileBytes;
+        ok = mbar_wait(&freed[stage], ((g / kTcStages) & 1) ^ 1, &sh->abort);      // (a fresh barrier passes a wait on parity 1)
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) return;
       }
-      unsigned char* dst = stage0 + ((wk.g + tile) % kTcStages) * kTcTileBytes + (u % kUnits) * (kBlocks * 16 * 128);
+      unsigned char* dst = tile_at + (u % kUnits) * (kBlocks * 16 * 128);
 #pragma unroll
       for (int j = 0; j < kBlocks; ++j) {
-        const __half2 f = tc_half_power(from.code[j] - most);
+        const __half2 f = *reinterpret_cast<const __half2*>(&from.factor[j]);
 #pragma unroll
         for (int i = 0; i < kPer16; ++i) {
           const uint4 v = from.raw[j * kPer16 + i];

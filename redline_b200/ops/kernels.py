@@ -10,8 +10,9 @@ from __future__ import annotations
 import ctypes
 import math
 import os
+import struct
 from concurrent.futures import ThreadPoolExecutor
-from ctypes import c_float, c_int, c_longlong, c_uint, c_void_p
+from ctypes import c_char_p, c_float, c_int, c_longlong, c_uint, c_void_p
 from functools import lru_cache
 from typing import Dict, Optional, Tuple
 
@@ -666,6 +667,13 @@ def attn_prefill(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, vcache: t
 
 KV8_DTYPE, KV8_SCALE_DTYPE = torch.float8_e4m3fn, torch.float8_e8m0fnu
 KV8_PAGE_SIZES = (16, 32, 64)
+_KV8_LAUNCH_ITEMS = 1024      # items of one launch (kMaxItems)
+# the entry points' arguments, packed (Kv8WriteCall, Kv8DecodeCall, Kv8PrefillCall)
+_KV8_WRITE, _KV8_DECODE, _KV8_PREFILL = struct.Struct("21q").pack, struct.Struct("19qd10q").pack, struct.Struct("20qd3q").pack
+
+
+def _kv8_ptr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _kv8(head_dim: int) -> ctypes.CDLL:
@@ -676,7 +684,8 @@ def _kv8(head_dim: int) -> ctypes.CDLL:
 
 
 # (A step of single tokens makes one of these calls per layer, and its GPU time is a few us: every attribute of a tensor is asked
-# for once, since each costs 0.1 to 0.3 us: kv8_write's call with its launch went from 15.7 to 12.9 us of one core.)
+# for once, since each costs 0.1 to 0.3 us, and the arguments go over in one piece: kv8_write's call with its launch went from 15.7 to
+# 11.1 us of one core.)
 def _kv8_check(what: str, kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch.Tensor, vscale: torch.Tensor, num_heads: int,
                num_kv_heads: int, head_dim: int, page_size: int) -> None:
     """The cache's tensors have the types and shapes that the kernels take."""
@@ -775,13 +784,11 @@ def kv8_write(qkv: torch.Tensor, positions: torch.Tensor, slots: Optional[torch.
         q_stride = _kv8_rows(what, "q_out", q_out, None, num_heads * head_dim, at)
         if q_out.dtype is not qkv.dtype or q_out.shape[0] < T:
             raise KernelError(f"{what}: q_out must be {qkv.dtype} with {T} rows")
-    f = _fn(_kv8(head_dim), "rl_kv8_write",
-            [c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
-             c_int, c_int, c_int, c_int, c_int, c_int, c_longlong, c_void_p, c_void_p])
+    f = _fn(_kv8(head_dim), "rl_kv8_write", [c_char_p])
     with _on(kcache):
-        _check(f(_code(qkv.dtype), qkv.data_ptr(), stride, positions.data_ptr(), _ptr(slots), _ptr(cos), _ptr(sin),
-                 kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(), vscale.data_ptr(), _ptr(q_out),
-                 q_stride, T, num_heads, num_kv_heads, page_size, max_pos, kcache.shape[0] * page_size, status.data_ptr(), _stream()),
+        _check(f(_KV8_WRITE(_code(qkv.dtype), qkv.data_ptr(), stride, positions.data_ptr(), _kv8_ptr(slots), _kv8_ptr(cos), _kv8_ptr(sin),
+                            kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(), vscale.data_ptr(), _kv8_ptr(q_out), q_stride, T,
+                            num_heads, num_kv_heads, page_size, max_pos, kcache.shape[0] * page_size, status.data_ptr(), _stream())),
                what)
 
 
@@ -830,17 +837,20 @@ def _kv8_decode(what: str, q, q_stride, kcache, vcache, kscale, vscale, block_ta
     seen = min(max_ctx, capacity) if max_ctx > 0 else capacity
     if window > 0:
         seen, sum_ctx = min(seen, window), min(sum_ctx, nitems * window)
-    f = _fn(_kv8(head_dim), "rl_kv8_attn_decode",
-            [c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p,
-             c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_int, c_int, c_longlong, c_void_p,
-             c_int, c_longlong, c_int, c_void_p])
+    if not 0 <= impl <= 4:
+        raise KernelError(f"{what}: impl {impl} is none of 0 to 4")
+    code = _code(q.dtype)
+    # (the kernel that stores the tokens on its way: rl_kv8_attn_decode)
+    fused = code == 1 and head_dim in (64, 128) and num_heads <= 16 * num_kv_heads and impl != 1 and page_size <= 32
+    launches = (nitems + _KV8_LAUNCH_ITEMS - 1) // _KV8_LAUNCH_ITEMS + (1 if store and not fused else 0)
+    f = _fn(_kv8(head_dim), "rl_kv8_attn_decode", [c_char_p])
     with _on(kcache):
-        _check(f(_code(q.dtype), q.data_ptr(), q_stride, kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(),
-                 vscale.data_ptr(), block_table.data_ptr(), blocks, items.data_ptr(), nitems, part.data_ptr(),
-                 counters.data_ptr(), out.data_ptr(), out_stride, num_heads, num_kv_heads, page_size, window, scale,
-                 _ptr(cos), _ptr(sin), max_pos, 1 if store else 0, kcache.shape[0] * page_size,
-                 status.data_ptr() if store else None, seen, sum_ctx, impl, _stream()),
-               what, 2 if store else 1)
+        _check(f(_KV8_DECODE(code, q.data_ptr(), q_stride, kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(), vscale.data_ptr(),
+                             block_table.data_ptr(), blocks, items.data_ptr(), nitems, part.data_ptr(), counters.data_ptr(),
+                             out.data_ptr(), out_stride, num_heads, num_kv_heads, page_size, window, scale, _kv8_ptr(cos),
+                             _kv8_ptr(sin), max_pos, 1 if store else 0, kcache.shape[0] * page_size,
+                             status.data_ptr() if store else 0, seen, sum_ctx, impl, _stream())),
+               what, launches)
 
 
 def kv8_attn_decode(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch.Tensor,
@@ -910,14 +920,14 @@ def kv8_attn_prefill(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, vcach
     _kv8_scale(what, window, scale)
     if tiles == 0:
         return
-    f = _fn(_kv8(head_dim), "rl_kv8_attn_prefill",
-            [c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
-             c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p])
+    if impl not in (0, 1, 3):
+        raise KernelError(f"{what}: impl {impl} is none of 0, 1 and 3")
+    f = _fn(_kv8(head_dim), "rl_kv8_attn_prefill", [c_char_p])
     with _on(kcache):
-        _check(f(_code(q.dtype), q.data_ptr(), q_stride, kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(), vscale.data_ptr(),
-                 block_table.data_ptr(), block_table.shape[1], tile_seq.data_ptr(), tile_tok.data_ptr(), tile_rows.data_ptr(),
-                 positions.data_ptr(), out.data_ptr(), out_stride, tiles, num_heads, num_kv_heads, page_size, window,
-                 scale, impl, tc_status(q.device).data_ptr(), _stream()), what)
+        _check(f(_KV8_PREFILL(_code(q.dtype), q.data_ptr(), q_stride, kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(),
+                              vscale.data_ptr(), block_table.data_ptr(), block_table.shape[1], tile_seq.data_ptr(),
+                              tile_tok.data_ptr(), tile_rows.data_ptr(), positions.data_ptr(), out.data_ptr(), out_stride, tiles,
+                              num_heads, num_kv_heads, page_size, window, scale, impl, tc_status(q.device).data_ptr(), _stream())), what)
 
 
 # ------------------------------------------- row-wise kernels of blocks with norms on both sides

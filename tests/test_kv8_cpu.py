@@ -86,6 +86,7 @@ def test_rows_that_are_refused(monkeypatch):
         (prefill, dict(out=torch.zeros(3, HEADS * DIM, dtype=torch.bfloat16)), "out must be"),
         (prefill, dict(tiles=2), "for 2 tiles"),
         (prefill, dict(window=-1), "window"),
+        (prefill, dict(impl=2), "impl 2"),
         (prefill, dict(scale=0.0), "scale must be positive"),
         (prefill, dict(scale=-1.0), "scale must be positive"),
         (prefill, dict(scale=float("nan")), "scale must be positive"),

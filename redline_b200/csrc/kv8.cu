@@ -160,10 +160,10 @@ kv8_write_kernel(const Kv8WriteArgs<T> a, int span, int tasks) {
         n += 32;
       }
     }
-    const T* src = a.qkv + static_cast<size_t>(t) * a.qkv_stride + static_cast<size_t>(a.hq + w) * kD + ch * 8;
+    const T* src = a.qkv + static_cast<size_t>(a.hq + w) * kD + ch * 8;
     const bool turn = !is_v && a.cos != nullptr;
     auto load = [&](int i, float* x) {                     // token i of the run
-      const T* p = src + static_cast<size_t>(i) * a.qkv_stride;
+      const T* p = src + static_cast<size_t>(a.items != nullptr ? a.items[t + i].x : t + i) * a.qkv_stride;
       load8(p, x);
       load8(p + kD / 2, x + 8);
       if (turn) {

@@ -383,6 +383,50 @@ def test_decode_with_the_tokens_own_keys(heads, kv_heads, dim, page, window, dty
     assert status.item() & 2
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim,page,dtype", [(4, 2, 64, 16, "bfloat16"), (4, 2, 64, 64, "bfloat16"), (4, 2, 64, 16, "float32"),
+                                                           (10, 2, 80, 32, "bfloat16"), (4, 1, 128, 64, "bfloat16")])
+def test_decode_of_items_in_another_order(heads, kv_heads, dim, page, dtype):
+    """Items name their rows: in another order than the rows, and only some of them, they store and attend the same."""
+    ctxs = (1, 17, 33, 64, 130)
+    cache, table = filled([max(n - 1, 1) for n in ctxs], heads, kv_heads, dim, page, seed=9, poison=False)
+    pages = cache[0].shape[0] + len(ctxs)
+    grown = empty_cache(pages, kv_heads, page, dim, 1)
+    for old, new in zip(cache, grown):
+        new[:old.shape[0]] = old
+    for s, n in enumerate(ctxs):
+        if (n - 1) % page == 0:
+            table[s, (n - 1) // page] = pages - 1 - s
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(len(ctxs) + 2, (heads + 2 * kv_heads) * dim, generator=g).to(DT[dtype]).to(DEV)
+    cos, sin = (t.to(DEV) for t in angles(140, dim))
+    work = kernels.kv8_decode_workspace(len(ctxs), heads, kv_heads, dim, torch.device(DEV))
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    results = []
+    row_of = (6, 2, 0, 5, 3)
+    for order in ((0, 1, 2, 3, 4), (3, 0, 4, 2, 1)):
+        gpu = on_gpu(grown)
+        out = torch.full((len(x), heads * dim), 9.0, dtype=x.dtype, device=DEV)
+        items = torch.tensor([(row_of[s], s, ctxs[s], 0) for s in order], dtype=torch.int32, device=DEV)
+        kernels.kv8_attn_decode_rope(x, x.stride(0), *gpu, table.to(DEV), items, work, out, len(order), heads, kv_heads, dim, page, 0,
+                                     1.0 / math.sqrt(dim), cos, sin, status, max_ctx=max(ctxs), sum_ctx=sum(ctxs))
+        results.append((out, *(t.view(torch.uint8).cpu() for t in gpu)))
+    assert status.item() == 0
+    positions = [n - 1 for n in ctxs]
+    slots = [int(table[s, p // page]) * page + p % page for s, p in enumerate(positions)]
+    k, v = (x.cpu().float()[list(row_of)][:, (heads + i * kv_heads) * dim:][:, :kv_heads * dim].reshape(-1, kv_heads, dim) for i in (0, 1))
+    P.store(P.rotate(k, cos.cpu()[positions], sin.cpu()[positions]), slots, grown[0], grown[2])
+    P.store(v, slots, grown[1], grown[3])
+    for out, *stored in results:
+        for got, want in zip(stored, grown):
+            assert torch.equal(got, want)
+        assert (out[[1, 4]] == 9.0).all()
+        keys, vals = P.values(grown[0], grown[2]), P.values(grown[1], grown[3])
+        for s, n in enumerate(ctxs):
+            q = P.rotate(x.cpu().float()[row_of[s], :heads * dim].view(1, heads, dim), cos.cpu()[n - 1:n], sin.cpu()[n - 1:n])
+            ref = P.attend(q, keys, vals, table[s], [n - 1], 0, 1.0 / math.sqrt(dim))
+            near(out[row_of[s]].view(1, heads, dim), ref, vals[table[s][:-(-n // page)].long()], dtype)
+
+
 PROMPT = [  # heads, kv heads, head size, page, window, (cached, new) of every sequence
     (4, 2, 64, 16, 0, ((0, 2), (0, 33), (5, 128), (100, 129))),
     (32, 8, 64, 16, 0, ((70, 200),)),

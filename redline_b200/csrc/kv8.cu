@@ -399,6 +399,7 @@ kv8_decode_kernel(const Kv8Args a) {
   const bool in_head = ch * 16 < kD;
   const Kv8Cut cut(kv8_units(a, start), gridDim.x);
   if (static_cast<int>(blockIdx.x) >= cut.shares) return;
+  bool bad = false;                          // a page id beyond the pool
   const int begin = cut.begin(blockIdx.x), end = cut.begin(blockIdx.x + 1);
   for (int u = begin; u < end;) {
     const Kv8Segment g = kv8_segment(a, start, u, end);
@@ -439,7 +440,7 @@ kv8_decode_kernel(const Kv8Args a) {
       for (int k0 = g.key_lo + warp * KPW; k0 < g.key_hi; k0 += KPW * (kGenThreads / 32)) {
         const int key = k0 + slot;
         const bool live = key < g.key_hi;
-        const size_t block = static_cast<size_t>(bt[(live ? key : k0) >> a.page_shift]) * a.hkv + g.kvh;
+        const size_t block = static_cast<size_t>(kv8_page(bt[(live ? key : k0) >> a.page_shift], a.pages, bad)) * a.hkv + g.kvh;
         const size_t at = (block * ps + (key & (ps - 1))) * kD + ch * 16;
         float s[kGenHeads] = {};
         uint4 vraw = make_uint4(0, 0, 0, 0);
@@ -547,6 +548,7 @@ kv8_decode_kernel(const Kv8Args a) {
     }
     u = g.next;
   }
+  if (bad) atomicOr(a.status, a.bad_page);
 }
 
 template <typename T>
@@ -568,6 +570,7 @@ struct Kv8PrefillArgs {
   int out_stride;
   int hq, hkv, page_shift, window;
   float scale;
+  int pages;                                   // of the pool
 };
 
 }  // namespace rl
@@ -593,7 +596,7 @@ constexpr size_t kPreSmem = sizeof(float) * (2 * kD * kPLd + kPK * kD + kPK * kP
 // heads of 128: 45 us.  What bounds it is the FFMA pipe and the reads of its operands from shared memory; few items do not fill the SMs.
 template <typename T>
 __global__ void __launch_bounds__(kPreThreads)
-kv8_prefill_kernel(const Kv8PrefillArgs<T> a) {
+kv8_prefill_kernel(const Kv8PrefillArgs<T> a, int* status) {
   extern __shared__ __align__(16) float tiles[];
   float* qs = tiles;                        // [D][68], scaled
   float* ks = qs + kD * kPLd;               // [D][68]
@@ -621,6 +624,7 @@ kv8_prefill_kernel(const Kv8PrefillArgs<T> a) {
   const int k_end = pos0 + rows;
   const int first = a.window > 0 && pos0 + 1 > a.window ? pos0 + 1 - a.window : 0;
   float m[4], l[4], acc[4][NC];
+  bool bad = false;                                       // a page id beyond the pool
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     m[i] = -INFINITY;
@@ -634,7 +638,7 @@ kv8_prefill_kernel(const Kv8PrefillArgs<T> a) {
       const int key = i % kPK, c = i / kPK, j = k0 + key;
       float k[16] = {}, v[16] = {};
       if (j < k_end && j >= first) {
-        const size_t block = static_cast<size_t>(bt[j >> a.page_shift]) * a.hkv + kvh;
+        const size_t block = static_cast<size_t>(kv8_page(bt[j >> a.page_shift], a.pages, bad)) * a.hkv + kvh;
         const size_t at = (block * page + (j & (page - 1))) * kD + c * 16;
         const float fk = kv8_scale(a.kscale[block]), fv = kv8_scale(a.vscale[block]);
         kv8_f16(*reinterpret_cast<const uint4*>(a.kcache + at), k);
@@ -709,6 +713,7 @@ kv8_prefill_kernel(const Kv8PrefillArgs<T> a) {
       }
     }
   }
+  if (bad) atomicOr(status, kKv8BadPage);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = ty * 4 + i;
@@ -1006,6 +1011,7 @@ struct Kv8DecodeCall {
   int64_t max_pos, store, num_slots;
   int* status;
   int64_t max_ctx, sum_ctx, impl;
+  int64_t bad_page;
   cudaStream_t stream;
 };
 
@@ -1020,11 +1026,11 @@ struct Kv8PrefillCall {
   void* out;
   int64_t out_stride, tiles, hq, hkv, page_size, window;
   double scale;
-  int64_t impl;
+  int64_t impl, pages;
   int* status;
   cudaStream_t stream;
 };
-static_assert(sizeof(Kv8WriteCall) == 21 * 8 && sizeof(Kv8DecodeCall) == 30 * 8 && sizeof(Kv8PrefillCall) == 24 * 8, "as they are packed");
+static_assert(sizeof(Kv8WriteCall) == 21 * 8 && sizeof(Kv8DecodeCall) == 31 * 8 && sizeof(Kv8PrefillCall) == 25 * 8, "as they are packed");
 
 // Which way of sharing out (2, 3 or 4; 0: the CUDA cores) a launch on the tensor cores would go by impl 0, or an error as a negative number.
 int rl_kv8_decode_choice(int dtype, int nitems, int hq, int hkv, int max_ctx, long long sum_ctx) {
@@ -1094,7 +1100,9 @@ int rl_kv8_attn_decode(const Kv8DecodeCall* c) {
   a.store = fused ? 1 : 0;
   a.sin = c->sin;
   a.max_pos = max_pos;
+  a.pages = static_cast<int>(c->num_slots / page_size);
   a.status = c->status;
+  a.bad_page = static_cast<int>(c->bad_page);
   for (int i0 = 0; i0 < nitems; i0 += kMaxItems) {         // (one launch unless there are very many items)
     a.items = c->items + i0;
     a.nitems = nitems - i0 < kMaxItems ? nitems - i0 : kMaxItems;
@@ -1128,7 +1136,7 @@ template <typename T>
 int launch_prefill(const void* q, int q_stride, const void* kc, const void* vc, const void* ks, const void* vs, const int32_t* bt,
                    int max_blocks, const int32_t* tile_seq, const int32_t* tile_tok, const int32_t* tile_rows,
                    const int32_t* positions, void* out, int out_stride, int tiles, int hq, int hkv, int page_size, int window,
-                   float scale, int impl, int* status, cudaStream_t stream) {
+                   float scale, int impl, int pages, int* status, cudaStream_t stream) {
   Kv8PrefillArgs<T> a;
   a.q = static_cast<const T*>(q);
   a.q_stride = q_stride;
@@ -1149,6 +1157,7 @@ int launch_prefill(const void* q, int q_stride, const void* kc, const void* vc, 
   a.page_shift = shift_of(page_size);
   a.window = window;
   a.scale = scale;
+  a.pages = pages;
   static bool tc_set[kMaxDevices], simt_set[kMaxDevices];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -1179,7 +1188,7 @@ int launch_prefill(const void* q, int q_stride, const void* kc, const void* vc, 
     if (e != cudaSuccess) return static_cast<int>(e);
     simt_set[dev] = true;
   }
-  launch_kernel(kv8_prefill_kernel<T>, dim3(tiles * 2, hq), dim3(kPreThreads), kPreSmem, stream, a);
+  launch_kernel(kv8_prefill_kernel<T>, dim3(tiles * 2, hq), dim3(kPreThreads), kPreSmem, stream, a, status);
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -1190,5 +1199,5 @@ extern "C" int rl_kv8_attn_prefill(const Kv8PrefillCall* c) {
   return run(c->q, static_cast<int>(c->q_stride), c->kc, c->vc, c->ks, c->vs, c->block_table, static_cast<int>(c->max_blocks), c->tile_seq,
              c->tile_tok, c->tile_rows, c->positions, c->out, static_cast<int>(c->out_stride), static_cast<int>(c->tiles),
              static_cast<int>(c->hq), static_cast<int>(c->hkv), static_cast<int>(c->page_size), static_cast<int>(c->window),
-             static_cast<float>(c->scale), static_cast<int>(c->impl), c->status, c->stream);
+             static_cast<float>(c->scale), static_cast<int>(c->impl), static_cast<int>(c->pages), c->status, c->stream);
 }

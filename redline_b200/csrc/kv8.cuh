@@ -79,6 +79,15 @@ __device__ __forceinline__ uint32_t kv8_pack2(float lo, float hi) {
 }
 __device__ __forceinline__ uint32_t kv8_pack4(const float* f) { return kv8_pack2(f[0], f[1]) | kv8_pack2(f[2], f[3]) << 16; }
 
+// A page id of a block table, if the pool has such a page; else page 0, the one that belongs to nobody, and `bad` is set.
+__device__ __forceinline__ int kv8_page(int page, int pages, bool& bad) {
+  const bool in = static_cast<unsigned>(page) < static_cast<unsigned>(pages);
+  bad |= !in;
+  return in ? page : 0;
+}
+
+constexpr int kKv8BadPage = 16;      // the bit of the tcgen05 kernels' status that a page id beyond the pool sets
+
 // ---- single tokens: how the keys of a launch are shared out
 //
 // A row is an (item, kv head): the query heads of one kv head of one sequence's token.  Its live keys are counted in
@@ -109,7 +118,9 @@ struct Kv8Args {
   const float* sin;
   int max_pos;
   int store;                   // q holds rows [q | k | v]: the tokens' keys and values are stored by the attention's kernel
+  int pages;                   // of the pool
   int* status;
+  int bad_page;                // the bit of *status that a page id beyond the pool sets
 };
 
 // What a part of a row's keys comes to, for one head, is left as D numerators times 2^(m + d) and a denominator times 2^m (log2

@@ -315,7 +315,8 @@ __device__ __forceinline__ void tc_run(const Kv8Args& a, const Kv8Segment& s, in
   auto page_of = [&](int key) { return page_last - min(max(key >> shift, page_first), page_last); };     // counted from the last
   // a window of 32 pages, a page to a lane: its id and the bytes of its scales (K, V), those of the window before, and the
   // ids of the next; and the scales of the window that the sums are in
-  int window = 0, my_page = bt[max(page_last - lane, page_first)], next_page = 0;
+  bool bad = false;                                      // a page id beyond the pool
+  int window = 0, my_page = kv8_page(bt[max(page_last - lane, page_first)], a.pages, bad), next_page = 0;
   const int top = sb0 + n - 1;
   const bool store = a.store && s.key_hi == s.ctx && top == (s.ctx - 1) / kSub;      // the newest page is this warp's
   TcRaw row, token;
@@ -346,7 +347,7 @@ __device__ __forceinline__ void tc_run(const Kv8Args& a, const Kv8Segment& s, in
       const int idx = page_of(key);
       if ((idx >> 5) != window) {
         window = idx >> 5;
-        my_page = next_page;
+        my_page = kv8_page(next_page, a.pages, bad);
         old_codes = my_codes;
         my_codes = codes_of(my_page);
         next_page = bt[max(page_last - window * 32 - 32 - lane, page_first)];
@@ -370,6 +371,8 @@ __device__ __forceinline__ void tc_run(const Kv8Args& a, const Kv8Segment& s, in
       const int4 other = a.items[i];
       if (other.z > 0 && a.block_table[static_cast<size_t>(other.y) * a.max_blocks + ((other.z - 1) >> shift)] == token_page) mine = false;
     }
+    // (a page beyond the pool stands as page 0 here, but nothing is stored there)
+    if (static_cast<unsigned>(bt[(s.ctx - 1) >> shift]) >= static_cast<unsigned>(a.pages)) mine = false;
     mine = __all_sync(0xffffffffu, mine);
     if (!mine && token_page != 0 && lane == 0) atomicOr(a.status, 8);
   }
@@ -570,6 +573,7 @@ __device__ __forceinline__ void tc_run(const Kv8Args& a, const Kv8Segment& s, in
       }
   }
   cp_async_wait<0>();
+  if (bad) atomicOr(a.status, a.bad_page);
 #pragma unroll
   for (int h = 0; h < NR; ++h)                           // the eight lanes of a head
 #pragma unroll

@@ -286,7 +286,8 @@ __device__ __forceinline__ uint32_t tc_half_power(int e) {
 // have put it.  Page ids and scales come 32 units at a time, a unit to a lane, a window ahead.
 template <typename Args>
 __device__ __forceinline__ void tc_load_eight_bit(const Args& a, PrefillTcShared* sh, unsigned char* q_s, unsigned char* k_s,
-                                                  unsigned char* v_s, bool is_v, int turn, int lane, int n_items, int pairs, int tiles) {
+                                                  unsigned char* v_s, bool is_v, int turn, int lane, int n_items, int pairs, int tiles,
+                                                  int* status) {
   constexpr int L = kTcLoaders8;
   constexpr int P = kD / 16, RPI = 32 / P;               // pieces of a row; rows that the warp's lanes cover at once
   constexpr int kPer16 = 16 / RPI;                       // pieces of a lane in 16 keys (of one page)
@@ -309,7 +310,7 @@ __device__ __forceinline__ void tc_load_eight_bit(const Args& a, PrefillTcShared
     uint4 raw[kPieces];
     uint32_t factor[kBlocks];
   };
-  bool ok = true;
+  bool ok = true, bad = false;                           // (bad: a page id beyond the pool)
   TcWalk wk;
   for (bool more = wk.first(a, n_items, pairs, tiles); more && ok; more = wk.next(a, n_items, pairs, tiles)) {
     const TcItem& w = wk.w;
@@ -320,7 +321,7 @@ __device__ __forceinline__ void tc_load_eight_bit(const Args& a, PrefillTcShared
     auto pages_of = [&](int u, int* page) {              // a lane's unit of the 32 from u on: its blocks' (page, head)
 #pragma unroll
       for (int j = 0; j < kBlocks; ++j)
-        page[j] = bt[min(max((w.k_begin + ((u + L * lane) * kBlocks + j) * 16) >> shift, first), last)] * a.hkv + w.kvh;
+        page[j] = kv8_page(bt[min(max((w.k_begin + ((u + L * lane) * kBlocks + j) * 16) >> shift, first), last)], a.pages, bad) * a.hkv + w.kvh;
     };
     auto codes_of = [&](const int* page, int* code) {
 #pragma unroll
@@ -333,7 +334,8 @@ __device__ __forceinline__ void tc_load_eight_bit(const Args& a, PrefillTcShared
     // the item's largest scale
     int most = 0;
 #pragma unroll 4
-    for (int pg = first + lane; pg <= last; pg += 32) most = max(most, static_cast<int>(scales[static_cast<size_t>(bt[pg]) * a.hkv + w.kvh]));
+    for (int pg = first + lane; pg <= last; pg += 32)
+      most = max(most, static_cast<int>(scales[static_cast<size_t>(kv8_page(bt[pg], a.pages, bad)) * a.hkv + w.kvh]));
     most = __reduce_max_sync(0xffffffffu, most);
     if (turn == 0 && lane == 0) (is_v ? sh->item_v : sh->item_k)[wk.it & 7] = kv8_scale(most);
     if (is_v && turn < (w.two ? 2 : 1)) {
@@ -466,6 +468,7 @@ __device__ __forceinline__ void tc_load_eight_bit(const Args& a, PrefillTcShared
     }
     if (ok) hand_over();
   }
+  if (bad) atomicOr(status, kKv8BadPage);
 }
 
 template <typename Args>
@@ -522,7 +525,7 @@ prefill_attn_tc_kernel(const Args a, int tiles, int* status) {
   if (Args::kEightBit && warp != kMma && warp != kMma + 1) {
     if constexpr (Args::kEightBit) {
       const int l = warp < kMma ? warp - kTcRowWarps : warp - kTcRowWarps - 2;      // first K's loaders, then V's
-      tc_load_eight_bit(a, sh, q_s, k_s, v_s, l >= kTcLoaders8, l % kTcLoaders8, lane, n_items, pairs, tiles);
+      tc_load_eight_bit(a, sh, q_s, k_s, v_s, l >= kTcLoaders8, l % kTcLoaders8, lane, n_items, pairs, tiles, status);
     }
   } else if (!Args::kEightBit && (warp == kTcRowWarps || warp == kTcRowWarps + 1)) {
     if constexpr (!Args::kEightBit) {

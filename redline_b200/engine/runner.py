@@ -286,6 +286,8 @@ class ModelRunner:
                 what.append("a wait inside the tcgen05 attention that ran out")
             if tc_code & 8:
                 what.append("a wait inside the tcgen05 product for few rows that ran out")
+            if tc_code & 16:
+                what.append("a page id beyond the pool of a cache in 8 bits")
             raise EngineError("a kernel met " + " and ".join(what))
 
     def set_op_profiling(self, on: bool) -> None:

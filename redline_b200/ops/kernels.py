@@ -331,7 +331,7 @@ _tc_status: Dict[int, torch.Tensor] = {}
 
 def tc_status(device: torch.device) -> torch.Tensor:
     """The device word in which the tcgen05 kernels report a wait that ran out (bit 0: gemm_tc,
-    bit 2: prompt-portion attention, bit 3: gemm_mid)."""
+    bit 2: prompt-portion attention, bit 3: gemm_mid); bit 4: attention over a cache in 8 bits met a page id beyond the pool."""
     i = device.index if device.index is not None else torch.cuda.current_device()
     if i not in _tc_status:
         _tc_status[i] = torch.zeros(1, dtype=torch.int32, device=device)
@@ -668,8 +668,9 @@ def attn_prefill(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, vcache: t
 KV8_DTYPE, KV8_SCALE_DTYPE = torch.float8_e4m3fn, torch.float8_e8m0fnu
 KV8_PAGE_SIZES = (16, 32, 64)
 _KV8_LAUNCH_ITEMS = 1024      # items of one launch (kMaxItems)
+_KV8_BAD_PAGE = 16            # bit of tc_status: a page id beyond the pool (kKv8BadPage)
 # the entry points' arguments, packed (Kv8WriteCall, Kv8DecodeCall, Kv8PrefillCall)
-_KV8_WRITE, _KV8_DECODE, _KV8_PREFILL = struct.Struct("21q").pack, struct.Struct("19qd10q").pack, struct.Struct("20qd3q").pack
+_KV8_WRITE, _KV8_DECODE, _KV8_PREFILL = struct.Struct("21q").pack, struct.Struct("19qd11q").pack, struct.Struct("20qd4q").pack
 
 
 def _kv8_ptr(t: Optional[torch.Tensor]) -> int:
@@ -702,6 +703,8 @@ def _kv8_check(what: str, kcache: torch.Tensor, vcache: torch.Tensor, kscale: to
             or len(scales) != 2 or scales[0] != shape[0] or scales[1] != num_kv_heads or vscale.shape != scales):
         raise KernelError(f"{what}: caches [pages, {num_kv_heads}, {page_size}, {head_dim}] and scales [pages, {num_kv_heads}]; "
                           f"got {tuple(shape)}, {tuple(vcache.shape)}, {tuple(kscale.shape)}, {tuple(vscale.shape)}")
+    if shape[0] < 1:
+        raise KernelError(f"{what}: a pool without a page")
     if not (kcache.is_contiguous() and vcache.is_contiguous() and kscale.is_contiguous() and vscale.is_contiguous()):
         raise KernelError(f"{what}: the cache and its scales must be contiguous")
     if (kcache.data_ptr() | vcache.data_ptr()) % 16:
@@ -805,6 +808,7 @@ def kv8_decode_workspace(nitems: int, num_heads: int, num_kv_heads: int, head_di
     """What ``kv8_attn_decode`` and ``kv8_attn_decode_rope`` need beside their arguments for up to ``nitems`` items: room for
     the pieces of rows that are shared out, and counters, which launches leave zero.  One stream uses a workspace at a time
     (two graphs that may run side by side need one each)."""
+    tc_status(device)           # (the attention reports there: not to be laid out first within a capture)
     return (torch.empty(kv8_part_floats(num_heads, num_kv_heads, head_dim), dtype=torch.float32, device=device),
             torch.zeros(max(nitems, 1) * num_kv_heads, dtype=torch.int32, device=device))
 
@@ -849,7 +853,8 @@ def _kv8_decode(what: str, q, q_stride, kcache, vcache, kscale, vscale, block_ta
                              block_table.data_ptr(), blocks, items.data_ptr(), nitems, part.data_ptr(), counters.data_ptr(),
                              out.data_ptr(), out_stride, num_heads, num_kv_heads, page_size, window, scale, _kv8_ptr(cos),
                              _kv8_ptr(sin), max_pos, 1 if store else 0, kcache.shape[0] * page_size,
-                             status.data_ptr() if store else 0, seen, sum_ctx, impl, _stream())),
+                             status.data_ptr() if store else tc_status(q.device).data_ptr(), seen, sum_ctx, impl,
+                             4 if store else _KV8_BAD_PAGE, _stream())),
                what, launches)
 
 
@@ -863,6 +868,7 @@ def kv8_attn_decode(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, vcache
     items      int32 [nitems, 4]: (token index of the query, sequence index, context length, 0); an item of context 0 has
                no keys, and its row of ``out`` is left as it was
     workspace  of kv8_decode_workspace
+    block_table  a page id beyond the pool is read as page 0, and bit 16 of ``tc_status`` tells
     max_ctx, sum_ctx  the longest context and their sum, as far as the host knows them (0: unknown); the work is shared out by
                the items' own contexts, these choose between ways to do so
     impl       0: the best kernel that applies; 1: CUDA cores; 2: tensor cores, a cluster or a group of warps to a row, or an
@@ -879,7 +885,8 @@ def kv8_attn_decode_rope(qkv: torch.Tensor, q_stride: int, kcache: torch.Tensor,
                          num_kv_heads: int, head_dim: int, page_size: int, window: int, scale: float, cos: torch.Tensor,
                          sin: torch.Tensor, status: torch.Tensor, max_ctx: int = 0, sum_ctx: int = 0, impl: int = 0) -> None:
     """``kv8_attn_decode`` from the UNROTATED rows [q | k | v] of the query tokens: a token's position is its context length - 1;
-    its rotated k and its v are stored there first (as kv8_write does), and q is rotated on its way into the attention."""
+    its rotated k and its v are stored there first (as kv8_write does), and q is rotated on its way into the attention.  A page id
+    beyond the pool is read as page 0, nothing is stored there, and bit 4 of ``status`` tells."""
     _kv8_decode("kv8_attn_decode_rope", qkv, q_stride, kcache, vcache, kscale, vscale, block_table, items, workspace, out, nitems,
                 num_heads, num_kv_heads, head_dim, page_size, window, scale, cos, sin, status, max_ctx, sum_ctx, impl)
 
@@ -903,8 +910,9 @@ def kv8_attn_prefill(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, vcach
                      tile_rows: torch.Tensor, positions: torch.Tensor, out: torch.Tensor, tiles: int, num_heads: int,
                      num_kv_heads: int, head_dim: int, page_size: int, window: int, scale: float, impl: int = 0) -> None:
     """``attn_prefill`` over a cache in 8 bits (kv8_write): tiles of up to 128 consecutive query tokens of one sequence
-    (tile_seq, tile_tok, tile_rows); rows of ``out`` that no tile names are left as they were.  impl 0: the best kernel that
-    applies (bfloat16 at head sizes 64 and 128: tcgen05; else CUDA cores); 1: CUDA cores; 3: the tcgen05 kernel or an error."""
+    (tile_seq, tile_tok, tile_rows); rows of ``out`` that no tile names are left as they were.  A page id beyond the pool is
+    read as page 0, and bit 16 of ``tc_status`` tells.  impl 0: the best kernel that applies (bfloat16 at head sizes 64 and 128:
+    tcgen05; else CUDA cores); 1: CUDA cores; 3: the tcgen05 kernel or an error."""
     what = "kv8_attn_prefill"
     _kv8_check(what, kcache, vcache, kscale, vscale, num_heads, num_kv_heads, head_dim, page_size)
     at = kcache.get_device()
@@ -927,7 +935,8 @@ def kv8_attn_prefill(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, vcach
         _check(f(_KV8_PREFILL(_code(q.dtype), q.data_ptr(), q_stride, kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(),
                               vscale.data_ptr(), block_table.data_ptr(), block_table.shape[1], tile_seq.data_ptr(),
                               tile_tok.data_ptr(), tile_rows.data_ptr(), positions.data_ptr(), out.data_ptr(), out_stride, tiles,
-                              num_heads, num_kv_heads, page_size, window, scale, impl, tc_status(q.device).data_ptr(), _stream())), what)
+                              num_heads, num_kv_heads, page_size, window, scale, impl, kcache.shape[0], tc_status(q.device).data_ptr(),
+                              _stream())), what)
 
 
 # ------------------------------------------- row-wise kernels of blocks with norms on both sides

@@ -1,0 +1,110 @@
+"""The cache in 8 bits: what the calls do with entries of device memory that the host cannot check (page ids beyond the pool)."""
+
+import math
+
+import pytest
+import torch
+
+import plain_kv8 as P
+from redline_b200.ops import kernels
+from test_kv8_gpu import DEV, DT, angles, empty_cache, filled, on_gpu, tiles_of
+
+pytestmark = pytest.mark.gpu
+BAD = (0, 5, 2 ** 20, 2 ** 31 - 1, -1, -2 ** 31)      # (0: just beyond the pool)
+
+
+def take_status():
+    t = kernels.tc_status(torch.device(DEV, 0))
+    code = t.item()
+    t.zero_()
+    return code
+
+
+def bytes_of(cache):
+    return [t.view(torch.uint8).cpu() for t in cache]
+
+
+KINDS = [(4, 2, 64, 16, "bfloat16", 0), (4, 2, 64, 16, "bfloat16", 2), (4, 2, 64, 32, "bfloat16", 3), (4, 2, 64, 64, "bfloat16", 4),
+         (3, 1, 128, 16, "bfloat16", 4), (3, 1, 128, 16, "bfloat16", 1), (4, 2, 64, 16, "float32", 0), (10, 2, 80, 16, "bfloat16", 0),
+         (24, 2, 128, 32, "bfloat16", 2)]
+
+
+def sequences(heads, kv_heads, dim, page, bad, poison):
+    """Four sequences; one page of the second is ``bad`` (counted from the pool's end, or negative), the first and the last of the
+    third as well."""
+    ctxs = (100, 3 * page + 5, 4 * page, 40)
+    cache, table = filled(ctxs, heads, kv_heads, dim, page, seed=dim + page, poison=poison)
+    cache[0][0], cache[1][0], cache[2][0], cache[3][0] = 3, 5, 120, 121         # page 0 is finite here: its values are looked at
+    pages = cache[0].shape[0]
+    wrong = table.clone()
+    for s, b in ((1, 1), (2, 0), (2, 3)):
+        wrong[s, b] = bad if bad < 0 else min(pages + bad, 2 ** 31 - 1)
+        table[s, b] = 0
+    return ctxs, cache, table, wrong
+
+
+@pytest.mark.parametrize("bad", BAD)
+@pytest.mark.parametrize("heads,kv_heads,dim,page,dtype,impl", KINDS)
+def test_pages_beyond_the_pool_read_as_page_0(heads, kv_heads, dim, page, dtype, impl, bad):
+    ctxs, cache, table, wrong = sequences(heads, kv_heads, dim, page, bad, True)
+    gpu = on_gpu(cache)
+    n, scale = len(ctxs), 1.0 / math.sqrt(dim)
+    items = torch.tensor([(i, i, c, 0) for i, c in enumerate(ctxs)], dtype=torch.int32, device=DEV)
+    work = kernels.kv8_decode_workspace(n, heads, kv_heads, dim, torch.device(DEV))
+    q = torch.randn(n, heads * dim, generator=torch.Generator().manual_seed(1)).to(DT[dtype]).to(DEV)
+    outs = []
+    for t, code in ((table, 0), (wrong, 16), (table, 0)):
+        out = torch.empty_like(q)
+        kernels.kv8_attn_decode(q, q.stride(0), *gpu, t.to(DEV), items, work, out, n, heads, kv_heads, dim, page, 0, scale, impl=impl)
+        assert take_status() == code
+        outs.append(out)
+    assert torch.isfinite(outs[0]).all() and torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+    assert all(torch.equal(a, b) for a, b in zip(bytes_of(gpu), cache))
+
+
+@pytest.mark.parametrize("bad", BAD)
+@pytest.mark.parametrize("heads,kv_heads,dim,page,dtype,impl", KINDS)
+def test_nothing_is_stored_beyond_the_pool(heads, kv_heads, dim, page, dtype, impl, bad):
+    """The third sequence's newest page is bad, the second has a bad one behind its newest: the other tokens are stored, bit 4 tells."""
+    ctxs, cache, table, wrong = sequences(heads, kv_heads, dim, page, bad, False)
+    gpu = on_gpu(cache)
+    n = len(ctxs)
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn(n, (heads + 2 * kv_heads) * dim, generator=g).to(DT[dtype])
+    cos, sin = angles(300, dim)
+    items = torch.tensor([(i, i, c, 0) for i, c in enumerate(ctxs)], dtype=torch.int32, device=DEV)
+    work = kernels.kv8_decode_workspace(n, heads, kv_heads, dim, torch.device(DEV))
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    xg, out = x.to(DEV), torch.empty(n, heads * dim, dtype=x.dtype, device=DEV)
+    kernels.kv8_attn_decode_rope(xg, xg.stride(0), *gpu, wrong.to(DEV), items, work, out, n, heads, kv_heads, dim, page, 0,
+                                 1.0 / math.sqrt(dim), cos.to(DEV), sin.to(DEV), status, impl=impl)
+    assert status.item() == 4 and take_status() == 0
+    at = [c - 1 for c in ctxs]
+    slots = [int(table[s, p // page]) * page + p % page if s != 2 else -1 for s, p in enumerate(at)]
+    k, v = x.float()[:, heads * dim:].split([kv_heads * dim] * 2, -1)
+    P.store(P.rotate(k.reshape(n, kv_heads, dim), cos[at], sin[at]), slots, cache[0], cache[2])
+    P.store(v.reshape(n, kv_heads, dim), slots, cache[1], cache[3])
+    for got, want in zip(bytes_of(gpu), cache):
+        assert torch.equal(got, want)
+    assert (work[1] == 0).all()
+
+
+@pytest.mark.parametrize("bad", BAD)
+@pytest.mark.parametrize("heads,kv_heads,dim,page,dtype,impl", [(4, 2, 64, 16, "bfloat16", 3), (3, 1, 128, 32, "bfloat16", 3),
+                                                                (4, 2, 64, 16, "bfloat16", 1), (4, 2, 64, 64, "float32", 0),
+                                                                (10, 2, 80, 16, "bfloat16", 0)])
+def test_prompts_over_pages_beyond_the_pool(heads, kv_heads, dim, page, dtype, impl, bad):
+    ctxs, cache, table, wrong = sequences(heads, kv_heads, dim, page, bad, True)
+    gpu = on_gpu(cache)
+    segments = [(c - min(c, 30), min(c, 30)) for c in ctxs]
+    positions = torch.tensor([p for a, n in segments for p in range(a, a + n)], dtype=torch.int32, device=DEV)
+    seq, tok, rows = tiles_of(segments)
+    q = torch.randn(len(positions), heads * dim, generator=torch.Generator().manual_seed(1)).to(DT[dtype]).to(DEV)
+    outs = []
+    for t, code in ((table, 0), (wrong, 16)):
+        out = torch.empty_like(q)
+        kernels.kv8_attn_prefill(q, q.stride(0), *gpu, t.to(DEV), seq, tok, rows, positions, out, len(seq), heads, kv_heads, dim, page, 0,
+                                 1.0 / math.sqrt(dim), impl=impl)
+        assert take_status() == code
+        outs.append(out)
+    assert torch.isfinite(outs[0]).all() and torch.equal(outs[0], outs[1])

@@ -144,9 +144,10 @@ kv8_write_kernel(const Kv8WriteArgs<T> a, int span, int tasks) {
     }
     const int off = static_cast<int>(slot & (ps - 1));
     const long long page = slot >> a.page_shift;
-    if (off > 0 && __shfl_sync(0xffffffffu, theirs, l - 1) == slot - 1) continue;      // not the first of its run
-    int n;                                                 // tokens of the run
-    {
+    // (an item is a run of its own: the attention's kernel, where it stores itself, could not take two)
+    if (a.items == nullptr && off > 0 && __shfl_sync(0xffffffffu, theirs, l - 1) == slot - 1) continue;      // not the first of its run
+    int n = 1;                                             // tokens of the run
+    if (a.items == nullptr) {
       // (lane l has its first token; those before stand for themselves)
       unsigned m = __ballot_sync(0xffffffffu, lane < l || (off + lane - l < ps && theirs == slot + lane - l));
       n = m == 0xffffffffu ? 32 - l : __ffs(~m) - 1 - l;
@@ -183,11 +184,13 @@ kv8_write_kernel(const Kv8WriteArgs<T> a, int span, int tasks) {
     uint8_t* scale = (is_v ? a.vscale : a.kscale) + static_cast<size_t>(page) * a.hkv + h;
     const int old = busy && off > 0 ? min(static_cast<int>(*scale), 254) : 0;
     // Two runs of one page in one call would each set its scale without the other's: only the first is stored.  (Page 0
-    // is the reserved one that padding rows write to: nothing to tell of there.)
+    // is the reserved one that padding rows write to: nothing to tell of there.)  Two items of one sequence likewise.
     bool before = false;
+    const int seq = a.items != nullptr ? a.items[t].y : 0;
     for (int i = threadIdx.x; i < t; i += kWriteThreads) {
       const long long s = kv8_slot(a, i);
       before |= s >= 0 && (s >> a.page_shift) == page;
+      if (a.items != nullptr) before |= a.items[i].z > 0 && a.items[i].y == seq;
     }
     if (__syncthreads_or(before)) {                        // (every thread has read its scale)
       if (threadIdx.x == 0 && page != 0) atomicOr(a.status, 8);
@@ -1105,6 +1108,7 @@ int rl_kv8_attn_decode(const Kv8DecodeCall* c) {
   a.bad_page = static_cast<int>(c->bad_page);
   for (int i0 = 0; i0 < nitems; i0 += kMaxItems) {         // (one launch unless there are very many items)
     a.items = c->items + i0;
+    a.before = i0;
     a.nitems = nitems - i0 < kMaxItems ? nitems - i0 : kMaxItems;
 #ifdef RL_KV8_TC
     if (tc) {

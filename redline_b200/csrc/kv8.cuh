@@ -108,6 +108,7 @@ struct Kv8Args {
   int max_blocks;
   const int4* items;           // (token index of the query, sequence index, context length, 0)
   int nitems;
+  int before;                  // items of the call before these (launches before this one have taken them)
   float* part;                 // [shares, 2, G, D + 4] pieces: numerators, d, m, denominator
   int* counters;               // [items * Hkv], zero between launches
   void* out;                   // [tokens, out_stride]

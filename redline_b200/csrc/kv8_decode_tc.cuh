@@ -365,11 +365,13 @@ __device__ __forceinline__ void tc_run(const Kv8Args& a, const Kv8Segment& s, in
   };
   const int token_page = __shfl_sync(0xffffffffu, my_page, 0);
   bool mine = true;
-  if (store) {                                           // (of several items that name one page the first stores: see kv8_write_kernel)
+  if (store) {                                           // (of several items of one page or sequence the first stores: see kv8_write_kernel)
 #pragma unroll 1
-    for (int i = lane; i < s.item; i += 32) {
+    for (int i = lane - a.before; i < s.item; i += 32) {
       const int4 other = a.items[i];
-      if (other.z > 0 && a.block_table[static_cast<size_t>(other.y) * a.max_blocks + ((other.z - 1) >> shift)] == token_page) mine = false;
+      if (other.z > 0 && (other.y == s.seq
+                          || a.block_table[static_cast<size_t>(other.y) * a.max_blocks + ((other.z - 1) >> shift)] == token_page))
+        mine = false;
     }
     // (a page beyond the pool stands as page 0 here, but nothing is stored there)
     if (static_cast<unsigned>(bt[(s.ctx - 1) >> shift]) >= static_cast<unsigned>(a.pages)) mine = false;

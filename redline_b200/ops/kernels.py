@@ -886,7 +886,10 @@ def kv8_attn_decode_rope(qkv: torch.Tensor, q_stride: int, kcache: torch.Tensor,
                          sin: torch.Tensor, status: torch.Tensor, max_ctx: int = 0, sum_ctx: int = 0, impl: int = 0) -> None:
     """``kv8_attn_decode`` from the UNROTATED rows [q | k | v] of the query tokens: a token's position is its context length - 1;
     its rotated k and its v are stored there first (as kv8_write does), and q is rotated on its way into the attention.  A page id
-    beyond the pool is read as page 0, nothing is stored there, and bit 4 of ``status`` tells."""
+    beyond the pool is read as page 0, nothing is stored there, and bit 4 of ``status`` tells.  The items are of different
+    sequences, which store in different pages: of several of one sequence or page only the first is stored, bit 8 of ``status`` tells
+    (not of page 0), and the rows of ``out`` of such a sequence are of no use (its tokens of one step go through ``kv8_write`` and
+    ``kv8_attn_prefill``)."""
     _kv8_decode("kv8_attn_decode_rope", qkv, q_stride, kcache, vcache, kscale, vscale, block_table, items, workspace, out, nitems,
                 num_heads, num_kv_heads, head_dim, page_size, window, scale, cos, sin, status, max_ctx, sum_ctx, impl)
 

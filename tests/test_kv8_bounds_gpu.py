@@ -1,4 +1,5 @@
-"""The cache in 8 bits: what the calls do with entries of device memory that the host cannot check (page ids beyond the pool)."""
+"""The cache in 8 bits: what the calls do with entries of device memory that the host cannot check (page ids beyond
+the pool, a sequence or a page under several items)."""
 
 import math
 
@@ -7,7 +8,7 @@ import torch
 
 import plain_kv8 as P
 from redline_b200.ops import kernels
-from test_kv8_gpu import DEV, DT, angles, empty_cache, filled, on_gpu, tiles_of
+from test_kv8_gpu import DEV, DT, angles, filled, near, on_gpu, tiles_of
 
 pytestmark = pytest.mark.gpu
 BAD = (0, 5, 2 ** 20, 2 ** 31 - 1, -1, -2 ** 31)      # (0: just beyond the pool)
@@ -108,3 +109,85 @@ def test_prompts_over_pages_beyond_the_pool(heads, kv_heads, dim, page, dtype, i
         assert take_status() == code
         outs.append(out)
     assert torch.isfinite(outs[0]).all() and torch.equal(outs[0], outs[1])
+
+
+def fresh(n, blocks, heads, kv_heads, dim, page, dtype, seed=1, extra=0):
+    """``n`` sequences of random finite pages and rows [q | k | v] for them."""
+    g = torch.Generator().manual_seed(seed)
+    pages = n * blocks + 1 + extra
+    cache = [torch.randint(0, 126, (pages, kv_heads, page, dim), generator=g).to(torch.uint8) for _ in range(2)]
+    cache += [torch.randint(115, 120, (pages, kv_heads), generator=g).to(torch.uint8) for _ in range(2)]
+    table = (torch.randperm(n * blocks, generator=g) + 1).view(n, blocks).int()
+    x = torch.randn(n, (heads + 2 * kv_heads) * dim, generator=g).to(DT[dtype])
+    return cache, table, x
+
+
+def stored(x, table, items, keep, cos, sin, cache, heads, kv_heads, dim, page):
+    """The restatement's store of the items' tokens, of those that are kept."""
+    at = [c - 1 for _, c in items]
+    slots = [int(table[s, p // page]) * page + p % page if k else -1 for (s, _), p, k in zip(items, at, keep)]
+    k, v = x.float()[:, heads * dim:].split([kv_heads * dim] * 2, -1)
+    P.store(P.rotate(k.reshape(len(x), kv_heads, dim), cos[at], sin[at]), slots, cache[0], cache[2])
+    P.store(v.reshape(len(x), kv_heads, dim), slots, cache[1], cache[3])
+
+
+def rope(x, gpu, table, items, cos, sin, heads, kv_heads, dim, page, impl):
+    n = len(items)
+    info = torch.tensor([(i, s, c, 0) for i, (s, c) in enumerate(items)], dtype=torch.int32, device=DEV)
+    work = kernels.kv8_decode_workspace(n, heads, kv_heads, dim, torch.device(DEV))
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    xg, out = x.to(DEV), torch.empty(len(x), heads * dim, dtype=x.dtype, device=DEV)
+    kernels.kv8_attn_decode_rope(xg, xg.stride(0), *gpu, table.to(DEV), info, work, out, n, heads, kv_heads, dim, page, 0,
+                                 1.0 / math.sqrt(dim), cos.to(DEV), sin.to(DEV), status, impl=impl)
+    assert (work[1] == 0).all()
+    return out, status.item()
+
+
+# items (sequence, context) and which of them are stored
+TWICE = [([(0, 20), (1, 18), (1, 19), (2, 40)], (1, 1, 0, 1)),          # one sequence, places that follow one another
+         ([(1, 64), (0, 20), (1, 65), (2, 40)], (1, 1, 0, 1)),          # one sequence, two pages
+         ([(3, 20), (4, 25), (0, 9), (3, 70)], (1, 0, 1, 0)),           # two sequences that name one page; one of them once more
+         ([(0, 0), (0, 33), (1, 1), (1, 1)], (0, 1, 1, 0))]             # (an item without keys stores nothing)
+
+
+@pytest.mark.parametrize("items,keep", TWICE)
+@pytest.mark.parametrize("heads,kv_heads,dim,page,dtype,impl", KINDS)
+def test_a_sequence_or_a_page_twice(heads, kv_heads, dim, page, dtype, impl, items, keep):
+    """Whichever kernel stores the tokens: the first is stored, the others are not, and bit 8 tells."""
+    cache, table, x = fresh(5, 8, heads, kv_heads, dim, page, dtype)
+    table[4] = table[3]
+    x = x[:len(items)].contiguous()
+    cos, sin = angles(300, dim)
+    gpu = on_gpu(cache)
+    _, code = rope(x, gpu, table, items, cos, sin, heads, kv_heads, dim, page, impl)
+    assert code == 8
+    stored(x, table, items, keep, cos, sin, cache, heads, kv_heads, dim, page)
+    for got, want in zip(bytes_of(gpu), cache):
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("twice", [False, True])
+@pytest.mark.parametrize("heads,kv_heads,dim,page,dtype,impl", [(4, 2, 64, 16, "bfloat16", 0), (4, 2, 64, 16, "bfloat16", 3),
+                                                                (4, 1, 128, 32, "bfloat16", 2), (2, 1, 64, 64, "bfloat16", 0),
+                                                                (2, 1, 64, 16, "float32", 0), (2, 1, 80, 16, "bfloat16", 0)])
+def test_more_items_than_a_launch_takes(heads, kv_heads, dim, page, dtype, impl, twice):
+    """Several launches over one workspace: tokens stored, rows attended, a sequence of the first launch in the last once more."""
+    n = 2100
+    cache, table, x = fresh(n, 2, heads, kv_heads, dim, page, dtype)
+    items = [(i, 1 + i * 7 % (2 * page)) for i in range(n)]
+    keep = [1] * n
+    if twice:
+        items[2090], keep[2090] = (3, items[3][1] + 1), 0
+    cos, sin = angles(2 * page + 2, dim)
+    gpu = on_gpu(cache)
+    out, code = rope(x, gpu, table, items, cos, sin, heads, kv_heads, dim, page, impl)
+    assert code == (8 if twice else 0)
+    stored(x, table, items, keep, cos, sin, cache, heads, kv_heads, dim, page)
+    for got, want in zip(bytes_of(gpu), cache):
+        assert torch.equal(got, want)
+    k, v = P.values(cache[0], cache[2]), P.values(cache[1], cache[3])
+    q = P.rotate(x.float()[:, :heads * dim].view(n, heads, dim), cos[[c - 1 for _, c in items]], sin[[c - 1 for _, c in items]])
+    for i in (0, 1, 500, 1022, 1023, 1024, 1025, 1500, 2047, 2048, 2049, 2098, 2099):
+        s, c = items[i]
+        ref = P.attend(q[i:i + 1], k, v, table[s], [c - 1], 0, 1.0 / math.sqrt(dim))
+        near(out[i].view(1, heads, dim), ref, v[table[s][:-(-c // page)].long()], dtype)

@@ -797,8 +797,17 @@ int launch_write(const void* qkv, int qkv_stride, const int32_t* positions, cons
   return static_cast<int>(cudaGetLastError());
 }
 
-// The largest number of shares that a launch is cut into: the workspace has two places for each.
+// The largest number of shares that a launch is cut into, whatever the device: the workspace has two places for each.  (148 SMs
+// times the 12 groups of a CTA.)
 constexpr int kMaxShares = 1776;
+
+// CTAs of a launch in shares, `groups` to a CTA, and pieces of a row, one to a CTA: as many as the device holds at once and the
+// workspace has places for.
+int shares_ctas(int resident, int groups) { return resident < kMaxShares / groups ? resident : kMaxShares / groups; }
+int most_pieces(int resident, long long rows) {
+  const long long k = (resident < kMaxShares ? resident : kMaxShares) / rows;
+  return static_cast<int>(k < 48 ? k : 48);
+}
 
 #ifdef RL_KV8_TC
 
@@ -889,10 +898,7 @@ void tc_rows(const TcDevice* d, long long rows, int G, int* csize, int* groups) 
 }
 
 // The pieces of a row where there is a CTA for each; the last to arrive adds them up, which takes some 0.2 us a piece.
-int tc_pieces(const TcDevice* d, long long rows) {
-  const long long k = d->resident[1] / rows;
-  return static_cast<int>(k < 48 ? k : 48);
-}
+int tc_pieces(const TcDevice* d, long long rows) { return most_pieces(d->resident[1], rows); }
 
 // Which of rows (2), shares (3) and pieces (4) is expected to take the shortest, in us: a start; then the longest of a warp's
 // run of sub-blocks, what the busiest SM reads and what all bytes take.  Fitted to 1017 launches (kv heads 1, 2 and 8, groups of
@@ -914,8 +920,7 @@ int kv8_choice(const TcDevice* d, int nitems, int hq, int hkv, int max_ctx, doub
   const double by_rows = (narrow ? 6.5 : 7.4) + longest(run * lat, (max_ctx + (groups * turns - 1) * mean) * key / csize / sm_rate, bytes / rate);
   const double by_shares = (narrow ? 17.1 : 21.5) + bytes / (narrow ? 4.12e6 : 5.09e6);
   double by_pieces = 1e30;
-  if (rows <= d->resident[1]) {
-    const int k = tc_pieces(d, rows);
+  if (const int k = tc_pieces(d, rows)) {
     by_pieces = (narrow ? 11.7 : 14.6) + longest((max_ctx / kSub + k * kDecWarps) / (k * kDecWarps) * lat, max_ctx * key / k / sm_rate, bytes / (narrow ? 7.1e6 : 7.8e6));
   }
   return by_rows <= by_shares && by_rows <= by_pieces ? 2 : (by_pieces <= by_shares ? 4 : 3);
@@ -933,7 +938,7 @@ int tc_plan(int nitems, int hq, int hkv, int max_ctx, long long sum_ctx, int imp
   plan->groups = 1;
   plan->parts = 0;
   if (impl == 0) impl = kv8_choice(d, nitems, hq, hkv, max_ctx, static_cast<double>(sum_ctx) / nitems);
-  if (impl == 4 && rows > resident) impl = 2;
+  if (impl == 4 && tc_pieces(d, rows) < 1) impl = 2;
   if (impl == 4) {
     plan->parts = tc_pieces(d, rows);
     plan->ctas = static_cast<int>(rows * plan->parts);
@@ -943,7 +948,7 @@ int tc_plan(int nitems, int hq, int hkv, int max_ctx, long long sum_ctx, int imp
   if (impl == 3) {
     plan->csize = 1;
     plan->parts = -1;
-    plan->ctas = resident;
+    plan->ctas = shares_ctas(resident, plan->groups);
     return 0;
   }
   const long long wanted = plan->csize > 1 ? rows : (rows + plan->groups - 1) / plan->groups;
@@ -1048,6 +1053,13 @@ int rl_kv8_decode_choice(int dtype, int nitems, int hq, int hkv, int max_ctx, lo
   return 0;
 }
 
+// The most pieces that a launch leaves in the workspace on a device that holds `resident` CTAs of `groups` groups at once: in shares
+// (rows 0) or with so many rows in pieces.
+long long rl_kv8_most_pieces(int resident, int groups, int rows) {
+  if (resident < 1 || groups < 1 || rows < 0) return -1;
+  return rows == 0 ? static_cast<long long>(shares_ctas(resident, groups)) * groups : static_cast<long long>(rows) * most_pieces(resident, rows);
+}
+
 // The floats of the workspace for groups of G heads (kv8.cuh: Kv8Args::part).
 long long rl_kv8_part_floats(int G) { return static_cast<long long>(kMaxShares) * 2 * G * (kD + 4); }
 
@@ -1120,7 +1132,7 @@ int rl_kv8_attn_decode(const Kv8DecodeCall* c) {
     if (impl > 1) return static_cast<int>(cudaErrorInvalidValue);
     // a CTA to a unit, as far as they are resident together
     const long long max_units = static_cast<long long>(a.nitems) * hkv * (max_ctx / kUnit + 2);
-    const int most = sms * 2 < kMaxShares ? sms * 2 : kMaxShares;
+    const int most = shares_ctas(sms * 2, 1);
     const int ctas = static_cast<int>(max_units < most ? max_units : most);
     if (single)
       launch_kernel(kv8_decode_kernel<float>, dim3(ctas), dim3(kGenThreads), 0, c->stream, a);

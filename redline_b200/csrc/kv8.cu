@@ -1075,14 +1075,16 @@ int rl_kv8_attn_decode(const Kv8DecodeCall* c) {
   const int page_size = static_cast<int>(c->page_size), impl = static_cast<int>(c->impl), max_pos = static_cast<int>(c->max_pos);
   const int max_ctx = static_cast<int>(c->max_ctx), q_stride = static_cast<int>(c->q_stride);
   const bool store = c->store != 0, single = c->dtype == 0;
+#ifdef RL_KV8_TC
+  const bool takes = !single && hq / hkv <= 16;
+#else
+  const bool takes = false;
+#endif
+  if (impl > 1 && !takes) return static_cast<int>(cudaErrorInvalidValue);      // (before anything is stored)
+  const bool tc = takes && impl != 1;
   int sms = 0;
   int e = device_sms(&sms);
   if (e) return e;
-#ifdef RL_KV8_TC
-  const bool tc = !single && hq / hkv <= 16 && impl != 1;
-#else
-  const bool tc = false;
-#endif
   // (pages of 64 tokens reach over two sub-blocks, which may be two warps': their tokens are stored by a kernel of its own)
   const bool fused = store && tc && page_size <= 32;
   if (store && !fused) {
@@ -1129,7 +1131,6 @@ int rl_kv8_attn_decode(const Kv8DecodeCall* c) {
       continue;
     }
 #endif
-    if (impl > 1) return static_cast<int>(cudaErrorInvalidValue);
     // a CTA to a unit, as far as they are resident together
     const long long max_units = static_cast<long long>(a.nitems) * hkv * (max_ctx / kUnit + 2);
     const int most = shares_ctas(sms * 2, 1);

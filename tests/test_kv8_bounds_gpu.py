@@ -191,3 +191,15 @@ def test_more_items_than_a_launch_takes(heads, kv_heads, dim, page, dtype, impl,
         s, c = items[i]
         ref = P.attend(q[i:i + 1], k, v, table[s], [c - 1], 0, 1.0 / math.sqrt(dim))
         near(out[i].view(1, heads, dim), ref, v[table[s][:-(-c // page)].long()], dtype)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,page,dtype", [(4, 2, 64, 16, "float32"), (10, 2, 80, 16, "bfloat16"), (40, 2, 64, 64, "bfloat16")])
+def test_a_refused_call_stores_nothing(heads, kv_heads, dim, page, dtype):
+    cache, table, x = fresh(3, 4, heads, kv_heads, dim, page, dtype)
+    cos, sin = angles(100, dim)
+    gpu = on_gpu(cache)
+    for impl in (2, 3, 4):
+        with pytest.raises(kernels.KernelError):
+            rope(x, gpu, table, [(0, 5), (1, 20), (2, 33)], cos, sin, heads, kv_heads, dim, page, impl)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(bytes_of(gpu), cache))

@@ -35,3 +35,14 @@ def test_a_launch_leaves_no_more_pieces_than_the_workspace_holds(head_dim):
         for rows in (1, 3, 8, 64, 147, 148, 149, 1776, 1777, 2000):
             assert 0 <= most(resident, 1, rows) <= min(places, resident)
     assert most(148, 1, 8) == 144 and most(148, 1, 149) == 0
+
+
+@pytest.mark.parametrize("head_dim,dtype,heads,impl", [(64, 0, 4, 2), (64, 0, 4, 4), (80, 1, 4, 3), (128, 1, 40, 2)])
+def test_a_kernel_that_does_not_take_the_call_is_refused_first(head_dim, dtype, heads, impl):
+    """Before the device is asked for anything, so before a token is stored (invalid argument, and not the error of a missing device)."""
+    f = kernels._kv8(head_dim).rl_kv8_attn_decode
+    f.restype, f.argtypes = ctypes.c_int, [ctypes.c_char_p]
+    names = ("dtype q q_stride k v ks vs table blocks items nitems part counters out out_stride hq hkv page_size window scale cos sin "
+             "max_pos store num_slots status max_ctx sum_ctx impl bad_page stream").split()
+    values = dict.fromkeys(names, 0) | dict(dtype=dtype, nitems=1, hq=heads, hkv=2, page_size=16, scale=0.5, store=1, impl=impl)
+    assert f(kernels._KV8_DECODE(*values.values())) == 1

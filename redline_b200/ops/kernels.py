@@ -808,7 +808,8 @@ def kv8_decode_workspace(nitems: int, num_heads: int, num_kv_heads: int, head_di
     """What ``kv8_attn_decode`` and ``kv8_attn_decode_rope`` need beside their arguments for up to ``nitems`` items: room for
     the pieces of rows that are shared out, and counters, which launches leave zero.  One stream uses a workspace at a time
     (two graphs that may run side by side need one each)."""
-    tc_status(device)           # (the attention reports there: not to be laid out first within a capture)
+    if torch.device(device).type == "cuda":
+        tc_status(torch.device(device))      # (the attention reports there: not to be laid out first within a capture)
     return (torch.empty(kv8_part_floats(num_heads, num_kv_heads, head_dim), dtype=torch.float32, device=device),
             torch.zeros(max(nitems, 1) * num_kv_heads, dtype=torch.int32, device=device))
 

@@ -3,6 +3,7 @@
 import ctypes
 
 import pytest
+import torch
 
 from redline_b200.ops import kernels
 from redline_b200.ops.kernels import KernelError
@@ -46,3 +47,8 @@ def test_a_kernel_that_does_not_take_the_call_is_refused_first(head_dim, dtype, 
              "max_pos store num_slots status max_ctx sum_ctx impl bad_page stream").split()
     values = dict.fromkeys(names, 0) | dict(dtype=dtype, nitems=1, hq=heads, hkv=2, page_size=16, scale=0.5, store=1, impl=impl)
     assert f(kernels._KV8_DECODE(*values.values())) == 1
+
+
+def test_a_workspace_can_be_laid_out_anywhere():
+    part, counters = kernels.kv8_decode_workspace(3, 4, 2, 64, torch.device("cpu"))
+    assert part.numel() == kernels.kv8_part_floats(4, 2, 64) and counters.numel() == 6 and not counters.any()

@@ -1042,6 +1042,7 @@ static_assert(sizeof(Kv8WriteCall) == 21 * 8 && sizeof(Kv8DecodeCall) == 31 * 8 
 
 // Which way of sharing out (2, 3 or 4; 0: the CUDA cores) a launch on the tensor cores would go by impl 0, or an error as a negative number.
 int rl_kv8_decode_choice(int dtype, int nitems, int hq, int hkv, int max_ctx, long long sum_ctx) {
+  if (hkv < 1 || hq < hkv) return -static_cast<int>(cudaErrorInvalidValue);
 #ifdef RL_KV8_TC
   if (dtype == 1 && hq / hkv <= 16 && nitems > 0) {
     const TcDevice* d = nullptr;

@@ -684,6 +684,11 @@ def _kv8(head_dim: int) -> ctypes.CDLL:
     return _lib(f"kv8_d{head_dim}", "kv8.cu", {"RL_HEAD_DIM": head_dim})
 
 
+def _kv8_heads(what: str, num_heads: int, num_kv_heads: int) -> None:
+    if num_kv_heads <= 0 or num_heads <= 0 or num_heads % num_kv_heads:
+        raise KernelError(f"{what}: {num_heads} query heads are no multiple of {num_kv_heads} kv heads")
+
+
 # (A step of single tokens makes one of these calls per layer, and its GPU time is a few us: every attribute of a tensor is asked
 # for once, since each costs 0.1 to 0.3 us, and the arguments go over in one piece: kv8_write's call with its launch went from 15.7 to
 # 11.1 us of one core.)
@@ -697,8 +702,7 @@ def _kv8_check(what: str, kcache: torch.Tensor, vcache: torch.Tensor, kscale: to
                           f"{vcache.dtype}, {kscale.dtype}, {vscale.dtype}")
     if page_size not in KV8_PAGE_SIZES:
         raise KernelError(f"{what}: pages of 16, 32 or 64 tokens; got {page_size}")
-    if num_kv_heads <= 0 or num_heads <= 0 or num_heads % num_kv_heads:
-        raise KernelError(f"{what}: {num_heads} query heads are no multiple of {num_kv_heads} kv heads")
+    _kv8_heads(what, num_heads, num_kv_heads)
     if (len(shape) != 4 or shape[1] != num_kv_heads or shape[2] != page_size or shape[3] != head_dim or vcache.shape != shape
             or len(scales) != 2 or scales[0] != shape[0] or scales[1] != num_kv_heads or vscale.shape != scales):
         raise KernelError(f"{what}: caches [pages, {num_kv_heads}, {page_size}, {head_dim}] and scales [pages, {num_kv_heads}]; "
@@ -798,6 +802,7 @@ def kv8_write(qkv: torch.Tensor, positions: torch.Tensor, slots: Optional[torch.
 @lru_cache(maxsize=None)
 def kv8_part_floats(num_heads: int, num_kv_heads: int, head_dim: int) -> int:
     """The floats of the first tensor of ``kv8_decode_workspace``, whatever the number of items."""
+    _kv8_heads("kv8_part_floats", num_heads, num_kv_heads)
     f = _kv8(head_dim).rl_kv8_part_floats
     f.restype, f.argtypes = c_longlong, [c_int]
     return f(num_heads // num_kv_heads)
@@ -899,6 +904,7 @@ def kv8_decode_choice(dtype: torch.dtype, nitems: int, num_heads: int, num_kv_he
                       window: int, device: torch.device) -> int:
     """Which way ``kv8_attn_decode`` with impl 0 would share out a launch of ``nitems`` rows of at most ``max_ctx`` and together
     ``sum_ctx`` keys (its impl 2, 3 or 4; 0: the CUDA cores): for callers that capture launches and replay them at other lengths."""
+    _kv8_heads("kv8_decode_choice", num_heads, num_kv_heads)
     if window > 0:
         max_ctx, sum_ctx = min(max_ctx, window), min(sum_ctx, nitems * window)
     f = _fn(_kv8(head_dim), "rl_kv8_decode_choice", [c_int, c_int, c_int, c_int, c_int, c_longlong])

@@ -52,3 +52,16 @@ def test_a_kernel_that_does_not_take_the_call_is_refused_first(head_dim, dtype, 
 def test_a_workspace_can_be_laid_out_anywhere():
     part, counters = kernels.kv8_decode_workspace(3, 4, 2, 64, torch.device("cpu"))
     assert part.numel() == kernels.kv8_part_floats(4, 2, 64) and counters.numel() == 6 and not counters.any()
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(4, 0), (0, 0), (0, 2), (4, -2), (4, 3), (2, 4)])
+def test_heads_that_are_no_groups(heads, kv_heads):
+    """Of every call that divides one number by the other."""
+    cpu = torch.device("cpu")
+    for call in (lambda: kernels.kv8_part_floats(heads, kv_heads, 64), lambda: kernels.kv8_decode_workspace(1, heads, kv_heads, 64, cpu),
+                 lambda: kernels.kv8_decode_choice(torch.bfloat16, 1, heads, kv_heads, 64, 10, 10, 0, cpu),
+                 lambda: write(num_heads=heads, num_kv_heads=kv_heads), lambda: prefill(num_heads=heads, num_kv_heads=kv_heads)):
+        with pytest.raises(KernelError, match="no multiple"):
+            call()
+    if kv_heads < 1 or heads < kv_heads:
+        assert kernels._kv8(64).rl_kv8_decode_choice(1, 1, heads, kv_heads, 10, ctypes.c_longlong(10)) == -1

@@ -717,6 +717,32 @@ kv8_prefill_kernel(const Kv8PrefillArgs<T> a, int* status) {
     }
   }
   if (bad) atomicOr(status, kKv8BadPage);
+  // A value that is not a number reaches the rows that see its key and no others, which a weight of 0 does not see to: rows that come out
+  // not finite are done once more by themselves.  (With a look at every weight in the tiles that reach past a row's own key four short
+  // portions took 59 us instead of 51.)
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < NC; ++j) odd |= !(fabsf(acc[i][j]) < INFINITY);
+  if (__syncthreads_or(odd)) {
+    constexpr int E = Kv8Row<kD>::E;
+    const int lane = threadIdx.x & 31;
+#pragma unroll 1
+    for (int r = threadIdx.x >> 5; r < rows; r += kPreThreads / 32) {
+      float q[E] = {}, o[E], top, den;
+      const int pos = pos0 + r, at = head * kD + lane * E;
+      if (Kv8Row<kD>::in_head(lane))
+#pragma unroll
+        for (int e = 0; e < E; ++e) q[e] = to_float(a.q[static_cast<size_t>(tok0 + r) * a.q_stride + at + e]);
+      kv8_row<kD>(a, a.tile_seq[tile], kvh, a.window > 0 && pos + 1 > a.window ? pos + 1 - a.window : 0, pos + 1, a.scale * kLog2e, lane,
+                  q, o, top, den);
+      if (Kv8Row<kD>::in_head(lane))
+#pragma unroll
+        for (int e = 0; e < E; ++e) a.out[static_cast<size_t>(tok0 + r) * a.out_stride + at + e] = from_float<T>(o[e] / den);
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = ty * 4 + i;

@@ -88,6 +88,97 @@ __device__ __forceinline__ int kv8_page(int page, int pages, bool& bad) {
 
 constexpr int kKv8BadPage = 16;      // the bit of the tcgen05 kernels' status that a page id beyond the pool sets
 
+// ---- one row by a warp: without the limits of the kernels that are built for speed, for the rows that meet them
+//
+// A query row of one head over the keys [lo, hi), in float32 throughout: scores by exponents of q and the page apart, values as they are,
+// a key that the row does not see not looked at.  Lane i has entries i E .. of q (`q`, as they are) and gets the numerators there (`o`,
+// relative to 2^m, m in log2 units as c is) and the denominator l.  Some 50 times slower than the kernels' own ways.
+template <int D>
+struct Kv8Row {
+  static constexpr int E = D <= 32 ? 1 : D <= 64 ? 2 : D <= 128 ? 4 : 8;
+  static __device__ __forceinline__ bool in_head(int lane) { return lane * E < D; }
+};
+
+template <int E>
+__device__ __forceinline__ void kv8_row_load(const uint8_t* p, float* f) {
+  if constexpr (E == 1) {
+    const uint32_t h = kv8_h2(*p);
+    f[0] = __low2float(*reinterpret_cast<const __half2*>(&h));
+  } else if constexpr (E == 2) {
+    const uint32_t h = kv8_h2(*reinterpret_cast<const uint16_t*>(p));
+    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    f[0] = x.x;
+    f[1] = x.y;
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; e += 4) kv8_f4(*reinterpret_cast<const uint32_t*>(p + e), f + e);
+  }
+}
+
+template <int D, typename Args>
+__device__ __forceinline__ void kv8_row(const Args& a, int seq, int kvh, int lo, int hi, float c, int lane, float* q, float* o, float& m, float& l) {
+  constexpr int E = Kv8Row<D>::E;
+  const bool in = Kv8Row<D>::in_head(lane);
+  const uint8_t *kc = reinterpret_cast<const uint8_t*>(a.kcache), *vc = reinterpret_cast<const uint8_t*>(a.vcache);
+  const int32_t* bt = a.block_table + static_cast<size_t>(seq) * a.max_blocks;
+  float amax = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    amax = fmaxf(amax, in ? fabsf(q[e]) : 0.f);
+    o[e] = 0.f;
+  }
+  amax = warp_max(amax);
+  const int ex = amax > 0.f && amax < INFINITY ? ilogbf(amax) : 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) q[e] = in ? ldexpf(q[e], -ex) : 0.f;
+  m = -INFINITY;
+  l = 0.f;
+#pragma unroll 1
+  for (int j0 = lo & ~15; j0 < hi; j0 += 16) {             // 16 keys of one page
+    bool bad = false;                                      // (told by whoever went over the keys before)
+    const size_t block = static_cast<size_t>(kv8_page(bt[j0 >> a.page_shift], a.pages, bad)) * a.hkv + kvh;
+    const int kcode = a.kscale[block];
+    const float fv = kv8_scale(a.vscale[block]);
+    const size_t base = ((block << a.page_shift) + (j0 & ((1 << a.page_shift) - 1))) * D + (in ? lane * E : 0);
+#pragma unroll 1
+    for (int j = 0; j < 16; j += 4) {
+      float x[4], v[4][E];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        float k[E];
+        kv8_row_load<E>(kc + base + static_cast<size_t>(j + u) * D, k);
+        kv8_row_load<E>(vc + base + static_cast<size_t>(j + u) * D, v[u]);
+        x[u] = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[u] += in ? q[e] * k[e] : 0.f;
+      }
+      float top = m;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int key = j0 + j + u;
+        x[u] = ldexpf(warp_sum(x[u]) * c, ex + kcode - 127);
+        if (kcode == 255) x[u] = __uint_as_float(0x7fc00000u);
+        if (key < lo || key >= hi) x[u] = -INFINITY;
+        top = fmaxf(top, x[u]);
+      }
+      const float use = top == -INFINITY ? 0.f : top, f = m == -INFINITY ? 0.f : exp2f(m - use);
+      l *= f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] *= f;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int key = j0 + j + u;
+        if (key < lo || key >= hi) continue;
+        const float p = exp2f(x[u] - use);
+        l += p;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] += p * (v[u][e] * fv);
+      }
+      m = top;
+    }
+  }
+}
+
 // ---- single tokens: how the keys of a launch are shared out
 //
 // A row is an (item, kv head): the query heads of one kv head of one sequence's token.  Its live keys are counted in

@@ -1215,13 +1215,13 @@ int launch_prefill(const void* q, int q_stride, const void* kc, const void* vc, 
       if (err) return err;
       if (!tc_set[dev]) {
         e = cudaFuncSetAttribute(prefill_attn_tc_kernel<Kv8PrefillArgs<bf16>>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 static_cast<int>(kPrefillTcSmem));
+                                 static_cast<int>(kPrefillTcSmem8));
         if (e != cudaSuccess) return static_cast<int>(e);
         tc_set[dev] = true;
       }
       const long long work = static_cast<long long>(tiles) * hkv * ((hq / hkv + 1) / 2);     // (tile, kv head, pair of heads)
       launch_kernel(prefill_attn_tc_kernel<Kv8PrefillArgs<bf16>>, dim3(static_cast<unsigned>(work < sms ? work : sms)), dim3(kTcThreads8),
-                    kPrefillTcSmem, stream, a, tiles, status);
+                    kPrefillTcSmem8, stream, a, tiles, status);
       return static_cast<int>(cudaGetLastError());
     }
   }

@@ -5,9 +5,10 @@
 // bytes through registers and convert them (one conversion and one product for two numbers; to bfloat16 it was four times as
 // many instructions, and a portion of 2,048 behind 6,144 keys took 419 us).  A page's scale goes in relative to the largest of the
 // item's pages, so that no half overflows: exact for pages down to 2^-15 of that, and rounded to 2^-25 of its unit below; the largest
-// goes into the exponent's factor (keys) and the epilogue's (values).  Queries are rounded to halves, so they are finite up to
-// 65,504 and exact from 2^-14 on.  P is a half too.  An item of work is a tile of up to 128 consecutive query rows of one
-// sequence for TWO query heads of one kv head (the last pair of an odd group has one): the two
+// goes into the exponent's factor (keys) and the epilogue's (values).  A row of Q is scaled by a power of two to at most 256, which
+// goes into the row's factor: as halves its entries keep their bits down to 2^-21 of its largest.  (Done by two of the loaders and not by
+// all six, three portions at head size 128 took 199 us instead of 172.)  P is a half too.  An item of work is a tile of up to 128
+// consecutive query rows of one sequence for TWO query heads of one kv head (the last pair of an odd group has one): the two
 // heads are the CTA's two "slots", they attend to the same keys and values, so a K tile and a V
 // tile are brought into shared memory once for both.  Persistent CTAs (one per SM) take items
 // one after another, longest first, and the pipeline runs on across items.  Per item the keys
@@ -87,9 +88,16 @@ struct PrefillTcShared {
   uint64_t o_free[2];                             // per slot: its four row warps have read the item's O
   uint32_t tmem_base;
   volatile int abort;
-  float item_k[8], item_v[8];                     // eight bits: an item's largest scales, by it % 8 (loaders are at most six items ahead)
 };
 constexpr size_t kPrefillTcSmem = 1024 + (2 + 2 * kTcStages) * kTcTileBytes + sizeof(PrefillTcShared);
+// With eight bits, by it % 8: an item's largest scales (loaders are at most six items ahead); by the slot's it % 4: what the products with
+// a row of Q are to be multiplied by (a slot's Q is loaded when the rows have begun with the item before).
+struct PrefillTcShared8 : PrefillTcShared {
+  float item_k[8], item_v[8];
+  float q_factor[4][2][kTcRows];
+};
+constexpr size_t kPrefillTcSmem8 = kPrefillTcSmem - sizeof(PrefillTcShared) + sizeof(PrefillTcShared8);
+static_assert(kPrefillTcSmem8 <= 227 * 1024, "a CTA's shared memory");
 
 // One item of a CTA's work: a tile of query rows for up to two query heads of one kv head.
 struct TcItem {
@@ -272,20 +280,25 @@ struct TcWalk {
   }
 };
 
+template <bool kEightBit>
+struct PrefillTcSharedOf { typedef PrefillTcShared T; };
+template <>
+struct PrefillTcSharedOf<true> { typedef PrefillTcShared8 T; };
+
 // 2^e as a pair of halves, for e <= 0 (0 below the halves' range).
 __device__ __forceinline__ uint32_t tc_half_power(int e) {
   const uint32_t b = e >= -14 ? static_cast<uint32_t>(e + 15) << 10 : (e >= -24 ? 1u << (e + 24) : 0u);
   return b | b << 16;
 }
 
-// The loaders of a cache in 8 bits: three warps K, three V (the first two of them a slot's Q as well).  The UNITS of a CTA's tiles, 16 or 32
+// The loaders of a cache in 8 bits: three warps K, three V, all of them Q.  The UNITS of a CTA's tiles, 16 or 32
 // keys each (four 16-byte pieces to a lane), go to a team's warps in turn, so all of them work on one tile.  (With a tile to a warp, each
 // with a stage of its own, a stage was empty for the whole time that one warp takes over a tile: 2,048 tokens behind 6,144 keys
 // 322 us, three portions at head size 128 212; with teams 276 and 169.  A ring of bytes in shared memory instead of registers: 357.)  A unit's
 // bytes come through registers, the next unit's on their way while one is converted and stored where the copies of a 16-bit cache would
 // have put it.  Page ids and scales come 32 units at a time, a unit to a lane, a window ahead.
 template <typename Args>
-__device__ __forceinline__ void tc_load_eight_bit(const Args& a, PrefillTcShared* sh, unsigned char* q_s, unsigned char* k_s,
+__device__ __forceinline__ void tc_load_eight_bit(const Args& a, PrefillTcShared8* sh, unsigned char* q_s, unsigned char* k_s,
                                                   unsigned char* v_s, bool is_v, int turn, int lane, int n_items, int pairs, int tiles,
                                                   int* status) {
   constexpr int L = kTcLoaders8;
@@ -338,39 +351,57 @@ __device__ __forceinline__ void tc_load_eight_bit(const Args& a, PrefillTcShared
       most = max(most, static_cast<int>(scales[static_cast<size_t>(kv8_page(bt[pg], a.pages, bad)) * a.hkv + w.kvh]));
     most = __reduce_max_sync(0xffffffffu, most);
     if (turn == 0 && lane == 0) (is_v ? sh->item_v : sh->item_k)[wk.it & 7] = kv8_scale(most);
-    if (is_v && turn < (w.two ? 2 : 1)) {
-      constexpr int CPR = kD / 8, QRI = 32 / CPR;
-      const int c = lane % CPR, qr = lane / CPR, s = turn;
-      const int n = s == 0 ? wk.it : wk.it1;             // the slot's items so far
-      const bf16* src = a.q + static_cast<size_t>(w.tok0) * a.q_stride + (w.head0 + s) * kD + c * 8;
-      unsigned char* dst = q_s + s * kTcTileBytes + static_cast<uint32_t>(c >> 3) * kTcHalfBytes;
-      ok = mbar_wait(&sh->q_free[s], (n & 1) ^ 1, &sh->abort);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
+    // Q of both slots, by all six warps: kQRows rows of a slot at a time
+    {
+      constexpr int CPR = kD / 8, QRI = 32 / CPR, kQ = 4, kQRows = kQ * QRI, kParts = kTcRows / kQRows;
+      const int c = lane % CPR, qr = lane / CPR, me = is_v ? L + turn : turn;
 #pragma unroll 1
-      for (int j = 0; j < kTcRows; j += 8 * QRI) {
-        uint4 v[8];
+      for (int s = 0; s < (w.two ? 2 : 1); ++s) {
+        const int n = s == 0 ? wk.it : wk.it1;             // the slot's items so far
+        const bf16* src = a.q + static_cast<size_t>(w.tok0) * a.q_stride + (w.head0 + s) * kD + c * 8;
+        unsigned char* dst = q_s + s * kTcTileBytes + static_cast<uint32_t>(c >> 3) * kTcHalfBytes;
+        float* factors = sh->q_factor[n & 3][s];
+        ok = mbar_wait(&sh->q_free[s], (n & 1) ^ 1, &sh->abort);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+#pragma unroll 1
+        for (int j = (me + s * kParts) % (2 * L); j < kParts; j += 2 * L) {
+          uint4 v[kQ];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const int row = j + u * QRI + qr;
-          v[u] = make_uint4(0, 0, 0, 0);
-          if (row < w.rows) v[u] = *reinterpret_cast<const uint4*>(src + static_cast<size_t>(row) * a.q_stride);
-        }
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const int row = j + u * QRI + qr;
-          uint32_t in[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const __half2 h = __floats2half2_rn(__uint_as_float(in[e] << 16), __uint_as_float(in[e] & 0xffff0000u));
-            in[e] = *reinterpret_cast<const uint32_t*>(&h);
+          for (int u = 0; u < kQ; ++u) {
+            const int row = j * kQRows + u * QRI + qr;
+            v[u] = make_uint4(0, 0, 0, 0);
+            if (row < w.rows) v[u] = *reinterpret_cast<const uint4*>(src + static_cast<size_t>(row) * a.q_stride);
           }
-          *reinterpret_cast<uint4*>(dst + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = make_uint4(in[0], in[1], in[2], in[3]);
+          // a row's largest magnitude: two bfloat16 of a word side by side, then the row's lanes
+          uint32_t top[kQ];
+#pragma unroll
+          for (int u = 0; u < kQ; ++u)
+            top[u] = __vmaxu2(__vmaxu2(v[u].x & 0x7fff7fffu, v[u].y & 0x7fff7fffu),
+                                   __vmaxu2(v[u].z & 0x7fff7fffu, v[u].w & 0x7fff7fffu));
+#pragma unroll
+          for (int o = 1; o < CPR; o <<= 1)
+#pragma unroll
+            for (int u = 0; u < kQ; ++u) top[u] = __vmaxu2(top[u], __shfl_xor_sync(0xffffffffu, top[u], o));
+#pragma unroll
+          for (int u = 0; u < kQ; ++u) {
+            const int row = j * kQRows + u * QRI + qr;
+            // the largest entry is 1.m * 2^(ex - 127), and is scaled to 1.m * 2^7
+            const int ex = static_cast<int>(max(top[u] >> 16, top[u] & 0xffffu) >> 7), up = min(134 - ex, 127);
+            const float mul = kv8_exp2i(up);
+            // (a row that is not finite is not a number)
+            if (c == 0) factors[row] = ex == 255 ? __uint_as_float(0x7fc00000u) : kv8_exp2i(-up);
+            uint32_t in[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) in[e] = pack_halves(__uint_as_float(in[e] << 16) * mul, __uint_as_float(in[e] & 0xffff0000u) * mul);
+            *reinterpret_cast<uint4*>(dst + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = make_uint4(in[0], in[1], in[2], in[3]);
+          }
         }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->q_full[s]);
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh->q_full[s]);
+      if (!ok) break;
     }
     uint32_t factor[kBlocks];
     auto factors_of = [&](const int* code) {
@@ -482,7 +513,8 @@ prefill_attn_tc_kernel(const Args a, int tiles, int* status) {
   unsigned char* q_s = base;                                        // one tile per slot
   unsigned char* k_s = base + 2 * kTcTileBytes;                     // kTcStages tiles
   unsigned char* v_s = base + (2 + kTcStages) * kTcTileBytes;       // kTcStages tiles
-  PrefillTcShared* sh = reinterpret_cast<PrefillTcShared*>(base + (2 + 2 * kTcStages) * kTcTileBytes);
+  typedef typename PrefillTcSharedOf<Args::kEightBit>::T Shared;
+  Shared* sh = reinterpret_cast<Shared*>(base + (2 + 2 * kTcStages) * kTcTileBytes);
   constexpr int kMma = Args::kEightBit ? 12 : kTcRowWarps + 2;      // the first of the two MMA warps
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int pairs = (a.hq / a.hkv + 1) / 2;
@@ -490,7 +522,7 @@ prefill_attn_tc_kernel(const Args a, int tiles, int* status) {
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&sh->q_full[s], 1);
+      mbar_init(&sh->q_full[s], Args::kEightBit ? 2 * kTcLoaders8 : 1);
       mbar_init(&sh->q_free[s], 1);
       mbar_init(&sh->qk_done[s], 1);
       mbar_init(&sh->pv_done[s], 1);
@@ -762,9 +794,9 @@ prefill_attn_tc_kernel(const Args a, int tiles, int* status) {
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
-        if constexpr (Args::kEightBit)      // (once there is a tile of the item, its loader has left the scale)
+        if constexpr (Args::kEightBit)      // (once there is a tile of the item, its loaders have left the scales)
           if (i == 0) {
-            sc = a.scale * kLog2e * sh->item_k[wk.it & 7];
+            sc = a.scale * kLog2e * sh->q_factor[(s == 0 ? wk.it : wk.it1) & 3][s][r] * sh->item_k[wk.it & 7];
             if (sc < 1.2e-38f) sc = 1.2e-38f;              // (times -inf it has to be -inf; so small a factor makes every score 0)
           }
         // only tiles that reach past the first row's position, before the last row's window or past the

@@ -1,4 +1,5 @@
-"""Attention over the cache in 8 bits where numbers are not finite: what is not a number reaches the rows that see it and no others."""
+"""Attention over the cache in 8 bits where numbers are not finite (what is not a number reaches the rows that see it and no others), or
+far apart."""
 
 import math
 
@@ -89,3 +90,82 @@ def test_single_tokens_over_what_is_not_a_number(heads, kv_heads, dim, page, dty
         for s, n in enumerate(ctxs):
             ref = P.attend(q[s].view(1, heads, dim), k, v, table[s], [n - 1], window, scale)
             same_where_finite(out[s].view(1, heads, dim), ref, v[table[s][:-(-n // page)].long()], dtype)
+
+
+def tight(out, q, k, v, table, positions, window, scale, dtype, rounded_q=False):
+    """``out`` [rows, heads, D] against the formula in float64, held to a bound of each number's own, with w_j the weights:
+
+      |error| <= r |result| + (p + 2 d) sum_j w_j |v_j|
+      r   the result's one rounding: 2^-8 (bfloat16), 2^-24 (float32)
+      p   the weights' rounding and the sums': 2^-11 for halves, and 2^-16 (chains of up to a few thousand terms in float32)
+      d   the largest error of a score, which moves weights by a factor of 1 + d and the denominator likewise: of the products' sums in
+          float32 2^-17 of sum_d |q_d k_d| (128 roundings of 2^-24), and 2^-11 more where q is rounded to halves on its way (``rounded_q``)
+
+    Returns the formula's result and the bound."""
+    heads, kv_heads, page = q.shape[1], k.shape[1], k.shape[2]
+    end = int(max(positions)) + 1
+    blocks = table[:-(-end // page)].long()
+    dev = out.device
+    keys = k.to(dev)[blocks.to(dev)].permute(1, 0, 2, 3).reshape(kv_heads, -1, k.shape[3])[:, :end]
+    vals = v.to(dev)[blocks.to(dev)].permute(1, 0, 2, 3).reshape(kv_heads, -1, k.shape[3])[:, :end]
+    keys, vals = (t.repeat_interleave(heads // kv_heads, 0) for t in (keys, vals))      # [heads, keys, D]
+    qd = q.to(dev).double().transpose(0, 1)
+    score, size = qd @ keys.transpose(1, 2) * scale, qd.abs() @ keys.abs().transpose(1, 2) * scale
+    at, key = torch.tensor(list(positions), device=dev), torch.arange(end, device=dev)
+    hide = key[None] > at[:, None]
+    if window:
+        hide |= key[None] <= at[:, None] - window
+    w = torch.softmax(score.masked_fill(hide, -math.inf), -1)
+    ref, spread = (w @ vals).transpose(0, 1), (w @ vals.abs()).transpose(0, 1)
+    d = size.masked_fill(hide, 0).amax(-1).transpose(0, 1)[..., None] * (2.0 ** -17 + (2.0 ** -11 if rounded_q else 0.0))
+    r, p = (2.0 ** -24, 2.0 ** -16) if dtype == "float32" else (2.0 ** -8, 2.0 ** -11 + 2.0 ** -16)
+    limit = r * ref.abs() + (p + 2 * d) * spread
+    assert torch.isfinite(out).all()
+    err = (out.double() - ref).abs()
+    assert (err <= limit).all(), f"{(err / limit.clamp(min=1e-300)).max().item():.2f} of the limit"
+    return ref, limit
+
+
+def magnitudes(lengths, kv_heads, dim, page, kexp, vexp, seed):
+    """``filled`` with keys of sequence s times 2^kexp[s], values times 2^vexp[s] (an exponent of a block moves its scale alone)."""
+    cache, table = filled(lengths, kv_heads, kv_heads, dim, page, seed=seed)
+    for s, n in enumerate(lengths):
+        mine = table[s][:-(-n // page)].long()
+        cache[2][mine] = (cache[2][mine].int() + kexp[s]).to(torch.uint8)
+        cache[3][mine] = (cache[3][mine].int() + vexp[s]).to(torch.uint8)
+    return cache, table
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,page,impl", [(4, 2, 64, 16, 3), (3, 1, 64, 32, 3), (4, 2, 128, 16, 3), (4, 2, 64, 16, 1),
+                                                          (10, 2, 80, 16, 0)])
+def test_prompts_of_queries_of_any_size(heads, kv_heads, dim, page, impl):
+    """Queries beyond what a half holds and far below it, over keys that make up for it; rows of other sizes beside them in a tile."""
+    qexp = (0, 17, 40, 100, -17, -40, -90, 110)
+    segments = tuple((20 * s, 70 + s) for s in range(len(qexp))) + ((0, 300),)
+    lengths = [a + n for a, n in segments]
+    cache, table = magnitudes(lengths, kv_heads, dim, page, [-e for e in qexp] + [0], [0, 60, -60, 90, 0, -90, 30, 0, 0], dim)
+    g = torch.Generator().manual_seed(5)
+    q = [torch.randn(n, heads * dim, generator=g) * 2.0 ** e for (_, n), e in zip(segments, qexp + (0,))]
+    q[-1] *= torch.exp2(-torch.randint(0, 120, (len(q[-1]), 1), generator=g).float())     # (every row its own size, down to all keys alike)
+    q[0][3] = 0.0
+    q = torch.cat(q).bfloat16()
+    scale = 1.0 / math.sqrt(dim)
+    out = prefill(q, on_gpu(cache), table, segments, heads, kv_heads, dim, page, 0, scale, impl)
+    k, v = P.values(cache[0], cache[2]), P.values(cache[1], cache[3])
+    row = 0
+    for s, (a, n) in enumerate(segments):
+        tight(out[row:row + n].view(n, heads, dim), q[row:row + n].view(n, heads, dim), k, v, table[s], range(a, a + n), 0, scale, "bfloat16")
+        row += n
+
+
+def test_prompts_of_queries_that_are_not_finite():
+    """Make their own rows not a number, and no others."""
+    heads, kv_heads, dim, page, n = 4, 2, 64, 16, 200
+    cache, table = filled((n,), heads, kv_heads, dim, page, seed=1)
+    q = torch.randn(n, heads * dim, generator=torch.Generator().manual_seed(1)).bfloat16()
+    q[50, 3], q[60, dim + 5], q[130, 2 * dim] = math.inf, math.nan, -math.inf
+    outs = [prefill(q, on_gpu(cache), table, ((0, n),), heads, kv_heads, dim, page, 0, 0.125, impl).view(n, heads, dim) for impl in (1, 3)]
+    nan = torch.zeros(n, heads, dim, dtype=torch.bool)
+    nan[50, 0] = nan[60, 1] = nan[130, 2] = True
+    for out in outs:
+        assert torch.equal(torch.isnan(out).cpu(), nan) and torch.isfinite(out[~nan.to(out.device)]).all()

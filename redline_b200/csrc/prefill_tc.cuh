@@ -7,10 +7,10 @@
 // item's pages, so that no half overflows: exact for pages down to 2^-15 of that, and rounded to 2^-25 of its unit below; the largest
 // goes into the exponent's factor (keys) and the epilogue's (values).  A row of Q is scaled by a power of two to at most 256, which
 // goes into the row's factor: as halves its entries keep their bits down to 2^-21 of its largest.  (Done by two of the loaders and not by
-// all six, three portions at head size 128 took 199 us instead of 172.)  P is a half too.  An item of work is a tile of up to 128
-// consecutive query rows of one sequence for TWO query heads of one kv head (the last pair of an odd group has one): the two
-// heads are the CTA's two "slots", they attend to the same keys and values, so a K tile and a V
-// tile are brought into shared memory once for both.  Persistent CTAs (one per SM) take items
+// all six, three portions at head size 128 took 199 us instead of 172.)  P is a half too, times 2^7.
+// An item of work is a tile of up to 128 consecutive query rows of one sequence for TWO query heads of one
+// kv head (the last pair of an odd group has one): the two heads are the CTA's two "slots", they attend to the same keys and
+// values, so a K tile and a V tile are brought into shared memory once for both.  Persistent CTAs (one per SM) take items
 // one after another, longest first, and the pipeline runs on across items.  Per item the keys
 // come in tiles of 128; for each slot and key tile:
 //   S = Q K^T      tcgen05.mma, 128 x 128, k = head size, accumulator in tensor memory
@@ -77,6 +77,7 @@ constexpr int kTcColP = 384;                            // with columns of its o
 constexpr int kTcThreads8 = 512, kTcRowRegs8 = 152, kTcOtherRegs8 = 104, kTcLoaders8 = 3;
 static_assert(256 * (kTcRowRegs8 + kTcOtherRegs8) <= 512 * 128, "the launch's registers");
 constexpr float kTcGrow = 8.f;                          // log2 of the growth of a row's maximum that moves the reference
+constexpr float kTcBase8 = 7.f;                         // eight bits: log2 of P at the reference, 2^15 at most: 11 bits down to 2^-21 of it
 
 struct PrefillTcShared {
   uint64_t q_full[2], q_free[2];                  // per slot: Q of an item has landed / its last S product has read it
@@ -845,7 +846,7 @@ prefill_attn_tc_kernel(const Args a, int tiles, int* status) {
           m_ref = m_new;
           moved = true;
         }
-        const float m_use = m_ref == -INFINITY ? 0.f : m_ref;  // a row without a live key so far
+        const float m_use = m_ref == -INFINITY ? 0.f : m_ref - (Args::kEightBit ? kTcBase8 : 0.f);  // a row without a live key so far
         const uint64_t sc2 = f32x2(sc, sc), nm2 = f32x2(-m_use, -m_use);
         uint64_t sum_a = f32x2(0.f, 0.f), sum_b = sum_a;
         auto add_sums = [](float& part, uint64_t a2, uint64_t b2) {

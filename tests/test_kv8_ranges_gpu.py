@@ -169,3 +169,22 @@ def test_prompts_of_queries_that_are_not_finite():
     nan[50, 0] = nan[60, 1] = nan[130, 2] = True
     for out in outs:
         assert torch.equal(torch.isnan(out).cpu(), nan) and torch.isfinite(out[~nan.to(out.device)]).all()
+
+
+@pytest.mark.parametrize("dim,impl", [(64, 3), (128, 3), (64, 1)])
+def test_prompts_of_many_small_weights(dim, impl):
+    """One key takes nearly all the weight and its value is nothing: what is left are thousands of keys of one small weight each."""
+    heads, kv_heads, page, n, past = 2, 1, 16, 130, 4000
+    cache, table = filled((past + n,), heads, kv_heads, dim, page, seed=2)
+    k, v = torch.zeros(past + n, kv_heads, dim), torch.ones(past + n, kv_heads, dim)
+    v *= 1.0 + torch.randint(0, 4, (past + n, 1, 1), generator=torch.Generator().manual_seed(1)) / 4.0
+    k[0, 0, 0], v[:16] = 1.0, 0.0
+    slot = [int(table[0, p // page]) * page + p % page for p in range(past + n)]
+    P.store(k, slot, cache[0], cache[2])
+    P.store(v, slot, cache[1], cache[3])
+    q = torch.zeros(n, heads, dim)
+    q[:, :, 0] = (torch.arange(n)[:, None] * 0.15 + torch.tensor([0.0, 0.07])) * math.log(2.0)      # weights from 1 to 2^-19.4 of the one key's
+    q = q.view(n, -1).bfloat16()
+    out = prefill(q, on_gpu(cache), table, ((past, n),), heads, kv_heads, dim, page, 0, 1.0, impl)
+    kd, vd = P.values(cache[0], cache[2]), P.values(cache[1], cache[3])
+    tight(out.view(n, heads, dim), q.view(n, heads, dim), kd, vd, table[0], range(past, past + n), 0, 1.0, "bfloat16")

@@ -3,9 +3,12 @@
 // Included by attention.cu, and by kv8.cu for a cache in 8 bits (the arguments' type says which: kEightBit).  Before it come
 // cp_async16_s, cp_async_commit, cp_async_wait and ex2_approx.  With eight bits the products are of halves: the loaders bring a tile's
 // bytes through registers and convert them (one conversion and one product for two numbers; to bfloat16 it was four times as
-// many instructions, and a portion of 2,048 behind 6,144 keys took 419 us).  A page's scale goes in relative to the largest of the
-// item's pages, so that no half overflows: exact for pages down to 2^-15 of that, and rounded to 2^-25 of its unit below; the largest
-// goes into the exponent's factor (keys) and the epilogue's (values).  A row of Q is scaled by a power of two to at most 256, which
+// many instructions, and a portion of 2,048 behind 6,144 keys took 419 us).  A page's scale goes in relative to 2^-7 of the largest of the
+// item's pages, so that no half overflows, which is exact for pages down to 2^-22 of that; the largest goes into the exponent's factor
+// (keys) and the epilogue's (values).  Items whose pages are farther apart than that are listed by the loaders, and items with a result that
+// is not finite by the rows (a value that is not a number reaches rows that do not see its key, too: a weight of 0 does not cover it); the
+// rows of a listed item are done once more at the end, one by one (kv8_row).  A page whose scale is the smallest is taken for one of
+// zeros here.  A row of Q is scaled by a power of two to at most 256, which
 // goes into the row's factor: as halves its entries keep their bits down to 2^-21 of its largest.  (Done by two of the loaders and not by
 // all six, three portions at head size 128 took 199 us instead of 172.)  P is a half too, times 2^7.
 // An item of work is a tile of up to 128 consecutive query rows of one sequence for TWO query heads of one
@@ -91,11 +94,14 @@ struct PrefillTcShared {
   volatile int abort;
 };
 constexpr size_t kPrefillTcSmem = 1024 + (2 + 2 * kTcStages) * kTcTileBytes + sizeof(PrefillTcShared);
+constexpr int kTcShift8 = 7, kTcSpread8 = 22;            // log2 of what the largest scale counts for, and of how far below a page's scale may be
+constexpr int kTcRedo8 = 60;
 // With eight bits, by it % 8: an item's largest scales (loaders are at most six items ahead); by the slot's it % 4: what the products with
 // a row of Q are to be multiplied by (a slot's Q is loaded when the rows have begun with the item before).
 struct PrefillTcShared8 : PrefillTcShared {
   float item_k[8], item_v[8];
   float q_factor[4][2][kTcRows];
+  int redo_n, redo[kTcRedo8];                     // items whose rows are to be done once more (some of them twice in the list; more than fit: all)
 };
 constexpr size_t kPrefillTcSmem8 = kPrefillTcSmem - sizeof(PrefillTcShared) + sizeof(PrefillTcShared8);
 static_assert(kPrefillTcSmem8 <= 227 * 1024, "a CTA's shared memory");
@@ -218,6 +224,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
+__device__ __forceinline__ float max_nan(float a, float b) {      // not a number if one of them is
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
 // Sets the scores of 32 keys that a row may not see to -inf: key j of them is live if jmin <= j <= jmax.
 // Without a window (the same for all threads) there is no lower limit to test.
 __device__ __forceinline__ void tc_mask32(uint32_t* sr, int jmax, int jmin, bool window) {
@@ -286,10 +298,15 @@ struct PrefillTcSharedOf { typedef PrefillTcShared T; };
 template <>
 struct PrefillTcSharedOf<true> { typedef PrefillTcShared8 T; };
 
-// 2^e as a pair of halves, for e <= 0 (0 below the halves' range).
+// 2^e as a pair of halves, for e < 16 (0 below the halves' range).
 __device__ __forceinline__ uint32_t tc_half_power(int e) {
   const uint32_t b = e >= -14 ? static_cast<uint32_t>(e + 15) << 10 : (e >= -24 ? 1u << (e + 24) : 0u);
   return b | b << 16;
+}
+
+__device__ __forceinline__ void tc_list(PrefillTcShared8* sh, int item) {
+  const int n = atomicAdd(&sh->redo_n, 1);
+  if (n < kTcRedo8) sh->redo[n] = item;
 }
 
 // The loaders of a cache in 8 bits: three warps K, three V, all of them Q.  The UNITS of a CTA's tiles, 16 or 32
@@ -345,13 +362,20 @@ __device__ __forceinline__ void tc_load_eight_bit(const Args& a, PrefillTcShared
     pages_of(x, page);
     codes_of(page, next_code);
     pages_of(x + 32 * L, next_page);
-    // the item's largest scale
-    int most = 0;
+    // the item's largest and smallest scales
+    int most = 0, least = 254;
 #pragma unroll 4
-    for (int pg = first + lane; pg <= last; pg += 32)
-      most = max(most, static_cast<int>(scales[static_cast<size_t>(kv8_page(bt[pg], a.pages, bad)) * a.hkv + w.kvh]));
+    for (int pg = first + lane; pg <= last; pg += 32) {
+      const int code = scales[static_cast<size_t>(kv8_page(bt[pg], a.pages, bad)) * a.hkv + w.kvh];
+      most = max(most, code);
+      least = min(least, code > 1 ? code : 254);
+    }
     most = __reduce_max_sync(0xffffffffu, most);
-    if (turn == 0 && lane == 0) (is_v ? sh->item_v : sh->item_k)[wk.it & 7] = kv8_scale(most);
+    least = __reduce_min_sync(0xffffffffu, least);
+    if (turn == 0 && lane == 0) {
+      (is_v ? sh->item_v : sh->item_k)[wk.it & 7] = kv8_scale(most) * 0x1p-7f;
+      if (most - least > kTcSpread8) tc_list(sh, wk.item);
+    }
     // Q of both slots, by all six warps: kQRows rows of a slot at a time
     {
       constexpr int CPR = kD / 8, QRI = 32 / CPR, kQ = 4, kQRows = kQ * QRI, kParts = kTcRows / kQRows;
@@ -407,7 +431,7 @@ __device__ __forceinline__ void tc_load_eight_bit(const Args& a, PrefillTcShared
     uint32_t factor[kBlocks];
     auto factors_of = [&](const int* code) {
 #pragma unroll
-      for (int j = 0; j < kBlocks; ++j) factor[j] = tc_half_power(code[j] - most);
+      for (int j = 0; j < kBlocks; ++j) factor[j] = tc_half_power(code[j] - most + kTcShift8);
     };
     factors_of(next_code);
     // asks for unit u, the r-th of the window
@@ -503,6 +527,25 @@ __device__ __forceinline__ void tc_load_eight_bit(const Args& a, PrefillTcShared
   if (bad) atomicOr(status, kKv8BadPage);
 }
 
+// Rows 32 q .. + 31 of slot s of an item once more, by the warp whose threads have written them.
+template <typename Args>
+__device__ __forceinline__ void tc_rows_again(const Args& a, const TcItem& w, int s, int q, int lane) {
+  constexpr int E = kD / 32;
+  static_assert(Kv8Row<kD>::E == E, "entries of a lane");
+  if (s == 1 && !w.two) return;
+#pragma unroll 1
+  for (int r = q * 32; r < min(q * 32 + 32, w.rows); ++r) {
+    const int pos = w.pos0 + r, at = (w.head0 + s) * kD + lane * E;
+    float x[E], o[E], m, l;
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = to_float(a.q[static_cast<size_t>(w.tok0 + r) * a.q_stride + at + e]);
+    kv8_row<kD>(a, w.seq, w.kvh, a.window > 0 && pos + 1 > a.window ? pos + 1 - a.window : 0, pos + 1, a.scale * 1.4426950408889634f, lane, x, o,
+                m, l);
+#pragma unroll
+    for (int e = 0; e < E; ++e) a.out[static_cast<size_t>(w.tok0 + r) * a.out_stride + at + e] = __float2bfloat16_rn(o[e] / l);
+  }
+}
+
 template <typename Args>
 __global__ void __launch_bounds__(Args::kEightBit ? kTcThreads8 : kTcThreads, 1)
 prefill_attn_tc_kernel(const Args a, int tiles, int* status) {
@@ -538,6 +581,7 @@ prefill_attn_tc_kernel(const Args a, int tiles, int* status) {
       mbar_init(&sh->v_free[b], 2);
     }
     sh->abort = 0;
+    if constexpr (Args::kEightBit) sh->redo_n = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kMma) {   // TMEM allocation is a whole-warp operation
@@ -931,6 +975,7 @@ prefill_attn_tc_kernel(const Args a, int tiles, int* status) {
       float inv = l_all > 0.f ? 1.f / l_all : 0.f;
       if constexpr (Args::kEightBit) inv *= sh->item_v[wk.it & 7];
       bf16* dst = a.out + static_cast<size_t>(w.tok0 + (r < rows ? r : 0)) * a.out_stride + (w.head0 + s) * kD;
+      float largest = 0.f;                                // of the row's results; not a number if one of them is
 #pragma unroll
       for (int c0 = 0; c0 < kD; c0 += 32) {
         uint32_t o[32];
@@ -942,11 +987,16 @@ prefill_attn_tc_kernel(const Args a, int tiles, int* status) {
             float v[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(o[d + e]) * inv;
+            if constexpr (Args::kEightBit)
+#pragma unroll
+              for (int e = 0; e < 8; ++e) largest = max_nan(largest, fabsf(v[e]));
             store16(dst + c0 + d, v);
           }
         }
       }
       tc_fence_before();
+      if constexpr (Args::kEightBit)
+        if (__any_sync(0xffffffffu, !(largest < INFINITY)) && lane == 0) tc_list(sh, wk.item);
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->o_free[s]);
     }
@@ -958,6 +1008,23 @@ prefill_attn_tc_kernel(const Args a, int tiles, int* status) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTcTmemCols) : "memory");
   }
   if (threadIdx.x == 0 && sh->abort) atomicOr(status, 4);
+  if constexpr (Args::kEightBit) {
+    // the listed items' rows (here and not behind the rows' loop, whose code was 3 % slower for it)
+    const int listed = sh->abort ? 0 : sh->redo_n;
+    if (listed > 0 && warp < kTcRowWarps) {
+      int round = 0;
+#pragma unroll 1
+      for (int i = 0;; ++i) {                              // the list, or (more than it holds) all the CTA's items
+        int item = -1;
+        if (listed > kTcRedo8) item = tc_next_item(round, n_items);
+        else if (i < listed) item = sh->redo[i];
+        if (item < 0) break;
+        bool had = false;
+        for (int j = 0; j < i && listed <= kTcRedo8; ++j) had |= sh->redo[j] == item;
+        if (!had) tc_rows_again(a, TcWalk::load(a, item, pairs, tiles), warp >> 2, warp & 3, lane);
+      }
+    }
+  }
 }
 
 }  // namespace rl

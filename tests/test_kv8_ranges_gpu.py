@@ -34,7 +34,8 @@ def same_where_finite(out, ref, v, dtype):
 
 @pytest.mark.parametrize("heads,kv_heads,dim,page,window,dtype,impl", [
     (4, 2, 64, 16, 0, "bfloat16", 1), (4, 2, 64, 16, 0, "float32", 0), (3, 1, 128, 32, 0, "bfloat16", 1), (4, 2, 64, 64, 90, "float32", 0),
-    (10, 2, 80, 16, 0, "bfloat16", 0), (2, 1, 16, 16, 25, "bfloat16", 0)])
+    (10, 2, 80, 16, 0, "bfloat16", 0), (2, 1, 16, 16, 25, "bfloat16", 0), (4, 2, 64, 16, 0, "bfloat16", 3), (3, 1, 128, 32, 0, "bfloat16", 3),
+    (4, 2, 64, 64, 90, "bfloat16", 3), (5, 1, 128, 16, 60, "bfloat16", 3)])
 def test_prompts_over_what_is_not_a_number(heads, kv_heads, dim, page, window, dtype, impl):
     """A key, an entry of a value and a page's scale in the middle of portions: the rows that see them, and only those."""
     segments = ((40, 200), (0, 70), (300, 150))
@@ -188,3 +189,63 @@ def test_prompts_of_many_small_weights(dim, impl):
     out = prefill(q, on_gpu(cache), table, ((past, n),), heads, kv_heads, dim, page, 0, 1.0, impl)
     kd, vd = P.values(cache[0], cache[2]), P.values(cache[1], cache[3])
     tight(out.view(n, heads, dim), q.view(n, heads, dim), kd, vd, table[0], range(past, past + n), 0, 1.0, "bfloat16")
+
+
+FAR = [(4, 2, 64, 16, 0, "bfloat16", 3), (3, 1, 128, 16, 0, "bfloat16", 3), (4, 2, 64, 32, 100, "bfloat16", 3), (4, 2, 64, 16, 0, "bfloat16", 1),
+       (4, 2, 64, 16, 0, "float32", 0), (10, 2, 80, 16, 0, "bfloat16", 0)]
+
+
+@pytest.mark.parametrize("far", [5, 20, 22, 23, 30, 60])
+@pytest.mark.parametrize("heads,kv_heads,dim,page,window,dtype,impl", FAR)
+def test_prompts_over_pages_far_apart(heads, kv_heads, dim, page, window, dtype, impl, far):
+    """Pages that only later rows of a tile see are 2^far larger, and queries are such that scores are of any one size; pages of all
+    sizes behind one another; every row right by its own measure."""
+    segments = ((0, 260), (100, 180), (0, 90))
+    lengths = [a + n for a, n in segments]
+    cache, table = filled(lengths, heads, kv_heads, dim, page, seed=dim + far)
+    small = 64 // page
+    for b, p in enumerate(table[0].tolist()):
+        if p and b < small:
+            cache[2][p] -= far
+            cache[3][p] -= far
+    for b, p in enumerate(table[1].tolist()):
+        if p:
+            cache[3][p] = (cache[3][p].int() + (-far, 0, far, 3, -far // 2)[b % 5]).to(torch.uint8)
+    g = torch.Generator().manual_seed(6)
+    q = torch.randn(sum(n for _, n in segments), heads * dim, generator=g)
+    q[:64] *= 2.0 ** far
+    q = q.to(DT[dtype])
+    scale = 1.0 / math.sqrt(dim)
+    out = prefill(q, on_gpu(cache), table, segments, heads, kv_heads, dim, page, window, scale, impl)
+    k, v = P.values(cache[0], cache[2]), P.values(cache[1], cache[3])
+    row = 0
+    for s, (a, n) in enumerate(segments):
+        tight(out[row:row + n].view(n, heads, dim), q[row:row + n].view(n, heads, dim), k, v, table[s], range(a, a + n), window, scale, dtype)
+        row += n
+
+
+def test_prompts_of_very_many_items_far_apart():
+    """More of them to a CTA than it keeps a list of."""
+    heads = kv_heads = 32
+    dim, page, n = 64, 16, 300
+    segments = ((15, 2),) * n
+    cache, table = filled((17,) * n, heads, kv_heads, dim, page, seed=3)
+    cache[3][table[:, 0].long()] -= 40
+    q = torch.randn(2 * n, heads * dim, generator=torch.Generator().manual_seed(6)).bfloat16()
+    out = prefill(q, on_gpu(cache), table, segments, heads, kv_heads, dim, page, 0, 0.125, 3)
+    k, v = P.values(cache[0], cache[2]), P.values(cache[1], cache[3])
+    for s in (0, 1, 77, 150, 298, 299):
+        tight(out[2 * s:2 * s + 2].view(2, heads, dim), q[2 * s:2 * s + 2].view(2, heads, dim), k, v, table[s], (15, 16), 0, 0.125, "bfloat16")
+
+
+def test_a_page_of_zeros_is_not_far_from_any():
+    """Its scale is the smallest there is."""
+    heads, kv_heads, dim, page, n = 4, 2, 64, 16, 200
+    cache, table = filled((n,), heads, kv_heads, dim, page, seed=3)
+    for b in (0, 3, 7):
+        p = int(table[0, b])
+        cache[0][p], cache[1][p], cache[2][p], cache[3][p] = 0, 0, 1, 1
+    q = torch.randn(n, heads * dim, generator=torch.Generator().manual_seed(6)).bfloat16()
+    out = prefill(q, on_gpu(cache), table, ((0, n),), heads, kv_heads, dim, page, 0, 0.125, 3)
+    k, v = P.values(cache[0], cache[2]), P.values(cache[1], cache[3])
+    tight(out.view(n, heads, dim), q.view(n, heads, dim), k, v, table[0], range(n), 0, 0.125, "bfloat16")

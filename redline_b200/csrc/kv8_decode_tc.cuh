@@ -11,7 +11,9 @@
 //                stands for is free, so a lane's 16 bytes of a key are four k steps of the A fragment as they lie.
 //   softmax      online, in log2 units, against a reference that moves only when some score exceeds it by 2^10: one vote a sub-block
 //                instead of shuffles.  The weights are halves, 2^5 at the reference: 11 bits down to 2^-19 of it, steps of 2^-29 below.
-//                For the product they carry the value scale of their page relative to the largest so far (2^-28 of that loses bits)
+//                For the product they carry the value scale of their page relative to the largest so far.  A run that meets pages more than
+//                2^10 apart is left and done by itself, a row after the other in float32 (kv8_row); a page whose scale is the smallest
+//                counts as zeros
 //   O^T += V^T P^T   ldmatrix transposes 16 x 16 bytes of V: four keys of an entry in a word; movmatrix transposes P
 // With the rotation in the kernel (a.store) the warp that has a row's newest page also stores the token's key and value there: it
 // takes that sub-block first, puts the token over what the copy brought, rescales the page if its scale rises, and goes on
@@ -120,6 +122,7 @@ __device__ __forceinline__ void store_cluster(float* p, uint32_t rank, float4 v)
 
 constexpr float kDecGrow = 10.f;        // log2 of how far a score may exceed the reference
 constexpr int kDecBase = 5;             // log2 of a weight at the reference: 2^15 at most
+constexpr int kDecSpread = 10;          // log2 of how far the value scales of a run's pages may be apart
 
 // One warp's result for its run.  Thread (g, t) holds entries 16 c + g (o[c][i][0 and 1]) and 16 c + 8 + g (2 and 3) of the heads
 // 8 i + 2 t and 8 i + 2 t + 1, and those heads' references and denominators (of its own keys until the end).
@@ -291,9 +294,10 @@ __device__ __forceinline__ uint32_t tc_store_token(const Kv8Args& a, const Kv8Se
   return static_cast<uint32_t>(kcode) | static_cast<uint32_t>(vcode) << 8;
 }
 
-// The run of sub-blocks [sb0, sb0 + n) of the segment, the last one first, through the warp's ring.
+// The run of sub-blocks [sb0, sb0 + n) of the segment, the last one first, through the warp's ring.  False: the pages are too far apart
+// (the token is stored, the result of no use).
 template <bool HI>
-__device__ __forceinline__ void tc_run(const Kv8Args& a, const Kv8Segment& s, int sb0, int n, uint32_t ring, int lane, TcState<HI>& st) {
+__device__ __forceinline__ bool tc_run(const Kv8Args& a, const Kv8Segment& s, int sb0, int n, uint32_t ring, int lane, TcState<HI>& st) {
   constexpr int KS = kD / 16, NC = kD / 16, NR = HI ? 2 : 1;
   constexpr int CPR = kD / 16;                           // 16-byte pieces of a key
   const int shift = a.page_shift, ps = 1 << shift;
@@ -307,7 +311,9 @@ __device__ __forceinline__ void tc_run(const Kv8Args& a, const Kv8Segment& s, in
     st.l[h][0] = st.l[h][1] = 0.f;
   }
   st.vref = -1000;
-  if (n <= 0) return;
+  int vleast = 1000;                                     // the smallest exponent of a page's values
+  bool near = true;
+  if (n <= 0) return true;
   const int32_t* bt = a.block_table + static_cast<size_t>(s.seq) * a.max_blocks;
   // (a sub-block may reach over either end of the live keys, into pages that need not be there any more: their places are
   // filled from the nearest live page)
@@ -476,9 +482,14 @@ __device__ __forceinline__ void tc_run(const Kv8Args& a, const Kv8Segment& s, in
       kf[b] = kv8_scale(c & 255);
       ve[b] = static_cast<int>(c >> 8) - 127;
       odd |= ve[b] == 128;
+      if (ve[b] > -126) vleast = min(vleast, ve[b]);
     }
     const int vref = max(st.vref, max(ve[0], ve[1]));
-    if (vref != st.vref) {                               // (the same for the warp)
+    if (vref - vleast > kDecSpread) {                    // (the same for the warp)
+      near = false;
+      break;
+    }
+    if (vref != st.vref) {
       const float f = kv8_exp2i(max(st.vref - vref, -127));
 #pragma unroll
       for (int c = 0; c < NC; ++c)
@@ -583,6 +594,31 @@ __device__ __forceinline__ void tc_run(const Kv8Args& a, const Kv8Segment& s, in
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) st.l[h][e] += __shfl_xor_sync(0xffffffffu, st.l[h][e], o);
   __syncwarp();
+  return near;
+}
+
+// The same run, a head after the other and a lane to kD / 32 entries, into the place of the warp's partial result.
+__device__ __noinline__ void tc_run_far(const Kv8Args& a, Kv8Segment s, int sb0, int n, int lane, float* to) {
+  constexpr int E = kD / 32;
+  const int G = a.hq / a.hkv, at = lane * E, dh = at % (kD / 2);
+#pragma unroll 1
+  for (int r = 0; r < G; ++r) {
+    const bf16* row = static_cast<const bf16*>(a.q) + static_cast<size_t>(s.tok) * a.q_stride + (s.kvh * G + r) * kD;
+    float x[E], o[E], m, l;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      x[e] = to_float(row[at + e]);
+      if (a.cos != nullptr) {
+        const size_t i = static_cast<size_t>(s.ctx - 1 < a.max_pos ? s.ctx - 1 : 0) * (kD / 2) + dh + e;
+        const float other = to_float(row[at < kD / 2 ? at + e + kD / 2 : dh + e]);
+        x[e] = at < kD / 2 ? x[e] * a.cos[i] - other * a.sin[i] : x[e] * a.cos[i] + other * a.sin[i];
+      }
+    }
+    kv8_row<kD>(a, s.seq, s.kvh, max(s.key_lo, sb0 * kSub), min(s.key_hi, (sb0 + n) * kSub), a.scale * 1.4426950408889634f, lane, x, o, m, l);
+#pragma unroll
+    for (int e = 0; e < E; ++e) to[r * kPartLd + at + e] = o[e];
+    if (lane == 0) *reinterpret_cast<float4*>(to + r * kPartLd + kD) = make_float4(0.f, m, l, 0.f);
+  }
 }
 
 __device__ __forceinline__ void tc_group_barrier(int bar, int gsize) {
@@ -649,7 +685,7 @@ __device__ __noinline__ void tc_fold(unsigned char* parts, int stride, int n, in
 // groups: of the CTA's warps, a divisor of their number.  parts: 0 rows, > 0 pieces of a row (one to a CTA), -1 shares.
 template <bool HI>
 __global__ void __launch_bounds__(kDecThreads, 1)
-kv8_decode_tc_kernel(const Kv8Args a, int groups, int parts) {
+kv8_decode_tc_kernel(const __grid_constant__ Kv8Args a, int groups, int parts) {
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ int start[kMaxItems + 1];
   __shared__ int last[kDecWarps];
@@ -704,17 +740,19 @@ kv8_decode_tc_kernel(const Kv8Args a, int groups, int parts) {
     const int first = s.key_lo / kSub, all = s.key_hi > s.key_lo ? (s.key_hi - 1) / kSub - first + 1 : 0;
     const int per = all / W, rem = all - per * W;
     TcState<HI> st;
-    tc_run<HI>(a, s, first + wi * per + min(wi, rem), per + (wi < rem ? 1 : 0), smem_u32(smem) + warp * kRingBytes, lane, st);
+    const int sb0 = first + wi * per + min(wi, rem), sbs = per + (wi < rem ? 1 : 0);
+    const bool near = tc_run<HI>(a, s, sb0, sbs, smem_u32(smem) + warp * kRingBytes, lane, st);
     bf16* out = static_cast<bf16*>(a.out) + static_cast<size_t>(s.tok) * a.out_stride + s.kvh * G * kD;
     // ---- its partial result into its ring
     float* mine = reinterpret_cast<float*>(smem + warp * kRingBytes);
     const int g = lane >> 2, t = lane & 3;
+    if (!near) tc_run_far(a, s, sb0, sbs, lane, mine);
 #pragma unroll
     for (int h = 0; h < (HI ? 2 : 1); ++h)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int r = 8 * h + 2 * t + e;
-        if (r >= G) continue;
+        if (r >= G || !near) continue;
 #pragma unroll
         for (int c = 0; c < kD / 16; ++c) {
           mine[r * kPartLd + 16 * c + g] = st.o[c][h][e];

@@ -880,6 +880,9 @@ def kv8_attn_decode(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, vcache
     impl       0: the best kernel that applies; 1: CUDA cores; 2: tensor cores, a cluster or a group of warps to a row, or an
                error; 3: tensor cores, the keys in equal shares, or an error; 4: tensor cores, every row in pieces (2 with more rows
                than SMs), or an error (tensor cores: bfloat16, head size 64 or 128, up to 16 query heads to a kv head)
+
+    On the tensor cores softmax weights are halves, 11 bits down to 2^-19 of a row's largest; what meets values of pages more than 2^10 apart
+    is done in float32, some 50 times slower.
     """
     _kv8_decode("kv8_attn_decode", q, q_stride, kcache, vcache, kscale, vscale, block_table, items, workspace, out, nitems,
                 num_heads, num_kv_heads, head_dim, page_size, window, scale, None, None, None, max_ctx, sum_ctx, impl)

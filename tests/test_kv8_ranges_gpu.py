@@ -8,7 +8,7 @@ import torch
 
 import plain_kv8 as P
 from redline_b200.ops import kernels
-from test_kv8_gpu import DEV, DT, filled, near, on_gpu, tiles_of
+from test_kv8_gpu import DEV, DT, angles, filled, near, on_gpu, tiles_of
 
 pytestmark = pytest.mark.gpu
 
@@ -249,3 +249,83 @@ def test_a_page_of_zeros_is_not_far_from_any():
     out = prefill(q, on_gpu(cache), table, ((0, n),), heads, kv_heads, dim, page, 0, 0.125, 3)
     k, v = P.values(cache[0], cache[2]), P.values(cache[1], cache[3])
     tight(out.view(n, heads, dim), q.view(n, heads, dim), k, v, table[0], range(n), 0, 0.125, "bfloat16")
+
+
+def decode(q, gpu, table, ctxs, heads, kv_heads, dim, page, window, scale, impl):
+    n = len(ctxs)
+    items = torch.tensor([(i, i, c, 0) for i, c in enumerate(ctxs)], dtype=torch.int32, device=DEV)
+    work = kernels.kv8_decode_workspace(n, heads, kv_heads, dim, torch.device(DEV))
+    qg, out = q.to(DEV), torch.empty(n, heads * dim, dtype=q.dtype, device=DEV)
+    kernels.kv8_attn_decode(qg, qg.stride(0), *gpu, table.to(DEV), items, work, out, n, heads, kv_heads, dim, page, window, scale, impl=impl)
+    assert (work[1] == 0).all()
+    return out
+
+
+SINGLE = [(4, 2, 64, 16, "bfloat16"), (16, 1, 64, 32, "bfloat16"), (3, 1, 128, 16, "bfloat16"), (16, 1, 128, 64, "bfloat16"),
+          (4, 2, 64, 16, "float32"), (10, 2, 80, 16, "bfloat16")]
+
+
+@pytest.mark.parametrize("far", [5, 10, 11, 30, 60])
+@pytest.mark.parametrize("heads,kv_heads,dim,page,dtype", SINGLE)
+@pytest.mark.parametrize("impl", [0, 1, 2, 3, 4])
+def test_single_tokens_over_pages_far_apart(heads, kv_heads, dim, page, dtype, impl, far):
+    """Values of pages 2^far apart: the large ones under weights that are next to nothing, and all sizes behind one another."""
+    if impl and (dtype == "float32" or dim == 80):
+        pytest.skip("one way only")
+    ctxs = (300, 1500, 64, 200, 900)
+    cache, table = filled(ctxs, heads, kv_heads, dim, page, seed=far)
+    g = torch.Generator().manual_seed(4)
+    q = torch.randn(len(ctxs), heads, dim, generator=g)
+    for s, n in enumerate(ctxs):
+        for b, p in enumerate(table[s].tolist()):
+            if not p:
+                continue
+            if s % 2:                            # every size, the token's own page among them
+                cache[3][p] = (cache[3][p].int() + (0, -far, far, 2, -far // 2)[b % 5]).to(torch.uint8)
+            elif b == 1:                         # one page of large values, its keys turned away from q
+                cache[3][p] += far
+                away = -q[s].view(kv_heads, heads // kv_heads, dim).sum(1) * (far * math.log(2.0) * 1.5 * math.sqrt(dim) / dim)
+                bytes_, scales = torch.zeros_like(cache[0][:1]), torch.zeros_like(cache[2][:1])
+                P.store(away[None].expand(page, -1, -1), range(page), bytes_, scales)
+                cache[0][p], cache[2][p] = bytes_[0], scales[0]
+    q = q.view(len(ctxs), -1).to(DT[dtype])
+    scale = 1.0 / math.sqrt(dim)
+    k, v = P.values(cache[0], cache[2]), P.values(cache[1], cache[3])
+    for window in (0, 100):
+        out = decode(q, on_gpu(cache), table, ctxs, heads, kv_heads, dim, page, window, scale, impl)
+        for s, n in enumerate(ctxs):
+            tight(out[s].view(1, heads, dim), q[s].view(1, heads, dim), k, v, table[s], [n - 1], window, scale, dtype)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,page,impl", [(4, 2, 64, 16, 2), (4, 2, 64, 32, 3), (3, 1, 128, 16, 4), (16, 1, 128, 32, 2),
+                                                          (4, 2, 64, 64, 2)])
+def test_tokens_stored_beside_pages_far_apart(heads, kv_heads, dim, page, impl):
+    """The token's own value far larger, or far smaller, than what the sequence holds: stored bit for bit, attended by its own measure."""
+    ctxs = (100, 130, 65, 200, 49, 33)
+    cache, table = filled(ctxs, heads, kv_heads, dim, page, seed=7, poison=False)
+    g = torch.Generator().manual_seed(3)
+    n = len(ctxs)
+    x = torch.randn(n, (heads + 2 * kv_heads) * dim, generator=g)
+    x[:, (heads + kv_heads) * dim:] *= 2.0 ** torch.tensor([40.0, -40.0, 12.0, -12.0, 90.0, 0.0])[:, None]
+    x = x.bfloat16()
+    cos, sin = angles(300, dim)
+    gpu = on_gpu(cache)
+    items = torch.tensor([(i, i, c, 0) for i, c in enumerate(ctxs)], dtype=torch.int32, device=DEV)
+    work = kernels.kv8_decode_workspace(n, heads, kv_heads, dim, torch.device(DEV))
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    xg, out = x.to(DEV), torch.empty(n, heads * dim, dtype=x.dtype, device=DEV)
+    scale = 1.0 / math.sqrt(dim)
+    kernels.kv8_attn_decode_rope(xg, xg.stride(0), *gpu, table.to(DEV), items, work, out, n, heads, kv_heads, dim, page, 0, scale,
+                                 cos.to(DEV), sin.to(DEV), status, impl=impl)
+    at = [c - 1 for c in ctxs]
+    slots = [int(table[s, p // page]) * page + p % page for s, p in enumerate(at)]
+    f = x.float()
+    P.store(P.rotate(f[:, heads * dim:-kv_heads * dim].reshape(n, kv_heads, dim), cos[at], sin[at]), slots, cache[0], cache[2])
+    P.store(f[:, -kv_heads * dim:].reshape(n, kv_heads, dim), slots, cache[1], cache[3])
+    for got, want in zip(gpu, cache):
+        assert torch.equal(got.view(torch.uint8).cpu(), want)
+    assert status.item() == 0
+    k, v = P.values(cache[0], cache[2]), P.values(cache[1], cache[3])
+    q = P.rotate(f[:, :heads * dim].view(n, heads, dim), cos[at], sin[at])
+    for s, c in enumerate(ctxs):
+        tight(out[s].view(1, heads, dim), q[s:s + 1], k, v, table[s], [c - 1], 0, scale, "bfloat16", rounded_q=True)

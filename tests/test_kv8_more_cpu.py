@@ -65,3 +65,12 @@ def test_heads_that_are_no_groups(heads, kv_heads):
             call()
     if kv_heads < 1 or heads < kv_heads:
         assert kernels._kv8(64).rl_kv8_decode_choice(1, 1, heads, kv_heads, 10, ctypes.c_longlong(10)) == -1
+
+
+def test_the_build_has_the_8_bit_cache_wherever_it_has_attention(monkeypatch):
+    """(a head size that it leaves out is compiled within the first request)"""
+    import __graft_entry__
+    asked = {}
+    monkeypatch.setattr(kernels, "build_all", lambda **kw: asked.update(kw))
+    __graft_entry__.build()
+    assert set(asked["head_dims"]) <= set(asked["kv8_dims"])

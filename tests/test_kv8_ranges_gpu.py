@@ -93,8 +93,8 @@ def test_single_tokens_over_what_is_not_a_number(heads, kv_heads, dim, page, dty
             same_where_finite(out[s].view(1, heads, dim), ref, v[table[s][:-(-n // page)].long()], dtype)
 
 
-def tight(out, q, k, v, table, positions, window, scale, dtype, rounded_q=False):
-    """``out`` [rows, heads, D] against the formula in float64, held to a bound of each number's own, with w_j the weights:
+def formula(q, k, v, table, positions, window, scale, dtype, rounded_q=False, times=None):
+    """Attention of q [rows, heads, D] in float64 and a bound of each number's own.  With w_j the weights:
 
       |error| <= r |result| + (p + 2 d) sum_j w_j |v_j|
       r   the result's one rounding: 2^-8 (bfloat16), 2^-24 (float32)
@@ -102,13 +102,13 @@ def tight(out, q, k, v, table, positions, window, scale, dtype, rounded_q=False)
       d   the largest error of a score, which moves weights by a factor of 1 + d and the denominator likewise: of the products' sums in
           float32 2^-17 of sum_d |q_d k_d| (128 roundings of 2^-24), and 2^-11 more where q is rounded to halves on its way (``rounded_q``)
 
-    Returns the formula's result and the bound."""
+    times: how often each key counts (for tests of the bound itself)."""
     heads, kv_heads, page = q.shape[1], k.shape[1], k.shape[2]
     end = int(max(positions)) + 1
-    blocks = table[:-(-end // page)].long()
-    dev = out.device
-    keys = k.to(dev)[blocks.to(dev)].permute(1, 0, 2, 3).reshape(kv_heads, -1, k.shape[3])[:, :end]
-    vals = v.to(dev)[blocks.to(dev)].permute(1, 0, 2, 3).reshape(kv_heads, -1, k.shape[3])[:, :end]
+    dev = k.device
+    blocks = table[:-(-end // page)].long().to(dev)
+    keys = k[blocks].permute(1, 0, 2, 3).reshape(kv_heads, -1, k.shape[3])[:, :end]
+    vals = v[blocks].permute(1, 0, 2, 3).reshape(kv_heads, -1, k.shape[3])[:, :end]
     keys, vals = (t.repeat_interleave(heads // kv_heads, 0) for t in (keys, vals))      # [heads, keys, D]
     qd = q.to(dev).double().transpose(0, 1)
     score, size = qd @ keys.transpose(1, 2) * scale, qd.abs() @ keys.abs().transpose(1, 2) * scale
@@ -116,15 +116,21 @@ def tight(out, q, k, v, table, positions, window, scale, dtype, rounded_q=False)
     hide = key[None] > at[:, None]
     if window:
         hide |= key[None] <= at[:, None] - window
+    if times is not None:
+        score = score + torch.log(times.to(dev))
     w = torch.softmax(score.masked_fill(hide, -math.inf), -1)
     ref, spread = (w @ vals).transpose(0, 1), (w @ vals.abs()).transpose(0, 1)
     d = size.masked_fill(hide, 0).amax(-1).transpose(0, 1)[..., None] * (2.0 ** -17 + (2.0 ** -11 if rounded_q else 0.0))
     r, p = (2.0 ** -24, 2.0 ** -16) if dtype == "float32" else (2.0 ** -8, 2.0 ** -11 + 2.0 ** -16)
-    limit = r * ref.abs() + (p + 2 * d) * spread
+    return ref, r * ref.abs() + (p + 2 * d) * spread
+
+
+def tight(out, q, k, v, table, positions, window, scale, dtype, rounded_q=False):
+    """``out`` [rows, heads, D] within the formula's bound."""
+    ref, limit = formula(q, k.to(out.device), v.to(out.device), table, positions, window, scale, dtype, rounded_q)
     assert torch.isfinite(out).all()
     err = (out.double() - ref).abs()
     assert (err <= limit).all(), f"{(err / limit.clamp(min=1e-300)).max().item():.2f} of the limit"
-    return ref, limit
 
 
 def magnitudes(lengths, kv_heads, dim, page, kexp, vexp, seed):

@@ -24,6 +24,7 @@
 #include <mutex>
 
 #include "common.cuh"
+#include "cp_async.cuh"
 
 #ifndef RL_HEAD_DIM
 #error "compile with -DRL_HEAD_DIM=<head size>"
@@ -626,9 +627,6 @@ __device__ __forceinline__ void cp_async16(void* smem, const void* gmem, bool pr
   const int bytes = pred ? 16 : 0;   // src-size 0: the 16 bytes are zero-filled
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(s), "l"(gmem), "r"(bytes));
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N)); }
 
 }  // namespace rl
 #include "decode_stream.cuh"

@@ -117,12 +117,6 @@ __device__ __forceinline__ void cursor_advance(StreamCursor& c, const StreamShar
   }
 }
 
-__device__ __forceinline__ float ex2_approx(float x) {      // 2^x; -inf gives 0
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 __device__ __forceinline__ int atomic_add_acq_rel(int* p, int v) {
   int old;
   asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], %2;" : "=r"(old) : "l"(p), "r"(v) : "memory");
@@ -134,13 +128,6 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
   return v;
-}
-__device__ __forceinline__ void cp_async16_s(uint32_t smem, const void* gmem) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(smem), "l"(gmem));
-}
-__device__ __forceinline__ void cp_async16_s(uint32_t smem, const void* gmem, bool pred) {
-  const int bytes = pred ? 16 : 0;   // src-size 0: the 16 bytes are zero-filled
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem), "l"(gmem), "r"(bytes));
 }
 
 // Merges the pieces of (item, kv head) into the output row of each of its heads; `nthreads` threads

@@ -1202,7 +1202,7 @@ int launch_prefill(const void* q, int q_stride, const void* kc, const void* vc, 
   a.window = window;
   a.scale = scale;
   a.pages = pages;
-  static bool tc_set[kMaxDevices], simt_set[kMaxDevices];
+  static bool simt_set[kMaxDevices];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return static_cast<int>(e);
@@ -1213,6 +1213,7 @@ int launch_prefill(const void* q, int q_stride, const void* kc, const void* vc, 
       int sms = 0;
       const int err = device_sms(&sms);
       if (err) return err;
+      static bool tc_set[kMaxDevices];
       if (!tc_set[dev]) {
         e = cudaFuncSetAttribute(prefill_attn_tc_kernel<Kv8PrefillArgs<bf16>>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  static_cast<int>(kPrefillTcSmem8));

@@ -35,6 +35,7 @@
 //   shares  the launch's keys in equal shares, one to a group (kv8.cuh): for rows of very different lengths
 #pragma once
 
+#include "cp_async.cuh"
 #include "tma.cuh"
 
 namespace rl {
@@ -48,27 +49,10 @@ constexpr int kMaxCluster = 8;
 constexpr int kPartLd = kD + 4;                          // floats to a head in a warp's partial result: kd numerators, d, m, denominator
 static_assert(16 * kPartLd * 4 <= kRingBytes, "a warp's partial result lies in its own ring");
 
-__device__ __forceinline__ void cp_async16_s(uint32_t smem, const void* gmem) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(smem), "l"(gmem));
-}
-__device__ __forceinline__ void cp_async16_s(uint32_t smem, const void* gmem, bool pred) {
-  const int bytes = pred ? 16 : 0;   // src-size 0: the 16 bytes are zero-filled
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem), "l"(gmem), "r"(bytes));
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
-}
 __device__ __forceinline__ uint4 lds16(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
   return v;
-}
-__device__ __forceinline__ float ex2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 // 16 rows of 16 bytes, a row's address in each of lanes 0 .. 15, and 16 more in lanes 16 .. 31: lane (g, t) gets rows
 // 4 t .. 4 t + 3 of column g in v[0], of column g + 8 in v[1], and of the second rows likewise in v[2] and v[3].

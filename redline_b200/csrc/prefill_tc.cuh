@@ -1,16 +1,15 @@
 // Prompt-portion attention on the fifth-generation tensor cores (bfloat16, head size 64 or 128).
 //
-// Included by attention.cu, and by kv8.cu for a cache in 8 bits (the arguments' type says which: kEightBit).  Before it come
-// cp_async16_s, cp_async_commit, cp_async_wait and ex2_approx.  With eight bits the products are of halves: the loaders bring a tile's
-// bytes through registers and convert them (one conversion and one product for two numbers; to bfloat16 it was four times as
-// many instructions, and a portion of 2,048 behind 6,144 keys took 419 us).  A page's scale goes in relative to 2^-7 of the largest of the
-// item's pages, so that no half overflows, which is exact for pages down to 2^-22 of that; the largest goes into the exponent's factor
-// (keys) and the epilogue's (values).  Items whose pages are farther apart than that are listed by the loaders, and items with a result that
-// is not finite by the rows (a value that is not a number reaches rows that do not see its key, too: a weight of 0 does not cover it); the
-// rows of a listed item are done once more at the end, one by one (kv8_row).  A page whose scale is the smallest is taken for one of
-// zeros here.  A row of Q is scaled by a power of two to at most 256, which
-// goes into the row's factor: as halves its entries keep their bits down to 2^-21 of its largest.  (Done by two of the loaders and not by
-// all six, three portions at head size 128 took 199 us instead of 172.)  P is a half too, times 2^7.
+// Included by attention.cu, and by kv8.cu for a cache in 8 bits (the arguments' type says which: kEightBit).
+// With eight bits the products are of halves: the loaders bring a tile's bytes through registers and convert them (one conversion and
+// one product for two numbers; to bfloat16 it was four times as many instructions, and a portion of 2,048 behind 6,144 keys took
+// 419 us).  A page's scale goes in relative to 2^-7 of the largest of the item's pages, so that no half overflows, which is exact for
+// pages down to 2^-22 of that; the largest goes into the exponent's factor (keys) and the epilogue's (values).  Items whose pages are
+// farther apart are listed by the loaders, and items with a result that is not finite by the rows (a value that is not a number
+// reaches rows that do not see its key, too: a weight of 0 does not cover it); the rows of a listed item are done once more at the
+// end, one by one (kv8_row).  A page whose scale is the smallest is taken for one of zeros here.  A row of Q is scaled by a power of
+// two to at most 256, which goes into the row's factor: as halves its entries keep their bits down to 2^-21 of its largest.  (Done by two
+// of the loaders and not by all six, three portions at head size 128 took 199 us instead of 172.)  P is a half too, times 2^7.
 // An item of work is a tile of up to 128 consecutive query rows of one sequence for TWO query heads of one
 // kv head (the last pair of an odd group has one): the two heads are the CTA's two "slots", they attend to the same keys and
 // values, so a K tile and a V tile are brought into shared memory once for both.  Persistent CTAs (one per SM) take items
@@ -57,6 +56,7 @@
 // loops, the copies in flight are waited for, TMEM is freed and bit 2 of *status is set.
 #pragma once
 
+#include "cp_async.cuh"
 #include "kv8.cuh"
 #include "umma.cuh"
 

@@ -127,6 +127,11 @@ __device__ __forceinline__ TcItem tc_item(const Args& a, int tile, int rem, int 
   w.rows = a.tile_rows[tile];
   w.pos0 = a.positions[w.tok0];
   w.k_end = w.pos0 + w.rows;
+  // (a tile without rows, which may stand in a list that was captured, goes through one key tile that nobody sees: every role counts it)
+  if (Args::kEightBit && w.rows <= 0) {
+    w.pos0 = 0;
+    w.k_end = 1;
+  }
   w.lo0 = (a.window > 0 && w.pos0 + 1 > a.window) ? w.pos0 + 1 - a.window : 0;
   w.k_begin = w.lo0 / kTcKeys * kTcKeys;
   w.nt = (w.k_end - w.k_begin + kTcKeys - 1) / kTcKeys;

@@ -923,8 +923,8 @@ def kv8_attn_prefill(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, vcach
                      tile_rows: torch.Tensor, positions: torch.Tensor, out: torch.Tensor, tiles: int, num_heads: int,
                      num_kv_heads: int, head_dim: int, page_size: int, window: int, scale: float, impl: int = 0) -> None:
     """``attn_prefill`` over a cache in 8 bits (kv8_write): tiles of up to 128 consecutive query tokens of one sequence
-    (tile_seq, tile_tok, tile_rows); rows of ``out`` that no tile names are left as they were.  A page id beyond the pool is
-    read as page 0, and bit 16 of ``tc_status`` tells.  impl 0: the best kernel that applies (bfloat16 at head sizes 64 and 128:
+    (tile_seq, tile_tok, tile_rows; a tile of no rows is passed over); rows of ``out`` that no tile names are left as they were.  A page id
+    beyond the pool is read as page 0, and bit 16 of ``tc_status`` tells.  impl 0: the best kernel that applies (bfloat16 at head sizes 64 and 128:
     tcgen05; else CUDA cores); 1: CUDA cores; 3: the tcgen05 kernel or an error.
 
     The tcgen05 kernel works on halves: softmax weights keep 11 bits down to 2^-21 of a row's largest.  Tiles whose pages' scales are more than

@@ -203,3 +203,32 @@ def test_a_refused_call_stores_nothing(heads, kv_heads, dim, page, dtype):
             rope(x, gpu, table, [(0, 5), (1, 20), (2, 33)], cos, sin, heads, kv_heads, dim, page, impl)
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(bytes_of(gpu), cache))
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,page,dtype,n", [(4, 2, 64, 16, "bfloat16", 5), (3, 1, 128, 16, "bfloat16", 5), (32, 8, 64, 32, "bfloat16", 40),
+                                                             (16, 8, 128, 16, "bfloat16", 40), (4, 2, 64, 16, "float32", 5), (10, 2, 80, 16, "bfloat16", 5)])
+def test_tiles_without_rows(heads, kv_heads, dim, page, dtype, n):
+    """Among the others, first and last, at positions that begin a key tile and others; a list of nothing else."""
+    segments = [(128 * (s % 3) + s % 2, 1 + 29 * s % 120) for s in range(n)]
+    lengths = [a + m for a, m in segments]
+    cache, table = filled(lengths, heads, kv_heads, dim, page, seed=1)
+    gpu = on_gpu(cache)
+    positions = torch.tensor([p for a, m in segments for p in range(a, a + m)], dtype=torch.int32, device=DEV)
+    seq, tok, rows = (t.tolist() for t in tiles_of(segments))
+    full = list(zip(seq, tok, rows))
+    with_empty = [(0, tok[0], 0)]
+    for i, t in enumerate(full):
+        with_empty += [t, (t[0], t[1], 0)] if i % 2 else [t]
+    q = torch.randn(len(positions), heads * dim, generator=torch.Generator().manual_seed(1)).to(DT[dtype]).to(DEV)
+
+    def run(tiles, out):
+        lists = [torch.tensor(t, dtype=torch.int32, device=DEV) for t in zip(*tiles)]
+        kernels.kv8_attn_prefill(q, q.stride(0), *gpu, table.to(DEV), *lists, positions, out, len(tiles), heads, kv_heads, dim, page, 0,
+                                 1.0 / math.sqrt(dim))
+        assert take_status() == 0
+        return out
+
+    want, got = run(full, torch.empty_like(q)), run(with_empty, torch.empty_like(q))
+    assert torch.isfinite(want).all() and torch.equal(want, got)
+    nothing = run([(0, 0, 0)] * 7, torch.full_like(q, 9.0))
+    assert (nothing == 9.0).all()

@@ -190,8 +190,9 @@ kv8_write_kernel(const Kv8WriteArgs<T> a, int span, int tasks) {
     for (int i = threadIdx.x; i < t; i += kWriteThreads) {
       const long long s = kv8_slot(a, i);
       before |= s >= 0 && (s >> a.page_shift) == page;
-      if (a.items != nullptr) before |= a.items[i].z > 0 && a.items[i].y == seq;
     }
+    if (a.items != nullptr)
+      for (int i = threadIdx.x; i < t; i += kWriteThreads) before |= a.items[i].z > 0 && a.items[i].y == seq;
     if (__syncthreads_or(before)) {                        // (every thread has read its scale)
       if (threadIdx.x == 0 && page != 0) atomicOr(a.status, 8);
       continue;

@@ -295,7 +295,7 @@ __device__ __forceinline__ bool tc_run(const Kv8Args& a, const Kv8Segment& s, in
     st.l[h][0] = st.l[h][1] = 0.f;
   }
   st.vref = -1000;
-  int vleast = 1000;                                     // the smallest exponent of a page's values
+  uint32_t vleast = 0x3fffffff;                          // the smallest exponent of a page's values, plus 125 (a page of zeros: a large number)
   bool near = true;
   if (n <= 0) return true;
   const int32_t* bt = a.block_table + static_cast<size_t>(s.seq) * a.max_blocks;
@@ -363,8 +363,7 @@ __device__ __forceinline__ bool tc_run(const Kv8Args& a, const Kv8Segment& s, in
                           || a.block_table[static_cast<size_t>(other.y) * a.max_blocks + ((other.z - 1) >> shift)] == token_page))
         mine = false;
     }
-    // (a page beyond the pool stands as page 0 here, but nothing is stored there)
-    if (static_cast<unsigned>(bt[(s.ctx - 1) >> shift]) >= static_cast<unsigned>(a.pages)) mine = false;
+    if (lane == 0 && bad) mine = false;                  // (a page beyond the pool stands as page 0 here, but nothing is stored there)
     mine = __all_sync(0xffffffffu, mine);
     if (!mine && token_page != 0 && lane == 0) atomicOr(a.status, 8);
   }
@@ -466,14 +465,15 @@ __device__ __forceinline__ bool tc_run(const Kv8Args& a, const Kv8Segment& s, in
       kf[b] = kv8_scale(c & 255);
       ve[b] = static_cast<int>(c >> 8) - 127;
       odd |= ve[b] == 128;
-      if (ve[b] > -126) vleast = min(vleast, ve[b]);
     }
     const int vref = max(st.vref, max(ve[0], ve[1]));
-    if (vref - vleast > kDecSpread) {                    // (the same for the warp)
-      near = false;
-      break;
-    }
-    if (vref != st.vref) {
+    const uint32_t least = min(static_cast<uint32_t>(ve[0] + 125), static_cast<uint32_t>(ve[1] + 125));
+    if (vref != st.vref || least < vleast) {             // (the same for the warp)
+      vleast = min(vleast, least);
+      if (vref + 125 - static_cast<int>(vleast) > kDecSpread) {
+        near = false;
+        break;
+      }
       const float f = kv8_exp2i(max(st.vref - vref, -127));
 #pragma unroll
       for (int c = 0; c < NC; ++c)

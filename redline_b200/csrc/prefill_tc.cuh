@@ -229,9 +229,9 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-__device__ __forceinline__ float max_nan(float a, float b) {      // not a number if one of them is
+__device__ __forceinline__ float max_nan(float a, float b, float c) {      // not a number if one of them is
   float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 
@@ -993,15 +993,14 @@ prefill_attn_tc_kernel(const Args a, int tiles, int* status) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(o[d + e]) * inv;
             if constexpr (Args::kEightBit)
-#pragma unroll
-              for (int e = 0; e < 8; ++e) largest = max_nan(largest, fabsf(v[e]));
+              largest = max_nan(max_nan(v[0], v[1], v[2]), max_nan(v[3], v[4], v[5]), max_nan(v[6], v[7], largest));
             store16(dst + c0 + d, v);
           }
         }
       }
       tc_fence_before();
       if constexpr (Args::kEightBit)
-        if (__any_sync(0xffffffffu, !(largest < INFINITY)) && lane == 0) tc_list(sh, wk.item);
+        if (__any_sync(0xffffffffu, largest != largest) && lane == 0) tc_list(sh, wk.item);
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->o_free[s]);
     }

@@ -593,6 +593,32 @@ constexpr int kPR = 64, kPK = 64, kPreThreads = 256;      // query rows and keys
 constexpr int kPLd = 68;                                  // floats to a row of 64 in shared memory
 constexpr size_t kPreSmem = sizeof(float) * (2 * kD * kPLd + kPK * kD + kPK * kPLd);
 
+// Rows tok0 .. + rows of one head once more, R to a warp.
+template <typename T>
+__device__ __noinline__ void kv8_prefill_again(const Kv8PrefillArgs<T>& a, int seq, int tok0, int rows, int pos0, int head) {
+  typedef Kv8Rows<kD> Rows;
+  const int lane = threadIdx.x & 31, at = head * kD + lane * Rows::E;
+#pragma unroll 1
+  for (int r0 = (threadIdx.x >> 5) * Rows::R; r0 < rows; r0 += kPreThreads / 32 * Rows::R) {
+    float q[Rows::R][Rows::E] = {}, o[Rows::R][Rows::E], top, den;
+#pragma unroll
+    for (int r = 0; r < Rows::R; ++r)
+      if (Rows::in_head(lane) && r0 + r < rows)
+#pragma unroll
+        for (int e = 0; e < Rows::E; ++e) q[r][e] = to_float(a.q[static_cast<size_t>(tok0 + r0 + r) * a.q_stride + at + e]);
+    const int mine = r0 + Rows::row_of(lane), pos = pos0 + mine;
+    kv8_rows<kD>(a, seq, head / (a.hq / a.hkv), a.window > 0 && pos + 1 > a.window ? pos + 1 - a.window : 0, mine < rows ? pos + 1 : 0,
+                 a.scale * 1.4426950408889634f, lane, q, o, top, den);
+#pragma unroll
+    for (int r = 0; r < Rows::R; ++r) {
+      const float d = __shfl_sync(0xffffffffu, den, r * 4 * Rows::L);
+      if (Rows::in_head(lane) && r0 + r < rows)
+#pragma unroll
+        for (int e = 0; e < Rows::E; ++e) a.out[static_cast<size_t>(tok0 + r0 + r) * a.out_stride + at + e] = from_float<T>(o[r][e] / d);
+    }
+  }
+}
+
 // Portions of prompts on the CUDA cores: a CTA to 64 consecutive query rows (half a tile of the launch) of one head;
 // keys in tiles of 64.  Thread (ty, tx) has rows 4 ty .. + 3; of S their keys 4 tx .. + 3 (operands as four rows and four
 // keys side by side: two 16-byte reads for 16 products), of O their columns tx + 16 j.  For float32 and the head sizes that the tcgen05
@@ -600,7 +626,7 @@ constexpr size_t kPreSmem = sizeof(float) * (2 * kD * kPLd + kPK * kD + kPK * kP
 // heads of 128: 45 us.  What bounds it is the FFMA pipe and the reads of its operands from shared memory; few items do not fill the SMs.
 template <typename T>
 __global__ void __launch_bounds__(kPreThreads)
-kv8_prefill_kernel(const Kv8PrefillArgs<T> a, int* status) {
+kv8_prefill_kernel(const __grid_constant__ Kv8PrefillArgs<T> a, int* status) {
   extern __shared__ __align__(16) float tiles[];
   float* qs = tiles;                        // [D][68], scaled
   float* ks = qs + kD * kPLd;               // [D][68]
@@ -727,21 +753,7 @@ kv8_prefill_kernel(const Kv8PrefillArgs<T> a, int* status) {
 #pragma unroll
     for (int j = 0; j < NC; ++j) odd |= !(fabsf(acc[i][j]) < INFINITY);
   if (__syncthreads_or(odd)) {
-    constexpr int E = Kv8Row<kD>::E;
-    const int lane = threadIdx.x & 31;
-#pragma unroll 1
-    for (int r = threadIdx.x >> 5; r < rows; r += kPreThreads / 32) {
-      float q[E] = {}, o[E], top, den;
-      const int pos = pos0 + r, at = head * kD + lane * E;
-      if (Kv8Row<kD>::in_head(lane))
-#pragma unroll
-        for (int e = 0; e < E; ++e) q[e] = to_float(a.q[static_cast<size_t>(tok0 + r) * a.q_stride + at + e]);
-      kv8_row<kD>(a, a.tile_seq[tile], kvh, a.window > 0 && pos + 1 > a.window ? pos + 1 - a.window : 0, pos + 1, a.scale * kLog2e, lane,
-                  q, o, top, den);
-      if (Kv8Row<kD>::in_head(lane))
-#pragma unroll
-        for (int e = 0; e < E; ++e) a.out[static_cast<size_t>(tok0 + r) * a.out_stride + at + e] = from_float<T>(o[e] / den);
-    }
+    kv8_prefill_again<T>(a, a.tile_seq[tile], tok0, rows, pos0, head);
     return;
   }
 #pragma unroll

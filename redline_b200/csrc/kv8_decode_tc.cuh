@@ -12,8 +12,7 @@
 //   softmax      online, in log2 units, against a reference that moves only when some score exceeds it by 2^10: one vote a sub-block
 //                instead of shuffles.  The weights are halves, 2^5 at the reference: 11 bits down to 2^-19 of it, steps of 2^-29 below.
 //                For the product they carry the value scale of their page relative to the largest so far.  A run that meets pages more than
-//                2^10 apart is left and done by itself, a row after the other in float32 (kv8_row); a page whose scale is the smallest
-//                counts as zeros
+//                2^10 apart is left and done in float32 (kv8_rows); a page whose scale is the smallest counts as zeros
 //   O^T += V^T P^T   ldmatrix transposes 16 x 16 bytes of V: four keys of an entry in a word; movmatrix transposes P
 // With the rotation in the kernel (a.store) the warp that has a row's newest page also stores the token's key and value there: it
 // takes that sub-block first, puts the token over what the copy brought, rescales the page if its scale rises, and goes on
@@ -581,27 +580,36 @@ __device__ __forceinline__ bool tc_run(const Kv8Args& a, const Kv8Segment& s, in
   return near;
 }
 
-// The same run, a head after the other and a lane to kD / 32 entries, into the place of the warp's partial result.
+// The same run in float32, into the place of the warp's partial result.
 __device__ __noinline__ void tc_run_far(const Kv8Args& a, Kv8Segment s, int sb0, int n, int lane, float* to) {
-  constexpr int E = kD / 32;
-  const int G = a.hq / a.hkv, at = lane * E, dh = at % (kD / 2);
+  typedef Kv8Rows<kD> Rows;
+  const int G = a.hq / a.hkv, at = lane * Rows::E, dh = at % (kD / 2);
 #pragma unroll 1
-  for (int r = 0; r < G; ++r) {
-    const bf16* row = static_cast<const bf16*>(a.q) + static_cast<size_t>(s.tok) * a.q_stride + (s.kvh * G + r) * kD;
-    float x[E], o[E], m, l;
+  for (int r0 = 0; r0 < G; r0 += Rows::R) {
+    float x[Rows::R][Rows::E] = {}, o[Rows::R][Rows::E], m, l;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      x[e] = to_float(row[at + e]);
-      if (a.cos != nullptr) {
-        const size_t i = static_cast<size_t>(s.ctx - 1 < a.max_pos ? s.ctx - 1 : 0) * (kD / 2) + dh + e;
-        const float other = to_float(row[at < kD / 2 ? at + e + kD / 2 : dh + e]);
-        x[e] = at < kD / 2 ? x[e] * a.cos[i] - other * a.sin[i] : x[e] * a.cos[i] + other * a.sin[i];
+    for (int r = 0; r < Rows::R; ++r) {
+      if (r0 + r >= G) continue;
+      const bf16* row = static_cast<const bf16*>(a.q) + static_cast<size_t>(s.tok) * a.q_stride + (s.kvh * G + r0 + r) * kD;
+#pragma unroll
+      for (int e = 0; e < Rows::E; ++e) {
+        x[r][e] = to_float(row[at + e]);
+        if (a.cos != nullptr) {
+          const size_t i = static_cast<size_t>(s.ctx - 1 < a.max_pos ? s.ctx - 1 : 0) * (kD / 2) + dh + e;
+          const float other = to_float(row[at < kD / 2 ? at + e + kD / 2 : dh + e]);
+          x[r][e] = at < kD / 2 ? x[r][e] * a.cos[i] - other * a.sin[i] : x[r][e] * a.cos[i] + other * a.sin[i];
+        }
       }
     }
-    kv8_row<kD>(a, s.seq, s.kvh, max(s.key_lo, sb0 * kSub), min(s.key_hi, (sb0 + n) * kSub), a.scale * 1.4426950408889634f, lane, x, o, m, l);
+    const int mine = r0 + Rows::row_of(lane);
+    kv8_rows<kD>(a, s.seq, s.kvh, max(s.key_lo, sb0 * kSub), mine < G ? min(s.key_hi, (sb0 + n) * kSub) : 0, a.scale * 1.4426950408889634f, lane,
+                 x, o, m, l);
 #pragma unroll
-    for (int e = 0; e < E; ++e) to[r * kPartLd + at + e] = o[e];
-    if (lane == 0) *reinterpret_cast<float4*>(to + r * kPartLd + kD) = make_float4(0.f, m, l, 0.f);
+    for (int r = 0; r < Rows::R; ++r)
+      if (r0 + r < G)
+#pragma unroll
+        for (int e = 0; e < Rows::E; ++e) to[(r0 + r) * kPartLd + at + e] = o[r][e];
+    if (mine < G && lane % (4 * Rows::L) == 0) *reinterpret_cast<float4*>(to + mine * kPartLd + kD) = make_float4(0.f, m, l, 0.f);
   }
 }
 

@@ -7,7 +7,7 @@
 // pages down to 2^-22 of that; the largest goes into the exponent's factor (keys) and the epilogue's (values).  Items whose pages are
 // farther apart are listed by the loaders, and items with a result that is not finite by the rows (a value that is not a number
 // reaches rows that do not see its key, too: a weight of 0 does not cover it); the rows of a listed item are done once more at the
-// end, one by one (kv8_row).  A page whose scale is the smallest is taken for one of zeros here.  A row of Q is scaled by a power of
+// end, by themselves (kv8_rows).  A page whose scale is the smallest is taken for one of zeros here.  A row of Q is scaled by a power of
 // two to at most 256, which goes into the row's factor: as halves its entries keep their bits down to 2^-21 of its largest.  (Done by two
 // of the loaders and not by all six, three portions at head size 128 took 199 us instead of 172.)  P is a half too, times 2^7.
 // An item of work is a tile of up to 128 consecutive query rows of one sequence for TWO query heads of one
@@ -535,19 +535,27 @@ __device__ __forceinline__ void tc_load_eight_bit(const Args& a, PrefillTcShared
 // Rows 32 q .. + 31 of slot s of an item once more, by the warp whose threads have written them.
 template <typename Args>
 __device__ __forceinline__ void tc_rows_again(const Args& a, const TcItem& w, int s, int q, int lane) {
-  constexpr int E = kD / 32;
-  static_assert(Kv8Row<kD>::E == E, "entries of a lane");
+  typedef Kv8Rows<kD> Rows;
   if (s == 1 && !w.two) return;
+  const int end = min(q * 32 + 32, w.rows), at = (w.head0 + s) * kD + lane * Rows::E;
 #pragma unroll 1
-  for (int r = q * 32; r < min(q * 32 + 32, w.rows); ++r) {
-    const int pos = w.pos0 + r, at = (w.head0 + s) * kD + lane * E;
-    float x[E], o[E], m, l;
+  for (int r0 = q * 32; r0 < end; r0 += Rows::R) {
+    float x[Rows::R][Rows::E] = {}, o[Rows::R][Rows::E], m, l;
 #pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = to_float(a.q[static_cast<size_t>(w.tok0 + r) * a.q_stride + at + e]);
-    kv8_row<kD>(a, w.seq, w.kvh, a.window > 0 && pos + 1 > a.window ? pos + 1 - a.window : 0, pos + 1, a.scale * 1.4426950408889634f, lane, x, o,
-                m, l);
+    for (int r = 0; r < Rows::R; ++r)
+      if (r0 + r < end)
 #pragma unroll
-    for (int e = 0; e < E; ++e) a.out[static_cast<size_t>(w.tok0 + r) * a.out_stride + at + e] = __float2bfloat16_rn(o[e] / l);
+        for (int e = 0; e < Rows::E; ++e) x[r][e] = to_float(a.q[static_cast<size_t>(w.tok0 + r0 + r) * a.q_stride + at + e]);
+    const int mine = r0 + Rows::row_of(lane), pos = w.pos0 + mine;
+    kv8_rows<kD>(a, w.seq, w.kvh, a.window > 0 && pos + 1 > a.window ? pos + 1 - a.window : 0, mine < end ? pos + 1 : 0,
+                 a.scale * 1.4426950408889634f, lane, x, o, m, l);
+#pragma unroll
+    for (int r = 0; r < Rows::R; ++r) {
+      const float d = __shfl_sync(0xffffffffu, l, r * 4 * Rows::L);
+      if (r0 + r < end)
+#pragma unroll
+        for (int e = 0; e < Rows::E; ++e) a.out[static_cast<size_t>(w.tok0 + r0 + r) * a.out_stride + at + e] = __float2bfloat16_rn(o[r][e] / d);
+    }
   }
 }
 

@@ -882,7 +882,7 @@ def kv8_attn_decode(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, vcache
                than SMs), or an error (tensor cores: bfloat16, head size 64 or 128, up to 16 query heads to a kv head)
 
     On the tensor cores softmax weights are halves, 11 bits down to 2^-19 of a row's largest; what meets values of pages more than 2^10 apart
-    is done in float32, some 50 times slower.
+    is done in float32, four times slower.
     """
     _kv8_decode("kv8_attn_decode", q, q_stride, kcache, vcache, kscale, vscale, block_table, items, workspace, out, nitems,
                 num_heads, num_kv_heads, head_dim, page_size, window, scale, None, None, None, max_ctx, sum_ctx, impl)
@@ -928,7 +928,7 @@ def kv8_attn_prefill(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, vcach
     tcgen05; else CUDA cores); 1: CUDA cores; 3: the tcgen05 kernel or an error.
 
     The tcgen05 kernel works on halves: softmax weights keep 11 bits down to 2^-21 of a row's largest.  Tiles whose pages' scales are more than
-    2^22 apart, or with a result that is not finite, are done once more row by row in float32, some 50 times slower."""
+    2^22 apart, or with a result that is not finite, are done once more in float32, 25 to 50 times slower."""
     what = "kv8_attn_prefill"
     _kv8_check(what, kcache, vcache, kscale, vscale, num_heads, num_kv_heads, head_dim, page_size)
     at = kcache.get_device()

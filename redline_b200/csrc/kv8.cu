@@ -84,7 +84,8 @@ __device__ __forceinline__ int kv8_position(const Kv8WriteArgs<T>& a, int pos) {
 
 constexpr int kWriteThreads = 256, kWriteWarps = kWriteThreads / 32;
 constexpr int kWriteTokens = 32 / (kD / 16);       // tokens that a warp takes at once: each D/16 lanes, 8 entries of either half of the head
-// Rounds of them that stay in registers between the two passes over a run: a page of 16 tokens at head sizes up to 128.
+// Rounds of them that are kept between the two passes over a run: a page of 16 tokens at head sizes up to 128.  (As floats, and with three CTAs an SM
+// a thread has 80 registers: 32 bytes of them are spilled at head size 64, 424 at 128.)
 constexpr int kWriteRounds = kD <= 64 ? 2 : 4;
 
 // gridDim.y = tasks + 1.  CTAs (x, y < tasks) store: where a RUN begins among the `span` tokens from x * span, the tokens that follow one
@@ -95,7 +96,8 @@ constexpr int kWriteRounds = kD <= 64 ? 2 : 4;
 // begin no run, and the CTAs are handed out one by one.
 // What bounds it is the way from the slots to the rows to the block's largest magnitude to the bytes; what does not depend on one
 // another is asked for together.  32 / 8 heads of 64: 8 single tokens 3.7 us, a prompt of 2,048 tokens 11.4 us (2.0 TB/s); nine portions
-// of 1 to 700 tokens at head size 128 26.6 us (2.3 TB/s).
+// of 1 to 700 tokens at head size 128 26.7 us (2.3 TB/s).  The look at all earlier tokens before a run is stored grows with the square: 16,384
+// tokens 94 us (1.9 TB/s), 65,536 679 us (1.1 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(kWriteThreads, 3)
 kv8_write_kernel(const Kv8WriteArgs<T> a, int span, int tasks) {
@@ -386,7 +388,7 @@ constexpr int kGenLanes = kD <= 16 ? 1 : kD <= 32 ? 2 : kD <= 64 ? 4 : kD <= 128
 // Single tokens on the CUDA cores.  A CTA to a share; a key to kGenLanes lanes of a warp, each with 16 entries of four
 // query heads and their numerators in registers and a running (max, denominator) of its own keys.  For float32 and the head sizes and groups
 // that the tensor-core kernel does not take; what bounds it is the conversions and products, 0.5 to 0.9 TB/s of the cache (32 / 8 heads in
-// bfloat16: 8 x 4,096 keys at head size 64 69 us against 16.6, 1 x 131,072 at 128 353 against 58).
+// bfloat16: 8 x 4,096 keys at head size 64 69 us against 17, 1 x 131,072 at 128 353 against 58; float32 8 x 4,096 60 us; 10 / 2 heads of 80 in bfloat16 70).
 template <typename T>
 __global__ void __launch_bounds__(kGenThreads)
 kv8_decode_kernel(const Kv8Args a) {
@@ -622,8 +624,8 @@ __device__ __noinline__ void kv8_prefill_again(const Kv8PrefillArgs<T>& a, int s
 // Portions of prompts on the CUDA cores: a CTA to 64 consecutive query rows (half a tile of the launch) of one head;
 // keys in tiles of 64.  Thread (ty, tx) has rows 4 ty .. + 3; of S their keys 4 tx .. + 3 (operands as four rows and four
 // keys side by side: two 16-byte reads for 16 products), of O their columns tx + 16 j.  For float32 and the head sizes that the tcgen05
-// kernel does not take (bfloat16 at 64: 2,048 tokens behind 6,144 keys 5,520 us against 276); float32, four portions of 33 to 129 tokens, 3 / 1
-// heads of 128: 45 us.  What bounds it is the FFMA pipe and the reads of its operands from shared memory; few items do not fill the SMs.
+// kernel does not take (bfloat16 at 64: 2,048 tokens behind 6,144 keys 5,520 us against 254); float32, four portions of 33 to 129 tokens, 3 / 1
+// heads of 128: 46 us; 512 tokens behind 512 in bfloat16, 12 / 4 heads of 96, 243 us.  What bounds it is the FFMA pipe and the reads of its operands from shared memory; few items do not fill the SMs.
 template <typename T>
 __global__ void __launch_bounds__(kPreThreads)
 kv8_prefill_kernel(const __grid_constant__ Kv8PrefillArgs<T> a, int* status) {

@@ -5,9 +5,9 @@
 // the sub-blocks of its run come by 16-byte asynchronous copies into a private ring, 8 to 16 KB on their way while one is worked on
 // (44 KB an SM cover the way from DRAM at full rate).  A sub-block:
 //   S = K Q^T    mma.sync.m16n8k16 on halves, 16 keys x 8 query heads: an e4m3 number is a half exactly (one conversion for two); q is
-//                scaled by a power of two per row to at most 256 and rounded to 11 bits.  (The instruction on e4m3 bytes is put together
-//                from conversions, products on halves and sums on this machine and was slower; with the heads as the wide side, half
-//                of its rows empty, there were twice as many products.)  Which entries of the head a k index of the product
+//                scaled by a power of two per row to at most 256 and rounded to 11 bits.  (The instruction on e4m3 bytes, k = 32, takes
+//                1.26 times as long as this one and would want q in three parts of four bits; with the heads as the wide side, half of
+//                its rows empty, there were twice as many products.)  Which entries of the head a k index of the product
 //                stands for is free, so a lane's 16 bytes of a key are four k steps of the A fragment as they lie.
 //   softmax      online, in log2 units, against a reference that moves only when some score exceeds it by 2^10: one vote a sub-block
 //                instead of shuffles.  The weights are halves, 2^5 at the reference: 11 bits down to 2^-19 of it, steps of 2^-29 below.
@@ -24,8 +24,8 @@
 // thread.
 //
 // What bounds a long launch is the copies' rate; a short one its chain of trips (0.7 us each) and the one fetch of every
-// instruction.  32 / 8 heads, the token's own write included at head size 64: one sequence of 513 keys 8.8 us, 8 of 4,096 16.6 us (2.0 TB/s),
-// 64 of 516 to 768 19.0; head size 128: one of 131,072 keys 58 us (4.6 TB/s), 24 of 64 to 8,192 62 us (3.6 TB/s).
+// instruction.  32 / 8 heads, the token's own write included at head size 64: one sequence of 513 keys 8.5 us, 8 of 4,096 17.0 us (1.9 TB/s),
+// 64 of 516 to 768 19.4; head size 128: one of 131,072 keys 58 us (4.6 TB/s), 24 of 64 to 8,192 62 us (3.6 TB/s).
 //
 // Where rows are shared out (see kv8_choice in kv8.cu for which):
 //   rows    a cluster of up to 8 CTAs to a row, whose partial results meet in the first one's shared memory; or, with more rows

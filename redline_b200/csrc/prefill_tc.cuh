@@ -44,9 +44,9 @@
 // head size 128, 333 tokens 21.9 (26.4), 2,048 70.4 (79.5), 8,192 834 (918), 16,384 3,146 (3,464), 2,048 behind 12,288
 // 724 (795).  So long rows at head size 64 are 1 to 2 % slower: half the row warps hide less of the hand-overs.
 // The two give the same bits: a row's denominator is summed in the two threads' chains still.
-// With eight bits, 32 / 8 heads of 64: 333 tokens behind 1,000 keys 35 us (16 bits 36), 2,048 behind 6,144 276 us, 436 TFLOP/s (227); three
-// portions of 300 to 900 tokens behind up to 2,000 at head size 128 169 us, 289 TFLOP/s.  The loaders' instructions are what it takes
-// longer: without them the long portion takes 249 us, without the conversions alone 280 of 284.
+// With eight bits, 32 / 8 heads of 64: 333 tokens behind 1,000 keys 37 us (16 bits 36), 2,048 behind 6,144 254 us, 474 TFLOP/s (227); three
+// portions of 300 to 900 tokens behind up to 2,000 at head size 128 168 us, 290 TFLOP/s.  The loaders' instructions are what it takes
+// longer: where the long portion took 276 us it took 249 with loaders that did nothing.
 // Warp roles: warps 0-3 rows of slot 0, warps 4-7 rows of slot 1 (warp w owns TMEM lanes
 // 32 (w % 4) ..), warp 8 brings both Q tiles once per item and the K tiles, warp 9 the V tiles,
 // from the paged cache with 16-byte cp.async copies (zero-filled outside the live keys), lane 0

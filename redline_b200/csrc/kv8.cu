@@ -1117,6 +1117,7 @@ int rl_kv8_attn_decode(const Kv8DecodeCall* c) {
   const int page_size = static_cast<int>(c->page_size), impl = static_cast<int>(c->impl), max_pos = static_cast<int>(c->max_pos);
   const int max_ctx = static_cast<int>(c->max_ctx), q_stride = static_cast<int>(c->q_stride);
   const bool store = c->store != 0, single = c->dtype == 0;
+  if (hkv < 1 || hq < hkv) return static_cast<int>(cudaErrorInvalidValue);
 #ifdef RL_KV8_TC
   const bool takes = !single && hq / hkv <= 16;
 #else
@@ -1255,6 +1256,7 @@ int launch_prefill(const void* q, int q_stride, const void* kc, const void* vc, 
 }  // namespace
 
 extern "C" int rl_kv8_attn_prefill(const Kv8PrefillCall* c) {
+  if (c->hkv < 1 || c->hq < c->hkv) return static_cast<int>(cudaErrorInvalidValue);
   auto run = c->dtype == 0 ? launch_prefill<float> : launch_prefill<bf16>;
   return run(c->q, static_cast<int>(c->q_stride), c->kc, c->vc, c->ks, c->vs, c->block_table, static_cast<int>(c->max_blocks), c->tile_seq,
              c->tile_tok, c->tile_rows, c->positions, c->out, static_cast<int>(c->out_stride), static_cast<int>(c->tiles),

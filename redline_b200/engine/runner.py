@@ -35,7 +35,7 @@ GRAPH_MAX_ROWS = 1024          # no graph is captured for more rows than this
 # head is then bound by its products and not by reading its table for every 64 rows).
 SCORE_LOGITS_BYTES = 256 << 20
 STATUS_MESSAGES = {1: "a token id outside the vocabulary", 2: "a position beyond the rotary table",
-                   4: "a cache slot beyond the pool", 8: "a second run of tokens in one page of a cache in 8 bits"}
+                   4: "a cache slot beyond the pool", 8: "a second run of tokens in one page, or of one sequence, of a cache in 8 bits"}
 
 
 class EngineError(RuntimeError):

@@ -74,3 +74,24 @@ def test_the_build_has_the_8_bit_cache_wherever_it_has_attention(monkeypatch):
     monkeypatch.setattr(kernels, "build_all", lambda **kw: asked.update(kw))
     __graft_entry__.build()
     assert set(asked["head_dims"]) <= set(asked["kv8_dims"])
+
+
+def test_native_calls_without_heads():
+    """(what the Python checks refuse, asked of the library itself)"""
+    lib = kernels._kv8(64)
+    for f, fields in ((lib.rl_kv8_attn_decode, 31), (lib.rl_kv8_attn_prefill, 25)):
+        f.restype, f.argtypes = ctypes.c_int, [ctypes.c_char_p]
+        assert f(bytes(8 * fields)) == 1
+
+
+@pytest.mark.parametrize("code,tc_code,said", [(4, 0, "a cache slot beyond the pool"), (8, 0, "a second run of tokens"), (0, 16, "a page id beyond the pool")])
+def test_what_an_engine_says_of_the_bits(monkeypatch, code, tc_code, said):
+    from types import SimpleNamespace
+    from redline_b200.engine import runner
+    word = torch.tensor([tc_code], dtype=torch.int32)
+    monkeypatch.setattr(runner.kernels, "tc_status", lambda device: word)
+    status = torch.tensor([code], dtype=torch.int32)
+    me = SimpleNamespace(builder=SimpleNamespace(status=status), device=None)
+    with pytest.raises(runner.EngineError, match=said):
+        runner.ModelRunner.check_status(me)
+    runner.ModelRunner.check_status(me)                  # (told once)

@@ -388,7 +388,8 @@ constexpr int kGenLanes = kD <= 16 ? 1 : kD <= 32 ? 2 : kD <= 64 ? 4 : kD <= 128
 // Single tokens on the CUDA cores.  A CTA to a share; a key to kGenLanes lanes of a warp, each with 16 entries of four
 // query heads and their numerators in registers and a running (max, denominator) of its own keys.  For float32 and the head sizes and groups
 // that the tensor-core kernel does not take; what bounds it is the conversions and products, 0.5 to 0.9 TB/s of the cache (32 / 8 heads in
-// bfloat16: 8 x 4,096 keys at head size 64 69 us against 17, 1 x 131,072 at 128 353 against 58; float32 8 x 4,096 60 us; 10 / 2 heads of 80 in bfloat16 70).
+// bfloat16: 8 x 4,096 keys at head size 64 69 us against 17, 1 x 131,072 at 128 353 against 58; 8 x 4,096 in float32 60 us, in
+// bfloat16 with 10 / 2 heads of 80 70).
 template <typename T>
 __global__ void __launch_bounds__(kGenThreads)
 kv8_decode_kernel(const Kv8Args a) {
@@ -625,7 +626,8 @@ __device__ __noinline__ void kv8_prefill_again(const Kv8PrefillArgs<T>& a, int s
 // keys in tiles of 64.  Thread (ty, tx) has rows 4 ty .. + 3; of S their keys 4 tx .. + 3 (operands as four rows and four
 // keys side by side: two 16-byte reads for 16 products), of O their columns tx + 16 j.  For float32 and the head sizes that the tcgen05
 // kernel does not take (bfloat16 at 64: 2,048 tokens behind 6,144 keys 5,520 us against 254); float32, four portions of 33 to 129 tokens, 3 / 1
-// heads of 128: 46 us; 512 tokens behind 512 in bfloat16, 12 / 4 heads of 96, 243 us.  What bounds it is the FFMA pipe and the reads of its operands from shared memory; few items do not fill the SMs.
+// heads of 128: 46 us; 512 tokens behind 512 in bfloat16, 12 / 4 heads of 96, 243 us.  What bounds it is the FFMA pipe and the
+// reads of its operands from shared memory; few items do not fill the SMs.
 template <typename T>
 __global__ void __launch_bounds__(kPreThreads)
 kv8_prefill_kernel(const __grid_constant__ Kv8PrefillArgs<T> a, int* status) {

@@ -408,7 +408,7 @@ __device__ __forceinline__ void tc_load_eight_bit(const Args& a, PrefillTcShared
 #pragma unroll
           for (int u = 0; u < kQ; ++u)
             top[u] = __vmaxu2(__vmaxu2(v[u].x & 0x7fff7fffu, v[u].y & 0x7fff7fffu),
-                                   __vmaxu2(v[u].z & 0x7fff7fffu, v[u].w & 0x7fff7fffu));
+                              __vmaxu2(v[u].z & 0x7fff7fffu, v[u].w & 0x7fff7fffu));
 #pragma unroll
           for (int o = 1; o < CPR; o <<= 1)
 #pragma unroll

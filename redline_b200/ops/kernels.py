@@ -871,8 +871,8 @@ def kv8_attn_decode(q: torch.Tensor, q_stride: int, kcache: torch.Tensor, vcache
                     sum_ctx: int = 0, impl: int = 0) -> None:
     """``attn_decode`` over a cache in 8 bits (kv8_write): one query token per item.
 
-    items      int32 [nitems, 4]: (token index of the query, sequence index, context length, 0); an item of context 0 has
-               no keys, and its row of ``out`` is left as it was
+    items      int32 [nitems, 4]: (token index of the query, sequence index, context length, 0), the context no longer than the
+               sequence's row of ``block_table``; an item of context 0 has no keys, and its row of ``out`` is left as it was
     workspace  of kv8_decode_workspace
     block_table  a page id beyond the pool is read as page 0, and bit 16 of ``tc_status`` tells
     max_ctx, sum_ctx  the longest context and their sum, as far as the host knows them (0: unknown); the work is shared out by
